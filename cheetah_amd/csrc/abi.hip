@@ -354,6 +354,111 @@ int cheetah_hip_attention_noalloc(const float *q, const cheetah_hip_kv_view *kv,
     return launch_attention(j, g_stream);
 }
 
+// What tree attention and tree commit ask of a cache view.
+static int check_tree_view(const cheetah_hip_kv_view &kv, uint32_t kv_format) {
+    if (!kv.k_pages || !kv.v_pages || !kv.page_table) return fail("HIP backend: tree call with a null cache pointer.");
+    if (kv_format > 1) return fail("HIP backend: kv_format must be 0 (BF16) or 1 (f32).");
+    if (kv.kv_heads == 0 || kv.kv_heads > 65535 || kv.page_size > INT32_MAX)
+        return fail("HIP backend: tree call with a cache geometry out of range.");
+    if (kv.page_size == 0 || kv.page_size % 64)
+        return fail("HIP backend: the KV page size must be a multiple of 64 positions.");
+    if (kv.head_dim != 64 && kv.head_dim != 128) return fail("HIP backend: attention supports head_dim 64 and 128.");
+    if (((uintptr_t)kv.k_pages | (uintptr_t)kv.v_pages) % 16 || (uintptr_t)kv.page_table % 4)
+        return fail("HIP backend: tree call with cache pointers that are not 16-byte aligned (page table 4).");
+    return 0;
+}
+
+int cheetah_hip_tree_attention(const float *q, const cheetah_hip_kv_view *kv, uint32_t kv_format, uint32_t q_heads,
+                               const int32_t *parents, size_t n, size_t offset, float *out) {
+    if (!q || !kv || !parents || !out) return fail("HIP backend: tree attention with a null pointer.");
+    if (n == 0 || n > CHEETAH_HIP_MAX_TREE_NODES)
+        return fail("HIP backend: a tree has 1 to " + std::to_string(CHEETAH_HIP_MAX_TREE_NODES) + " nodes.");
+    CHIP_TRY(check_tree_view(*kv, kv_format));
+    if (q_heads == 0 || q_heads > 65535 || q_heads % kv->kv_heads)
+        return fail("HIP backend: q_heads must be a multiple of kv_heads.");
+    if (q_heads / kv->kv_heads > 8) return fail("HIP backend: attention supports 1..8 query heads per KV head.");
+    if (offset > (size_t)INT32_MAX - n) return fail("HIP backend: tree position out of range.");
+    if (((uintptr_t)q | (uintptr_t)out) % 16 || (uintptr_t)parents % 4)
+        return fail("HIP backend: tree attention needs 16-byte aligned q and out, 4-byte aligned parents.");
+    CHIP_TRY(ensure_ready());
+    TreeJob j;
+    j.q = q;
+    j.out = out;
+    j.k = kv->k_pages;
+    j.v = kv->v_pages;
+    j.g = KvGeom{kv->page_table, (int)kv->page_size, (int)kv->kv_heads, (int)kv->head_dim, (int)kv_format};
+    j.q_heads = (int)q_heads;
+    j.parents = parents;
+    j.n = n;
+    j.offset = offset;
+    return launch_tree_attention(j, g_stream);
+}
+
+int cheetah_hip_tree_commit(const cheetah_hip_kv_view *views, size_t nviews, uint32_t kv_format, size_t offset,
+                            const uint32_t *nodes, size_t count) {
+    if (!views || nviews == 0 || (!nodes && count)) return fail("HIP backend: tree commit with a null argument.");
+    for (size_t i = 0; i < nviews; ++i) {
+        CHIP_TRY(check_tree_view(views[i], kv_format));
+        if (views[i].page_size != views[0].page_size || views[i].kv_heads != views[0].kv_heads ||
+            views[i].head_dim != views[0].head_dim)
+            return fail("HIP backend: tree commit needs views of one geometry.");
+    }
+    for (size_t j = 0; j < count; ++j)
+        if (nodes[j] >= CHEETAH_HIP_MAX_TREE_NODES || (j && nodes[j] <= nodes[j - 1]))
+            return fail("HIP backend: a branch is strictly increasing nodes below " +
+                        std::to_string(CHEETAH_HIP_MAX_TREE_NODES) + ".");
+    if (offset > (size_t)INT32_MAX - CHEETAH_HIP_MAX_TREE_NODES)
+        return fail("HIP backend: tree position out of range.");
+    CHIP_TRY(ensure_ready());
+    const KvGeom g{nullptr, (int)views[0].page_size, (int)views[0].kv_heads, (int)views[0].head_dim, (int)kv_format};
+    for (size_t v0 = 0; v0 < nviews; v0 += kCommitViews) {
+        KvLayer layers[kCommitViews];
+        const int32_t *tables[kCommitViews];
+        const size_t n = std::min(nviews - v0, (size_t)kCommitViews);
+        for (size_t i = 0; i < n; ++i) {
+            layers[i] = KvLayer{(void *)views[v0 + i].k_pages, (void *)views[v0 + i].v_pages};
+            tables[i] = views[v0 + i].page_table;
+        }
+        CHIP_TRY(launch_tree_commit(layers, tables, n, g, offset, nodes, count, g_stream));
+    }
+    return 0;
+}
+
+int cheetah_hip_logprobs(const void *logits, uint32_t logit_format, size_t rows, size_t vocab, size_t stride,
+                         const uint32_t *tokens, uint32_t top, float *logprobs, float *entropy, uint32_t *top_ids,
+                         float *top_logprobs) {
+    if (!logits) return fail("HIP backend: logprobs with a null pointer.");
+    if (logit_format > 1) return fail("HIP backend: logit_format must be 0 (BF16) or 1 (f32).");
+    if (rows == 0 || vocab == 0 || rows > (size_t)INT32_MAX || vocab > (size_t)INT32_MAX || stride > (size_t)INT32_MAX)
+        return fail("HIP backend: logprobs shape out of range.");
+    if (stride < vocab) return fail("HIP backend: logprobs rows overlap (stride below vocab).");
+    if (top > CHEETAH_HIP_MAX_TOP || top > vocab)
+        return fail("HIP backend: logprobs returns at most " + std::to_string(CHEETAH_HIP_MAX_TOP) +
+                    " alternatives, and at most the vocabulary.");
+    if (!logprobs && !entropy && !top) return fail("HIP backend: logprobs without an output.");
+    if (logprobs && !tokens) return fail("HIP backend: logprobs of tokens needs the tokens.");
+    if ((top != 0) != (top_ids != nullptr) || (top != 0) != (top_logprobs != nullptr))
+        return fail("HIP backend: logprobs needs ids and log probabilities of the alternatives, or none.");
+    const size_t elem = logit_format ? 4 : 2;
+    if ((uintptr_t)logits % elem || ((uintptr_t)tokens | (uintptr_t)logprobs | (uintptr_t)entropy | (uintptr_t)top_ids |
+                                     (uintptr_t)top_logprobs) % 4)
+        return fail("HIP backend: logprobs with a misaligned pointer.");
+    CHIP_TRY(ensure_ready());
+    LogprobJob j;
+    j.x = logits;
+    j.f32 = logit_format == 1;
+    j.rows = rows;
+    j.vocab = vocab;
+    j.stride = stride;
+    j.tokens = tokens;
+    j.top = (int)top;
+    j.logprobs = logprobs;
+    j.entropy = entropy;
+    j.ids = top_ids;
+    j.tops = top_logprobs;
+    return launch_logprobs(j, g_stream);
+}
+
 int cheetah_hip_time_gemv(uint32_t fmt, const void *const *w, size_t nbuf, size_t rows, size_t cols,
                           const float *x, float *y, size_t iters, float *ms) {
     CHIP_TRY(ensure_ready());

@@ -225,6 +225,47 @@ int attention_prefill_splits(size_t ctx, int span = kDefaultPrefillSpan);
 // kF32PrefillSpan).
 int attention_prefill_span(size_t kv_capacity, bool kv_f32);
 
+// ---------------------------------------------------------------------------
+// Drafted tokens (tree.hip).
+// ---------------------------------------------------------------------------
+constexpr int kMaxTreeNodes = 256;  // CHEETAH_HIP_MAX_TREE_NODES
+// Views a launch of the commit moves (its arguments hold them).
+constexpr int kCommitViews = 128;
+
+// Attention of a tree's n nodes; node i's K/V row is at position offset + i.
+struct TreeJob {
+    const float *q = nullptr;  // [n][q_heads * head_dim]
+    float *out = nullptr;      // [n][q_heads * head_dim]
+    const void *k = nullptr, *v = nullptr;
+    KvGeom g;
+    int q_heads = 0;
+    const int32_t *parents = nullptr;  // device [n]
+    size_t n = 0, offset = 0;
+};
+int launch_tree_attention(const TreeJob &job, hipStream_t s);
+// In every view (a layer's pools and its page table) the K/V rows of positions
+// offset + nodes[j] move to offset + j, j = 0 .. count - 1. nodes (host): below
+// kMaxTreeNodes, strictly increasing.
+int launch_tree_commit(const KvLayer *layers, const int32_t *const *page_tables, size_t views, const KvGeom &g,
+                       size_t offset, const uint32_t *nodes, size_t count, hipStream_t s);
+
+// ---------------------------------------------------------------------------
+// Log probabilities (logprobs.hip): rows of `vocab` logits, `stride` elements
+// apart, BF16 or f32. Null outputs are left out; ids / tops hold `top` a row.
+// ---------------------------------------------------------------------------
+constexpr int kMaxTop = 64;  // CHEETAH_HIP_MAX_TOP
+struct LogprobJob {
+    const void *x = nullptr;
+    bool f32 = true;
+    size_t rows = 0, vocab = 0, stride = 0;
+    const uint32_t *tokens = nullptr;  // device [rows], with logprobs
+    int top = 0;
+    float *logprobs = nullptr, *entropy = nullptr;
+    uint32_t *ids = nullptr;
+    float *tops = nullptr;
+};
+int launch_logprobs(const LogprobJob &job, hipStream_t s);
+
 // Greedy argmax (ties -> last index, total order) of logits[n]; writes the
 // index to *out_token. When `step` is set (the device-side decode loop,
 // step[0] = token, step[1] = position) it also records the index as the

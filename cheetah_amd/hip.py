@@ -71,6 +71,9 @@ SIGNATURES = {
     "cheetah_hip_dequant_q4": (_c.c_int, [_VP, _SZ, _SZ, _VP]),
     "cheetah_hip_attention": (_c.c_int, [_VP, _c.POINTER(KvView), _c.c_uint32, _SZ, _SZ, _VP]),
     "cheetah_hip_attention_noalloc": (_c.c_int, [_VP, _c.POINTER(KvView), _c.c_uint32, _SZ, _SZ, _VP]),
+    "cheetah_hip_tree_attention": (_c.c_int, [_VP, _c.POINTER(KvView), _c.c_uint32, _c.c_uint32, _VP, _SZ, _SZ, _VP]),
+    "cheetah_hip_tree_commit": (_c.c_int, [_c.POINTER(KvView), _SZ, _c.c_uint32, _SZ, _U32P, _SZ]),
+    "cheetah_hip_logprobs": (_c.c_int, [_VP, _c.c_uint32, _SZ, _SZ, _SZ, _VP, _c.c_uint32, _VP, _VP, _VP, _VP]),
     "cheetah_hip_model_create": (_VP, [_c.POINTER(Config), _c.c_uint32, _c.c_uint32, _SZ, _SZ]),
     "cheetah_hip_model_set_unit": (_c.c_int, [_VP, _c.c_char_p, _VP, _SZ, _c.c_uint32,
                                               _c.POINTER(_c.c_uint64), _SZ]),
@@ -276,6 +279,78 @@ def attention(q: np.ndarray, kp: np.ndarray, vp: np.ndarray, table: np.ndarray, 
     fn = lib().cheetah_hip_attention_noalloc if noalloc else lib().cheetah_hip_attention
     check(fn(qd.ptr, _c.byref(view), q_heads, rows, offset, od.ptr))
     return od.download(np.float32, rows * q_heads * hd).reshape(rows, q_heads * hd)
+
+
+def tree_attention(q: np.ndarray, kp: np.ndarray, vp: np.ndarray, table: np.ndarray, q_heads: int, parents,
+                   offset: int) -> np.ndarray:
+    """cheetah_hip_tree_attention: q f32 [n, q_heads*hd]; kp/vp BF16 (uint16)
+    or f32 pages; table int32; parents: each node's parent, -1 = a root."""
+    parents = np.ascontiguousarray(parents, np.int32)
+    n = parents.size
+    _, kvh, ps, hd = kp.shape
+    if kp.dtype != vp.dtype or kp.dtype not in (np.uint16, np.float32):
+        raise ValueError("K/V pages must both be BF16 (uint16) or both f32")
+    if q.size != n * q_heads * hd or vp.shape != kp.shape:
+        raise ValueError("tree_attention shape mismatch")
+    if offset + n > table.size * ps:
+        raise ValueError("the page table ends before the tree's positions")
+    if table.size and not 0 <= int(table.min()) <= int(table.max()) < kp.shape[0]:
+        raise ValueError("page table entry outside the pool")
+    qd = DeviceBuffer.from_array(np.ascontiguousarray(q, np.float32))
+    kd, vd, td = DeviceBuffer.from_array(kp), DeviceBuffer.from_array(vp), DeviceBuffer.from_array(table)
+    pd, od = DeviceBuffer.from_array(parents), DeviceBuffer(max(n, 1) * q_heads * hd * 4)
+    view = KvView(kd.ptr, vd.ptr, td.ptr, ps, kvh, hd)
+    check(lib().cheetah_hip_tree_attention(qd.ptr, _c.byref(view), int(kp.dtype == np.float32), q_heads, pd.ptr, n,
+                                           offset, od.ptr))
+    return od.download(np.float32, n * q_heads * hd).reshape(n, q_heads * hd)
+
+
+def tree_commit(caches, offset: int, nodes) -> list:
+    """cheetah_hip_tree_commit over caches [(kp, vp, table), ...] (pages as in
+    tree_attention); returns the moved [(kp, vp), ...]."""
+    nodes = np.ascontiguousarray(nodes, np.uint32)
+    held, views = [], []
+    for kp, vp, table in caches:
+        if kp.dtype != caches[0][0].dtype or vp.dtype != kp.dtype or kp.dtype not in (np.uint16, np.float32):
+            raise ValueError("K/V pages must all be BF16 (uint16) or all f32")
+        if kp.shape != vp.shape:
+            raise ValueError("K and V pages must have one shape")
+        if nodes.size and offset + int(nodes.max()) >= table.size * kp.shape[2]:
+            raise ValueError("the page table ends before the tree's positions")
+        if table.size and not 0 <= int(table.min()) <= int(table.max()) < kp.shape[0]:
+            raise ValueError("page table entry outside the pool")
+        b = [DeviceBuffer.from_array(t) for t in (kp, vp, np.ascontiguousarray(table, np.int32))]
+        held.append(b)
+        views.append(KvView(b[0].ptr, b[1].ptr, b[2].ptr, kp.shape[2], kp.shape[1], kp.shape[3]))
+    f32 = int(bool(caches) and caches[0][0].dtype == np.float32)
+    check(lib().cheetah_hip_tree_commit((KvView * max(len(views), 1))(*views), len(views), f32, offset,
+                                        nodes.ctypes.data_as(_U32P), nodes.size))
+    return [(b[0].download(c[0].dtype, c[0].size).reshape(c[0].shape),
+             b[1].download(c[1].dtype, c[1].size).reshape(c[1].shape)) for b, c in zip(held, caches)]
+
+
+def logprobs(logits: np.ndarray, tokens=None, top: int = 0, vocab: int | None = None):
+    """cheetah_hip_logprobs of logits [rows, stride], f32 or BF16 (uint16), the
+    first `vocab` of each row (default: all): (log probabilities of `tokens` or
+    None, entropies, ids [rows, top] and log probabilities of the `top` most
+    likely)."""
+    logits = np.ascontiguousarray(logits)
+    if logits.dtype not in (np.uint16, np.float32) or logits.ndim != 2:
+        raise ValueError("logits must be a matrix of f32 or BF16 (uint16)")
+    rows, stride = logits.shape
+    vocab = stride if vocab is None else vocab
+    tokens = None if tokens is None else np.ascontiguousarray(tokens, np.uint32)
+    if tokens is not None and tokens.size != rows:
+        raise ValueError("one token a row")
+    xd = DeviceBuffer.from_array(logits)
+    td = None if tokens is None else DeviceBuffer.from_array(tokens)
+    lp, ent = DeviceBuffer(max(rows, 1) * 4), DeviceBuffer(max(rows, 1) * 4)
+    ids, tops = (DeviceBuffer(max(rows * top, 1) * 4) for _ in range(2))
+    check(lib().cheetah_hip_logprobs(xd.ptr, int(logits.dtype == np.float32), rows, vocab, stride, td and td.ptr, top,
+                                     td and lp.ptr, ent.ptr, ids.ptr if top else None, tops.ptr if top else None))
+    return (lp.download(np.float32, rows) if td else None, ent.download(np.float32, rows),
+            ids.download(np.uint32, rows * top).reshape(rows, top),
+            tops.download(np.float32, rows * top).reshape(rows, top))
 
 
 # ---------------------------------------------------------------------------

@@ -122,6 +122,56 @@ int cheetah_hip_attention_noalloc(const float *q, const cheetah_hip_kv_view *kv,
                                   size_t offset, float *out);
 
 /* ------------------------------------------------------------------------
+ * Drafted tokens and scoring, op level. No counterpart in the reference (it
+ * decodes one token at a time and reads the last row's logits). Buffers the
+ * calls read or write may be any memory of the library's device; work on them
+ * that runs on other streams must have finished, as for every op-level call.
+ * ---------------------------------------------------------------------- */
+
+/* Most nodes of a tree of drafted tokens. */
+#define CHEETAH_HIP_MAX_TREE_NODES 256
+/* Attention for a tree of n drafted tokens that continue a cached sequence of
+ * `offset` positions. parents (device int32 [n]) holds each node's parent, an
+ * earlier node; a value outside [0, i) makes node i a root. Node i's K/V row is
+ * already in the cache, at position offset + i. Every node attends to the
+ * positions [0, offset), its ancestors and itself: never to other branches or to
+ * positions past the tree, whatever their rows hold (NaN, unwritten memory).
+ * kv: the paged view of cheetah_hip_attention; kv_format 0 = BF16 pools, 1 =
+ * f32 (k_pages / v_pages then point to f32 elements). Page size a multiple of
+ * 64, head_dim 64 or 128, 1 to 8 query heads per KV head, 16-byte aligned
+ * buffers. q: device f32 [n][q_heads*head_dim] (each rotated for its own
+ * position, offset + depth); out: device f32, the same shape. */
+int cheetah_hip_tree_attention(const float *q, const cheetah_hip_kv_view *kv, uint32_t kv_format, uint32_t q_heads,
+                               const int32_t *parents, size_t n, size_t offset, float *out);
+/* Keeps one branch of a tree: in each of the nviews caches (one per layer) the
+ * K/V rows of positions offset + nodes[j] move to offset + j, j = 0 .. count-1.
+ * nodes (host) is strictly increasing and below CHEETAH_HIP_MAX_TREE_NODES: a
+ * root and its descendants in order. The views (host array) may have page
+ * tables of their own but one page size, KV head count and head_dim, and no
+ * cache may be listed twice. Rows past the branch are left as they are. */
+int cheetah_hip_tree_commit(const cheetah_hip_kv_view *views, size_t nviews, uint32_t kv_format, size_t offset,
+                            const uint32_t *nodes, size_t count);
+
+/* Most alternatives a row of cheetah_hip_logprobs returns. */
+#define CHEETAH_HIP_MAX_TOP 64
+/* For each of `rows` rows of `vocab` logits (device, `stride` >= vocab elements
+ * apart; logit_format 0 = BF16, 1 = f32), in natural logarithms:
+ *   logprobs[r] = x[tokens[r]] - log sum exp x   (tokens: device uint32 [rows];
+ *                 NaN where the id is not below vocab)
+ *   entropy[r]  = - sum p log p
+ *   top_ids[r][i], top_logprobs[r][i], i < top: the `top` largest logits in
+ *                 descending order, equal ones by ascending id.
+ * top is at most CHEETAH_HIP_MAX_TOP and vocab. Outputs are device arrays; any
+ * may be null (tokens too, without logprobs), but not all of them, and top_ids
+ * and top_logprobs go together with top > 0. -inf logits have probability 0; a
+ * row of nothing else has log probabilities of -inf and entropy 0. A row that
+ * holds a NaN or +inf has NaN for each log probability and its entropy; its
+ * alternatives are ordered with NaN as -inf. */
+int cheetah_hip_logprobs(const void *logits, uint32_t logit_format, size_t rows, size_t vocab, size_t stride,
+                         const uint32_t *tokens, uint32_t top, float *logprobs, float *entropy, uint32_t *top_ids,
+                         float *top_logprobs);
+
+/* ------------------------------------------------------------------------
  * Model: the HIP implementation of ModelForward (registry.rs:57-85) for the
  * qwen2 and llama families (registrations/qwen2.rs, llama.rs).
  * ---------------------------------------------------------------------- */
