@@ -315,13 +315,10 @@ static AttnJob attention_job(const float *q, const cheetah_hip_kv_view *kv, uint
     return j;
 }
 
-static int attention_op(const float *q, const cheetah_hip_kv_view *kv, uint32_t q_heads, size_t rows, size_t offset,
-                        float *out) {
-    CHIP_TRY(check_attention_args(q, kv, q_heads, rows, out));
+// Split partials of the op-level attention calls (grown on demand, per thread).
+static int attention_scratch(size_t need, float **out, size_t *out_floats) {
     static thread_local float *part = nullptr;
     static thread_local size_t part_floats = 0;
-    size_t need = 0;
-    AttnJob j = attention_job(q, kv, q_heads, rows, offset, out, &need);
     if (need > part_floats) {
         CHIP_CHECK(hipStreamSynchronize(g_stream));
         if (part) CHIP_CHECK(hipFree(part));
@@ -330,6 +327,18 @@ static int attention_op(const float *q, const cheetah_hip_kv_view *kv, uint32_t 
         CHIP_CHECK(hipMalloc(&part, need * sizeof(float)));
         part_floats = need;
     }
+    *out = part;
+    *out_floats = part_floats;
+    return 0;
+}
+
+static int attention_op(const float *q, const cheetah_hip_kv_view *kv, uint32_t q_heads, size_t rows, size_t offset,
+                        float *out) {
+    CHIP_TRY(check_attention_args(q, kv, q_heads, rows, out));
+    size_t need = 0, part_floats = 0;
+    float *part = nullptr;
+    AttnJob j = attention_job(q, kv, q_heads, rows, offset, out, &need);
+    CHIP_TRY(attention_scratch(need, &part, &part_floats));
     j.part = part;
     j.part_floats = part_floats;
     return launch_attention(j, g_stream);
@@ -391,6 +400,9 @@ int cheetah_hip_tree_attention(const float *q, const cheetah_hip_kv_view *kv, ui
     j.parents = parents;
     j.n = n;
     j.offset = offset;
+    const int splits = tree_attention_splits(j);
+    if (splits > 1)
+        CHIP_TRY(attention_scratch(attention_part_floats(n, j.q_heads, splits, j.g.head_dim), &j.part, &j.part_floats));
     return launch_tree_attention(j, g_stream);
 }
 

@@ -214,6 +214,10 @@ int launch_attention(const AttnJob &job, hipStream_t s);
 // rotary width = head_dim.
 bool attention_decode_fuses_rope(const KvGeom &g, int q_heads, int rotary_dim);
 size_t attention_part_floats(size_t rows, int q_heads, int splits, int head_dim);
+// The splits' partials of rows x q_heads ([row][head][split][head_dim values,
+// maximum (log2 units), weight sum]) merged in order; nothing for one split.
+int launch_attention_merge(const float *part, int splits, size_t rows, int q_heads, int head_dim, float *out,
+                           uint16_t *out_hi, uint16_t *out_lo, hipStream_t s);
 // Split count of a decode-style launch (one row per query position) over ctx
 // keys: one or two blocks per CU (matrix-core or VALU kernel), at most one
 // split per 64-position tile, one for a short BF16 context.
@@ -241,7 +245,14 @@ struct TreeJob {
     int q_heads = 0;
     const int32_t *parents = nullptr;  // device [n]
     size_t n = 0, offset = 0;
+    // Partials: attention_part_floats(n, q_heads, tree_attention_splits(job),
+    // head_dim) floats; fewer mean fewer splits.
+    float *part = nullptr;
+    size_t part_floats = 0;
+    // Optional BF16 halves of out (as AttnJob's); out may then be null.
+    uint16_t *out_hi = nullptr, *out_lo = nullptr;
 };
+int tree_attention_splits(const TreeJob &job);
 int launch_tree_attention(const TreeJob &job, hipStream_t s);
 // In every view (a layer's pools and its page table) the K/V rows of positions
 // offset + nodes[j] move to offset + j, j = 0 .. count - 1. nodes (host): below
