@@ -1657,20 +1657,6 @@ size_t attention_part_floats(size_t rows, int q_heads, int splits, int head_dim)
 
 int attention_max_splits() { return kMaxSplits; }
 
-int launch_attention_merge(const float *part, int splits, size_t rows, int q_heads, int head_dim, float *out,
-                           uint16_t *out_hi, uint16_t *out_lo, hipStream_t s) {
-    if (splits > kMaxSplits) return fail("HIP backend: attention merge of too many splits.");
-    AttnJob j;
-    j.rows = rows;
-    j.q_heads = q_heads;
-    AttnArgs a{};
-    a.part = (float *)part;
-    a.out = out;
-    a.out_hi = out_hi;
-    a.out_lo = out_lo;
-    return head_dim == 64 ? launch_merge2<64>(j, a, splits, s) : launch_merge2<128>(j, a, splits, s);
-}
-
 // Split-K of a decode-style launch: across the KV heads and rows about one
 // block per CU for the matrix-core kernel (BF16 K/V; measured 13 % faster
 // than two at 16K keys, where the K/V stream, not the block count, sets the

@@ -214,10 +214,6 @@ int launch_attention(const AttnJob &job, hipStream_t s);
 // rotary width = head_dim.
 bool attention_decode_fuses_rope(const KvGeom &g, int q_heads, int rotary_dim);
 size_t attention_part_floats(size_t rows, int q_heads, int splits, int head_dim);
-// The splits' partials of rows x q_heads ([row][head][split][head_dim values,
-// maximum (log2 units), weight sum]) merged in order; nothing for one split.
-int launch_attention_merge(const float *part, int splits, size_t rows, int q_heads, int head_dim, float *out,
-                           uint16_t *out_hi, uint16_t *out_lo, hipStream_t s);
 // Split count of a decode-style launch (one row per query position) over ctx
 // keys: one or two blocks per CU (matrix-core or VALU kernel), at most one
 // split per 64-position tile, one for a short BF16 context.

@@ -22,7 +22,8 @@ struct TreeArgs {
     const void *k, *v;
     const int32_t *page_table;
     const int32_t *parents;
-    float *part;
+    float *part;  // [row][head][split][HD]: weighted sums
+    float2 *ml;   // [row][head][split]: maximum (log2 units), weight sum
     float *out;
     uint16_t *out_hi, *out_lo;  // BF16 halves of out (null: not written)
     int page_size, kv_heads, q_heads, offset, n;
@@ -47,7 +48,8 @@ __device__ __forceinline__ void store_out4(const TreeArgs &a, size_t i, f32x4 v)
 // The ancestors of every node, themselves among them, as 256-bit words in LDS,
 // by the whole block (thread i: node i). up[i] is the nearest ancestor that
 // anc[i] does not hold yet, so each round doubles the length of the paths held:
-// log2(depth) rounds, whatever the tree's shape.
+// log2(depth) rounds, whatever the tree's shape. The caller's next barrier
+// makes them visible.
 constexpr int kAncWords = kMaxTreeNodes / 64;
 struct TreeLds {
     uint64_t anc[kMaxTreeNodes][kAncWords];
@@ -56,28 +58,45 @@ struct TreeLds {
     int sick_prefix;           // an infinity or NaN in the prefix's V (f32)
     int16_t up[kMaxTreeNodes];
 };
-__device__ __forceinline__ void find_ancestors(const int32_t *parents, int n, TreeLds &t) {
-    static_assert(kThreads == kMaxTreeNodes, "a thread per node");
-    const int i = threadIdx.x;
-    int p = i < n ? parents[i] : -1;
-    if (p >= i) p = -1;
-    uint64_t w[kAncWords];
-#pragma unroll
-    for (int k = 0; k < kAncWords; ++k) t.anc[i][k] = w[k] = i >> 6 == k ? 1ull << (i & 63) : 0;
-    t.up[i] = (int16_t)(p < 0 ? -1 : p);
+__device__ __forceinline__ void find_ancestors(int p, int n, TreeLds &t) {  // p: parents[thread]
+    const int i = threadIdx.x;  // nodes are the first kMaxTreeNodes threads
+    if (i >= n || p >= i) p = -1;
     if (i < kAncWords) t.sick[i] = 0;
+    if (n <= 64) {  // one wave, in registers
+        if (i >= 64) return;
+        uint64_t w = 1ull << i;
+        while (__any(p >= 0)) {
+            const int from = max(p, 0);
+            const uint64_t up = (uint64_t)(uint32_t)__shfl((int)w, from, 64) |
+                                (uint64_t)(uint32_t)__shfl((int)(w >> 32), from, 64) << 32;
+            const int q = __shfl(p, from, 64);
+            w = p >= 0 ? w | up : w;
+            p = p >= 0 ? q : p;
+        }
+        t.anc[i][0] = w;
+#pragma unroll
+        for (int k = 1; k < kAncWords; ++k) t.anc[i][k] = 0;
+        return;
+    }
+    uint64_t w[kAncWords];
+    const bool mine = i < kMaxTreeNodes;
+    if (mine) {
+#pragma unroll
+        for (int k = 0; k < kAncWords; ++k) t.anc[i][k] = w[k] = i >> 6 == k ? 1ull << (i & 63) : 0;
+        t.up[i] = (int16_t)max(p, -1);
+    }
     while (__syncthreads_or(p >= 0)) {
         if (p >= 0) {
 #pragma unroll
             for (int k = 0; k < kAncWords; ++k) w[k] |= t.anc[p][k];
             p = t.up[p];
-        } else {
-            p = -1;
         }
         __syncthreads();  // every path is read before one grows
+        if (mine) {
 #pragma unroll
-        for (int k = 0; k < kAncWords; ++k) t.anc[i][k] = w[k];
-        t.up[i] = (int16_t)p;
+            for (int k = 0; k < kAncWords; ++k) t.anc[i][k] = w[k];
+            t.up[i] = (int16_t)max(p, -1);
+        }
     }
 }
 
@@ -118,11 +137,11 @@ __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int hea
 #pragma unroll
         for (int d = 0; d < D; ++d) o[d] = fmaf(w, kv_value((const KT *)a.v + at + lane + 64 * d), o[d] * alpha);
     }
-    float *part = a.part + (((size_t)node * a.q_heads + head) * S + split) * (HD + 2);
+    const size_t at = ((size_t)node * a.q_heads + head) * S + split;
 #pragma unroll
     for (int d = 0; d < D; ++d) {
         if (S > 1) {
-            part[lane + 64 * d] = o[d];
+            a.part[at * HD + lane + 64 * d] = o[d];
         } else {
             const float v = o[d] / l;
             if (a.out) a.out[row + lane + 64 * d] = v;
@@ -133,16 +152,76 @@ __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int hea
             }
         }
     }
-    if (S > 1 && lane == 0) {
-        part[HD] = l == l ? m : INFINITY;  // a NaN row: no split outweighs it
-        part[HD + 1] = l;
+    if (S > 1 && lane == 0) a.ml[at] = make_float2(l == l ? m : INFINITY, l);  // a NaN row: no split outweighs it
+}
+
+// Eight values as three BF16 parts, each the top 8 bits of what the ones before
+// leave: all 24 bits of a value (no roundings: 11 instructions a pair where
+// split3x8's rounded parts take 16).
+__device__ __forceinline__ void cut3x8(const float (&v)[8], bf16x8 (&out)[3]) {
+    u32x4 w[3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t x[2], y[2], z[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            x[k] = __float_as_uint(v[2 * i + k]);
+            const float r = v[2 * i + k] - __uint_as_float(x[k] & 0xFFFF0000u);
+            y[k] = __float_as_uint(r);
+            z[k] = __float_as_uint(r - __uint_as_float(y[k] & 0xFFFF0000u));
+        }
+        w[0][i] = __builtin_amdgcn_perm(x[1], x[0], 0x07060302u);
+        w[1][i] = __builtin_amdgcn_perm(y[1], y[0], 0x07060302u);
+        w[2][i] = __builtin_amdgcn_perm(z[1], z[0], 0x07060302u);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) out[k] = __builtin_bit_cast(bf16x8, w[k]);
+}
+
+// read_vt of two blocks of 16 positions, OFF and OFF + 16 rows, in one wait.
+template <int HD>
+__device__ __forceinline__ void read_vt2(const uint32_t (&addr)[HD / 32], bf16x8 (&v0)[HD / 32], bf16x8 (&v1)[HD / 32]) {
+    s16x4_t r[2][HD / 32][2];
+    if constexpr (HD == 128) {
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:%20\n\t"
+            "ds_read_b64_tr_b16 %2, %17\n\tds_read_b64_tr_b16 %3, %17 offset:%20\n\t"
+            "ds_read_b64_tr_b16 %4, %18\n\tds_read_b64_tr_b16 %5, %18 offset:%20\n\t"
+            "ds_read_b64_tr_b16 %6, %19\n\tds_read_b64_tr_b16 %7, %19 offset:%20\n\t"
+            "ds_read_b64_tr_b16 %8, %16 offset:%21\n\tds_read_b64_tr_b16 %9, %16 offset:%22\n\t"
+            "ds_read_b64_tr_b16 %10, %17 offset:%21\n\tds_read_b64_tr_b16 %11, %17 offset:%22\n\t"
+            "ds_read_b64_tr_b16 %12, %18 offset:%21\n\tds_read_b64_tr_b16 %13, %18 offset:%22\n\t"
+            "ds_read_b64_tr_b16 %14, %19 offset:%21\n\tds_read_b64_tr_b16 %15, %19 offset:%22\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(r[0][0][0]), "=&v"(r[0][0][1]), "=&v"(r[0][1][0]), "=&v"(r[0][1][1]), "=&v"(r[0][2][0]),
+              "=&v"(r[0][2][1]), "=&v"(r[0][3][0]), "=&v"(r[0][3][1]), "=&v"(r[1][0][0]), "=&v"(r[1][0][1]),
+              "=&v"(r[1][1][0]), "=&v"(r[1][1][1]), "=&v"(r[1][2][0]), "=&v"(r[1][2][1]), "=&v"(r[1][3][0]),
+              "=&v"(r[1][3][1])
+            : "v"(addr[0]), "v"(addr[1]), "v"(addr[2]), "v"(addr[3]), "i"(4 * HD * 2), "i"(16 * HD * 2), "i"(20 * HD * 2)
+            : "memory");
+    } else {
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+            "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%10\n\t"
+            "ds_read_b64_tr_b16 %4, %8 offset:%11\n\tds_read_b64_tr_b16 %5, %8 offset:%12\n\t"
+            "ds_read_b64_tr_b16 %6, %9 offset:%11\n\tds_read_b64_tr_b16 %7, %9 offset:%12\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(r[0][0][0]), "=&v"(r[0][0][1]), "=&v"(r[0][1][0]), "=&v"(r[0][1][1]), "=&v"(r[1][0][0]),
+              "=&v"(r[1][0][1]), "=&v"(r[1][1][0]), "=&v"(r[1][1][1])
+            : "v"(addr[0]), "v"(addr[1]), "i"(4 * HD * 2), "i"(16 * HD * 2), "i"(20 * HD * 2)
+            : "memory");
+    }
+#pragma unroll
+    for (int u = 0; u < HD / 32; ++u) {
+        v0[u] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[0][u][0], r[0][u][1], 0, 1, 2, 3, 4, 5, 6, 7));
+        v1[u] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(r[1][u][0], r[1][u][1], 0, 1, 2, 3, 4, 5, 6, 7));
     }
 }
 
 // ---------------------------------------------------------------------------
 // On the matrix cores. The M = n G rows (node, head of the group) of a KV head
-// are cut into waves of 32 and blocks of WR row waves; the 4 / WR key waves of
-// a row wave take 32-position steps of the block's tiles in turn and are joined
+// are cut into waves of 32 and blocks of WR row waves; the WK key waves of a
+// row wave take 32-position steps of the block's tiles in turn and are joined
 // at the end. Per step, as attn_prefill_kernel's:
 //   S^T = K Q^T     K rows from LDS, Q^T in registers
 //   O^T += V^T P^T  V read transposed, P^T as the scores' registers lie
@@ -152,38 +231,38 @@ __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int hea
 // products give 1e-6. An f32 cache's K and V are three parts too, and six of
 // the nine part products are taken (attn_prefill_f32_kernel's).
 //
-// BF16 tiles of T positions go global to LDS, the next one while the current
+// BF16 tiles of 128 positions go global to LDS, the next one while the current
 // one computes; f32 tiles of 64 wait in registers and are split while staged.
+// Two waves a SIMD, one's softmax beside the other's products, in one block:
+// two blocks of four waves a CU ran at the pace of their ages, and the younger
+// alone at the end.
 //
-// Splits are runs of `chunk` positions (whole tiles); merged by the attention
-// merge. Blocks with the same (split, KV head) and other rows are 8 apart, on
-// one XCD: they read the same tiles through its L2.
+// Splits are runs of whole tiles, joined by tree_merge_kernel. Blocks with
+// the same (split, KV head) and other rows are 8 apart, on one XCD: they read
+// the same tiles through its L2.
 // ---------------------------------------------------------------------------
-template <int WR, class KT>
-constexpr int tree_tile() { return WR == 1 && sizeof(KT) == 2 ? 128 : 64; }
-template <int HD, int WR, class KT>
+template <class KT>
+constexpr int tree_tile() { return sizeof(KT) == 2 ? 128 : 64; }
+template <int HD, class KT>
 constexpr size_t tree_tile_lds() {  // two BF16 tiles, or one of three parts
-    return sizeof(KT) == 2 ? (size_t)4 * tree_tile<WR, KT>() * HD * 2 : (size_t)6 * 64 * HD * 2;
+    return sizeof(KT) == 2 ? (size_t)4 * tree_tile<KT>() * HD * 2 : (size_t)6 * tree_tile<KT>() * HD * 2;
 }
-template <int HD, int WR, class KT>
-constexpr size_t tree_lds_bytes() { return tree_tile_lds<HD, WR, KT>() + sizeof(TreeLds); }
-// Blocks of a CU: what its LDS and registers let in.
-template <int HD, int WR, class KT>
-constexpr int tree_blocks_per_cu() { return HD == 128 && (WR == 1 || sizeof(KT) == 4) ? 1 : 2; }
+template <int HD, class KT>
+constexpr size_t tree_lds_bytes() { return tree_tile_lds<HD, KT>() + sizeof(TreeLds); }
 
-template <int HD, int WR, class KT>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(tree_blocks_per_cu<HD, WR, KT>())))
-void tree_attn_kernel(TreeArgs a, int S, int chunk) {
+template <int HD, int WR, int WK, class KT>
+__global__ __launch_bounds__(64 * WR * WK) __attribute__((amdgpu_waves_per_eu(WR * WK / 4)))
+void tree_attn_kernel(TreeArgs a, int S, int tiles) {
     constexpr bool F32 = sizeof(KT) == 4;
-    constexpr int WK = 4 / WR, T = tree_tile<WR, KT>(), STEPS = T / (32 * WK);
+    constexpr int NW = WR * WK, T = tree_tile<KT>(), STEPS = T / (32 * WK);
     constexpr int KSTEPS = HD / 16, UT = HD / 32;
     constexpr int CPR = HD / 8;       // 16-byte chunks per LDS row
-    constexpr int HC = HD / 32;       // BF16: a wave's copies for 64 positions; f32: a thread's 8-dim units of a tile
+    constexpr int HC = HD / 8 / NW;   // BF16: a wave's copies for 64 positions; f32: a thread's 8-dim units of a tile
     constexpr int PL = F32 ? 3 : 1;   // parts (planes) of K and V
     constexpr int TB = T * HD * 2;    // bytes of a tile's plane
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    extern __shared__ __attribute__((aligned(256))) uint8_t smem[];
     uint8_t *ks = smem, *vs = smem + (F32 ? 3 : 2) * TB;
-    TreeLds &tree = *(TreeLds *)(smem + tree_tile_lds<HD, WR, KT>());
+    TreeLds &tree = *(TreeLds *)(smem + tree_tile_lds<HD, KT>());
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int wr = wave % WR, wk = wave / WR;
@@ -195,26 +274,45 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
     const int m0 = rb * 32 * WR, m = m0 + wr * 32 + n;
     const bool rvalid = m < M;
     const int node = rvalid ? m / G : 0, head = g * G + (rvalid ? m % G : 0);
-    const int start = split * chunk;
-    const int end = min(start + chunk, a.offset + (min(M, m0 + 32 * WR) - 1) / G + 1);
-    float *part = a.part + (((size_t)node * a.q_heads + head) * S + split) * (HD + 2);
+    // tiles / S tiles a split, the first ones one more. (Block-uniform, said to
+    // the compiler: the quotients come from vector registers.)
+    const int each = tiles / S, extra = tiles % S;
+    const int t_first = split * each + min(split, extra);
+    const int start = __builtin_amdgcn_readfirstlane(t_first * T);
+    const int end = __builtin_amdgcn_readfirstlane(
+        (int)min((unsigned)(t_first + each + (split < extra)) * T, (unsigned)(a.offset + (min(M, m0 + 32 * WR) - 1) / G + 1)));
+    const size_t at_part = ((size_t)node * a.q_heads + head) * S + split;
     if (start >= end) {  // no row of the block reaches the split
-        if (rvalid && wk == 0 && half == 0) part[HD] = -INFINITY;
+        if (rvalid && wk == 0 && half == 0) a.ml[at_part] = make_float2(-INFINITY, 0.f);
         return;
     }
     const bool in_tree = end > a.offset;  // block-uniform
-    const int last = (end - 1) / 64 * 64;  // the last 64 positions with a row in them
-    auto page_of = [&](int p) {  // a scalar load, one tile ahead of its use
-        return ((const __attribute__((address_space(4))) int32_t *)a.page_table)[p / a.page_size];
-    };
-    int page[T / 64];  // of the next tile to fetch
+    // Page table entries held_0 .. + 63, a lane each: the loop looks pages up
+    // without a load (a scalar load in flight would make each wait for an LDS
+    // read a wait for all of them).
+    const int last_page = (end - 1) / a.page_size;
+    int page_i = __builtin_amdgcn_readfirstlane(start / a.page_size), held_0 = page_i;
+    int page_at = start - page_i * a.page_size;
+    int held = a.page_table[min(held_0 + lane, last_page)];
+    int page[T / 64], row0[T / 64];  // of the next tile to fetch
     auto next_pages = [&](int t0) {
 #pragma unroll
-        for (int x = 0; x < T / 64; ++x) page[x] = page_of(min(t0 + 64 * x, last));
+        for (int x = 0; x < T / 64; ++x) {
+            if (t0 + 64 * x >= end) break;
+            if (page_i - held_0 == 64) {
+                held_0 = page_i;
+                held = a.page_table[min(held_0 + lane, last_page)];
+                asm volatile("" : "+v"(held));  // waited for here, not by every lookup
+            }
+            page[x] = __builtin_amdgcn_readlane(held, page_i - held_0);
+            row0[x] = page_at;
+            page_at += 64;
+            if (page_at == a.page_size) page_at = 0, ++page_i;
+        }
     };
 
     // BF16 copies of a tile: copy c of a wave fills 1 KB, 64 / CPR rows, of the
-    // block's 4 KB; K rows at krow_of, chunks swizzled (attn_prefill_kernel's).
+    // block's NW KB; K rows at krow_of, chunks swizzled (attn_prefill_kernel's).
     // Positions past the block's rows may hold stale bytes: masked, and V cleared.
     const int lr = wave * (64 / CPR) + lane / CPR;
     const int koff = krow_of(lr) * HD * 2 + 16 * ((lane % CPR) ^ (lr % CPR));
@@ -224,13 +322,12 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
     auto fetch = [&](int t0, int b) {
 #pragma unroll
         for (int x = 0; x < T / 64; ++x) {
-            const int p0 = t0 + 64 * x;
-            if (p0 >= end) break;
-            const size_t tile = (((size_t)page[x] * a.kv_heads + g) * a.page_size + p0 % a.page_size) * HD;
+            if (t0 + 64 * x >= end) break;
+            const size_t tile = (((size_t)page[x] * a.kv_heads + g) * a.page_size + row0[x]) * HD;
             if constexpr (F32) {
 #pragma unroll
                 for (int c = 0; c < HC; ++c) {
-                    const int idx = (int)threadIdx.x + kThreads * c;
+                    const int idx = (int)threadIdx.x + 64 * NW * c;
                     const float *kp = (const float *)a.k + tile + (size_t)idx * 8;
                     const float *vp = (const float *)a.v + tile + (size_t)idx * 8;
                     kr[c][0] = *(const f32x4 *)kp;
@@ -245,9 +342,9 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
                 const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
                     (void *)((const uint16_t *)a.v + tile), (short)0, 64 * HD * 2, 0x00020000);
 #pragma unroll
-                for (int c = 0; c < HC; ++c) buf_to_lds<16>(rk, ks + at + 4096 * c, koff, 4096 * c);
+                for (int c = 0; c < HC; ++c) buf_to_lds<16>(rk, ks + at + 1024 * NW * c, koff, 1024 * NW * c);
 #pragma unroll
-                for (int c = 0; c < HC; ++c) buf_to_lds<16>(rv, vs + at + 4096 * c, voff, 4096 * c);
+                for (int c = 0; c < HC; ++c) buf_to_lds<16>(rv, vs + at + 1024 * NW * c, voff, 1024 * NW * c);
             }
         }
     };
@@ -263,9 +360,9 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
     };
     auto clean_v = [&](int t0, int b) {
         for (int c = 0; c < HC * T / 64; ++c) {
-            const int p = t0 + lr + 256 / CPR * c;
+            const int p = t0 + lr + 64 * NW / CPR * c;
             if (p < a.offset) continue;
-            u32x4 *at = (u32x4 *)(vs + b * TB + wave * 1024 + 4096 * c + 16 * lane);
+            u32x4 *at = (u32x4 *)(vs + b * TB + wave * 1024 + 1024 * NW * c + 16 * lane);
             bool bad = p >= end;
             if (!bad) {
                 const u32x4 w = *at;
@@ -280,7 +377,7 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
     auto stage = [&](int t0) {
 #pragma unroll
         for (int c = 0; c < (F32 ? HC : 0); ++c) {
-            const int idx = (int)threadIdx.x + kThreads * c, r = idx / CPR, ch = idx % CPR, kr_ = krow_of(r);
+            const int idx = (int)threadIdx.x + 64 * NW * c, r = idx / CPR, ch = idx % CPR, kr_ = krow_of(r);
             const float kv[8] = {kr[c][0][0], kr[c][0][1], kr[c][0][2], kr[c][0][3],
                                  kr[c][1][0], kr[c][1][1], kr[c][1][2], kr[c][1][3]};
             float vv[8] = {vr[c][0][0], vr[c][0][1], vr[c][0][2], vr[c][0][3],
@@ -293,21 +390,23 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) vv[i] = fine && !past ? vv[i] : 0.f;
             bf16x8 w[3];
-            split3x8(kv, w);
+            cut3x8(kv, w);
 #pragma unroll
             for (int k = 0; k < 3; ++k) *(bf16x8 *)(ks + k * TB + kr_ * HD * 2 + 16 * (ch ^ (kr_ % CPR))) = w[k];
-            split3x8(vv, w);
+            cut3x8(vv, w);
 #pragma unroll
             for (int k = 0; k < 3; ++k) *(bf16x8 *)(vs + k * TB + r * HD * 2 + 16 * (ch ^ vseg<HD>(r))) = w[k];
         }
     };
 
+    // The parents first: behind the tile's copies they would arrive after them.
+    const int parent = in_tree && (int)threadIdx.x < a.n ? a.parents[threadIdx.x] : -1;
     next_pages(start);
     fetch(start, 0);
     next_pages(start + T);
     if (threadIdx.x < 4) tree.odd[threadIdx.x] = 0;
     if (threadIdx.x == 0) tree.sick_prefix = 0;
-    if (in_tree) find_ancestors(a.parents, a.n, tree);
+    if (in_tree) find_ancestors(parent, a.n, tree);
 
     bf16x8 q3[KSTEPS][3];
     {
@@ -324,18 +423,17 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
         for (int s = 0; s < KSTEPS; ++s) {
             const float v[8] = {raw[s][0][0] * sq, raw[s][0][1] * sq, raw[s][0][2] * sq, raw[s][0][3] * sq,
                                 raw[s][1][0] * sq, raw[s][1][1] * sq, raw[s][1][2] * sq, raw[s][1][3] * sq};
-            split3x8(v, q3[s]);
+            cut3x8(v, q3[s]);
         }
     }
     // This lane's transposing V reads in a 16-position block: rows
     // 8 half + i / 4 (and + 4), dims 32 u + 16 ((lane / 16) % 2) + 4 (i % 4).
     const int vi = lane & 15, vrow = 8 * half + (vi >> 2);
-    uint32_t vaddr[UT];
-#pragma unroll
-    for (int u = 0; u < UT; ++u) {
-        const int c = (4 * u + 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1)) ^ vseg<HD>(vrow);
-        vaddr[u] = (uint32_t)(uintptr_t)(vs + vrow * HD * 2 + 16 * c + 8 * (vi & 1));
-    }
+    // The chunk swizzles touch address bits that u and s alone set besides them:
+    // one base, and an exclusive or for each read.
+    const uint32_t vbase = (uint32_t)(uintptr_t)(vs + vrow * HD * 2 + 8 * (vi & 1) +
+                                                 16 * ((2 * ((lane >> 4) & 1) + ((vi & 3) >> 1)) ^ vseg<HD>(vrow)));
+    const int kbase = n * HD * 2 + 16 * (half ^ (n % CPR));
 
     f32x16 oacc[UT];
 #pragma unroll
@@ -343,7 +441,10 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
     float m2 = -INFINITY, l = 0.f;
     if constexpr (!F32) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (start + T > a.offset) clean_v(start, 0);
+        if (start + T > a.offset) {
+            __syncthreads();  // the marks start at none
+            clean_v(start, 0);
+        }
     }
     __syncthreads();
     int b = 0;
@@ -363,31 +464,38 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
             if (t0 + p0 >= end) break;
             uint32_t vad[UT];
 #pragma unroll
-            for (int u = 0; u < UT; ++u) vad[u] = vaddr[u] + b * TB + p0 * HD * 2;
-            f32x16 sacc = f32x16{}, slow = f32x16{};
+            for (int u = 0; u < UT; ++u) vad[u] = (vbase + b * TB + p0 * HD * 2) ^ (64 * u);
+            const int kat = kbase + b * TB + p0 * HD * 2;
+            bf16x8 ka[F32 ? 1 : KSTEPS][PL];
+            auto read_k = [&](int s, bf16x8 (&k)[PL]) {
+#pragma unroll
+                for (int x = 0; x < PL; ++x) k[x] = *(const bf16x8 *)(ks + (kat ^ (32 * s)) + x * TB);
+            };
+            if constexpr (!F32) {
+#pragma unroll
+                for (int s = 0; s < KSTEPS; ++s) read_k(s, ka[s]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // f32 caches add the small products up by themselves.
+            f32x16 sacc = f32x16{}, small = f32x16{};
+            f32x16 &slow = F32 ? small : sacc;
 #pragma unroll
             for (int s = 0; s < KSTEPS; ++s) {
-                const int r = p0 + n;
-                const uint8_t *kp = ks + b * TB + r * HD * 2 + 16 * ((2 * s + half) ^ (r % CPR));
-                bf16x8 ka[PL];
-#pragma unroll
-                for (int k = 0; k < PL; ++k) ka[k] = *(const bf16x8 *)(kp + k * TB);
+                auto &k = ka[F32 ? 0 : s];
                 if constexpr (F32) {
-                    slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[2], q3[s][0], slow, 0, 0, 0);
-                    slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[1], q3[s][1], slow, 0, 0, 0);
+                    read_k(s, k);
+                    slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[2], q3[s][0], slow, 0, 0, 0);
+                    slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[1], q3[s][1], slow, 0, 0, 0);
                 }
-                slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[0], q3[s][2], slow, 0, 0, 0);
-                sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[0], q3[s][0], sacc, 0, 0, 0);
-                if constexpr (F32) slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[1], q3[s][0], slow, 0, 0, 0);
-                slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[0], q3[s][1], slow, 0, 0, 0);
+                slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], q3[s][2], slow, 0, 0, 0);
+                if constexpr (F32) slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[1], q3[s][0], slow, 0, 0, 0);
+                slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], q3[s][1], slow, 0, 0, 0);
+                sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], q3[s][0], sacc, 0, 0, 0);
             }
-            sacc += slow;
+            if constexpr (F32) sacc += small;
             // The step's V^T fragments, while the score products drain.
             bf16x8 va[F32 ? 1 : 2][PL][UT];
-            if constexpr (!F32) {
-                read_vt<HD, 0>(vad, va[0][0]);
-                read_vt<HD, 16 * HD * 2>(vad, va[1][0]);
-            }
+            if constexpr (!F32) read_vt2<HD>(vad, va[0][0], va[F32 ? 0 : 1][0]);
             // Register r holds position 8 half + (r & 3) + (r & 4) + 2 (r & 8) of the step.
             const int x0 = t0 + p0 - a.offset;  // node of the step's first position
             if (x0 + 32 > 0) {
@@ -407,11 +515,12 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
             float tmax = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, sacc[r]);
-            tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
             // Exponentials against a maximum that is raised only by more than 8
-            // (log2 units), so weights are at most 256 and rescaling is rare.
-            const bool raise = tmax > m2 + 8.0f;
-            if (__any(raise)) {
+            // (log2 units), so weights are at most 256 and rescaling is rare. The
+            // two lanes of a row share it; each sums its own weights.
+            if (__any(tmax > m2 + 8.0f)) {
+                tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
+                const bool raise = tmax > m2 + 8.0f;
                 const float mnew = raise ? tmax : m2;
                 const float alpha = raise ? __builtin_amdgcn_exp2f(m2 - mnew) : 1.f;  // 0 from -inf
                 l *= alpha;
@@ -430,7 +539,6 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
                 sacc[r] = pv;
                 tsum += pv;
             }
-            tsum += __shfl_xor(tsum, 32, 64);
             l += tsum;
             auto mix = [&](auto block) {
                 constexpr int s2 = decltype(block)::value;
@@ -438,7 +546,7 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) pv[j] = sacc[8 * s2 + j];
                 bf16x8 p3[3];
-                split3x8(pv, p3);
+                cut3x8(pv, p3);
                 auto product = [&](const bf16x8 (&v)[UT], const bf16x8 &p) {
 #pragma unroll
                     for (int u = 0; u < UT; ++u)
@@ -472,11 +580,12 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
         __syncthreads();
     }
 
+    l += __shfl_xor(l, 32, 64);
     // Key waves past the first leave their rows in the tiles' LDS (rows padded
     // by 16 bytes, off each other's banks), the first adds them up in order.
     if constexpr (WK > 1) {
         constexpr int LD = HD + 4;
-        static_assert((size_t)(WK - 1) * WR * 32 * (LD + 2) * 4 <= tree_tile_lds<HD, WR, KT>(), "joined in the tiles' LDS");
+        static_assert((size_t)(WK - 1) * WR * 32 * (LD + 2) * 4 <= tree_tile_lds<HD, KT>(), "joined in the tiles' LDS");
         auto rows_of = [&](int w) { return (float *)smem + ((w - 1) * WR + wr) * 32 * (LD + 2); };
         if (wk > 0) {
             float *so = rows_of(wk);
@@ -536,21 +645,78 @@ void tree_attn_kernel(TreeArgs a, int S, int chunk) {
             for (int u = 0; u < UT; ++u)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    *(f32x4 *)(part + 32 * u + 8 * q + 4 * half) =
+                    *(f32x4 *)(a.part + at_part * HD + 32 * u + 8 * q + 4 * half) =
                         f32x4{oacc[u][4 * q], oacc[u][4 * q + 1], oacc[u][4 * q + 2], oacc[u][4 * q + 3]};
-            if (half == 0) {
-                part[HD] = m2;
-                part[HD + 1] = l;
-            }
+            if (half == 0) a.ml[at_part] = make_float2(m2, l);
         }
     }
     __syncthreads();
 #pragma unroll 1
-    for (int r = wave; r < 32 * WR; r += 4)
+    for (int r = wave; r < 32 * WR; r += NW)
         if (tree.odd[r >> 5] >> (r & 31) & 1) {
             const int i = (m0 + r) / G;
             plain_row<HD, KT>(a, tree, i, g * G + (m0 + r) % G, g, start, min(end, a.offset + i + 1), S, split);
         }
+}
+
+// Joins the splits of one (row, head): W waves of a block each add up every
+// W-th split's values in order, then their sums in order. Every load of a batch
+// is in flight at once, the first batch beside the maxima.
+template <int HD, int W>
+__global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a, int S, int items) {
+    constexpr int D = HD / 64, B = 8;
+    typedef float vec __attribute__((ext_vector_type(D)));
+    __shared__ float so[kThreads / 64][HD];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int item = (int)blockIdx.x * (kThreads / 64 / W) + wave / W, w0 = wave % W;
+    if (W == 1 && item >= items) return;
+    const float2 *ml = a.ml + (size_t)item * S;
+    const float *part = a.part + (size_t)item * S * HD + D * lane;
+    vec v[B];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) v[i] = *(const vec *)(part + (size_t)min(s0 + W * i, S - 1) * HD);
+    };
+    const float2 x = ml[min(lane, S - 1)], y = ml[min(lane + 64, S - 1)];
+    load(w0);
+    const float m0 = lane < S ? x.x : -INFINITY, m1 = lane + 64 < S ? y.x : -INFINITY;
+    const float M = wave_max(fmaxf(m0, m1));
+    const float f0 = m0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
+    const float f1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - M);
+    const float L = wave_sum((f0 != 0.f ? f0 * x.y : 0.f) + (f1 != 0.f ? f1 * y.y : 0.f));
+    vec o = {};
+    for (int s0 = w0; s0 < S; s0 += W * B) {
+        if (s0 != w0) load(s0);
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            // A split without a key of the row (and what a lane past S read) holds no
+            // values; selected, not branched around: a load would sink into the branch.
+            const int s = s0 + W * i;
+            const float f = s >= S ? 0.f : s < 64 ? lane_read(f0, s) : lane_read(f1, s - 64);
+#pragma unroll
+            for (int d = 0; d < D; ++d) o[d] = fmaf(f, f != 0.f ? v[i][d] : 0.f, o[d]);
+        }
+    }
+    if constexpr (W > 1) {
+        *(vec *)&so[wave][D * lane] = o;
+        __syncthreads();
+        if (w0) return;
+#pragma unroll
+        for (int w = 1; w < W; ++w) o += *(const vec *)&so[wave + w][D * lane];
+    }
+    const float inv = 1.0f / L;
+    const size_t at = (size_t)item * HD + D * lane;
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+        const float r = o[d] * inv;
+        if (a.out) a.out[at + d] = r;
+        if (a.out_hi) {
+            const __bf16 hb = (__bf16)r;
+            a.out_hi[at + d] = __builtin_bit_cast(uint16_t, hb);
+            a.out_lo[at + d] = __builtin_bit_cast(uint16_t, (__bf16)(r - (float)hb));
+        }
+    }
 }
 
 // The move of a branch, by value in the launch's arguments: no device copy of
@@ -598,49 +764,63 @@ __global__ __launch_bounds__(kThreads) void tree_commit_kernel(CommitArgs a, int
 
 namespace {
 
-// Row waves of a block: as many as hold the rows, up to 4. An f32 tile has room
-// for two key waves only.
+// Row waves of a block: one for up to 32 rows, else two or four, the fewer
+// where four would leave two of the last block without rows. f32: two or four.
 int tree_row_waves(const TreeJob &j) {
-    const int rows = (int)j.n * (j.q_heads / j.g.kv_heads);
-    return rows <= 32 && !j.g.kv_f32 ? 1 : rows <= 64 ? 2 : 4;
+    const int rows = (int)j.n * (j.q_heads / j.g.kv_heads), waves = (rows + 31) / 32;
+    if (waves == 1 && !j.g.kv_f32) return 1;
+    return waves <= 2 || waves % 4 == 1 || waves % 4 == 2 ? 2 : 4;
 }
 
-template <int HD, int WR, class KT>
-int launch_tree_blocks(const TreeArgs &a, int S, int chunk, hipStream_t s) {
-    constexpr size_t lds = tree_lds_bytes<HD, WR, KT>();
+template <int HD, int WR, int WK, class KT>
+int launch_tree_blocks(const TreeArgs &a, int S, int tiles, hipStream_t s) {
+    constexpr size_t lds = tree_lds_bytes<HD, KT>();
     static std::atomic<uint64_t> lds_set{0};
-    CHIP_TRY(allow_dynamic_lds((const void *)tree_attn_kernel<HD, WR, KT>, lds, lds_set));
+    CHIP_TRY(allow_dynamic_lds((const void *)tree_attn_kernel<HD, WR, WK, KT>, lds, lds_set));
     const int rb = (a.n * (a.q_heads / a.kv_heads) + 32 * WR - 1) / (32 * WR);
     const size_t blocks = ((size_t)S * a.kv_heads + 7) / 8 * 8 * (size_t)rb;
     if (blocks > (size_t)INT32_MAX) return fail("HIP backend: tree attention grid out of range.");
-    hipLaunchKernelGGL((tree_attn_kernel<HD, WR, KT>), dim3((unsigned)blocks), dim3(kThreads), lds, s, a, S, chunk);
+    hipLaunchKernelGGL((tree_attn_kernel<HD, WR, WK, KT>), dim3((unsigned)blocks), dim3(64 * WR * WK), lds, s, a, S,
+                       tiles);
     CHIP_CHECK(hipGetLastError());
     return 0;
 }
 
 template <int HD>
-int launch_tree_h(const TreeJob &j, const TreeArgs &a, int S, int chunk, hipStream_t s) {
+int launch_tree_h(const TreeJob &j, const TreeArgs &a, int S, int tiles, hipStream_t s) {
     const int wr = tree_row_waves(j);
-    if (j.g.kv_f32)
-        return wr == 2 ? launch_tree_blocks<HD, 2, float>(a, S, chunk, s) : launch_tree_blocks<HD, 4, float>(a, S, chunk, s);
-    return wr == 1   ? launch_tree_blocks<HD, 1, uint16_t>(a, S, chunk, s)
-           : wr == 2 ? launch_tree_blocks<HD, 2, uint16_t>(a, S, chunk, s)
-                     : launch_tree_blocks<HD, 4, uint16_t>(a, S, chunk, s);
+    if (j.g.kv_f32) {
+        if (wr == 2) CHIP_TRY((launch_tree_blocks<HD, 2, 2, float>(a, S, tiles, s)));
+        else CHIP_TRY((launch_tree_blocks<HD, 4, 1, float>(a, S, tiles, s)));
+    } else {
+        if (wr == 1) CHIP_TRY((launch_tree_blocks<HD, 1, 4, uint16_t>(a, S, tiles, s)));
+        else if (wr == 2) CHIP_TRY((launch_tree_blocks<HD, 2, 4, uint16_t>(a, S, tiles, s)));
+        else CHIP_TRY((launch_tree_blocks<HD, 4, 2, uint16_t>(a, S, tiles, s)));
+    }
+    if (S == 1) return 0;
+    const int items = (int)j.n * j.q_heads;
+    if (S > 16)
+        hipLaunchKernelGGL((tree_merge_kernel<HD, 4>), dim3((unsigned)items), dim3(kThreads), 0, s, a, S, items);
+    else
+        hipLaunchKernelGGL((tree_merge_kernel<HD, 1>), dim3((unsigned)((items + 3) / 4)), dim3(kThreads), 0, s, a, S, items);
+    CHIP_CHECK(hipGetLastError());
+    return 0;
 }
 
-int tree_tile_of(const TreeJob &j) { return tree_row_waves(j) == 1 ? 128 : 64; }
+int tree_tile_of(const TreeJob &j) { return j.g.kv_f32 ? tree_tile<float>() : tree_tile<uint16_t>(); }
 
 }  // namespace
 
-// Splits of the keys: as many as fill the chip with blocks, of whole tiles.
+// Splits of the keys: as many as fill the chip with one block a CU (f32 at
+// head_dim 64: two), of whole tiles; at least 8 (split, KV head) pairs go to the
+// XCDs in turn, so that their number is brought down to a multiple of 8.
 int tree_attention_splits(const TreeJob &j) {
     const int rows = (int)j.n * (j.q_heads / j.g.kv_heads), wr = tree_row_waves(j);
     const size_t tile = (size_t)tree_tile_of(j), tiles = (j.offset + j.n + tile - 1) / tile;
-    const size_t per_cu = j.g.head_dim == 128 && (wr == 1 || j.g.kv_f32) ? 1 : 2;
-    const size_t blocks = (size_t)((rows + 32 * wr - 1) / (32 * wr)) * (size_t)j.g.kv_heads;
-    const size_t want = std::max<size_t>(per_cu * (size_t)std::max(device_cus(), 1) / blocks, 1);
-    const size_t S = std::min({want, tiles, (size_t)attention_max_splits()}), each = (tiles + S - 1) / S;
-    return (int)((tiles + each - 1) / each);
+    const size_t slots = (j.g.kv_f32 && j.g.head_dim == 64 ? 2 : 1) * (size_t)std::max(device_cus(), 8);
+    const size_t rb = (size_t)((rows + 32 * wr - 1) / (32 * wr)), kvh = (size_t)j.g.kv_heads;
+    const size_t pairs = std::max<size_t>(slots / 8 / rb, 1) * 8;
+    return (int)std::min({std::max<size_t>(pairs / kvh, 1), tiles, (size_t)attention_max_splits()});
 }
 
 int launch_tree_attention(const TreeJob &j, hipStream_t s) {
@@ -651,8 +831,8 @@ int launch_tree_attention(const TreeJob &j, hipStream_t s) {
     int S = tree_attention_splits(j);
     const size_t split_floats = attention_part_floats(j.n, j.q_heads, 1, j.g.head_dim);
     if (S > 1) S = (int)std::min<size_t>((size_t)S, std::max<size_t>(j.part ? j.part_floats / split_floats : 1, 1));
-    const size_t tile = (size_t)tree_tile_of(j), tiles = (j.offset + j.n + tile - 1) / tile, each = (tiles + S - 1) / S;
-    S = (int)((tiles + each - 1) / each);
+    const size_t tile = (size_t)tree_tile_of(j);
+    const int tiles = (int)((j.offset + j.n + tile - 1) / tile), items = (int)j.n * j.q_heads;
     TreeArgs a{};
     a.q = j.q;
     a.k = j.k;
@@ -660,6 +840,7 @@ int launch_tree_attention(const TreeJob &j, hipStream_t s) {
     a.page_table = j.g.page_table;
     a.parents = j.parents;
     a.part = j.part;
+    a.ml = (float2 *)(j.part + (size_t)items * S * j.g.head_dim);
     a.out = j.out;
     a.out_hi = j.out_hi;
     a.out_lo = j.out_lo;
@@ -668,10 +849,8 @@ int launch_tree_attention(const TreeJob &j, hipStream_t s) {
     a.q_heads = j.q_heads;
     a.offset = (int)j.offset;
     a.n = (int)j.n;
-    const int chunk = (int)(each * tile);
-    if (j.g.head_dim == 64) CHIP_TRY(launch_tree_h<64>(j, a, S, chunk, s));
-    else CHIP_TRY(launch_tree_h<128>(j, a, S, chunk, s));
-    return launch_attention_merge(j.part, S, j.n, j.q_heads, j.g.head_dim, j.out, j.out_hi, j.out_lo, s);
+    if (j.g.head_dim == 64) return launch_tree_h<64>(j, a, S, tiles, s);
+    return launch_tree_h<128>(j, a, S, tiles, s);
 }
 
 int launch_tree_commit(const KvLayer *layers, const int32_t *const *page_tables, size_t views, const KvGeom &g,
