@@ -237,7 +237,7 @@ __device__ __forceinline__ void read_vt2(const uint32_t (&addr)[HD / 32], bf16x8
 // two blocks of four waves a CU ran at the pace of their ages, and the younger
 // alone at the end.
 //
-// Splits are runs of whole tiles, joined by tree_merge_kernel. Blocks with
+// Splits are runs of positions, joined by tree_merge_kernel. Blocks with
 // the same (split, KV head) and other rows are 8 apart, on one XCD: they read
 // the same tiles through its L2.
 // ---------------------------------------------------------------------------
@@ -252,7 +252,7 @@ constexpr size_t tree_lds_bytes() { return tree_tile_lds<HD, KT>() + sizeof(Tree
 
 template <int HD, int WR, int WK, class KT>
 __global__ __launch_bounds__(64 * WR * WK) __attribute__((amdgpu_waves_per_eu(WR * WK / 4)))
-void tree_attn_kernel(TreeArgs a, int S, int tiles) {
+void tree_attn_kernel(TreeArgs a, int S, int units, int unit) {
     constexpr bool F32 = sizeof(KT) == 4;
     constexpr int NW = WR * WK, T = tree_tile<KT>(), STEPS = T / (32 * WK);
     constexpr int KSTEPS = HD / 16, UT = HD / 32;
@@ -274,13 +274,13 @@ void tree_attn_kernel(TreeArgs a, int S, int tiles) {
     const int m0 = rb * 32 * WR, m = m0 + wr * 32 + n;
     const bool rvalid = m < M;
     const int node = rvalid ? m / G : 0, head = g * G + (rvalid ? m % G : 0);
-    // tiles / S tiles a split, the first ones one more. (Block-uniform, said to
-    // the compiler: the quotients come from vector registers.)
-    const int each = tiles / S, extra = tiles % S;
-    const int t_first = split * each + min(split, extra);
-    const int start = __builtin_amdgcn_readfirstlane(t_first * T);
+    // units / S runs of `unit` positions a split, the first ones one more. (Block-
+    // uniform, said to the compiler: the quotients come from vector registers.)
+    const int each = units / S, extra = units % S;
+    const int first = split * each + min(split, extra);
+    const int start = __builtin_amdgcn_readfirstlane(first * unit);
     const int end = __builtin_amdgcn_readfirstlane(
-        (int)min((unsigned)(t_first + each + (split < extra)) * T, (unsigned)(a.offset + (min(M, m0 + 32 * WR) - 1) / G + 1)));
+        (int)min((unsigned)(first + each + (split < extra)) * unit, (unsigned)(a.offset + (min(M, m0 + 32 * WR) - 1) / G + 1)));
     const size_t at_part = ((size_t)node * a.q_heads + head) * S + split;
     if (start >= end) {  // no row of the block reaches the split
         if (rvalid && wk == 0 && half == 0) a.ml[at_part] = make_float2(-INFINITY, 0.f);
@@ -460,12 +460,14 @@ void tree_attn_kernel(TreeArgs a, int S, int tiles) {
         }
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) {
-            const int p0 = 32 * (wk * STEPS + st);
+            const int p0 = 32 * (st * WK + wk);
             if (t0 + p0 >= end) break;
             uint32_t vad[UT];
 #pragma unroll
             for (int u = 0; u < UT; ++u) vad[u] = (vbase + b * TB + p0 * HD * 2) ^ (64 * u);
             const int kat = kbase + b * TB + p0 * HD * 2;
+            // BF16: every K fragment of the step in flight at once. (f32: three parts
+            // of each would take the registers of the second wave at head_dim 64.)
             bf16x8 ka[F32 ? 1 : KSTEPS][PL];
             auto read_k = [&](int s, bf16x8 (&k)[PL]) {
 #pragma unroll
@@ -581,73 +583,76 @@ void tree_attn_kernel(TreeArgs a, int S, int tiles) {
     }
 
     l += __shfl_xor(l, 32, 64);
-    // Key waves past the first leave their rows in the tiles' LDS (rows padded
-    // by 16 bytes, off each other's banks), the first adds them up in order.
+    // The key waves of a row join in LDS, in the tiles' place: each leaves the
+    // blocks of 32 dims that others own (block u: wave u % WK) and adds up its own,
+    // in wave order. Rows padded by 16 bytes, off each other's banks.
     if constexpr (WK > 1) {
-        constexpr int LD = HD + 4;
-        static_assert((size_t)(WK - 1) * WR * 32 * (LD + 2) * 4 <= tree_tile_lds<HD, KT>(), "joined in the tiles' LDS");
-        auto rows_of = [&](int w) { return (float *)smem + ((w - 1) * WR + wr) * 32 * (LD + 2); };
-        if (wk > 0) {
-            float *so = rows_of(wk);
+        constexpr int LD = 32 + 4;
+        static_assert((size_t)WR * UT * (WK - 1) * 32 * LD * 4 + (size_t)NW * 32 * 8 <= tree_tile_lds<HD, KT>(),
+                      "joined in the tiles' LDS");
+        auto block = [&](int w, int u) {  // of key wave w, without its own ones
+            const int own_before = WK <= UT ? w * (UT / WK) : min(w, UT), own_below = u > w ? (u - w - 1) / WK + 1 : 0;
+            return (float *)smem + (wr * UT * (WK - 1) + w * UT - own_before + u - own_below) * 32 * LD + n * LD + 4 * half;
+        };
+        float2 *ml = (float2 *)((float *)smem + WR * UT * (WK - 1) * 32 * LD) + wr * WK * 32 + n;
 #pragma unroll
-            for (int u = 0; u < UT; ++u)
+        for (int u = 0; u < UT; ++u)
+            if (u % WK != wk)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    *(f32x4 *)(so + n * LD + 32 * u + 8 * q + 4 * half) =
+                    *(f32x4 *)(block(wk, u) + 8 * q) =
                         f32x4{oacc[u][4 * q], oacc[u][4 * q + 1], oacc[u][4 * q + 2], oacc[u][4 * q + 3]};
-            if (half == 0) {
-                so[32 * LD + 2 * n] = m2;
-                so[32 * LD + 2 * n + 1] = l;
-            }
-        }
+        if (half == 0) ml[32 * wk] = make_float2(m2, l);
         __syncthreads();
-        if (wk == 0) {
+        float2 x[WK];
+        m2 = -INFINITY;
 #pragma unroll
-            for (int w = 1; w < WK; ++w) {
-                const float *si = rows_of(w);
-                const float mi = si[32 * LD + 2 * n], li = si[32 * LD + 2 * n + 1];
-                const float mn = fmaxf(m2, mi);
-                // A wave that saw no key (m = -inf) adds nothing.
-                const float fa = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - mn);
-                const float fb = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - mn);
-                m2 = mn;
-                l = fmaf(fb, li, l * fa);
+        for (int w = 0; w < WK; ++w) {
+            x[w] = ml[32 * w];
+            m2 = fmaxf(m2, x[w].x);
+        }
+        l = 0.f;
 #pragma unroll
-                for (int u = 0; u < UT; ++u)
+        for (int w = 0; w < WK; ++w) {  // a wave that saw no key (-inf) adds nothing
+            x[w].x = x[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[w].x - m2);
+            l = fmaf(x[w].x, x[w].y, l);
+        }
+#pragma unroll
+        for (int u = 0; u < UT; ++u)
+            if (u % WK == wk) {
+                const f32x16 own = oacc[u];
+                oacc[u] = f32x16{};
+#pragma unroll
+                for (int w = 0; w < WK; ++w)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const f32x4 v = *(const f32x4 *)(si + n * LD + 32 * u + 8 * q + 4 * half);
+                        const f32x4 v = w == wk ? f32x4{own[4 * q], own[4 * q + 1], own[4 * q + 2], own[4 * q + 3]}
+                                                : *(const f32x4 *)(block(w, u) + 8 * q);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) oacc[u][4 * q + e] = fmaf(fb, v[e], oacc[u][4 * q + e] * fa);
+                        for (int e = 0; e < 4; ++e) oacc[u][4 * q + e] = fmaf(x[w].x, v[e], oacc[u][4 * q + e]);
                     }
             }
-        }
     }
-    if (wk == 0 && rvalid) {
+    if (rvalid) {
         bool odd = l != l || (F32 && tree.sick_prefix);
         if (in_tree)
 #pragma unroll
             for (int k = 0; k < kAncWords; ++k) odd |= (tree.anc[node][k] & tree.sick[k]) != 0;
+        const float inv = 1.0f / l;
         if (odd) {
-            if (half == 0) atomicOr(&tree.odd[wr], 1u << n);
-        } else if (S == 1) {
-            const float inv = 1.0f / l;
-            const size_t ob = ((size_t)node * a.q_heads + head) * HD;
-#pragma unroll
-            for (int u = 0; u < UT; ++u)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    store_out4(a, ob + 32 * u + 8 * q + 4 * half,
-                               f32x4{oacc[u][4 * q] * inv, oacc[u][4 * q + 1] * inv, oacc[u][4 * q + 2] * inv,
-                                     oacc[u][4 * q + 3] * inv});
+            if (wk == 0 && half == 0) atomicOr(&tree.odd[wr], 1u << n);
         } else {
+            const size_t ob = ((size_t)node * a.q_heads + head) * HD + 4 * half;
 #pragma unroll
             for (int u = 0; u < UT; ++u)
+                if (u % WK == wk)
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *(f32x4 *)(a.part + at_part * HD + 32 * u + 8 * q + 4 * half) =
-                        f32x4{oacc[u][4 * q], oacc[u][4 * q + 1], oacc[u][4 * q + 2], oacc[u][4 * q + 3]};
-            if (half == 0) a.ml[at_part] = make_float2(m2, l);
+                    for (int q = 0; q < 4; ++q) {
+                        const f32x4 v = {oacc[u][4 * q], oacc[u][4 * q + 1], oacc[u][4 * q + 2], oacc[u][4 * q + 3]};
+                        if (S == 1) store_out4(a, ob + 32 * u + 8 * q, v * inv);
+                        else *(f32x4 *)(a.part + at_part * HD + 32 * u + 8 * q + 4 * half) = v;
+                    }
+            if (S > 1 && wk == 0 && half == 0) a.ml[at_part] = make_float2(m2, l);
         }
     }
     __syncthreads();
@@ -773,7 +778,7 @@ int tree_row_waves(const TreeJob &j) {
 }
 
 template <int HD, int WR, int WK, class KT>
-int launch_tree_blocks(const TreeArgs &a, int S, int tiles, hipStream_t s) {
+int launch_tree_blocks(const TreeArgs &a, int S, int units, int unit, hipStream_t s) {
     constexpr size_t lds = tree_lds_bytes<HD, KT>();
     static std::atomic<uint64_t> lds_set{0};
     CHIP_TRY(allow_dynamic_lds((const void *)tree_attn_kernel<HD, WR, WK, KT>, lds, lds_set));
@@ -781,21 +786,21 @@ int launch_tree_blocks(const TreeArgs &a, int S, int tiles, hipStream_t s) {
     const size_t blocks = ((size_t)S * a.kv_heads + 7) / 8 * 8 * (size_t)rb;
     if (blocks > (size_t)INT32_MAX) return fail("HIP backend: tree attention grid out of range.");
     hipLaunchKernelGGL((tree_attn_kernel<HD, WR, WK, KT>), dim3((unsigned)blocks), dim3(64 * WR * WK), lds, s, a, S,
-                       tiles);
+                       units, unit);
     CHIP_CHECK(hipGetLastError());
     return 0;
 }
 
 template <int HD>
-int launch_tree_h(const TreeJob &j, const TreeArgs &a, int S, int tiles, hipStream_t s) {
+int launch_tree_h(const TreeJob &j, const TreeArgs &a, int S, int units, int unit, hipStream_t s) {
     const int wr = tree_row_waves(j);
     if (j.g.kv_f32) {
-        if (wr == 2) CHIP_TRY((launch_tree_blocks<HD, 2, 2, float>(a, S, tiles, s)));
-        else CHIP_TRY((launch_tree_blocks<HD, 4, 1, float>(a, S, tiles, s)));
+        if (wr == 2) CHIP_TRY((launch_tree_blocks<HD, 2, 2, float>(a, S, units, unit, s)));
+        else CHIP_TRY((launch_tree_blocks<HD, 4, 1, float>(a, S, units, unit, s)));
     } else {
-        if (wr == 1) CHIP_TRY((launch_tree_blocks<HD, 1, 4, uint16_t>(a, S, tiles, s)));
-        else if (wr == 2) CHIP_TRY((launch_tree_blocks<HD, 2, 4, uint16_t>(a, S, tiles, s)));
-        else CHIP_TRY((launch_tree_blocks<HD, 4, 2, uint16_t>(a, S, tiles, s)));
+        if (wr == 1) CHIP_TRY((launch_tree_blocks<HD, 1, 4, uint16_t>(a, S, units, unit, s)));
+        else if (wr == 2) CHIP_TRY((launch_tree_blocks<HD, 2, 4, uint16_t>(a, S, units, unit, s)));
+        else CHIP_TRY((launch_tree_blocks<HD, 4, 2, uint16_t>(a, S, units, unit, s)));
     }
     if (S == 1) return 0;
     const int items = (int)j.n * j.q_heads;
@@ -807,19 +812,21 @@ int launch_tree_h(const TreeJob &j, const TreeArgs &a, int S, int tiles, hipStre
     return 0;
 }
 
-int tree_tile_of(const TreeJob &j) { return j.g.kv_f32 ? tree_tile<float>() : tree_tile<uint16_t>(); }
-
 }  // namespace
 
 // Splits of the keys: as many as fill the chip with one block a CU (f32 at
-// head_dim 64: two), of whole tiles; at least 8 (split, KV head) pairs go to the
+// head_dim 64: two), of a tile at least; at least 8 (split, KV head) pairs go to the
 // XCDs in turn, so that their number is brought down to a multiple of 8.
 int tree_attention_splits(const TreeJob &j) {
     const int rows = (int)j.n * (j.q_heads / j.g.kv_heads), wr = tree_row_waves(j);
-    const size_t tile = (size_t)tree_tile_of(j), tiles = (j.offset + j.n + tile - 1) / tile;
+    const size_t tile = j.g.kv_f32 ? tree_tile<float>() : tree_tile<uint16_t>();
+    const size_t tiles = (j.offset + j.n + tile - 1) / tile;
     const size_t slots = (j.g.kv_f32 && j.g.head_dim == 64 ? 2 : 1) * (size_t)std::max(device_cus(), 8);
     const size_t rb = (size_t)((rows + 32 * wr - 1) / (32 * wr)), kvh = (size_t)j.g.kv_heads;
     const size_t pairs = std::max<size_t>(slots / 8 / rb, 1) * 8;
+    // One block walks two BF16 tiles sooner than two blocks join (5 nodes on 250,
+    // 14 / 2 heads of 64: 9.1 and 10.6 us; 24 on 120, 32 / 8 of 128: 15.9 and 17.1).
+    if (!j.g.kv_f32 && tiles <= 2) return 1;
     return (int)std::min({std::max<size_t>(pairs / kvh, 1), tiles, (size_t)attention_max_splits()});
 }
 
@@ -831,8 +838,13 @@ int launch_tree_attention(const TreeJob &j, hipStream_t s) {
     int S = tree_attention_splits(j);
     const size_t split_floats = attention_part_floats(j.n, j.q_heads, 1, j.g.head_dim);
     if (S > 1) S = (int)std::min<size_t>((size_t)S, std::max<size_t>(j.part ? j.part_floats / split_floats : 1, 1));
-    const size_t tile = (size_t)tree_tile_of(j);
-    const int tiles = (int)((j.offset + j.n + tile - 1) / tile), items = (int)j.n * j.q_heads;
+    // Splits of whole tiles, or of half ones where that makes the longest shorter
+    // (64 nodes on 16k, 9 or 8.5 tiles: 57.2 -> 55.4 us; 256 on 4k, 9 either way:
+    // 55.6, with half tiles 57.0).
+    const int tile = j.g.kv_f32 ? tree_tile<float>() : tree_tile<uint16_t>(), items = (int)j.n * j.q_heads;
+    auto units_of = [&](int unit) { return (int)((j.offset + j.n - 1) / (size_t)unit) + 1; };
+    auto longest = [&](int unit) { return (long)((units_of(unit) + S - 1) / S) * unit; };
+    const int unit = longest(64) < longest(tile) ? 64 : tile, units = units_of(unit);
     TreeArgs a{};
     a.q = j.q;
     a.k = j.k;
@@ -849,8 +861,8 @@ int launch_tree_attention(const TreeJob &j, hipStream_t s) {
     a.q_heads = j.q_heads;
     a.offset = (int)j.offset;
     a.n = (int)j.n;
-    if (j.g.head_dim == 64) return launch_tree_h<64>(j, a, S, tiles, s);
-    return launch_tree_h<128>(j, a, S, tiles, s);
+    if (j.g.head_dim == 64) return launch_tree_h<64>(j, a, S, units, unit, s);
+    return launch_tree_h<128>(j, a, S, units, unit, s);
 }
 
 int launch_tree_commit(const KvLayer *layers, const int32_t *const *page_tables, size_t views, const KvGeom &g,
