@@ -441,7 +441,7 @@ int cheetah_hip_logprobs(const void *logits, uint32_t logit_format, size_t rows,
                          float *top_logprobs) {
     if (!logits) return fail("HIP backend: logprobs with a null pointer.");
     if (logit_format > 1) return fail("HIP backend: logit_format must be 0 (BF16) or 1 (f32).");
-    if (rows == 0 || vocab == 0 || rows > (size_t)INT32_MAX || vocab > (size_t)INT32_MAX || stride > (size_t)INT32_MAX)
+    if (rows == 0 || vocab == 0 || rows > (size_t)INT32_MAX || vocab > (size_t)INT32_MAX - 64)
         return fail("HIP backend: logprobs shape out of range.");
     if (stride < vocab) return fail("HIP backend: logprobs rows overlap (stride below vocab).");
     if (top > CHEETAH_HIP_MAX_TOP || top > vocab)
@@ -468,6 +468,20 @@ int cheetah_hip_logprobs(const void *logits, uint32_t logit_format, size_t rows,
     j.entropy = entropy;
     j.ids = top_ids;
     j.tops = top_logprobs;
+    // Segment results (grown on demand, per thread).
+    static thread_local void *ws = nullptr;
+    static thread_local size_t ws_bytes = 0;
+    const size_t need = logprobs_workspace_bytes(rows, vocab, j.top);
+    if (need > ws_bytes) {
+        CHIP_CHECK(hipStreamSynchronize(g_stream));
+        if (ws) CHIP_CHECK(hipFree(ws));
+        ws = nullptr;
+        ws_bytes = 0;
+        CHIP_CHECK(hipMalloc(&ws, need));
+        ws_bytes = need;
+    }
+    j.ws = ws;
+    j.ws_bytes = ws_bytes;
     return launch_logprobs(j, g_stream);
 }
 

@@ -270,7 +270,10 @@ struct LogprobJob {
     float *logprobs = nullptr, *entropy = nullptr;
     uint32_t *ids = nullptr;
     float *tops = nullptr;
+    void *ws = nullptr;  // logprobs_workspace_bytes of it
+    size_t ws_bytes = 0;
 };
+size_t logprobs_workspace_bytes(size_t rows, size_t vocab, int top);
 int launch_logprobs(const LogprobJob &job, hipStream_t s);
 
 // Greedy argmax (ties -> last index, total order) of logits[n]; writes the

@@ -4,110 +4,445 @@
 //   log p_t = (x_t - M) - log(c + S),   H = log(c + S) + A / (c + S).
 // S leaves the largest logits out, so that log(1 + S) keeps its digits where one
 // token is nearly certain; every term of H is positive.
+//
+// One pass over the logits. A row is cut into segments, a block each
+// (logprobs_kernel); a block walks its segment in chunks that sit in registers,
+// each thread with its own running maximum and sums (f32 over a chunk's at most
+// 32 logits, in 64 bits from chunk to chunk), the block with the best `top`
+// logits so far. A logit joins those only if it is larger than the last of them
+// (ids rise, so an equal one loses), which is rare after the first chunk. Few
+// rows have many segments, joined by logprobs_join_kernel; many rows have one
+// each and are done in one launch.
+#include <algorithm>
+#include <type_traits>
+
 #include "kernels.hpp"
 
 namespace chip {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kCap = 512;       // candidates a block holds beside its best
+constexpr int kJoinPer = 16;    // picks of a thread in the join
+constexpr int kMaxSegs = 64;    // a lane of the join's waves each
+static_assert(kMaxSegs * kMaxTop <= kThreads * kJoinPer, "the join holds every pick");
+constexpr float kLog2e = 1.44269504088896340736f;
 
-__device__ __forceinline__ float logit(const float *x, size_t i) { return x[i]; }
-__device__ __forceinline__ float logit(const uint16_t *x, size_t i) { return bf16_f32(x[i]); }
+// A row's sums over a part of it: the maximum, the logits equal to it, the sum
+// over the others, the sum of the entropy's terms.
+struct Sums {
+    double S, A;
+    float m;
+    int c;
+};
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+struct LogprobArgs {
+    const void *x;
+    const uint32_t *tokens;
+    float *logprobs, *entropy;
+    uint32_t *ids;
+    float *tops;
+    size_t stride;
+    unsigned vocab, seg;  // logits of a row, of a segment
+    int top, segs;
+    Sums *sums;       // [row][segment]
+    uint64_t *picks;  // [row][segment][top]: keys
+};
+
+// Alternatives are ordered by their keys: the value's bits in order, then the
+// id from the largest. -0 counts as 0 and NaN as -inf. 0 is no logit's key.
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t id) {
+    const float v = x == x ? x + 0.f : -INFINITY;
+    const uint32_t u = __float_as_uint(v), o = u & 0x80000000u ? ~u : u | 0x80000000u;
+    return (uint64_t)o << 32 | (0xFFFFFFFFu - id);
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+    const uint32_t o = (uint32_t)(key >> 32);
+    return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+__device__ __forceinline__ uint32_t key_id(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {  // wave_sum's steps
+    v += dpp_f64<kDppXor1>(v);
+    v += dpp_f64<kDppXor2>(v);
+    v += dpp_f64<kDppHalfMirror>(v);
+    v += dpp_f64<kDppMirror>(v);
+    return (lane_f64(v, 0) + lane_f64(v, 16)) + (lane_f64(v, 32) + lane_f64(v, 48));
 }
 
-// One block a row: the maximum, the sums, then `top` times the best logit after
-// the last one (larger, or equal with a larger id).
+// Sums about their own maximum -> about the larger m. Without a finite logit
+// (-inf) they are 0, or NaN, which stays.
+__device__ __forceinline__ void raise(Sums &s, float m) {
+    if (s.m == m) return;
+    const float d = s.m - m;
+    const double f = s.m == -INFINITY ? 0.0 : (double)__builtin_amdgcn_exp2f(d * kLog2e), w = s.c + s.S;
+    s.A = f == 0.0 ? 0.0 * w : f * (s.A - (double)d * w);
+    s.S = f * w;
+    s.c = 0;
+    s.m = m;
+}
+
+// The wave's sums about m, the largest maximum.
+__device__ __forceinline__ Sums wave_join(Sums s, float m) {
+    raise(s, m);
+    Sums t;
+    t.m = m;
+    t.S = wave_sum_f64(s.S);
+    t.A = wave_sum_f64(s.A);
+    t.c = (int)wave_sum((float)s.c);  // at most the few ties of threads: below 2^24 a lane
+    return t;
+}
+
+// A row's results from its sums, alternatives from their keys (any LDS or
+// global array), by the threads of a block.
+struct Result {
+    double m, logsum;
+    bool empty;
+    __device__ Result(const Sums &s) : m(s.m), logsum(log1p((double)(s.c - 1) + s.S)), empty(s.m == -INFINITY && s.S == 0) {}
+    __device__ float logprob(float x) const { return empty ? -INFINITY : (float)((double)x - m - logsum); }
+};
 template <class T>
-__global__ __launch_bounds__(kThreads) void logprobs_kernel(const T *x, size_t vocab, size_t stride,
-                                                            const uint32_t *tokens, int top, float *logprobs,
-                                                            float *entropy, uint32_t *ids, float *tops) {
-    __shared__ float red[kWaves];
-    __shared__ double red64[3][kWaves];
-    __shared__ unsigned long long best[kWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const size_t row = blockIdx.x;
-    x += row * stride;
-    float m = -INFINITY;
-    for (size_t i = tid; i < vocab; i += kThreads) m = fmaxf(m, logit(x, i));
-    m = wave_max(m);
-    if (lane == 0) red[wave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float ref = m == -INFINITY ? 0.f : m;
-    double c = 0, S = 0, A = 0;
-    for (size_t i = tid; i < vocab; i += kThreads) {
-        const float d = logit(x, i) - ref, e = expf(d);
-        if (d == 0.f) c += 1;
-        else S += e;
-        if (!(e == 0.f)) A -= (double)e * d;  // a NaN reaches both sums
-    }
-    c = wave_sum_f64(c);
-    S = wave_sum_f64(S);
-    A = wave_sum_f64(A);
-    if (lane == 0) {
-        red64[0][wave] = c;
-        red64[1][wave] = S;
-        red64[2][wave] = A;
-    }
-    __syncthreads();
-    c = S = A = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        c += red64[0][w];
-        S += red64[1][w];
-        A += red64[2][w];
-    }
-    const bool empty = m == -INFINITY && S == 0;
-    const double logsum = c == 1 ? log1p(S) : log(c + S);
-    auto logprob = [&](float v) { return empty ? -INFINITY : (float)((double)v - (double)m - logsum); };
-    if (tid == 0) {
-        if (logprobs) {
-            const uint32_t t = tokens[row];
-            logprobs[row] = t < vocab ? logprob(logit(x, t)) : NAN;
+__device__ __forceinline__ void store_row(const LogprobArgs &a, const T *x, size_t row, const Sums &s, const uint64_t *best) {
+    const int tid = threadIdx.x;
+    const Result r(s);
+    if (tid == 0 && a.logprobs) {
+        const uint32_t t = a.tokens[row];
+        float v = NAN;
+        if (t < a.vocab) {
+            if constexpr (sizeof(T) == 4) v = r.logprob(x[t]);
+            else v = r.logprob(bf16_f32(x[t]));
         }
-        if (entropy) entropy[row] = empty ? 0.f : (float)(logsum + A / (c + S));
+        a.logprobs[row] = v;
     }
-    // Keys: the value in order, then the id descending.
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < top; ++k) {
-        unsigned long long b = 0;
-        for (size_t i = tid; i < vocab; i += kThreads) {
-            float v = logit(x, i) + 0.f;  // -0 and 0 are equal
-            if (v != v) v = -INFINITY;
-            const uint32_t u = __float_as_uint(v), o = u & 0x80000000u ? ~u : u | 0x80000000u;
-            const unsigned long long key = ((unsigned long long)o << 32) | (0xFFFFFFFFu - (uint32_t)i);
-            if (key < last && key > b) b = key;
-        }
+    if (tid == 0 && a.entropy) a.entropy[row] = r.empty ? 0.f : (float)(r.logsum + s.A / ((double)s.c + s.S));
+    if (tid < a.top) {
+        const uint64_t k = best[tid];
+        a.ids[row * a.top + tid] = key_id(k);
+        a.tops[row * a.top + tid] = r.logprob(key_value(k));
+    }
+}
+
+// The best `top` keys that a block has seen, in order, and candidates behind
+// them. Every function is called by the whole block.
+struct Best {
+    uint64_t key[kMaxTop + kCap];
+    float wave_value[kWaves];
+    uint64_t wave_key[kWaves];
+    int count;  // keys held, the best among them
+};
+
+// Sorts the keys held and keeps the first `top`: each thread ranks its keys
+// among all of them.
+__device__ __forceinline__ void best_prune(Best &b, int top) {
+    constexpr int R = (kMaxTop + kCap + kThreads - 1) / kThreads;
+    const int tid = threadIdx.x, n = b.count;
+    uint64_t mine[R];
+    int rank[R];
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) b = max(b, (unsigned long long)__shfl_xor(b, off, 64));
-        __syncthreads();
-        if (lane == 0) best[wave] = b;
-        __syncthreads();
-        last = max(max(best[0], best[1]), max(best[2], best[3]));
-        if (tid == 0) {
-            const uint32_t id = 0xFFFFFFFFu - (uint32_t)last;
-            ids[row * top + k] = id;
-            tops[row * top + k] = logprob(logit(x, id));
+    for (int i = 0; i < R; ++i) {
+        mine[i] = tid + kThreads * i < n ? b.key[tid + kThreads * i] : 0;
+        rank[i] = 0;
+    }
+    if (n <= kThreads) {
+        if (tid < (n + 63) / 64 * 64)
+            for (int j = 0; j < n; ++j) rank[0] += b.key[j] > mine[0];
+    } else {
+        for (int j = 0; j < n; ++j) {
+            const uint64_t k = b.key[j];
+#pragma unroll
+            for (int i = 0; i < R; ++i) rank[i] += k > mine[i];
         }
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (tid + kThreads * i < n && rank[i] < top) b.key[rank[i]] = mine[i];
+    if (tid == 0) b.count = min(n, top);
+    __syncthreads();
+}
+
+// Takes the block's next logits, x[i] with ids id(i) where ok(i), thread by
+// thread; `most` is the thread's largest. Keys of logits that cannot be among
+// the best `top` are left out: while `full`, those up to the last of them.
+template <int PER, class Id, class Ok>
+__device__ __forceinline__ void best_take(Best &b, int top, bool &full, float &last, const float (&x)[PER], float most,
+                                          Id id, Ok ok) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    most = most == most ? most : -INFINITY;  // (a signalling NaN came last)
+    auto open = [&](int i, float from) { return ok(i) && (full ? x[i] > last : true) && !(x[i] < from); };
+    auto append = [&](float from) {  // every open logit from `from` on; the count may pass the room
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) n += open(i, from);
+        if (n) {
+            int at = atomicAdd(&b.count, n);
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (open(i, from)) {
+                    if (at < kMaxTop + kCap) b.key[at] = key_of(x[i], id(i));
+                    ++at;
+                }
+        }
+        __syncthreads();
+    };
+    auto settle = [&]() {
+        best_prune(b, top);
+        full = b.count == top;
+        last = full ? key_value(b.key[top - 1]) : -INFINITY;
+    };
+    const int held = b.count;
+    __syncthreads();
+    if (full) {
+        append(-INFINITY);
+        if (b.count <= kMaxTop + kCap) {
+            if (b.count >= top + 64) settle();
+            return;
+        }
+        __syncthreads();
+        if (tid == 0) b.count = held;
+        __syncthreads();
+        settle();
+    }
+    // Too many: at least `top` logits reach the smallest of the waves' (top / 4)-th
+    // largest thread maxima.
+    {
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < 64; ++j) {
+            const float v = lane_read(most, j);
+            rank += v > most || (v == most && j < lane);
+        }
+        const uint64_t at = __ballot(rank == (top + kWaves - 1) / kWaves - 1);
+        if (lane == 0) b.wave_value[wave] = at ? lane_read(most, __builtin_ctzll(at)) : -INFINITY;
+    }
+    __syncthreads();
+    const float from = fminf(fminf(b.wave_value[0], b.wave_value[1]), fminf(b.wave_value[2], b.wave_value[3]));
+    const int before = b.count;
+    __syncthreads();
+    append(from);
+    if (b.count > kMaxTop + kCap) {
+        // Ties without end: the best open logit after the last one, `top` times.
+        __syncthreads();
+        if (tid == 0) b.count = before;
+        uint64_t prev = ~0ull;
+        for (int r = 0; r < top; ++r) {
+            uint64_t k = 0;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const uint64_t q = open(i, -INFINITY) ? key_of(x[i], id(i)) : 0;
+                if (q < prev && q > k) k = q;
+            }
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) {
+                const uint64_t q = (uint64_t)__shfl_xor((unsigned long long)k, off, 64);
+                k = q > k ? q : k;
+            }
+            __syncthreads();
+            if (lane == 0) b.wave_key[wave] = k;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) k = max(k, b.wave_key[w]);
+            if (k == 0) break;  // no more (the same in every thread)
+            if (tid == 0) b.key[b.count++] = k;
+            prev = k;
+        }
+        __syncthreads();
+    }
+    settle();
+}
+
+// One segment of a row, kThreads * PER logits at a time.
+template <class T, int PER>
+__global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
+    constexpr int VE = 16 / sizeof(T), NV = PER / VE;  // logits of a 16-byte load, loads of a thread
+    constexpr unsigned CHUNK = kThreads * PER;
+    __shared__ Best best;
+    __shared__ Sums part[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const size_t row = blockIdx.x / (unsigned)a.segs;
+    const unsigned seg = blockIdx.x % (unsigned)a.segs;
+    const T *x_row = (const T *)a.x + row * a.stride;
+    // 16-byte loads from the row's last boundary on: logit e of them has id
+    // e - head. A load holds at least one logit of the row.
+    const unsigned head = (unsigned)((uintptr_t)x_row & 15) / sizeof(T), all = head + a.vocab;
+    const T *from = x_row - head;
+    const unsigned begin = seg * a.seg, end = min(begin + a.seg, all), last_load = (all - 1) / VE * VE;
+    u32x4 raw[NV];
+    auto load = [&](unsigned e0) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) raw[v] = *(const u32x4 *)(from + min(e0 + (kThreads * v + tid) * VE, last_load));
+    };
+    load(begin);
+    if (tid == 0) best.count = 0;
+    __syncthreads();
+    Sums s{0.0, 0.0, -INFINITY, 0};
+    bool full = false;
+    float last = -INFINITY;
+    for (unsigned e0 = begin; e0 < end; e0 += CHUNK) {
+        float x[PER];
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    x[4 * v + i] = __uint_as_float(raw[v][i]);
+                } else {
+                    x[8 * v + 2 * i] = bf16_lo(raw[v][i]);
+                    x[8 * v + 2 * i + 1] = bf16_hi(raw[v][i]);
+                }
+            }
+        if (e0 + CHUNK < end) load(e0 + CHUNK);
+        auto at = [&](int i) { return e0 + (kThreads * (i / VE) + tid) * VE + i % VE; };
+        auto ok = [&](int i) { return at(i) >= head && at(i) < end; };
+        const bool whole = e0 >= head && e0 + CHUNK <= end;
+        if (!whole)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) x[i] = ok(i) ? x[i] : -INFINITY;
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) most = fmaxf(most, x[i]);
+        raise(s, fmaxf(s.m, most));
+        const float m = s.m == -INFINITY ? 0.f : s.m;
+        float S = 0.f, A = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const float d = x[i] - m, e = __builtin_amdgcn_exp2f(d * kLog2e), o = d == 0.f ? 0.f : e;
+            s.c += d == 0.f;
+            S += o;
+            A = fmaf(o, -fmaxf(d, -150.f), A);  // 0 from -150 on, -inf too
+        }
+        s.S += S;
+        s.A += A;
+        if (a.top && __syncthreads_or(!full || most > last))
+            best_take(best, a.top, full, last, x, most, [&](int i) { return at(i) - head; },
+                      [&](int i) { return whole || ok(i); });
+    }
+    // The block's sums.
+    const float wm = wave_max(s.m);
+    const Sums t = wave_join(s, wm);
+    if (lane == 0) part[wave] = t;
+    __syncthreads();
+    Sums all_waves = part[0];
+    float m = all_waves.m;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, part[w].m);
+    raise(all_waves, m);
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) {
+        Sums u = part[w];
+        raise(u, m);
+        all_waves.S += u.S;
+        all_waves.A += u.A;
+        all_waves.c += u.c;
+    }
+    if (a.top && best.count != a.top) {  // candidates left, or a segment of fewer logits than `top`
+        __syncthreads();
+        best_prune(best, a.top);
+    }
+    if (a.segs == 1) {
+        store_row(a, x_row, row, all_waves, best.key);
+        return;
+    }
+    const size_t at = row * a.segs + seg;
+    if (tid == 0) a.sums[at] = all_waves;
+    if (tid < a.top) a.picks[at * a.top + tid] = tid < best.count ? best.key[tid] : 0;
+}
+
+// The segments of a row.
+template <class T>
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a) {
+    __shared__ Best best;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const size_t row = blockIdx.x;
+    Sums s{0.0, 0.0, -INFINITY, 0};
+    if (lane < a.segs) s = a.sums[row * a.segs + lane];
+    uint64_t key[kJoinPer];
+    float x[kJoinPer], most = -INFINITY;
+    const int n = a.segs * a.top;
+#pragma unroll
+    for (int i = 0; i < kJoinPer; ++i) {
+        const int e = kThreads * i + tid;
+        key[i] = e < n ? a.picks[row * n + e] : 0;
+        x[i] = key[i] ? key_value(key[i]) : -INFINITY;
+        most = fmaxf(most, x[i]);
+    }
+    if (tid == 0) best.count = 0;
+    __syncthreads();
+    s = wave_join(s, wave_max(s.m));
+    if (a.top) {
+        bool full = false;
+        float last = -INFINITY;
+        best_take(best, a.top, full, last, x, most, [&](int i) { return key_id(key[i]); }, [&](int i) { return key[i] != 0; });
+    }
+    store_row(a, (const T *)a.x + row * a.stride, row, s, best.key);
+}
+
+// Segments of a row: enough for two blocks a CU, of at least a small chunk.
+int logprob_segs(size_t rows, size_t vocab) {
+    const size_t want = 2 * (size_t)std::max(device_cus(), 1) / rows, most = (vocab + 2047) / 2048;
+    return (int)std::max<size_t>(std::min({want, most, (size_t)kMaxSegs}), 1);
+}
+
+template <class T>
+int launch_logprobs_t(const LogprobJob &j, LogprobArgs &a, hipStream_t s) {
+    const size_t blocks = j.rows * (size_t)a.segs;
+    if (blocks > (size_t)INT32_MAX) return fail("HIP backend: logprobs grid out of range.");
+    if (a.seg <= (unsigned)(8 * kThreads))
+        hipLaunchKernelGGL((logprobs_kernel<T, 8>), dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
+    else
+        hipLaunchKernelGGL((logprobs_kernel<T, 32>), dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
+    CHIP_CHECK(hipGetLastError());
+    if (a.segs == 1) return 0;
+    hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3((unsigned)j.rows), dim3(kThreads), 0, s, a);
+    CHIP_CHECK(hipGetLastError());
+    return 0;
 }
 
 }  // namespace
 
+size_t logprobs_workspace_bytes(size_t rows, size_t vocab, int top) {
+    const size_t segs = (size_t)logprob_segs(rows, vocab);
+    return segs == 1 ? 0 : rows * segs * (sizeof(Sums) + (size_t)top * sizeof(uint64_t));
+}
+
 int launch_logprobs(const LogprobJob &j, hipStream_t s) {
-    const dim3 grid((unsigned)j.rows);
-    if (j.f32)
-        hipLaunchKernelGGL((logprobs_kernel<float>), grid, dim3(kThreads), 0, s, (const float *)j.x, j.vocab, j.stride,
-                           j.tokens, j.top, j.logprobs, j.entropy, j.ids, j.tops);
-    else
-        hipLaunchKernelGGL((logprobs_kernel<uint16_t>), grid, dim3(kThreads), 0, s, (const uint16_t *)j.x, j.vocab,
-                           j.stride, j.tokens, j.top, j.logprobs, j.entropy, j.ids, j.tops);
-    CHIP_CHECK(hipGetLastError());
-    return 0;
+    if (!j.x || j.rows == 0 || j.vocab == 0 || j.vocab > (size_t)INT32_MAX - 64 || j.stride < j.vocab || j.top < 0 ||
+        j.top > kMaxTop || (size_t)j.top > j.vocab)
+        return fail("HIP backend: logprobs shape out of range.");
+    LogprobArgs a{};
+    a.x = j.x;
+    a.tokens = j.tokens;
+    a.logprobs = j.logprobs;
+    a.entropy = j.entropy;
+    a.ids = j.ids;
+    a.tops = j.tops;
+    a.stride = j.stride;
+    a.vocab = (unsigned)j.vocab;
+    a.top = j.top;
+    a.segs = logprob_segs(j.rows, j.vocab);
+    // Up to seven logits of another row or of padding come before the row's first.
+    a.seg = ((unsigned)j.vocab + 7 + (unsigned)a.segs - 1) / (unsigned)a.segs;
+    a.seg = (a.seg + 7) / 8 * 8;
+    if (a.segs > 1) {
+        if (!j.ws || j.ws_bytes < logprobs_workspace_bytes(j.rows, j.vocab, j.top))
+            return fail("HIP backend: logprobs workspace too small.");
+        a.sums = (Sums *)j.ws;
+        a.picks = (uint64_t *)(a.sums + j.rows * (size_t)a.segs);
+    }
+    return j.f32 ? launch_logprobs_t<float>(j, a, s) : launch_logprobs_t<uint16_t>(j, a, s);
 }
 
 }  // namespace chip
