@@ -23,9 +23,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kCap = 512;       // candidates a block holds beside its best
-constexpr int kJoinPer = 16;    // picks of a thread in the join
-constexpr int kMaxSegs = 64;    // a lane of the join's waves each
-static_assert(kMaxSegs * kMaxTop <= kThreads * kJoinPer, "the join holds every pick");
+constexpr int kMaxSegs = 128;   // two a lane of the join's waves
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // A row's sums over a part of it: the maximum, the logits equal to it, the sum
@@ -137,35 +135,39 @@ __device__ __forceinline__ void store_row(const LogprobArgs &a, const T *x, size
 
 // The best `top` keys that a block has seen, in order, and candidates behind
 // them. Every function is called by the whole block.
+constexpr int kRoom = kMaxTop + kCap;  // keys held; up to kMaxTop ties go behind them
 struct Best {
-    uint64_t key[kMaxTop + kCap];
+    uint64_t key[kRoom + kMaxTop + 8];
     float wave_value[kWaves];
     uint64_t wave_key[kWaves];
+    int ties[kWaves];
     int count;  // keys held, the best among them
 };
 
 // Sorts the keys held and keeps the first `top`: each thread ranks its keys
-// among all of them.
-__device__ __forceinline__ void best_prune(Best &b, int top) {
-    constexpr int R = (kMaxTop + kCap + kThreads - 1) / kThreads;
-    const int tid = threadIdx.x, n = b.count;
+// among all of them, eight reads in flight.
+template <int R>
+__device__ __forceinline__ void best_rank(Best &b, int top, int n) {
+    const int tid = threadIdx.x;
     uint64_t mine[R];
     int rank[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        mine[i] = tid + kThreads * i < n ? b.key[tid + kThreads * i] : 0;
+        mine[i] = tid + kThreads * i < n ? b.key[tid + kThreads * i] : ~0ull;
         rank[i] = 0;
     }
-    if (n <= kThreads) {
-        if (tid < (n + 63) / 64 * 64)
-            for (int j = 0; j < n; ++j) rank[0] += b.key[j] > mine[0];
-    } else {
-        for (int j = 0; j < n; ++j) {
-            const uint64_t k = b.key[j];
+    if (tid < 8) b.key[n + tid] = 0;  // above no key
+    __syncthreads();
+    if (R > 1 || tid < (n + 63) / 64 * 64)
+        for (int j = 0; j < n; j += 8) {
+            uint64_t k[8];
 #pragma unroll
-            for (int i = 0; i < R; ++i) rank[i] += k > mine[i];
+            for (int q = 0; q < 8; ++q) k[q] = b.key[j + q];
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+#pragma unroll
+                for (int i = 0; i < R; ++i) rank[i] += k[q] > mine[i];
         }
-    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < R; ++i)
@@ -173,95 +175,173 @@ __device__ __forceinline__ void best_prune(Best &b, int top) {
     if (tid == 0) b.count = min(n, top);
     __syncthreads();
 }
+__device__ __forceinline__ void best_prune(Best &b, int top) {
+    constexpr int R = (kRoom + kMaxTop + kThreads - 1) / kThreads;
+    const int n = b.count;
+    if (n <= kThreads) best_rank<1>(b, top, n);
+    else best_rank<R>(b, top, n);
+}
 
-// Takes the block's next logits, x[i] with ids id(i) where ok(i), thread by
-// thread; `most` is the thread's largest. Keys of logits that cannot be among
-// the best `top` are left out: while `full`, those up to the last of them.
-template <int PER, class Id, class Ok>
-__device__ __forceinline__ void best_take(Best &b, int top, bool &full, float &last, const float (&x)[PER], float most,
-                                          Id id, Ok ok) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    most = most == most ? most : -INFINITY;  // (a signalling NaN came last)
-    auto open = [&](int i, float from) { return ok(i) && (full ? x[i] > last : true) && !(x[i] < from); };
-    auto append = [&](float from) {  // every open logit from `from` on; the count may pass the room
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) n += open(i, from);
-        if (n) {
-            int at = atomicAdd(&b.count, n);
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (open(i, from)) {
-                    if (at < kMaxTop + kCap) b.key[at] = key_of(x[i], id(i));
-                    ++at;
-                }
-        }
-        __syncthreads();
+// What the best are taken from, 16 bytes of logits a thread and vector or a
+// pick; equal ones' ids rise with (vector, thread, place in it). Read again
+// from memory: the registers that hold a chunk would not do for both.
+template <class T>
+struct Logits {
+    static constexpr int VE = 16 / sizeof(T);
+    const T *from;
+    unsigned e0, head, end, last_load;
+    int vectors;
+    struct Vec {
+        u32x4 w;
+        unsigned e;
     };
-    auto settle = [&]() {
-        best_prune(b, top);
-        full = b.count == top;
-        last = full ? key_value(b.key[top - 1]) : -INFINITY;
-    };
-    const int held = b.count;
-    __syncthreads();
-    if (full) {
-        append(-INFINITY);
-        if (b.count <= kMaxTop + kCap) {
-            if (b.count >= top + 64) settle();
-            return;
-        }
-        __syncthreads();
-        if (tid == 0) b.count = held;
-        __syncthreads();
-        settle();
+    __device__ Vec load(int v) const {
+        const unsigned e = e0 + (kThreads * v + threadIdx.x) * VE;
+        return Vec{*(const u32x4 *)(from + min(e, last_load)), e};
     }
-    // Too many: at least `top` logits reach the smallest of the waves' (top / 4)-th
-    // largest thread maxima.
+    __device__ bool ok(const Vec &v, int q) const { return v.e + q >= head && v.e + q < end; }
+    __device__ uint32_t id(const Vec &v, int q) const { return v.e + q - head; }
+    __device__ float value(const Vec &v, int q) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(v.w[q]);
+        else return q & 1 ? bf16_hi(v.w[q >> 1]) : bf16_lo(v.w[q >> 1]);
+    }
+};
+struct Picks {
+    static constexpr int VE = 1;
+    const uint64_t *key;
+    int n, vectors;
+    typedef uint64_t Vec;
+    __device__ Vec load(int v) const {
+        const int e = kThreads * v + (int)threadIdx.x;
+        return e < n ? key[e] : 0;
+    }
+    __device__ bool ok(Vec v, int) const { return v != 0; }
+    __device__ uint32_t id(Vec v, int) const { return key_id(v); }
+    __device__ float value(Vec v, int) const { return key_value(v); }
+};
+
+__device__ __forceinline__ void best_settle(Best &b, int top, bool &full, float &last) {
+    best_prune(b, top);
+    full = b.count == top;
+    last = full ? key_value(b.key[top - 1]) : -INFINITY;
+}
+
+// Takes a chunk of which any number may belong to the best: those above `last`
+// while `full`, all otherwise. `most`: the thread's largest value of it.
+template <class Src>
+__device__ __forceinline__ void best_refill(Best &b, int top, bool &full, float &last, const Src &src, float most) {
+    constexpr int VE = Src::VE;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int held = b.count;
+    // At least `top` logits reach the smallest of the waves' (top / 4) largest
+    // thread maxima. (Ranked by their ordered bits, the lowest six the lane's, so
+    // that every lane has a rank of its own.)
     {
+        most = most == most ? most : -INFINITY;  // (a signalling NaN came last)
+        const uint32_t u = __float_as_uint(most), o = u & 0x80000000u ? ~u : u | 0x80000000u;
+        const uint32_t mine = (o & ~63u) | lane;
         int rank = 0;
-#pragma unroll 8
-        for (int j = 0; j < 64; ++j) {
-            const float v = lane_read(most, j);
-            rank += v > most || (v == most && j < lane);
-        }
-        const uint64_t at = __ballot(rank == (top + kWaves - 1) / kWaves - 1);
-        if (lane == 0) b.wave_value[wave] = at ? lane_read(most, __builtin_ctzll(at)) : -INFINITY;
+#pragma unroll 16
+        for (int j = 0; j < 64; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)mine, j) > mine;
+        const float least = -wave_max(rank < (top + kWaves - 1) / kWaves ? -most : -INFINITY);
+        if (lane == 0) b.wave_value[wave] = least;
     }
     __syncthreads();
     const float from = fminf(fminf(b.wave_value[0], b.wave_value[1]), fminf(b.wave_value[2], b.wave_value[3]));
-    const int before = b.count;
-    __syncthreads();
-    append(from);
-    if (b.count > kMaxTop + kCap) {
-        // Ties without end: the best open logit after the last one, `top` times.
-        __syncthreads();
-        if (tid == 0) b.count = before;
-        uint64_t prev = ~0ull;
-        for (int r = 0; r < top; ++r) {
-            uint64_t k = 0;
+    auto open = [&](float v) { return !full || v > last; };
+    // Every open logit from `from` on (`above`: only larger ones); the count may
+    // pass the room.
+    auto append = [&](bool above) {
+        for (int v = 0; v < src.vectors; ++v) {
+            const auto w = src.load(v);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const uint64_t q = open(i, -INFINITY) ? key_of(x[i], id(i)) : 0;
-                if (q < prev && q > k) k = q;
+            for (int q = 0; q < VE; ++q) {
+                const float x = src.value(w, q);
+                if (src.ok(w, q) && open(x) && (above ? x > from : !(x < from))) {
+                    const int at = atomicAdd(&b.count, 1);
+                    if (at < kRoom) b.key[at] = key_of(x, src.id(w, q));
+                }
             }
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) {
-                const uint64_t q = (uint64_t)__shfl_xor((unsigned long long)k, off, 64);
-                k = q > k ? q : k;
-            }
-            __syncthreads();
-            if (lane == 0) b.wave_key[wave] = k;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) k = max(k, b.wave_key[w]);
-            if (k == 0) break;  // no more (the same in every thread)
-            if (tid == 0) b.key[b.count++] = k;
-            prev = k;
         }
         __syncthreads();
+    };
+    auto back = [&]() {
+        __syncthreads();
+        if (tid == 0) b.count = held;
+        __syncthreads();
+    };
+    append(false);
+    if (b.count > kRoom) {
+        // Ties (a mask's, most likely): the larger ones, and the first `top` of those
+        // equal to `from`.
+        back();
+        append(true);
+        const int larger = b.count;
+        if (larger <= kRoom) {
+            auto tie = [&](const typename Src::Vec &w, int q) {
+                const float x = src.value(w, q);
+                return src.ok(w, q) && open(x) && !(x < from) && !(x > from);
+            };
+            int base = 0;
+            for (int v = 0; v < src.vectors && base < top; ++v) {
+                const auto w = src.load(v);
+                int n = 0, before = 0;
+#pragma unroll
+                for (int q = 0; q < VE; ++q) {
+                    const uint64_t m = __ballot(tie(w, q));
+                    n += __builtin_popcountll(m);
+                    before += __builtin_popcountll(m & ((1ull << lane) - 1));
+                }
+                if (lane == 0) b.ties[wave] = n;
+                __syncthreads();
+                int at = base + before;
+                for (int x = 0; x < kWaves; ++x) {
+                    if (x < wave) at += b.ties[x];
+                    base += b.ties[x];
+                }
+#pragma unroll
+                for (int q = 0; q < VE; ++q)
+                    if (tie(w, q)) {
+                        if (at < top) b.key[larger + at] = key_of(src.value(w, q), src.id(w, q));
+                        ++at;
+                    }
+                __syncthreads();
+            }
+            if (tid == 0) b.count = larger + min(base, top);
+            __syncthreads();
+        } else {
+            // Logits that rise with their ids: the best open one after the last, `top` times.
+            back();
+            uint64_t prev = ~0ull;
+            for (int r = 0; r < top; ++r) {
+                uint64_t k = 0;
+                for (int v = 0; v < src.vectors; ++v) {
+                    const auto w = src.load(v);
+#pragma unroll
+                    for (int q = 0; q < VE; ++q) {
+                        const float x = src.value(w, q);
+                        const uint64_t c = src.ok(w, q) && open(x) ? key_of(x, src.id(w, q)) : 0;
+                        if (c < prev && c > k) k = c;
+                    }
+                }
+#pragma unroll
+                for (int off = 32; off > 0; off >>= 1) {
+                    const uint64_t c = (uint64_t)__shfl_xor((unsigned long long)k, off, 64);
+                    k = c > k ? c : k;
+                }
+                __syncthreads();
+                if (lane == 0) b.wave_key[wave] = k;
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) k = max(k, b.wave_key[w]);
+                if (k == 0) break;  // no more (the same in every thread)
+                if (tid == 0) b.key[b.count++] = k;
+                prev = k;
+            }
+            __syncthreads();
+        }
     }
-    settle();
+    best_settle(b, top, full, last);
 }
 
 // One segment of a row, kThreads * PER logits at a time.
@@ -326,9 +406,30 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
         }
         s.S += S;
         s.A += A;
-        if (a.top && __syncthreads_or(!full || most > last))
-            best_take(best, a.top, full, last, x, most, [&](int i) { return at(i) - head; },
-                      [&](int i) { return whole || ok(i); });
+        if (a.top && __syncthreads_or(!full || most > last)) {
+            const Logits<T> src{from, e0, head, end, last_load, (int)((min(end - e0, CHUNK) + kThreads * VE - 1) / (kThreads * VE))};
+            if (full) {  // few: straight from the registers
+                const int held = best.count;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (x[i] > last) {  // (never a logit that is not ok: -inf)
+                        const int k = atomicAdd(&best.count, 1);
+                        if (k < kRoom) best.key[k] = key_of(x[i], at(i) - head);
+                    }
+                __syncthreads();
+                const int n = best.count;
+                if (n <= kRoom) {
+                    if (n >= a.top + 64) best_settle(best, a.top, full, last);
+                    continue;
+                }
+                __syncthreads();
+                if (tid == 0) best.count = held;
+                __syncthreads();
+                best_settle(best, a.top, full, last);
+            }
+            best_refill(best, a.top, full, last, src, most);
+        }
     }
     // The block's sums.
     const float wm = wave_max(s.m);
@@ -348,7 +449,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
         all_waves.A += u.A;
         all_waves.c += u.c;
     }
-    if (a.top && best.count != a.top) {  // candidates left, or a segment of fewer logits than `top`
+    if (a.top && best.count > a.top) {  // candidates left
         __syncthreads();
         best_prune(best, a.top);
     }
@@ -367,32 +468,35 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a) 
     __shared__ Best best;
     const int tid = threadIdx.x, lane = tid & 63;
     const size_t row = blockIdx.x;
-    Sums s{0.0, 0.0, -INFINITY, 0};
+    Sums s{0.0, 0.0, -INFINITY, 0}, s2 = s;
     if (lane < a.segs) s = a.sums[row * a.segs + lane];
-    uint64_t key[kJoinPer];
-    float x[kJoinPer], most = -INFINITY;
+    if (lane + 64 < a.segs) s2 = a.sums[row * a.segs + lane + 64];
     const int n = a.segs * a.top;
-#pragma unroll
-    for (int i = 0; i < kJoinPer; ++i) {
-        const int e = kThreads * i + tid;
-        key[i] = e < n ? a.picks[row * n + e] : 0;
-        x[i] = key[i] ? key_value(key[i]) : -INFINITY;
-        most = fmaxf(most, x[i]);
+    const Picks src{a.picks + row * n, n, (n + kThreads - 1) / kThreads};
+    float most = -INFINITY;
+    for (int v = 0; v < src.vectors; ++v) {
+        const uint64_t k = src.load(v);
+        most = fmaxf(most, k ? key_value(k) : -INFINITY);
     }
     if (tid == 0) best.count = 0;
     __syncthreads();
-    s = wave_join(s, wave_max(s.m));
+    const float m = wave_max(fmaxf(s.m, s2.m));
+    s = wave_join(s, m);
+    s2 = wave_join(s2, m);
+    s.S += s2.S;
+    s.A += s2.A;
+    s.c += s2.c;
     if (a.top) {
         bool full = false;
         float last = -INFINITY;
-        best_take(best, a.top, full, last, x, most, [&](int i) { return key_id(key[i]); }, [&](int i) { return key[i] != 0; });
+        best_refill(best, a.top, full, last, src, most);
     }
     store_row(a, (const T *)a.x + row * a.stride, row, s, best.key);
 }
 
 // Segments of a row: enough for two blocks a CU, of at least a small chunk.
 int logprob_segs(size_t rows, size_t vocab) {
-    const size_t want = 2 * (size_t)std::max(device_cus(), 1) / rows, most = (vocab + 2047) / 2048;
+    const size_t want = 2 * (size_t)std::max(device_cus(), 1) / rows, most = (vocab + 2039) / 2040;
     return (int)std::max<size_t>(std::min({want, most, (size_t)kMaxSegs}), 1);
 }
 
