@@ -44,7 +44,7 @@ struct LogprobArgs {
     unsigned vocab, seg;  // logits of a row, of a segment
     int top, segs;
     Sums *sums;       // [row][segment]
-    uint64_t *picks;  // [row][segment][top]: keys
+    uint64_t *picks;  // [row][top][segment]: keys, 0 for none
 };
 
 // Alternatives are ordered by their keys: the value's bits in order, then the
@@ -134,14 +134,15 @@ __device__ __forceinline__ void store_row(const LogprobArgs &a, const T *x, size
 }
 
 // The best `top` keys that a block has seen, in order, and candidates behind
-// them. Every function is called by the whole block.
-constexpr int kRoom = kMaxTop + kCap;  // keys held; up to kMaxTop ties go behind them
+// them. Logits of -inf (and NaN) are never among them: fill_masked adds the first
+// of those at the end where others are fewer than `top`. Every function is called
+// by the whole block and ends with its results visible.
+constexpr int kRoom = kMaxTop + kCap;
 struct Best {
-    uint64_t key[kRoom + kMaxTop + 8];
+    uint64_t key[kRoom + 8];
     float wave_value[kWaves];
-    uint64_t wave_key[kWaves];
-    int ties[kWaves];
-    int count;  // keys held, the best among them
+    int hist[256], wave_total[kWaves], found[3];
+    int count;  // keys held, the best among them; past kRoom: some had no room
 };
 
 // Sorts the keys held and keeps the first `top`: each thread ranks its keys
@@ -175,21 +176,49 @@ __device__ __forceinline__ void best_rank(Best &b, int top, int n) {
     if (tid == 0) b.count = min(n, top);
     __syncthreads();
 }
-__device__ __forceinline__ void best_prune(Best &b, int top) {
-    constexpr int R = (kRoom + kMaxTop + kThreads - 1) / kThreads;
+
+// Prunes to the best `top`, says above what a logit would join them and how many
+// are held (the count itself may grow again before every wave has read it).
+__device__ __forceinline__ int best_settle(Best &b, int top, float &last) {
+    constexpr int R = (kRoom + kThreads - 1) / kThreads;
     const int n = b.count;
     if (n <= kThreads) best_rank<1>(b, top, n);
     else best_rank<R>(b, top, n);
+    last = n < top ? -INFINITY : key_value(b.key[top - 1]);
+    return min(n, top);
 }
 
-// What the best are taken from, 16 bytes of logits a thread and vector or a
-// pick; equal ones' ids rise with (vector, thread, place in it). Read again
-// from memory: the registers that hold a chunk would not do for both.
+// A value that at least `top` of the logits reach whose thread maxima are `most`:
+// the smallest of the waves' (top / 4) largest. (Ranked by their ordered bits, the
+// lowest six the lane's, so that every lane has a rank of its own.)
+__device__ __forceinline__ float best_bound(Best &b, int top, float most) {
+    const int lane = threadIdx.x & 63;
+    most = most == most ? most + 0.f : -INFINITY;  // (NaN: a signalling one came last)
+    const uint32_t u = __float_as_uint(most), o = u & 0x80000000u ? ~u : u | 0x80000000u, mine = (o & ~63u) | lane;
+    int rank = 0;
+#pragma unroll 16
+    for (int j = 0; j < 64; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)mine, j) > mine;
+    const float least = -wave_max(rank < (top + kWaves - 1) / kWaves ? -most : -INFINITY);
+    if (lane == 0) b.wave_value[threadIdx.x >> 6] = least;
+    __syncthreads();
+    return fminf(fminf(b.wave_value[0], b.wave_value[1]), fminf(b.wave_value[2], b.wave_value[3]));
+}
+
+// The largest value below v.
+__device__ __forceinline__ float just_below(float v) {
+    if (v == 0.f) return __uint_as_float(0x80000001u);
+    const uint32_t u = __float_as_uint(v);
+    return v == -INFINITY ? v : __uint_as_float(v > 0.f ? u - 1 : u + 1);
+}
+
+// Logits, 16 bytes a thread and vector, or segments' picks, as keys read from
+// memory: 0 where there is none, or none above `last`.
 template <class T>
 struct Logits {
     static constexpr int VE = 16 / sizeof(T);
     const T *from;
     unsigned e0, head, end, last_load;
+    float last;
     int vectors;
     struct Vec {
         u32x4 w;
@@ -199,149 +228,113 @@ struct Logits {
         const unsigned e = e0 + (kThreads * v + threadIdx.x) * VE;
         return Vec{*(const u32x4 *)(from + min(e, last_load)), e};
     }
-    __device__ bool ok(const Vec &v, int q) const { return v.e + q >= head && v.e + q < end; }
-    __device__ uint32_t id(const Vec &v, int q) const { return v.e + q - head; }
-    __device__ float value(const Vec &v, int q) const {
-        if constexpr (sizeof(T) == 4) return __uint_as_float(v.w[q]);
-        else return q & 1 ? bf16_hi(v.w[q >> 1]) : bf16_lo(v.w[q >> 1]);
+    __device__ uint64_t key(const Vec &v, int q) const {
+        float x;
+        if constexpr (sizeof(T) == 4) x = __uint_as_float(v.w[q]);
+        else x = q & 1 ? bf16_hi(v.w[q >> 1]) : bf16_lo(v.w[q >> 1]);
+        return v.e + q >= head && v.e + q < end && x > last ? key_of(x, v.e + q - head) : 0;
     }
 };
 struct Picks {
     static constexpr int VE = 1;
-    const uint64_t *key;
+    const uint64_t *picks;
     int n, vectors;
     typedef uint64_t Vec;
     __device__ Vec load(int v) const {
         const int e = kThreads * v + (int)threadIdx.x;
-        return e < n ? key[e] : 0;
+        return e < n ? picks[e] : 0;
     }
-    __device__ bool ok(Vec v, int) const { return v != 0; }
-    __device__ uint32_t id(Vec v, int) const { return key_id(v); }
-    __device__ float value(Vec v, int) const { return key_value(v); }
+    __device__ uint64_t key(Vec v, int) const { return v; }
 };
 
-__device__ __forceinline__ void best_settle(Best &b, int top, bool &full, float &last) {
-    best_prune(b, top);
-    full = b.count == top;
-    last = full ? key_value(b.key[top - 1]) : -INFINITY;
-}
-
-// Takes a chunk of which any number may belong to the best: those above `last`
-// while `full`, all otherwise. `most`: the thread's largest value of it.
+// Takes the keys of which there are too many for a bound to tell apart (ties):
+// the `top`-th largest by its digits, eight bits at a time, until those from it on
+// have room. Keys are unique, so that they do in the end.
 template <class Src>
-__device__ __forceinline__ void best_refill(Best &b, int top, bool &full, float &last, const Src &src, float most) {
-    constexpr int VE = Src::VE;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int held = b.count;
-    // At least `top` logits reach the smallest of the waves' (top / 4) largest
-    // thread maxima. (Ranked by their ordered bits, the lowest six the lane's, so
-    // that every lane has a rank of its own.)
-    {
-        most = most == most ? most : -INFINITY;  // (a signalling NaN came last)
-        const uint32_t u = __float_as_uint(most), o = u & 0x80000000u ? ~u : u | 0x80000000u;
-        const uint32_t mine = (o & ~63u) | lane;
-        int rank = 0;
-#pragma unroll 16
-        for (int j = 0; j < 64; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)mine, j) > mine;
-        const float least = -wave_max(rank < (top + kWaves - 1) / kWaves ? -most : -INFINITY);
-        if (lane == 0) b.wave_value[wave] = least;
-    }
-    __syncthreads();
-    const float from = fminf(fminf(b.wave_value[0], b.wave_value[1]), fminf(b.wave_value[2], b.wave_value[3]));
-    auto open = [&](float v) { return !full || v > last; };
-    // Every open logit from `from` on (`above`: only larger ones); the count may
-    // pass the room.
-    auto append = [&](bool above) {
+__device__ __forceinline__ void best_select(Best &b, int top, const Src &src) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, room = kRoom - b.count;
+    uint64_t prefix = 0, from = 0;
+    int need = top, taken = 0;
+    for (int shift = 56;; shift -= 8) {
+        __syncthreads();
+        b.hist[tid] = 0;
+        __syncthreads();
         for (int v = 0; v < src.vectors; ++v) {
             const auto w = src.load(v);
 #pragma unroll
-            for (int q = 0; q < VE; ++q) {
-                const float x = src.value(w, q);
-                if (src.ok(w, q) && open(x) && (above ? x > from : !(x < from))) {
-                    const int at = atomicAdd(&b.count, 1);
-                    if (at < kRoom) b.key[at] = key_of(x, src.id(w, q));
+            for (int q = 0; q < Src::VE; ++q) {
+                const uint64_t k = src.key(w, q);
+                const bool in = k && (shift == 56 || k >> (shift + 8) == prefix);
+                const int digit = (int)(k >> shift) & 255;
+                const uint64_t m = __ballot(in);
+                if (!m) continue;
+                const int first = __builtin_amdgcn_readlane(digit, __builtin_ctzll(m));
+                if (__ballot(in && digit != first) == 0) {  // one bin, as ties have
+                    if (lane == 0) atomicAdd(&b.hist[first], __builtin_popcountll(m));
+                } else if (in) {
+                    atomicAdd(&b.hist[digit], 1);
                 }
             }
         }
         __syncthreads();
-    };
-    auto back = [&]() {
+        // Keys with this thread's digit or a larger one.
+        const int h = b.hist[tid];
+        int sum = h;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int other = __shfl_down(sum, off, 64);
+            if (lane + off < 64) sum += other;
+        }
+        if (lane == 0) b.wave_total[wave] = sum;
         __syncthreads();
-        if (tid == 0) b.count = held;
+        for (int w = wave + 1; w < kWaves; ++w) sum += b.wave_total[w];
+        if (sum >= need && sum - h < need) {
+            b.found[0] = tid;
+            b.found[1] = sum - h;
+            b.found[2] = h;
+        }
         __syncthreads();
-    };
-    append(false);
-    if (b.count > kRoom) {
-        // Ties (a mask's, most likely): the larger ones, and the first `top` of those
-        // equal to `from`.
-        back();
-        append(true);
-        const int larger = b.count;
-        if (larger <= kRoom) {
-            auto tie = [&](const typename Src::Vec &w, int q) {
-                const float x = src.value(w, q);
-                return src.ok(w, q) && open(x) && !(x < from) && !(x > from);
-            };
-            int base = 0;
-            for (int v = 0; v < src.vectors && base < top; ++v) {
-                const auto w = src.load(v);
-                int n = 0, before = 0;
+        prefix = prefix << 8 | (uint64_t)b.found[0];
+        taken += b.found[1];
+        need -= b.found[1];
+        from = prefix << shift;
+        if (taken + b.found[2] <= room || shift == 0) break;
+    }
+    for (int v = 0; v < src.vectors; ++v) {
+        const auto w = src.load(v);
 #pragma unroll
-                for (int q = 0; q < VE; ++q) {
-                    const uint64_t m = __ballot(tie(w, q));
-                    n += __builtin_popcountll(m);
-                    before += __builtin_popcountll(m & ((1ull << lane) - 1));
-                }
-                if (lane == 0) b.ties[wave] = n;
-                __syncthreads();
-                int at = base + before;
-                for (int x = 0; x < kWaves; ++x) {
-                    if (x < wave) at += b.ties[x];
-                    base += b.ties[x];
-                }
-#pragma unroll
-                for (int q = 0; q < VE; ++q)
-                    if (tie(w, q)) {
-                        if (at < top) b.key[larger + at] = key_of(src.value(w, q), src.id(w, q));
-                        ++at;
-                    }
-                __syncthreads();
-            }
-            if (tid == 0) b.count = larger + min(base, top);
-            __syncthreads();
-        } else {
-            // Logits that rise with their ids: the best open one after the last, `top` times.
-            back();
-            uint64_t prev = ~0ull;
-            for (int r = 0; r < top; ++r) {
-                uint64_t k = 0;
-                for (int v = 0; v < src.vectors; ++v) {
-                    const auto w = src.load(v);
-#pragma unroll
-                    for (int q = 0; q < VE; ++q) {
-                        const float x = src.value(w, q);
-                        const uint64_t c = src.ok(w, q) && open(x) ? key_of(x, src.id(w, q)) : 0;
-                        if (c < prev && c > k) k = c;
-                    }
-                }
-#pragma unroll
-                for (int off = 32; off > 0; off >>= 1) {
-                    const uint64_t c = (uint64_t)__shfl_xor((unsigned long long)k, off, 64);
-                    k = c > k ? c : k;
-                }
-                __syncthreads();
-                if (lane == 0) b.wave_key[wave] = k;
-                __syncthreads();
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w) k = max(k, b.wave_key[w]);
-                if (k == 0) break;  // no more (the same in every thread)
-                if (tid == 0) b.key[b.count++] = k;
-                prev = k;
-            }
-            __syncthreads();
+        for (int q = 0; q < Src::VE; ++q) {
+            const uint64_t k = src.key(w, q);
+            if (k && k >= from) b.key[atomicAdd(&b.count, 1)] = k;
         }
     }
-    best_settle(b, top, full, last);
+    __syncthreads();
+}
+
+// The first of the row's logits without a probability, up to `top` alternatives.
+template <class T>
+__device__ __forceinline__ void fill_masked(Best &b, int top, const T *x, unsigned vocab) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int at = b.count;  // (no more change it)
+    for (unsigned i0 = 0; at < top && i0 < vocab; i0 += kThreads) {
+        const unsigned i = i0 + tid;
+        bool masked = false;
+        if (i < vocab) {
+            if constexpr (sizeof(T) == 4) masked = !(x[i] > -INFINITY);
+            else masked = !(bf16_f32(x[i]) > -INFINITY);
+        }
+        const uint64_t m = __ballot(masked);
+        __syncthreads();
+        if (lane == 0) b.wave_total[wave] = __builtin_popcountll(m);
+        __syncthreads();
+        int mine = at + __builtin_popcountll(m & ((1ull << lane) - 1));
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) mine += b.wave_total[w];
+            at += b.wave_total[w];
+        }
+        if (masked && mine < top) b.key[mine] = key_of(-INFINITY, i);
+    }
+    __syncthreads();
 }
 
 // One segment of a row, kThreads * PER logits at a time.
@@ -369,9 +362,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
     if (tid == 0) best.count = 0;
     __syncthreads();
     Sums s{0.0, 0.0, -INFINITY, 0};
-    bool full = false;
+    // A logit above `last` may be among the best. Waves hand theirs over as they
+    // go; the block looks at them after the first chunk and every kSettle-th, and
+    // takes the chunks since (from `since`) again where they had no room.
+    constexpr int kSettle = 4;
     float last = -INFINITY;
-    for (unsigned e0 = begin; e0 < end; e0 += CHUNK) {
+    unsigned since = begin;
+    int held = 0, chunk = 0;
+    for (unsigned e0 = begin; e0 < end; e0 += CHUNK, ++chunk) {
         float x[PER];
 #pragma unroll
         for (int v = 0; v < NV; ++v)
@@ -386,11 +384,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
             }
         if (e0 + CHUNK < end) load(e0 + CHUNK);
         auto at = [&](int i) { return e0 + (kThreads * (i / VE) + tid) * VE + i % VE; };
-        auto ok = [&](int i) { return at(i) >= head && at(i) < end; };
-        const bool whole = e0 >= head && e0 + CHUNK <= end;
-        if (!whole)
+        if (e0 < head || e0 + CHUNK > end)
 #pragma unroll
-            for (int i = 0; i < PER; ++i) x[i] = ok(i) ? x[i] : -INFINITY;
+            for (int i = 0; i < PER; ++i) x[i] = at(i) >= head && at(i) < end ? x[i] : -INFINITY;
         float most = -INFINITY;
 #pragma unroll
         for (int i = 0; i < PER; ++i) most = fmaxf(most, x[i]);
@@ -406,29 +402,32 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
         }
         s.S += S;
         s.A += A;
-        if (a.top && __syncthreads_or(!full || most > last)) {
-            const Logits<T> src{from, e0, head, end, last_load, (int)((min(end - e0, CHUNK) + kThreads * VE - 1) / (kThreads * VE))};
-            if (full) {  // few: straight from the registers
-                const int held = best.count;
-                __syncthreads();
+        if (!a.top) continue;
+        float above = last;
+        if (chunk == 0) above = just_below(best_bound(best, a.top, most));  // all of them would be too many
+        if (__any(most > above))
 #pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    if (x[i] > last) {  // (never a logit that is not ok: -inf)
-                        const int k = atomicAdd(&best.count, 1);
-                        if (k < kRoom) best.key[k] = key_of(x[i], at(i) - head);
-                    }
-                __syncthreads();
-                const int n = best.count;
-                if (n <= kRoom) {
-                    if (n >= a.top + 64) best_settle(best, a.top, full, last);
-                    continue;
+            for (int i = 0; i < PER; ++i)
+                if (x[i] > above) {
+                    const int k = atomicAdd(&best.count, 1);
+                    if (k < kRoom) best.key[k] = key_of(x[i], at(i) - head);
                 }
-                __syncthreads();
+        if (chunk % kSettle == 0 || e0 + CHUNK >= end) {
+            __syncthreads();
+            const int n = best.count;
+            __syncthreads();  // the same in every wave, before one goes on
+            if (n > kRoom) {
+                // Ties, or logits that rise with their ids.
                 if (tid == 0) best.count = held;
                 __syncthreads();
-                best_settle(best, a.top, full, last);
+                const unsigned upto = min(end, e0 + CHUNK);
+                const Logits<T> src{from, since, head, upto, last_load, last, (int)((upto - since + kThreads * VE - 1) / (kThreads * VE))};
+                best_select(best, a.top, src);
             }
-            best_refill(best, a.top, full, last, src, most);
+            if (n >= a.top + 64 || chunk == 0 || e0 + CHUNK >= end) {
+                held = best_settle(best, a.top, last);
+                since = e0 + CHUNK;
+            }
         }
     }
     // The block's sums.
@@ -449,17 +448,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
         all_waves.A += u.A;
         all_waves.c += u.c;
     }
-    if (a.top && best.count > a.top) {  // candidates left
-        __syncthreads();
-        best_prune(best, a.top);
-    }
     if (a.segs == 1) {
+        if (held < a.top) fill_masked(best, a.top, x_row, a.vocab);
         store_row(a, x_row, row, all_waves, best.key);
         return;
     }
     const size_t at = row * a.segs + seg;
     if (tid == 0) a.sums[at] = all_waves;
-    if (tid < a.top) a.picks[at * a.top + tid] = tid < best.count ? best.key[tid] : 0;
+    if (tid < a.top) a.picks[(row * a.top + tid) * a.segs + seg] = tid < held ? best.key[tid] : 0;
 }
 
 // The segments of a row.
@@ -487,9 +483,24 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a) 
     s.A += s2.A;
     s.c += s2.c;
     if (a.top) {
-        bool full = false;
-        float last = -INFINITY;
-        best_refill(best, a.top, full, last, src, most);
+        const float from = best_bound(best, a.top, most);
+        for (int v = 0; v < src.vectors; ++v) {
+            const uint64_t k = src.load(v);
+            if (k && key_value(k) >= from) {
+                const int i = atomicAdd(&best.count, 1);
+                if (i < kRoom) best.key[i] = k;
+            }
+        }
+        __syncthreads();
+        const bool many = best.count > kRoom;
+        __syncthreads();
+        if (many) {
+            if (tid == 0) best.count = 0;
+            __syncthreads();
+            best_select(best, a.top, src);
+        }
+        float last;
+        if (best_settle(best, a.top, last) < a.top) fill_masked(best, a.top, (const T *)a.x + row * a.stride, a.vocab);
     }
     store_row(a, (const T *)a.x + row * a.stride, row, s, best.key);
 }
