@@ -8,7 +8,7 @@
 // One pass over the logits. A row is cut into segments, a block each
 // (logprobs_kernel); a block walks its segment in chunks that sit in registers,
 // each thread with its own running maximum and sums (f32 over a chunk's at most
-// 32 logits, in 64 bits from chunk to chunk), the block with the best `top`
+// 16 logits, in 64 bits from chunk to chunk), the block with the best `top`
 // logits so far. A logit joins those only if it is larger than the last of them
 // (ids rise, so an equal one loses), which is rare after the first chunk. Few
 // rows have many segments, joined by logprobs_join_kernel; many rows have one
@@ -25,6 +25,10 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kCap = 512;       // candidates a block holds beside its best
 constexpr int kMaxSegs = 128;   // two a lane of the join's waves
 constexpr float kLog2e = 1.44269504088896340736f;
+
+// Block barrier that waits on LDS traffic only: the next chunk's loads stay in
+// flight across it.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // A row's sums over a part of it: the maximum, the logits equal to it, the sum
 // over the others, the sum of the entropy's terms.
@@ -158,7 +162,7 @@ __device__ __forceinline__ void best_rank(Best &b, int top, int n) {
         rank[i] = 0;
     }
     if (tid < 8) b.key[n + tid] = 0;  // above no key
-    __syncthreads();
+    lds_barrier();
     if (R > 1 || tid < (n + 63) / 64 * 64)
         for (int j = 0; j < n; j += 8) {
             uint64_t k[8];
@@ -169,12 +173,12 @@ __device__ __forceinline__ void best_rank(Best &b, int top, int n) {
 #pragma unroll
                 for (int i = 0; i < R; ++i) rank[i] += k[q] > mine[i];
         }
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int i = 0; i < R; ++i)
         if (tid + kThreads * i < n && rank[i] < top) b.key[rank[i]] = mine[i];
     if (tid == 0) b.count = min(n, top);
-    __syncthreads();
+    lds_barrier();
 }
 
 // Prunes to the best `top`, says above what a logit would join them and how many
@@ -200,7 +204,7 @@ __device__ __forceinline__ float best_bound(Best &b, int top, float most) {
     for (int j = 0; j < 64; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)mine, j) > mine;
     const float least = -wave_max(rank < (top + kWaves - 1) / kWaves ? -most : -INFINITY);
     if (lane == 0) b.wave_value[threadIdx.x >> 6] = least;
-    __syncthreads();
+    lds_barrier();
     return fminf(fminf(b.wave_value[0], b.wave_value[1]), fminf(b.wave_value[2], b.wave_value[3]));
 }
 
@@ -256,9 +260,9 @@ __device__ __forceinline__ void best_select(Best &b, int top, const Src &src) {
     uint64_t prefix = 0, from = 0;
     int need = top, taken = 0;
     for (int shift = 56;; shift -= 8) {
-        __syncthreads();
+        lds_barrier();
         b.hist[tid] = 0;
-        __syncthreads();
+        lds_barrier();
         for (int v = 0; v < src.vectors; ++v) {
             const auto w = src.load(v);
 #pragma unroll
@@ -276,7 +280,7 @@ __device__ __forceinline__ void best_select(Best &b, int top, const Src &src) {
                 }
             }
         }
-        __syncthreads();
+        lds_barrier();
         // Keys with this thread's digit or a larger one.
         const int h = b.hist[tid];
         int sum = h;
@@ -286,14 +290,14 @@ __device__ __forceinline__ void best_select(Best &b, int top, const Src &src) {
             if (lane + off < 64) sum += other;
         }
         if (lane == 0) b.wave_total[wave] = sum;
-        __syncthreads();
+        lds_barrier();
         for (int w = wave + 1; w < kWaves; ++w) sum += b.wave_total[w];
         if (sum >= need && sum - h < need) {
             b.found[0] = tid;
             b.found[1] = sum - h;
             b.found[2] = h;
         }
-        __syncthreads();
+        lds_barrier();
         prefix = prefix << 8 | (uint64_t)b.found[0];
         taken += b.found[1];
         need -= b.found[1];
@@ -308,7 +312,7 @@ __device__ __forceinline__ void best_select(Best &b, int top, const Src &src) {
             if (k && k >= from) b.key[atomicAdd(&b.count, 1)] = k;
         }
     }
-    __syncthreads();
+    lds_barrier();
 }
 
 // The first of the row's logits without a probability, up to `top` alternatives.
@@ -324,9 +328,9 @@ __device__ __forceinline__ void fill_masked(Best &b, int top, const T *x, unsign
             else masked = !(bf16_f32(x[i]) > -INFINITY);
         }
         const uint64_t m = __ballot(masked);
-        __syncthreads();
+        lds_barrier();
         if (lane == 0) b.wave_total[wave] = __builtin_popcountll(m);
-        __syncthreads();
+        lds_barrier();
         int mine = at + __builtin_popcountll(m & ((1ull << lane) - 1));
         for (int w = 0; w < kWaves; ++w) {
             if (w < wave) mine += b.wave_total[w];
@@ -334,7 +338,7 @@ __device__ __forceinline__ void fill_masked(Best &b, int top, const T *x, unsign
         }
         if (masked && mine < top) b.key[mine] = key_of(-INFINITY, i);
     }
-    __syncthreads();
+    lds_barrier();
 }
 
 // One segment of a row, kThreads * PER logits at a time.
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
     };
     load(begin);
     if (tid == 0) best.count = 0;
-    __syncthreads();
+    lds_barrier();
     Sums s{0.0, 0.0, -INFINITY, 0};
     // A logit above `last` may be among the best. Waves hand theirs over as they
     // go; the block looks at them after the first chunk and every kSettle-th, and
@@ -413,13 +417,13 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
                     if (k < kRoom) best.key[k] = key_of(x[i], at(i) - head);
                 }
         if (chunk % kSettle == 0 || e0 + CHUNK >= end) {
-            __syncthreads();
+            lds_barrier();
             const int n = best.count;
-            __syncthreads();  // the same in every wave, before one goes on
+            lds_barrier();  // the same in every wave, before one goes on
             if (n > kRoom) {
                 // Ties, or logits that rise with their ids.
                 if (tid == 0) best.count = held;
-                __syncthreads();
+                lds_barrier();
                 const unsigned upto = min(end, e0 + CHUNK);
                 const Logits<T> src{from, since, head, upto, last_load, last, (int)((upto - since + kThreads * VE - 1) / (kThreads * VE))};
                 best_select(best, a.top, src);
@@ -434,7 +438,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
     const float wm = wave_max(s.m);
     const Sums t = wave_join(s, wm);
     if (lane == 0) part[wave] = t;
-    __syncthreads();
+    lds_barrier();
     Sums all_waves = part[0];
     float m = all_waves.m;
 #pragma unroll
@@ -475,7 +479,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a) 
         most = fmaxf(most, k ? key_value(k) : -INFINITY);
     }
     if (tid == 0) best.count = 0;
-    __syncthreads();
+    lds_barrier();
     const float m = wave_max(fmaxf(s.m, s2.m));
     s = wave_join(s, m);
     s2 = wave_join(s2, m);
@@ -491,12 +495,12 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a) 
                 if (i < kRoom) best.key[i] = k;
             }
         }
-        __syncthreads();
+        lds_barrier();
         const bool many = best.count > kRoom;
-        __syncthreads();
+        lds_barrier();
         if (many) {
             if (tid == 0) best.count = 0;
-            __syncthreads();
+            lds_barrier();
             best_select(best, a.top, src);
         }
         float last;
@@ -518,7 +522,7 @@ int launch_logprobs_t(const LogprobJob &j, LogprobArgs &a, hipStream_t s) {
     if (a.seg <= (unsigned)(8 * kThreads))
         hipLaunchKernelGGL((logprobs_kernel<T, 8>), dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
     else
-        hipLaunchKernelGGL((logprobs_kernel<T, 32>), dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL((logprobs_kernel<T, 16>), dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
     CHIP_CHECK(hipGetLastError());
     if (a.segs == 1) return 0;
     hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3((unsigned)j.rows), dim3(kThreads), 0, s, a);
