@@ -158,10 +158,12 @@ int qkv_perm_row(int stored_row, int q_heads, int kv_heads, int head_dim, int ro
 // sums ws[nchunks][rows][q_dim + 2*kv_dim] folded as the GEMM folds them (the
 // first ceil(n / 2) in order, the rest in order, the two added), times sc (if
 // set), plus bias (if set) - the GEMM epilogue's arithmetic; qkv is unused.
+// angles (device [rows], optional): row i is rotated for position angles[i]
+// and still appended at pos0 + i (a tree's nodes: depths, and slots in order).
 int launch_rope_append(const float *qkv, float *qrot, size_t rows, int q_heads, const KvGeom &g, const KvLayer &kv,
                        const float *rope_cos, const float *rope_sin, int rotary_dim, size_t offset,
                        const int32_t *pos_dev, hipStream_t s, const float *ws = nullptr, int nchunks = 0,
-                       const float *sc = nullptr, const float *bias = nullptr);
+                       const float *sc = nullptr, const float *bias = nullptr, const int32_t *angles = nullptr);
 
 // dst[r][:] = src[map[r]][:] for rows of row_bytes bytes (load-time layout).
 int launch_gather_rows(const uint8_t *src, uint8_t *dst, const int32_t *map, size_t rows, size_t row_bytes,
@@ -283,7 +285,10 @@ int launch_logprobs(const LogprobJob &job, hipStream_t s);
 // it in step[0] and advances step[1] by one.
 int launch_argmax(const float *logits, size_t n, uint32_t *out_token, int32_t *step, uint32_t *hist,
                   size_t hist_cap, void *scratch, hipStream_t s);
-size_t argmax_scratch_bytes();
+size_t argmax_scratch_bytes(size_t rows = 1);
+// The same argmax of each of `rows` rows of n logits; scratch holds
+// argmax_scratch_bytes(rows).
+int launch_argmax_rows(const float *logits, size_t n, size_t rows, uint32_t *out_tokens, void *scratch, hipStream_t s);
 
 // step[0] = token, step[1] = pos, in stream order.
 int launch_set_step(int32_t *step, int32_t token, int32_t pos, hipStream_t s);

@@ -235,6 +235,7 @@ __global__ __launch_bounds__(kThreads) void rope_append_kernel(const float *__re
                                                                const int32_t *__restrict__ page_table, int page_size,
                                                                KT *__restrict__ kc, KT *__restrict__ vc, long offset,
                                                                const int32_t *__restrict__ pos_dev,
+                                                               const int32_t *__restrict__ angles,
                                                                const float *__restrict__ ws, int nchunks,
                                                                const float *__restrict__ sc,
                                                                const float *__restrict__ bias) {
@@ -263,8 +264,9 @@ __global__ __launch_bounds__(kThreads) void rope_append_kernel(const float *__re
         }
     };
     const int half = rotary_dim / 2;
-    const float *cr = cos_t + (size_t)pos * half;
-    const float *sr = sin_t + (size_t)pos * half;
+    const long angle = angles ? (long)angles[row] : pos;
+    const float *cr = cos_t + (size_t)angle * half;
+    const float *sr = sin_t + (size_t)angle * half;
     // rope_elem's arithmetic on element d of the head starting at column base.
     auto rot = [&](int base, int d) -> float {
         if (d >= rotary_dim) return val(base + d);
@@ -330,7 +332,11 @@ __device__ __forceinline__ void block_argmax(int &key, uint32_t &idx) {
 
 constexpr int kArgmaxBlocks = 64;
 
+// blockIdx.y is the row of n logits.
 __global__ __launch_bounds__(kThreads) void argmax_partial_kernel(const float *x, int n, int *pkey, uint32_t *pidx) {
+    x += (size_t)blockIdx.y * n;
+    pkey += (size_t)blockIdx.y * gridDim.x;
+    pidx += (size_t)blockIdx.y * gridDim.x;
     int key = INT_MIN;
     uint32_t idx = 0;
     for (int i = blockIdx.x * kThreads + threadIdx.x; i < n; i += gridDim.x * kThreads)
@@ -342,15 +348,18 @@ __global__ __launch_bounds__(kThreads) void argmax_partial_kernel(const float *x
     }
 }
 
+// blockIdx.x is the row; step and hist are a single row's.
 __global__ __launch_bounds__(kThreads) void argmax_final_kernel(const int *pkey, const uint32_t *pidx, int parts,
                                                                 uint32_t *out, int32_t *step, uint32_t *hist,
                                                                 long hist_cap) {
+    pkey += (size_t)blockIdx.x * parts;
+    pidx += (size_t)blockIdx.x * parts;
     int key = INT_MIN;
     uint32_t idx = 0;
     for (int i = threadIdx.x; i < parts; i += kThreads) better(key, idx, pkey[i], pidx[i]);
     block_argmax(key, idx);
     if (threadIdx.x == 0) {
-        if (out) *out = idx;
+        if (out) out[blockIdx.x] = idx;
         if (step) {
             const long next = (long)step[1] + 1;
             if (hist && next < hist_cap) hist[next] = idx;
@@ -458,7 +467,7 @@ int qkv_perm_row(int stored, int q_heads, int kv_heads, int head_dim, int rotary
 int launch_rope_append(const float *qkv, float *qrot, size_t rows, int q_heads, const KvGeom &g, const KvLayer &kv,
                        const float *rope_cos, const float *rope_sin, int rotary_dim, size_t offset,
                        const int32_t *pos_dev, hipStream_t s, const float *ws, int nchunks, const float *sc,
-                       const float *bias) {
+                       const float *bias, const int32_t *angles) {
     if (rows == 0) return 0;
     if (rotary_dim <= 0 || rotary_dim > g.head_dim || rotary_dim % 2)
         return fail("HIP backend: rotary_dim must be even and at most head_dim.");
@@ -469,7 +478,7 @@ int launch_rope_append(const float *qkv, float *qrot, size_t rows, int q_heads, 
 #define CHIP_ROPE(KT, SUM)                                                                                      \
     hipLaunchKernelGGL((rope_append_kernel<KT, SUM>), grid, dim3(kThreads), 0, s, qkv, qrot, q_heads, g.kv_heads, \
                        g.head_dim, rotary_dim, rope_cos, rope_sin, g.page_table, g.page_size, (KT *)kv.k,         \
-                       (KT *)kv.v, (long)offset, pos_dev, ws, nchunks, sc, bias)
+                       (KT *)kv.v, (long)offset, pos_dev, angles, ws, nchunks, sc, bias)
     if (g.kv_f32) {
         if (nchunks > 0) CHIP_ROPE(float, true);
         else CHIP_ROPE(float, false);
@@ -490,7 +499,7 @@ int launch_gather_rows(const uint8_t *src, uint8_t *dst, const int32_t *map, siz
     return 0;
 }
 
-size_t argmax_scratch_bytes() { return kArgmaxBlocks * (sizeof(int) + sizeof(uint32_t)); }
+size_t argmax_scratch_bytes(size_t rows) { return rows * kArgmaxBlocks * (sizeof(int) + sizeof(uint32_t)); }
 
 int launch_argmax(const float *logits, size_t n, uint32_t *out_token, int32_t *step, uint32_t *hist,
                   size_t hist_cap, void *scratch, hipStream_t s) {
@@ -501,6 +510,20 @@ int launch_argmax(const float *logits, size_t n, uint32_t *out_token, int32_t *s
     CHIP_CHECK(hipGetLastError());
     hipLaunchKernelGGL(argmax_final_kernel, dim3(1), dim3(kThreads), 0, s, (const int *)pkey, (const uint32_t *)pidx,
                        kArgmaxBlocks, out_token, step, hist, (long)hist_cap);
+    CHIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+int launch_argmax_rows(const float *logits, size_t n, size_t rows, uint32_t *out_tokens, void *scratch, hipStream_t s) {
+    if (n == 0 || n > (size_t)INT32_MAX || rows == 0 || rows > 65535)
+        return fail("HIP backend: argmax over empty or oversized rows.");
+    int *pkey = (int *)scratch;
+    uint32_t *pidx = (uint32_t *)(pkey + rows * kArgmaxBlocks);
+    hipLaunchKernelGGL(argmax_partial_kernel, dim3(kArgmaxBlocks, (unsigned)rows), dim3(kThreads), 0, s, logits, (int)n,
+                       pkey, pidx);
+    CHIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL(argmax_final_kernel, dim3((unsigned)rows), dim3(kThreads), 0, s, (const int *)pkey,
+                       (const uint32_t *)pidx, kArgmaxBlocks, out_tokens, nullptr, nullptr, 0L);
     CHIP_CHECK(hipGetLastError());
     return 0;
 }

@@ -19,10 +19,17 @@
 // residual}, LM head GEMV with fused final norm, argmax. The token and
 // position live in device memory, so the same graph replays every step and
 // the greedy loop can run back to back with no host round trip.
+//
+// Drafted tokens: forward_tree runs a tree of candidates as one chunk (K/V of
+// node i in slot len + i, rotated for position len + depth, the layers'
+// attention along the tree's branches, the LM head over every row) and leaves
+// the cached length alone; commit_tree moves the accepted branch's rows to the
+// front of those slots and lengthens the cache by it.
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -236,6 +243,20 @@ struct cheetah_hip_model {
     unsigned slot_epoch[2] = {};
     hipEvent_t ready[2] = {}, released[2] = {};
     Layer fed[2];
+    // Every row's logits of a tree or of a scored chunk, and the attention
+    // partials of a tree (both grown on demand).
+    float *row_logits = nullptr, *tree_part = nullptr;
+    size_t row_logits_floats = 0, tree_part_floats = 0;
+    // The tree whose nodes' K/V rows are at positions [len, len + tree_n); 0:
+    // none. Pinned staging and its device copy: tokens, parents, rotation
+    // positions, then the nodes' argmaxes (kMaxTreeNodes words each).
+    size_t tree_n = 0;
+    int32_t *tree_host = nullptr, *tree_dev = nullptr;
+    void *row_scratch = nullptr;  // argmax over kMaxTreeNodes rows
+    // Scored chunks: the targets and results of a call, the segments' sums.
+    uint32_t *score_dev = nullptr;
+    uint8_t *score_ws = nullptr;
+    size_t score_words = 0, score_ws_bytes = 0;
 
     ~cheetah_hip_model() {
         if (stream) (void)hipStreamSynchronize(stream);
@@ -252,6 +273,7 @@ struct cheetah_hip_model {
         if (stream) (void)hipStreamDestroy(stream);
         if (words_host) (void)hipHostFree(words_host);
         if (tokens_host) (void)hipHostFree(tokens_host);
+        if (tree_host) (void)hipHostFree(tree_host);
         if (logits_host) (void)hipHostFree(logits_host);
         for (int p : pages) sh->page_unref(p);
     }
@@ -708,6 +730,10 @@ int init_instance(cheetah_hip_model *m) {
     CHIP_CHECK(hipHostMalloc((void **)&m->logits_host, (size_t)c.vocab_size * sizeof(float), hipHostMallocDefault));
     CHIP_CHECK(hipHostGetDevicePointer((void **)&m->logits_out, m->logits_host, 0));
     m->page_host.assign(sh.num_pages, 0);
+    CHIP_CHECK(hipHostMalloc((void **)&m->tree_host, 4 * kMaxTreeNodes * sizeof(int32_t), hipHostMallocDefault));
+    CHIP_TRY(m->mem.alloc(&m->tree_dev, 4 * kMaxTreeNodes));
+    CHIP_TRY(m->mem.alloc(&scratch, argmax_scratch_bytes(kMaxTreeNodes)));
+    m->row_scratch = scratch;
     return init_fused(m);
 }
 
@@ -984,9 +1010,30 @@ int launch_decode(cheetah_hip_model *m, size_t pos, bool sample) {
     return 0;
 }
 
-// One prefill chunk of `rows` tokens at absolute position `pos`.
-// tokens_dev holds the chunk's ids (already on the device).
-int enqueue_chunk(cheetah_hip_model *m, const uint32_t *tokens_dev, size_t rows, size_t pos, bool last_chunk) {
+// A chunk's rows as a tree's nodes (device arrays): parents and the positions
+// they are rotated for.
+struct TreeRows {
+    const int32_t *parents, *angles;
+};
+
+// `tree` (with tree_part large enough) in slots pos .. pos + rows - 1.
+TreeJob tree_job(const cheetah_hip_model *m, const TreeRows &tree, size_t rows, size_t pos) {
+    TreeJob tj;
+    tj.q = m->qrot;
+    tj.g = geom(m);
+    tj.q_heads = (int)C(m).q_heads;
+    tj.parents = tree.parents;
+    tj.n = rows;
+    tj.offset = pos;
+    tj.part = m->tree_part;
+    tj.part_floats = m->tree_part_floats;
+    return tj;
+}
+
+// One prefill chunk of `rows` tokens at absolute position `pos`, or the nodes
+// of a tree there. tokens_dev holds the chunk's ids (already on the device).
+int enqueue_chunk(cheetah_hip_model *m, const uint32_t *tokens_dev, size_t rows, size_t pos, bool last_chunk,
+                  const TreeRows *tree = nullptr) {
     Shared &sh = *m->sh;
     const auto &c = sh.cfg;
     hipStream_t s = m->stream;
@@ -1028,28 +1075,38 @@ int enqueue_chunk(cheetah_hip_model *m, const uint32_t *tokens_dev, size_t rows,
         CHIP_TRY(launch_gemm(qkv, s));
         CHIP_TRY(launch_rope_append(m->qkv, m->qrot, rows, (int)c.q_heads, geom(m), L.kv, sh.rope_cos, sh.rope_sin,
                                     (int)c.rotary_dim, pos, nullptr, s, m->gemm_ws, qkv_chunks, L.qkv.scales(),
-                                    L.qkv_bias));
-        AttnJob aj;
-        aj.q = m->qrot;
-        aj.q_stride = sh.q_dim();
-        aj.out = attn;
-        aj.k = L.kv.k;
-        aj.v = L.kv.v;
-        aj.g = geom(m);
-        aj.q_heads = (int)c.q_heads;
-        aj.rows = rows;
-        aj.offset = pos;
-        aj.part = m->part;
-        aj.part_floats = m->part_floats;
-        aj.prefill = true;
-        // Absolute spans of positions, fixed per model: a position's attention
-        // output does not depend on how the prompt was cut into chunks (KV
-        // continuation stays bit-exact, decoder.rs:1710-1728).
-        aj.span = attention_prefill_span(sh.kv_capacity, sh.kv_f32 != 0);
-        // The prefill attention writes the o_proj input halves itself.
-        aj.out_hi = m->xh;
-        aj.out_lo = m->xl;
-        CHIP_TRY(launch_attention(aj, s));
+                                    L.qkv_bias, tree ? tree->angles : nullptr));
+        // Either attention writes the o_proj input halves itself.
+        if (tree) {
+            TreeJob tj = tree_job(m, *tree, rows, pos);
+            tj.out = attn;
+            tj.k = L.kv.k;
+            tj.v = L.kv.v;
+            tj.out_hi = m->xh;
+            tj.out_lo = m->xl;
+            CHIP_TRY(launch_tree_attention(tj, s));
+        } else {
+            AttnJob aj;
+            aj.q = m->qrot;
+            aj.q_stride = sh.q_dim();
+            aj.out = attn;
+            aj.k = L.kv.k;
+            aj.v = L.kv.v;
+            aj.g = geom(m);
+            aj.q_heads = (int)c.q_heads;
+            aj.rows = rows;
+            aj.offset = pos;
+            aj.part = m->part;
+            aj.part_floats = m->part_floats;
+            aj.prefill = true;
+            // Absolute spans of positions, fixed per model: a position's attention
+            // output does not depend on how the prompt was cut into chunks (KV
+            // continuation stays bit-exact, decoder.rs:1710-1728).
+            aj.span = attention_prefill_span(sh.kv_capacity, sh.kv_f32 != 0);
+            aj.out_hi = m->xh;
+            aj.out_lo = m->xl;
+            CHIP_TRY(launch_attention(aj, s));
+        }
         GemmJob o;
         o.w = L.o;
         o.x = attn;
@@ -1119,6 +1176,51 @@ int enqueue_chunk(cheetah_hip_model *m, const uint32_t *tokens_dev, size_t rows,
     return 0;
 }
 
+// The logits of `rows` of the chunk's hidden rows from `first` on, into
+// row_logits [rows][vocab]: the final norm and the LM head as a GEMM.
+int enqueue_head_rows(cheetah_hip_model *m, size_t first, size_t rows) {
+    Shared &sh = *m->sh;
+    const auto &c = sh.cfg;
+    const size_t H = c.hidden_size;
+    float *normed = gemm_takes_halves(H) ? nullptr : m->normed;
+    CHIP_TRY(launch_rmsnorm_rows(m->hidden + first * H, sh.final_norm, c.rms_eps, rows, H, normed, m->stream, m->xh,
+                                 m->xl));
+    GemmJob head;
+    head.w = sh.head;
+    head.x = normed;
+    head.n = rows;
+    head.y = m->row_logits;
+    head.ws = m->gemm_ws;
+    head.ws_floats = m->gemm_ws_floats;
+    head.xh = m->xh;
+    head.xl = m->xl;
+    return launch_gemm(head, m->stream);
+}
+
+// A buffer of at least `need` elements: replaced by a larger one once the
+// stream has done with it.
+template <class T>
+int grow(cheetah_hip_model *m, T **p, size_t *have, size_t need) {
+    if (need <= *have) return 0;
+    CHIP_CHECK(hipStreamSynchronize(m->stream));
+    if (*p) m->mem.release(*p);
+    *p = nullptr;
+    *have = 0;
+    CHIP_TRY(m->mem.alloc(p, need));
+    *have = need;
+    return 0;
+}
+
+// A call whose host containers may run out of memory, at the C boundary.
+template <class F>
+int guarded(F call) {
+    try {
+        return call();
+    } catch (const std::exception &) {
+        return fail("HIP backend: out of host memory.");
+    }
+}
+
 int check_model(const cheetah_hip_model *m) {
     if (!m) return fail("HIP backend: no model.");
     if (!m->sh->finalized) return fail("HIP backend: model not finalized; call cheetah_hip_model_finalize.");
@@ -1158,6 +1260,7 @@ int run_forward(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t o
     CHIP_TRY(refresh_weights(m));
     if (chunk_rows == 0) chunk_rows = 256;
     chunk_rows = std::min(chunk_rows, m->sh->max_chunk);
+    m->tree_n = 0;
     CHIP_TRY(reserve_positions(m, n));
     if (n == 1) {
         CHIP_TRY(launch_set_step(m->step_dev, (int32_t)tokens[0], (int32_t)offset, m->stream));
@@ -1182,6 +1285,142 @@ int run_forward(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t o
     }
     CHIP_TRY(launch_export(want_logits ? m->logits : nullptr, C(m).vocab_size, m->logits_out, m->next_dev, nullptr,
                            m->words_out, m->stream));
+    CHIP_CHECK(hipStreamSynchronize(m->stream));
+    m->len = offset + n;
+    return 0;
+}
+
+// Runs a tree's nodes behind the cached positions and waits: their K/V rows
+// in slots [offset, offset + n), their logits in row_logits, with `sample` their
+// argmaxes in the fourth row of tree_host. The tree is then the pending one.
+int run_tree(cheetah_hip_model *m, const uint32_t *tokens, const int32_t *parents, size_t n, size_t offset,
+             bool sample) {
+    CHIP_TRY(check_model(m));
+    if (n > (size_t)kMaxTreeNodes || (n && n > m->sh->max_chunk))
+        return fail("HIP backend: a tree has at most " + std::to_string(kMaxTreeNodes) +
+                    " nodes, and at most the model's chunk rows.");
+    CHIP_TRY(validate(m, tokens, n, offset));
+    if (!parents) return fail("HIP backend: null parents pointer.");
+    for (size_t i = 0; i < n; ++i)
+        if (parents[i] < -1 || parents[i] >= (long)i)
+            return fail("HIP backend: a node's parent comes before it (-1: a child of the cached text).");
+    CHIP_TRY(refresh_weights(m));
+    m->tree_n = 0;
+    CHIP_TRY(grow(m, &m->row_logits, &m->row_logits_floats, n * C(m).vocab_size));
+    CHIP_TRY(reserve_positions(m, n));
+    CHIP_CHECK(hipStreamSynchronize(m->stream));  // tree_host reuse
+    constexpr size_t N = kMaxTreeNodes;
+    int32_t *host = m->tree_host, *dev = m->tree_dev;
+    for (size_t i = 0; i < n; ++i) {
+        host[i] = (int32_t)tokens[i];
+        host[N + i] = parents[i];
+        host[2 * N + i] = parents[i] < 0 ? (int32_t)offset : host[2 * N + parents[i]] + 1;
+    }
+    CHIP_CHECK(hipMemcpyAsync(dev, host, 3 * N * sizeof(int32_t), hipMemcpyHostToDevice, m->stream));
+    const TreeRows tree{dev + N, dev + 2 * N};
+    const int splits = tree_attention_splits(tree_job(m, tree, n, offset));
+    CHIP_TRY(grow(m, &m->tree_part, &m->tree_part_floats,
+                  attention_part_floats(n, (int)C(m).q_heads, splits, (int)C(m).head_dim)));
+    CHIP_TRY(enqueue_chunk(m, (const uint32_t *)dev, n, offset, false, &tree));
+    CHIP_TRY(enqueue_head_rows(m, 0, n));
+    if (sample) {
+        CHIP_TRY(launch_argmax_rows(m->row_logits, C(m).vocab_size, n, (uint32_t *)(dev + 3 * N), m->row_scratch,
+                                    m->stream));
+        CHIP_CHECK(hipMemcpyAsync(host + 3 * N, dev + 3 * N, n * sizeof(int32_t), hipMemcpyDeviceToHost, m->stream));
+    }
+    CHIP_CHECK(hipStreamSynchronize(m->stream));
+    m->tree_n = n;
+    return 0;
+}
+
+// Keeps a branch of the pending tree (checked): its rows move behind the
+// cached positions, the rest of the tree is dropped.
+int keep_branch(cheetah_hip_model *m, const uint32_t *nodes, size_t count) {
+    Shared &sh = *m->sh;
+    if (count) {
+        // A page that a snapshot taken since shares is copied before its rows move.
+        CHIP_TRY(reserve_positions(m, m->tree_n));
+        KvLayer layers[kCommitViews];
+        const int32_t *tables[kCommitViews];
+        for (int i = 0; i < kCommitViews; ++i) tables[i] = m->page_dev;
+        for (size_t l0 = 0; l0 < sh.layers.size(); l0 += kCommitViews) {
+            const size_t views = std::min(sh.layers.size() - l0, (size_t)kCommitViews);
+            for (size_t i = 0; i < views; ++i) layers[i] = sh.layers[l0 + i].kv;
+            CHIP_TRY(launch_tree_commit(layers, tables, views, geom(m), m->len, nodes, count, m->stream));
+        }
+        CHIP_CHECK(hipStreamSynchronize(m->stream));
+    }
+    m->len += count;
+    m->tree_n = 0;
+    return 0;
+}
+
+// Prefill that also scores every position (run_forward's chunks, the LM head
+// over all of their rows).
+int run_scored(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t offset, size_t chunk_rows,
+               const uint32_t *targets, uint32_t top, float *logprobs, float *entropy, uint32_t *top_ids,
+               float *top_logprobs) {
+    CHIP_TRY(check_model(m));
+    CHIP_TRY(validate(m, tokens, n, offset));
+    if (top > (uint32_t)kMaxTop || top > C(m).vocab_size)
+        return fail("HIP backend: logprobs returns at most " + std::to_string(kMaxTop) +
+                    " alternatives, and at most the vocabulary.");
+    if (!logprobs && !entropy && !top) return fail("HIP backend: logprobs without an output.");
+    if (logprobs && !targets) return fail("HIP backend: logprobs of tokens needs the tokens.");
+    if ((top != 0) != (top_ids != nullptr) || (top != 0) != (top_logprobs != nullptr))
+        return fail("HIP backend: logprobs needs ids and log probabilities of the alternatives, or none.");
+    CHIP_TRY(refresh_weights(m));
+    if (chunk_rows == 0) chunk_rows = 256;
+    chunk_rows = std::min(chunk_rows, m->sh->max_chunk);
+    // Rows whose logits are held at once: enough for the LM head's products to
+    // be bound by the matrix cores.
+    const size_t V = C(m).vocab_size, group = std::min({n, chunk_rows, (size_t)256});
+    m->tree_n = 0;
+    CHIP_TRY(grow(m, &m->row_logits, &m->row_logits_floats, group * V));
+    CHIP_TRY(grow(m, &m->score_dev, &m->score_words, n * (3 + 2 * (size_t)top)));
+    size_t ws = 0;
+    for (size_t r = 1; r <= group; ++r) ws = std::max(ws, logprobs_workspace_bytes(r, V, (int)top));
+    CHIP_TRY(grow(m, &m->score_ws, &m->score_ws_bytes, ws));
+    CHIP_TRY(reserve_positions(m, n));
+    CHIP_CHECK(hipStreamSynchronize(m->stream));  // tokens_host reuse
+    std::memcpy(m->tokens_host, tokens, n * sizeof(uint32_t));
+    CHIP_CHECK(hipMemcpyAsync(m->tokens_dev, m->tokens_host, n * sizeof(uint32_t), hipMemcpyHostToDevice, m->stream));
+    uint32_t *want = m->score_dev;
+    float *lp = (float *)(want + n), *ent = lp + n;
+    uint32_t *ids = (uint32_t *)(ent + n);
+    float *tops = (float *)(ids + n * top);
+    if (logprobs)
+        CHIP_CHECK(hipMemcpyAsync(want, targets, n * sizeof(uint32_t), hipMemcpyHostToDevice, m->stream));
+    for (size_t start = 0; start < n; start += chunk_rows) {
+        const size_t rows = std::min(chunk_rows, n - start);
+        CHIP_TRY(enqueue_chunk(m, m->tokens_dev + start, rows, offset + start, false));
+        for (size_t r0 = 0; r0 < rows; r0 += group) {
+            const size_t at = start + r0;
+            LogprobJob j;
+            j.x = m->row_logits;
+            j.rows = std::min(group, rows - r0);
+            j.vocab = j.stride = V;
+            j.tokens = logprobs ? want + at : nullptr;
+            j.top = (int)top;
+            j.logprobs = logprobs ? lp + at : nullptr;
+            j.entropy = entropy ? ent + at : nullptr;
+            j.ids = top ? ids + at * top : nullptr;
+            j.tops = top ? tops + at * top : nullptr;
+            j.ws = m->score_ws;
+            j.ws_bytes = m->score_ws_bytes;
+            CHIP_TRY(enqueue_head_rows(m, r0, j.rows));
+            CHIP_TRY(launch_logprobs(j, m->stream));
+        }
+    }
+    auto get = [&](void *dst, const void *src, size_t words) -> int {
+        if (!dst) return 0;
+        CHIP_CHECK(hipMemcpyAsync(dst, src, words * sizeof(uint32_t), hipMemcpyDeviceToHost, m->stream));
+        return 0;
+    };
+    CHIP_TRY(get(logprobs, lp, n));
+    CHIP_TRY(get(entropy, ent, n));
+    CHIP_TRY(get(top_ids, ids, n * top));
+    CHIP_TRY(get(top_logprobs, tops, n * top));
     CHIP_CHECK(hipStreamSynchronize(m->stream));
     m->len = offset + n;
     return 0;
@@ -1326,6 +1565,7 @@ int cheetah_hip_decode_greedy(cheetah_hip_model *m, uint32_t token, size_t offse
     if (!tokens_out) return fail("HIP backend: null tokens_out.");
     CHIP_TRY(validate_decode(m, token, offset, steps));
     CHIP_TRY(refresh_weights(m));
+    m->tree_n = 0;
     CHIP_TRY(reserve_positions(m, steps));
     CHIP_TRY(launch_set_step(m->step_dev, (int32_t)token, (int32_t)offset, m->stream));
     if (fused_fits(m, offset, steps)) CHIP_TRY(run_fused(m, offset, steps));
@@ -1338,12 +1578,64 @@ int cheetah_hip_decode_greedy(cheetah_hip_model *m, uint32_t token, size_t offse
     return 0;
 }
 
+int cheetah_hip_forward_tree(cheetah_hip_model *m, const uint32_t *tokens, const int32_t *parents, size_t n,
+                             size_t offset, uint32_t *next_tokens, float *logits_out) {
+    if (!next_tokens && !logits_out) return fail("HIP backend: forward_tree without an output.");
+    if (guarded([&] { return run_tree(m, tokens, parents, n, offset, next_tokens != nullptr); })) return -1;
+    if (next_tokens) std::memcpy(next_tokens, m->tree_host + 3 * kMaxTreeNodes, n * sizeof(uint32_t));
+    if (logits_out)
+        CHIP_CHECK(hipMemcpy(logits_out, m->row_logits, n * C(m).vocab_size * sizeof(float), hipMemcpyDeviceToHost));
+    return 0;
+}
+
+int cheetah_hip_commit_tree(cheetah_hip_model *m, const uint32_t *nodes, size_t count) {
+    CHIP_TRY(check_model(m));
+    if (!nodes && count) return fail("HIP backend: null nodes pointer.");
+    if (m->tree_n == 0)
+        return fail("HIP backend: no tree to commit (forward_tree must be the last call that wrote the cache).");
+    if (count > m->tree_n) return fail("HIP backend: the branch has more nodes than the tree.");
+    const int32_t *parents = m->tree_host + kMaxTreeNodes;
+    for (size_t j = 0; j < count; ++j)
+        if (nodes[j] >= m->tree_n || parents[nodes[j]] != (j ? (int32_t)nodes[j - 1] : -1))
+            return fail("HIP backend: a branch goes from a root to a node, each node followed by a child.");
+    return guarded([&] { return keep_branch(m, nodes, count); });
+}
+
+int cheetah_hip_verify_tree(cheetah_hip_model *m, const uint32_t *tokens, const int32_t *parents, size_t n,
+                            size_t offset, uint32_t *accepted, size_t *count, uint32_t *next_token) {
+    if (!accepted || !count || !next_token) return fail("HIP backend: verify_tree with a null output.");
+    if (parents)
+        for (size_t i = 0; i < n && i < (size_t)kMaxTreeNodes; ++i)
+            if ((parents[i] < 0) != (i == 0))
+                return fail("HIP backend: verify_tree takes one root, node 0: the last token sampled.");
+    if (guarded([&] { return run_tree(m, tokens, parents, n, offset, true); })) return -1;
+    const uint32_t *next = (const uint32_t *)(m->tree_host + 3 * kMaxTreeNodes);
+    uint32_t branch[kMaxTreeNodes] = {0};
+    size_t len = 1, cur = 0;
+    for (size_t i = 1; i < n; ++i)
+        if (parents[i] == (int32_t)cur && tokens[i] == next[cur]) branch[len++] = (uint32_t)(cur = i);
+    if (guarded([&] { return keep_branch(m, branch, len); })) return -1;
+    std::memcpy(accepted, branch, len * sizeof(uint32_t));
+    *count = len;
+    *next_token = next[cur];
+    return 0;
+}
+
+int cheetah_hip_forward_logprobs(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t offset,
+                                 size_t chunk_rows, const uint32_t *targets, uint32_t top, float *logprobs,
+                                 float *entropy, uint32_t *top_ids, float *top_logprobs) {
+    return guarded([&] {
+        return run_scored(m, tokens, n, offset, chunk_rows, targets, top, logprobs, entropy, top_ids, top_logprobs);
+    });
+}
+
 int cheetah_hip_time_decode(cheetah_hip_model *m, uint32_t token, size_t offset, size_t steps, float *ms_per_step,
                             float *gemv_ms, uint32_t *tokens_out) {
     CHIP_TRY(check_model(m));
     if (steps == 0 || !ms_per_step) return fail("HIP backend: time_decode needs steps and an output.");
     CHIP_TRY(validate_decode(m, token, offset, steps));
     CHIP_TRY(refresh_weights(m));
+    m->tree_n = 0;
     CHIP_TRY(reserve_positions(m, steps));
     CHIP_TRY(launch_set_step(m->step_dev, (int32_t)token, (int32_t)offset, m->stream));
     hipEvent_t e0, e1;
@@ -1472,6 +1764,7 @@ void cheetah_hip_clear_cache(cheetah_hip_model *m) {
     for (int p : m->pages) m->sh->page_unref(p);
     m->pages.clear();
     m->len = 0;
+    m->tree_n = 0;
 }
 
 cheetah_hip_model *cheetah_hip_clone(const cheetah_hip_model *src) {

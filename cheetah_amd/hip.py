@@ -26,6 +26,7 @@ _c = ctypes
 _SZ = _c.c_size_t
 _VP = _c.c_void_p
 _U32P = _c.POINTER(_c.c_uint32)
+_I32P = _c.POINTER(_c.c_int32)
 _F32P = _c.POINTER(_c.c_float)
 
 
@@ -81,6 +82,11 @@ SIGNATURES = {
     "cheetah_hip_forward": (_c.c_int, [_VP, _U32P, _SZ, _SZ, _SZ, _F32P]),
     "cheetah_hip_forward_greedy": (_c.c_int, [_VP, _U32P, _SZ, _SZ, _SZ, _U32P, _F32P]),
     "cheetah_hip_decode_greedy": (_c.c_int, [_VP, _c.c_uint32, _SZ, _SZ, _U32P]),
+    "cheetah_hip_forward_tree": (_c.c_int, [_VP, _U32P, _I32P, _SZ, _SZ, _U32P, _F32P]),
+    "cheetah_hip_commit_tree": (_c.c_int, [_VP, _U32P, _SZ]),
+    "cheetah_hip_verify_tree": (_c.c_int, [_VP, _U32P, _I32P, _SZ, _SZ, _U32P, _c.POINTER(_SZ), _U32P]),
+    "cheetah_hip_forward_logprobs": (_c.c_int, [_VP, _U32P, _SZ, _SZ, _SZ, _U32P, _c.c_uint32, _F32P, _F32P, _U32P,
+                                                _F32P]),
     "cheetah_hip_clear_cache": (None, [_VP]),
     "cheetah_hip_clone": (_VP, [_VP]),
     "cheetah_hip_kv_len": (_SZ, [_VP]),
@@ -429,6 +435,59 @@ class HipForward:
         out = np.zeros(steps, np.uint32)
         check(lib().cheetah_hip_decode_greedy(self._h, int(token), offset, steps, out.ctypes.data_as(_U32P)))
         return out
+
+    def forward_tree(self, tokens, parents, offset: int, want_logits: bool = False):
+        """Runs a tree of drafted tokens behind the cache (parents[i] < i, -1:
+        a child of the cached text) and leaves it pending for commit_tree: every
+        node's argmax, with want_logits also every node's logits [n, vocab]."""
+        toks = np.ascontiguousarray(tokens, dtype=np.uint32)
+        par = np.ascontiguousarray(parents, dtype=np.int32)
+        if toks.size != par.size:
+            raise ValueError("one parent a token")
+        nxt = np.zeros(toks.size, np.uint32)
+        logits = np.empty((toks.size, self.shape.vocab_size), np.float32) if want_logits else None
+        check(lib().cheetah_hip_forward_tree(self._h, toks.ctypes.data_as(_U32P), par.ctypes.data_as(_I32P), toks.size,
+                                             offset, nxt.ctypes.data_as(_U32P),
+                                             logits.ctypes.data_as(_F32P) if want_logits else None))
+        return (nxt, logits) if want_logits else nxt
+
+    def commit_tree(self, nodes) -> None:
+        """Keeps a branch of the pending tree (its nodes from a root on; none
+        drops the tree)."""
+        nodes = np.ascontiguousarray(nodes, dtype=np.uint32)
+        check(lib().cheetah_hip_commit_tree(self._h, nodes.ctypes.data_as(_U32P), nodes.size))
+
+    def verify_tree(self, tokens, parents, offset: int):
+        """forward_tree, the greedy walk from node 0 (the last token sampled)
+        and the commit of what it accepts: (accepted nodes, next token)."""
+        toks = np.ascontiguousarray(tokens, dtype=np.uint32)
+        par = np.ascontiguousarray(parents, dtype=np.int32)
+        if toks.size != par.size:
+            raise ValueError("one parent a token")
+        accepted = np.zeros(max(toks.size, 1), np.uint32)
+        count, nxt = _SZ(0), _c.c_uint32(0)
+        check(lib().cheetah_hip_verify_tree(self._h, toks.ctypes.data_as(_U32P), par.ctypes.data_as(_I32P), toks.size,
+                                            offset, accepted.ctypes.data_as(_U32P), _c.byref(count), _c.byref(nxt)))
+        return accepted[:count.value], int(nxt.value)
+
+    def forward_logprobs(self, tokens, offset: int, targets=None, top: int = 0, chunk_rows: int = 0):
+        """forward that scores every position: (log probabilities of `targets`
+        or None, entropies, ids [n, top] and log probabilities of the `top` most
+        likely next tokens)."""
+        toks = np.ascontiguousarray(tokens, dtype=np.uint32)
+        want = None if targets is None else np.ascontiguousarray(targets, dtype=np.uint32)
+        if want is not None and want.size != toks.size:
+            raise ValueError("one target a token")
+        n = toks.size
+        lp = None if want is None else np.empty(n, np.float32)
+        ent = np.empty(n, np.float32)
+        ids, tops = np.empty((n, top), np.uint32), np.empty((n, top), np.float32)
+        check(lib().cheetah_hip_forward_logprobs(
+            self._h, toks.ctypes.data_as(_U32P), n, offset, chunk_rows,
+            None if want is None else want.ctypes.data_as(_U32P), top,
+            None if lp is None else lp.ctypes.data_as(_F32P), ent.ctypes.data_as(_F32P),
+            ids.ctypes.data_as(_U32P) if top else None, tops.ctypes.data_as(_F32P) if top else None))
+        return lp, ent, ids, tops
 
     def time_decode(self, token: int, offset: int, steps: int):
         ms = _c.c_float(0)

@@ -230,6 +230,42 @@ int cheetah_hip_forward_greedy(cheetah_hip_model *m, const uint32_t *tokens, siz
  * the sampled ids to tokens_out[steps]. */
 int cheetah_hip_decode_greedy(cheetah_hip_model *m, uint32_t token, size_t offset, size_t steps,
                               uint32_t *tokens_out);
+/* Verification of drafted tokens (speculative decoding; no counterpart in the
+ * reference). A tree of candidate tokens is run in one forward behind the
+ * cached positions. tokens[n]; parents[n]: parents[i] in [-1, i), -1 for a child
+ * of the cached text; n at most CHEETAH_HIP_MAX_TREE_NODES and max_chunk_rows.
+ * Node i attends to the cache, its ancestors and itself, at position offset +
+ * depth; offset must equal the cached length, and offset + n must fit the
+ * capacity.
+ *   forward_tree: next_tokens[n] (or NULL) receives every node's argmax (ties
+ *     to the last index), logits_out[n * vocab_size] (or NULL) every node's
+ *     logits. The cached length stays; the nodes' K/V rows wait behind it until
+ *     commit_tree or until anything else runs on this instance or clears or
+ *     restores its cache, which drops them.
+ *   commit_tree: keeps a branch of that tree, nodes[count] from a child of the
+ *     cached text to any node, each followed by a child of it; the cache is then
+ *     as if the branch's tokens had been run alone. count 0 drops the tree.
+ *   verify_tree: forward_tree and commit_tree in one call, greedily. Node 0 is
+ *     the only root: the last token sampled, not yet in the cache. From it the
+ *     walk goes to the child whose token is the argmax while there is one (the
+ *     first such child). accepted[n] receives the walk's nodes, *count (at least
+ *     1) their number, *next_token the argmax behind the last of them: what
+ *     `count` steps of greedy decoding would have sampled. The cache then holds
+ *     the accepted tokens. */
+int cheetah_hip_forward_tree(cheetah_hip_model *m, const uint32_t *tokens, const int32_t *parents, size_t n,
+                             size_t offset, uint32_t *next_tokens, float *logits_out);
+int cheetah_hip_commit_tree(cheetah_hip_model *m, const uint32_t *nodes, size_t count);
+int cheetah_hip_verify_tree(cheetah_hip_model *m, const uint32_t *tokens, const int32_t *parents, size_t n,
+                            size_t offset, uint32_t *accepted, size_t *count, uint32_t *next_token);
+/* forward that scores every position (cheetah_hip_logprobs of each one's
+ * logits; no counterpart in the reference): targets[n] are the tokens whose
+ * log probabilities go to logprobs[n] (both may be NULL; for a text's own tokens
+ * targets[i] = the token after tokens[i]; one past the vocabulary gives NaN),
+ * entropy[n] may be NULL, top_ids and top_logprobs [n * top] are NULL when top
+ * is 0. Chunks and cache as cheetah_hip_forward. */
+int cheetah_hip_forward_logprobs(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t offset,
+                                 size_t chunk_rows, const uint32_t *targets, uint32_t top, float *logprobs,
+                                 float *entropy, uint32_t *top_ids, float *top_logprobs);
 /* ModelForward::clear_cache (registry.rs:62). */
 void cheetah_hip_clear_cache(cheetah_hip_model *m);
 /* Boxed clone per generation (registry.rs:95-117, ops.rs:1017-1029): shares

@@ -110,3 +110,22 @@ def test_host_wrappers_check_their_arrays(hip):
         hip.logprobs(np.zeros((3, 5), np.float32), [1, 2])
     with pytest.raises(ValueError, match="matrix"):
         hip.logprobs(np.zeros((3, 5), np.float64))
+
+
+def test_model_calls_refuse_what_they_see_first(hip):
+    """Null outputs, a second root and a null model, before any device work."""
+    L = hip.lib()
+    toks, par = (ctypes.c_uint32 * 3)(1, 2, 3), (ctypes.c_int32 * 3)(-1, 0, -1)
+    out, count, f = (ctypes.c_uint32 * 3)(), ctypes.c_size_t(0), (ctypes.c_float * 3)()
+    refused(hip, L.cheetah_hip_forward_tree(None, toks, par, 3, 0, None, None), "without an output")
+    refused(hip, L.cheetah_hip_forward_tree(None, toks, par, 3, 0, out, None), "no model")
+    refused(hip, L.cheetah_hip_commit_tree(None, out, 1), "no model")
+    refused(hip, L.cheetah_hip_verify_tree(None, toks, par, 3, 0, None, ctypes.byref(count), out), "null output")
+    refused(hip, L.cheetah_hip_verify_tree(None, toks, par, 3, 0, out, None, out), "null output")
+    refused(hip, L.cheetah_hip_verify_tree(None, toks, par, 3, 0, out, ctypes.byref(count), None), "null output")
+    refused(hip, L.cheetah_hip_verify_tree(None, toks, par, 3, 0, out, ctypes.byref(count), out), "one root")
+    par[2] = 1
+    refused(hip, L.cheetah_hip_verify_tree(None, toks, par, 3, 0, out, ctypes.byref(count), out), "no model")
+    par[0] = 0
+    refused(hip, L.cheetah_hip_verify_tree(None, toks, par, 3, 0, out, ctypes.byref(count), out), "one root")
+    refused(hip, L.cheetah_hip_forward_logprobs(None, toks, 3, 0, 0, None, 0, None, f, None, None), "no model")
