@@ -478,6 +478,7 @@ int cheetah_hip_logprobs(const void *logits, uint32_t logit_format, size_t rows,
         ws = nullptr;
         ws_bytes = 0;
         CHIP_CHECK(hipMalloc(&ws, need));
+        CHIP_TRY(logprobs_workspace_clear(ws, g_stream));
         ws_bytes = need;
     }
     j.ws = ws;

@@ -272,10 +272,13 @@ struct LogprobJob {
     float *logprobs = nullptr, *entropy = nullptr;
     uint32_t *ids = nullptr;
     float *tops = nullptr;
-    void *ws = nullptr;  // logprobs_workspace_bytes of it
+    // logprobs_workspace_bytes of it, cleared once after its allocation (every
+    // launch leaves it so for the next), for one stream's launches at a time.
+    void *ws = nullptr;
     size_t ws_bytes = 0;
 };
 size_t logprobs_workspace_bytes(size_t rows, size_t vocab, int top);
+int logprobs_workspace_clear(void *ws, hipStream_t s);
 int launch_logprobs(const LogprobJob &job, hipStream_t s);
 
 // Greedy argmax (ties -> last index, total order) of logits[n]; writes the

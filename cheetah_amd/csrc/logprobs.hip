@@ -10,9 +10,19 @@
 // each thread with its own running maximum and sums (f32 over a chunk's at most
 // 16 logits, in 64 bits from chunk to chunk), the block with the best `top`
 // logits so far. A logit joins those only if it is larger than the last of them
-// (ids rise, so an equal one loses), which is rare after the first chunk. Few
-// rows have many segments, joined by logprobs_join_kernel; many rows have one
-// each and are done in one launch.
+// (ids rise, so an equal one loses), which is rare after the first chunk. Many
+// rows have one segment each; few rows have many, whose results go through memory
+// to the row's last block, which joins them in the same launch.
+//
+// Bound: 512 f32 rows of 152064 (311 MB) with 5 alternatives take 60.7 us, 5.13
+// TB/s, a large copy's rate; BF16 rows take 0.86 of the time (the exponentials then
+// count: 16 of them a thread and chunk). Fewer rows are bound by the steps before
+// and behind the loop, each a memory or LDS round trip: of 64 rows' 20.4 us with 20
+// alternatives the loop ends at 13, the segment's sums and picks are in memory at
+// 14.6, counted at 15.2, read by the last block at 15.6, ranked at 17.6. As two
+// launches these 64 rows took 23.4 us, one row 11.6 (11.6 in one). A release
+// fence in place of the write-through stores (it writes the whole L2 back) made
+// them 29.6 and 12.2.
 #include <algorithm>
 #include <type_traits>
 
@@ -38,6 +48,25 @@ struct Sums {
     int c;
 };
 
+// Words that blocks of one launch hand on. An agent-scope access goes past the
+// caches of its own XCD, so that a block anywhere reads what is there.
+__device__ __forceinline__ void agent_store(uint64_t *p, uint64_t v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t agent_load(const uint64_t *p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+constexpr int kCountStride = 32;  // a row's count has a cache line of its own
+constexpr int kSumWords = sizeof(Sums) / sizeof(uint64_t);
+__device__ __forceinline__ Sums agent_load(const Sums *p) {
+    uint64_t w[kSumWords];
+#pragma unroll
+    for (int i = 0; i < kSumWords; ++i) w[i] = agent_load((const uint64_t *)p + i);
+    Sums s;
+    __builtin_memcpy(&s, w, sizeof(s));
+    return s;
+}
+
 struct LogprobArgs {
     const void *x;
     const uint32_t *tokens;
@@ -47,8 +76,9 @@ struct LogprobArgs {
     size_t stride;
     unsigned vocab, seg;  // logits of a row, of a segment
     int top, segs;
-    Sums *sums;       // [row][segment]
-    uint64_t *picks;  // [row][top][segment]: keys, 0 for none
+    Sums *sums;         // [row][segment]
+    uint64_t *picks;    // [row][segment][top]: keys, 0 for none
+    uint32_t *arrived;  // [row][kCountStride]: segments done, 0 between launches
 };
 
 // Alternatives are ordered by their keys: the value's bits in order, then the
@@ -108,27 +138,29 @@ __device__ __forceinline__ Sums wave_join(Sums s, float m) {
     return t;
 }
 
-// A row's results from its sums, alternatives from their keys (any LDS or
-// global array), by the threads of a block.
+// The given token's logit, in the first thread; NaN where there is none. Read at
+// a block's start, its two round trips to memory pass beside the first chunk's.
+template <class T>
+__device__ __forceinline__ float token_logit(const LogprobArgs &a, const T *x, size_t row) {
+    if (!a.logprobs || threadIdx.x) return NAN;
+    const uint32_t t = a.tokens[row];
+    if (t >= a.vocab) return NAN;
+    if constexpr (sizeof(T) == 4) return x[t];
+    else return bf16_f32(x[t]);
+}
+
+// A row's results from its sums, alternatives from their keys, by the threads of
+// a block.
 struct Result {
     double m, logsum;
     bool empty;
     __device__ Result(const Sums &s) : m(s.m), logsum(log1p((double)(s.c - 1) + s.S)), empty(s.m == -INFINITY && s.S == 0) {}
     __device__ float logprob(float x) const { return empty ? -INFINITY : (float)((double)x - m - logsum); }
 };
-template <class T>
-__device__ __forceinline__ void store_row(const LogprobArgs &a, const T *x, size_t row, const Sums &s, const uint64_t *best) {
+__device__ __forceinline__ void store_row(const LogprobArgs &a, size_t row, float token, const Sums &s, const uint64_t *best) {
     const int tid = threadIdx.x;
     const Result r(s);
-    if (tid == 0 && a.logprobs) {
-        const uint32_t t = a.tokens[row];
-        float v = NAN;
-        if (t < a.vocab) {
-            if constexpr (sizeof(T) == 4) v = r.logprob(x[t]);
-            else v = r.logprob(bf16_f32(x[t]));
-        }
-        a.logprobs[row] = v;
-    }
+    if (tid == 0 && a.logprobs) a.logprobs[row] = token == token ? r.logprob(token) : NAN;
     if (tid == 0 && a.entropy) a.entropy[row] = r.empty ? 0.f : (float)(r.logsum + s.A / ((double)s.c + s.S));
     if (tid < a.top) {
         const uint64_t k = best[tid];
@@ -144,39 +176,53 @@ __device__ __forceinline__ void store_row(const LogprobArgs &a, const T *x, size
 constexpr int kRoom = kMaxTop + kCap;
 struct Best {
     uint64_t key[kRoom + 8];
+    uint16_t above[kWaves][kRoom];
     float wave_value[kWaves];
     int hist[256], wave_total[kWaves], found[3];
     int count;  // keys held, the best among them; past kRoom: some had no room
 };
 
-// Sorts the keys held and keeps the first `top`: each thread ranks its keys
-// among all of them, eight reads in flight.
+// Sorts the keys held and keeps the first `top`. Every wave takes all the keys, R a
+// lane, and a quarter of them to compare with, eight reads in flight; a key's rank
+// is the sum of the waves' counts of larger ones. (A thread with a key of its own
+// and all the others to compare: 160 keys 2.2 us, so 1.5.)
 template <int R>
 __device__ __forceinline__ void best_rank(Best &b, int top, int n) {
-    const int tid = threadIdx.x;
-    uint64_t mine[R];
+    constexpr int OWN = (64 * R + kThreads - 1) / kThreads;  // keys whose ranks a thread adds up
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int part = (n + 8 * kWaves - 1) / (8 * kWaves) * 8, j0 = min(wave * part, n), j1 = min(j0 + part, n);
+    uint64_t mine[R], own[OWN];
     int rank[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        mine[i] = tid + kThreads * i < n ? b.key[tid + kThreads * i] : ~0ull;
+        mine[i] = lane + 64 * i < n ? b.key[lane + 64 * i] : ~0ull;
         rank[i] = 0;
     }
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) own[i] = tid + kThreads * i < n ? b.key[tid + kThreads * i] : 0;
     if (tid < 8) b.key[n + tid] = 0;  // above no key
     lds_barrier();
-    if (R > 1 || tid < (n + 63) / 64 * 64)
-        for (int j = 0; j < n; j += 8) {
-            uint64_t k[8];
+    for (int j = j0; j < j1; j += 8) {
+        uint64_t k[8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) k[q] = b.key[j + q];
+        for (int q = 0; q < 8; ++q) k[q] = b.key[j + q];
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
+        for (int q = 0; q < 8; ++q)
 #pragma unroll
-                for (int i = 0; i < R; ++i) rank[i] += k[q] > mine[i];
-        }
+            for (int i = 0; i < R; ++i) rank[i] += k[q] > mine[i];
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) b.above[wave][lane + 64 * i] = (uint16_t)rank[i];
     lds_barrier();
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-        if (tid + kThreads * i < n && rank[i] < top) b.key[rank[i]] = mine[i];
+    for (int i = 0; i < OWN; ++i) {
+        const int at = tid + kThreads * i;
+        if (at >= n) break;
+        int r = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) r += b.above[w][at];
+        if (r < top) b.key[r] = own[i];
+    }
     if (tid == 0) b.count = min(n, top);
     lds_barrier();
 }
@@ -184,10 +230,10 @@ __device__ __forceinline__ void best_rank(Best &b, int top, int n) {
 // Prunes to the best `top`, says above what a logit would join them and how many
 // are held (the count itself may grow again before every wave has read it).
 __device__ __forceinline__ int best_settle(Best &b, int top, float &last) {
-    constexpr int R = (kRoom + kThreads - 1) / kThreads;
     const int n = b.count;
-    if (n <= kThreads) best_rank<1>(b, top, n);
-    else best_rank<R>(b, top, n);
+    if (n <= 128) best_rank<2>(b, top, n);
+    else if (n <= 256) best_rank<4>(b, top, n);
+    else best_rank<kRoom / 64>(b, top, n);
     last = n < top ? -INFINITY : key_value(b.key[top - 1]);
     return min(n, top);
 }
@@ -242,11 +288,12 @@ struct Logits {
 struct Picks {
     static constexpr int VE = 1;
     const uint64_t *picks;
-    int n, vectors;
+    int segs, top, vectors;
     typedef uint64_t Vec;
+    // In the order of their ranks, so that a thread's largest is of its own segment.
     __device__ Vec load(int v) const {
         const int e = kThreads * v + (int)threadIdx.x;
-        return e < n ? picks[e] : 0;
+        return e < segs * top ? agent_load(picks + (e % segs * top + e / segs)) : 0;
     }
     __device__ uint64_t key(Vec v, int) const { return v; }
 };
@@ -341,6 +388,54 @@ __device__ __forceinline__ void fill_masked(Best &b, int top, const T *x, unsign
     lds_barrier();
 }
 
+// The segments of a row, by the block that was the last to end one.
+template <class T>
+__device__ __forceinline__ void join_row(const LogprobArgs &a, Best &best, const T *x_row, size_t row, float token) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    Sums s{0.0, 0.0, -INFINITY, 0}, s2 = s;
+    if (lane < a.segs) s = agent_load(a.sums + row * a.segs + lane);
+    if (lane + 64 < a.segs) s2 = agent_load(a.sums + row * a.segs + lane + 64);
+    const int n = a.segs * a.top;
+    const Picks src{a.picks + row * n, a.segs, a.top, (n + kThreads - 1) / kThreads};
+    float most = -INFINITY;
+    for (int v = 0; v < src.vectors; ++v) {
+        const uint64_t k = src.load(v);
+        most = fmaxf(most, k ? key_value(k) : -INFINITY);
+    }
+    if (tid == 0) best.count = 0;
+    lds_barrier();
+    const float m = wave_max(fmaxf(s.m, s2.m));
+    if (a.segs > 64) {
+        raise(s, m);
+        raise(s2, m);
+        s.S += s2.S;
+        s.A += s2.A;
+        s.c += s2.c;
+    }
+    s = wave_join(s, m);
+    if (a.top) {
+        const float from = n <= kThreads ? -INFINITY : best_bound(best, a.top, most);
+        for (int v = 0; v < src.vectors; ++v) {
+            const uint64_t k = src.load(v);
+            if (k && key_value(k) >= from) {
+                const int i = atomicAdd(&best.count, 1);
+                if (i < kRoom) best.key[i] = k;
+            }
+        }
+        lds_barrier();
+        const bool many = best.count > kRoom;
+        lds_barrier();
+        if (many) {
+            if (tid == 0) best.count = 0;
+            lds_barrier();
+            best_select(best, a.top, src);
+        }
+        float last;
+        if (best_settle(best, a.top, last) < a.top) fill_masked(best, a.top, x_row, a.vocab);
+    }
+    store_row(a, row, token, s, best.key);
+}
+
 // One segment of a row, kThreads * PER logits at a time.
 template <class T, int PER>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
@@ -348,6 +443,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
     constexpr unsigned CHUNK = kThreads * PER;
     __shared__ Best best;
     __shared__ Sums part[kWaves];
+    __shared__ bool last_here;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const size_t row = blockIdx.x / (unsigned)a.segs;
     const unsigned seg = blockIdx.x % (unsigned)a.segs;
@@ -363,6 +459,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
         for (int v = 0; v < NV; ++v) raw[v] = *(const u32x4 *)(from + min(e0 + (kThreads * v + tid) * VE, last_load));
     };
     load(begin);
+    const float token = token_logit(a, x_row, row);
     if (tid == 0) best.count = 0;
     lds_barrier();
     Sums s{0.0, 0.0, -INFINITY, 0};
@@ -409,13 +506,18 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
         if (!a.top) continue;
         float above = last;
         if (chunk == 0) above = just_below(best_bound(best, a.top, most));  // all of them would be too many
-        if (__any(most > above))
+        if (most > above) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) n += x[i] > above;
+            int k = atomicAdd(&best.count, n);
 #pragma unroll
             for (int i = 0; i < PER; ++i)
                 if (x[i] > above) {
-                    const int k = atomicAdd(&best.count, 1);
                     if (k < kRoom) best.key[k] = key_of(x[i], at(i) - head);
+                    ++k;
                 }
+        }
         if (chunk % kSettle == 0 || e0 + CHUNK >= end) {
             lds_barrier();
             const int n = best.count;
@@ -454,60 +556,31 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
     }
     if (a.segs == 1) {
         if (held < a.top) fill_masked(best, a.top, x_row, a.vocab);
-        store_row(a, x_row, row, all_waves, best.key);
+        store_row(a, row, token, all_waves, best.key);
         return;
     }
+    // The first wave leaves the segment's results and counts it; the row's last
+    // block joins them, in the segments' order whichever it is.
     const size_t at = row * a.segs + seg;
-    if (tid == 0) a.sums[at] = all_waves;
-    if (tid < a.top) a.picks[(row * a.top + tid) * a.segs + seg] = tid < held ? best.key[tid] : 0;
+    if (wave == 0) {
+        uint64_t w[kSumWords];
+        __builtin_memcpy(w, &all_waves, sizeof(all_waves));
+#pragma unroll
+        for (int i = 0; i < kSumWords; ++i)
+            if (tid == i) agent_store((uint64_t *)(a.sums + at) + i, w[i]);
+        if (tid < a.top) agent_store(a.picks + at * a.top + tid, tid < held ? best.key[tid] : 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // they are there before the count says so
+        if (tid == 0) {
+            uint32_t *count = a.arrived + row * kCountStride;
+            last_here = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)a.segs - 1;
+            if (last_here) *count = 0;
+        }
+    }
+    lds_barrier();
+    if (!last_here) return;
+    join_row(a, best, x_row, row, token);
 }
 
-// The segments of a row.
-template <class T>
-__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a) {
-    __shared__ Best best;
-    const int tid = threadIdx.x, lane = tid & 63;
-    const size_t row = blockIdx.x;
-    Sums s{0.0, 0.0, -INFINITY, 0}, s2 = s;
-    if (lane < a.segs) s = a.sums[row * a.segs + lane];
-    if (lane + 64 < a.segs) s2 = a.sums[row * a.segs + lane + 64];
-    const int n = a.segs * a.top;
-    const Picks src{a.picks + row * n, n, (n + kThreads - 1) / kThreads};
-    float most = -INFINITY;
-    for (int v = 0; v < src.vectors; ++v) {
-        const uint64_t k = src.load(v);
-        most = fmaxf(most, k ? key_value(k) : -INFINITY);
-    }
-    if (tid == 0) best.count = 0;
-    lds_barrier();
-    const float m = wave_max(fmaxf(s.m, s2.m));
-    s = wave_join(s, m);
-    s2 = wave_join(s2, m);
-    s.S += s2.S;
-    s.A += s2.A;
-    s.c += s2.c;
-    if (a.top) {
-        const float from = best_bound(best, a.top, most);
-        for (int v = 0; v < src.vectors; ++v) {
-            const uint64_t k = src.load(v);
-            if (k && key_value(k) >= from) {
-                const int i = atomicAdd(&best.count, 1);
-                if (i < kRoom) best.key[i] = k;
-            }
-        }
-        lds_barrier();
-        const bool many = best.count > kRoom;
-        lds_barrier();
-        if (many) {
-            if (tid == 0) best.count = 0;
-            lds_barrier();
-            best_select(best, a.top, src);
-        }
-        float last;
-        if (best_settle(best, a.top, last) < a.top) fill_masked(best, a.top, (const T *)a.x + row * a.stride, a.vocab);
-    }
-    store_row(a, (const T *)a.x + row * a.stride, row, s, best.key);
-}
 
 // Segments of a row: enough for two blocks a CU, of at least a small chunk.
 int logprob_segs(size_t rows, size_t vocab) {
@@ -524,17 +597,23 @@ int launch_logprobs_t(const LogprobJob &j, LogprobArgs &a, hipStream_t s) {
     else
         hipLaunchKernelGGL((logprobs_kernel<T, 16>), dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
     CHIP_CHECK(hipGetLastError());
-    if (a.segs == 1) return 0;
-    hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3((unsigned)j.rows), dim3(kThreads), 0, s, a);
-    CHIP_CHECK(hipGetLastError());
     return 0;
 }
 
 }  // namespace
 
+// The rows' counts at a workspace's start (rows in segments are at most half the
+// blocks of two a CU).
+constexpr size_t kCountBytes = 1024 * kCountStride * sizeof(uint32_t);
+
+int logprobs_workspace_clear(void *ws, hipStream_t s) {
+    CHIP_CHECK(hipMemsetAsync(ws, 0, kCountBytes, s));
+    return 0;
+}
+
 size_t logprobs_workspace_bytes(size_t rows, size_t vocab, int top) {
     const size_t segs = (size_t)logprob_segs(rows, vocab);
-    return segs == 1 ? 0 : rows * segs * (sizeof(Sums) + (size_t)top * sizeof(uint64_t));
+    return segs == 1 ? 0 : kCountBytes + rows * segs * (sizeof(Sums) + (size_t)top * sizeof(uint64_t));
 }
 
 int launch_logprobs(const LogprobJob &j, hipStream_t s) {
@@ -558,7 +637,9 @@ int launch_logprobs(const LogprobJob &j, hipStream_t s) {
     if (a.segs > 1) {
         if (!j.ws || j.ws_bytes < logprobs_workspace_bytes(j.rows, j.vocab, j.top))
             return fail("HIP backend: logprobs workspace too small.");
-        a.sums = (Sums *)j.ws;
+        if (j.rows > kCountBytes / (kCountStride * sizeof(uint32_t))) return fail("HIP backend: logprobs grid out of range.");
+        a.arrived = (uint32_t *)j.ws;
+        a.sums = (Sums *)((uint8_t *)j.ws + kCountBytes);
         a.picks = (uint64_t *)(a.sums + j.rows * (size_t)a.segs);
     }
     return j.f32 ? launch_logprobs_t<float>(j, a, s) : launch_logprobs_t<uint16_t>(j, a, s);

@@ -1380,7 +1380,10 @@ int run_scored(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t of
     CHIP_TRY(grow(m, &m->score_dev, &m->score_words, n * (3 + 2 * (size_t)top)));
     size_t ws = 0;
     for (size_t r = 1; r <= group; ++r) ws = std::max(ws, logprobs_workspace_bytes(r, V, (int)top));
-    CHIP_TRY(grow(m, &m->score_ws, &m->score_ws_bytes, ws));
+    if (ws > m->score_ws_bytes) {
+        CHIP_TRY(grow(m, &m->score_ws, &m->score_ws_bytes, ws));
+        CHIP_TRY(logprobs_workspace_clear(m->score_ws, m->stream));
+    }
     CHIP_TRY(reserve_positions(m, n));
     CHIP_CHECK(hipStreamSynchronize(m->stream));  // tokens_host reuse
     std::memcpy(m->tokens_host, tokens, n * sizeof(uint32_t));
