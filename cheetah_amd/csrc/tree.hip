@@ -17,6 +17,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Block barrier that waits on LDS traffic only: loads stay in flight across it.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 struct TreeArgs {
     const float *q;
     const void *k, *v;
@@ -56,6 +59,7 @@ struct TreeLds {
     uint64_t sick[kAncWords];  // nodes with an infinity or NaN in V
     uint32_t odd[4];           // a row wave's rows to compute again
     int sick_prefix;           // an infinity or NaN in the prefix's V (f32)
+    int32_t pages[64];         // the split's first page table entries
     int16_t up[kMaxTreeNodes];
 };
 __device__ __forceinline__ void find_ancestors(int p, int n, TreeLds &t) {  // p: parents[thread]
@@ -261,7 +265,7 @@ void tree_attn_kernel(TreeArgs a, int S, int units, int unit) {
     constexpr int PL = F32 ? 3 : 1;   // parts (planes) of K and V
     constexpr int TB = T * HD * 2;    // bytes of a tile's plane
     extern __shared__ __attribute__((aligned(256))) uint8_t smem[];
-    uint8_t *ks = smem, *vs = smem + (F32 ? 3 : 2) * TB;
+    uint8_t *ks = smem, *vs = smem + PL * TB;  // the second BF16 tile, 2 TB on
     TreeLds &tree = *(TreeLds *)(smem + tree_tile_lds<HD, KT>());
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -293,7 +297,10 @@ void tree_attn_kernel(TreeArgs a, int S, int units, int unit) {
     const int last_page = (end - 1) / a.page_size;
     int page_i = __builtin_amdgcn_readfirstlane(start / a.page_size), held_0 = page_i;
     int page_at = start - page_i * a.page_size;
-    int held = a.page_table[min(held_0 + lane, last_page)];
+    // The first ones by one wave, for all: a CU's loads return in order, and the
+    // second four waves' own would come behind the first four's copies (at 2.7 us
+    // where the first four's come at 0.7).
+    int held = wave == 0 ? a.page_table[min(held_0 + lane, last_page)] : 0;
     int page[T / 64], row0[T / 64];  // of the next tile to fetch
     auto next_pages = [&](int t0) {
 #pragma unroll
@@ -336,7 +343,7 @@ void tree_attn_kernel(TreeArgs a, int S, int units, int unit) {
                     vr[c][1] = *(const f32x4 *)(vp + 4);
                 }
             } else {
-                const int at = b * TB + x * 64 * HD * 2 + wave * 1024;
+                const int at = b * 2 * TB + x * 64 * HD * 2 + wave * 1024;
                 const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
                     (void *)((const uint16_t *)a.k + tile), (short)0, 64 * HD * 2, 0x00020000);
                 const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
@@ -362,7 +369,7 @@ void tree_attn_kernel(TreeArgs a, int S, int units, int unit) {
         for (int c = 0; c < HC * T / 64; ++c) {
             const int p = t0 + lr + 64 * NW / CPR * c;
             if (p < a.offset) continue;
-            u32x4 *at = (u32x4 *)(vs + b * TB + wave * 1024 + 1024 * NW * c + 16 * lane);
+            u32x4 *at = (u32x4 *)(vs + b * 2 * TB + wave * 1024 + 1024 * NW * c + 16 * lane);
             bool bad = p >= end;
             if (!bad) {
                 const u32x4 w = *at;
@@ -399,33 +406,61 @@ void tree_attn_kernel(TreeArgs a, int S, int units, int unit) {
         }
     };
 
-    // The parents first: behind the tile's copies they would arrive after them.
+    // What the tile's copies would hold up is asked for before them: the parents,
+    // and the queries. The key waves of a row wave load and cut a part of its
+    // fragments each (cutting all of them takes a wave 0.8 us) and hand them on in
+    // LDS, where the first tile does not come: f32 the tile's place itself, BF16
+    // the second tile's, in as many rounds as it takes.
+    constexpr int OWN = KSTEPS / WK;
+    constexpr int ROUNDS = WK == 1 ? 1 : (WR * KSTEPS * 3072 + (F32 ? 6 : 2) * TB - 1) / ((F32 ? 6 : 2) * TB);
+    constexpr int KR = KSTEPS / ROUNDS;
+    static_assert(KR % WK == 0, "a wave has a step of every round");
     const int parent = in_tree && (int)threadIdx.x < a.n ? a.parents[threadIdx.x] : -1;
+    f32x4 raw[OWN][2];
+    {
+        const float *qp = a.q + ((size_t)node * a.q_heads + head) * HD + 8 * half;
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+            raw[i][0] = *(const f32x4 *)(qp + 16 * (i * WK + wk));
+            raw[i][1] = *(const f32x4 *)(qp + 16 * (i * WK + wk) + 4);
+        }
+    }
+    if (wave == 0) tree.pages[lane] = held;
+    if (threadIdx.x < 4) tree.odd[threadIdx.x] = 0;
+    if (threadIdx.x == 0) tree.sick_prefix = 0;
+    lds_barrier();
+    held = tree.pages[lane];
     next_pages(start);
     fetch(start, 0);
     next_pages(start + T);
-    if (threadIdx.x < 4) tree.odd[threadIdx.x] = 0;
-    if (threadIdx.x == 0) tree.sick_prefix = 0;
-    if (in_tree) find_ancestors(parent, a.n, tree);
 
     bf16x8 q3[KSTEPS][3];
-    {
-        const float sl2 = (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f;
-        const float *qp = a.q + ((size_t)node * a.q_heads + head) * HD + 8 * half;
-        const float sq = rvalid ? sl2 : 0.f;  // rows without a query: their scores are not used
-        f32x4 raw[KSTEPS][2];  // every load before the first use: one round trip
+    const float sq = rvalid ? (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f : 0.f;  // (no query: scores not used)
 #pragma unroll
-        for (int s = 0; s < KSTEPS; ++s) {
-            raw[s][0] = *(const f32x4 *)(qp + 16 * s);
-            raw[s][1] = *(const f32x4 *)(qp + 16 * s + 4);
+    for (int round = 0; round < ROUNDS; ++round) {
+        uint8_t *at = smem + (F32 ? 0 : 2 * TB) + wr * KR * 3072 + lane * 16;
+        if (round) lds_barrier();  // the last one's are read
+#pragma unroll
+        for (int i = round * KR / WK; i < (round + 1) * KR / WK; ++i) {
+            const float v[8] = {raw[i][0][0] * sq, raw[i][0][1] * sq, raw[i][0][2] * sq, raw[i][0][3] * sq,
+                                raw[i][1][0] * sq, raw[i][1][1] * sq, raw[i][1][2] * sq, raw[i][1][3] * sq};
+            bf16x8 w[3];
+            cut3x8(v, w);
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+                if constexpr (WK == 1) q3[i][k] = w[k];
+                else *(bf16x8 *)(at + ((i * WK + wk - round * KR) * 3 + k) * 1024) = w[k];
         }
+        if constexpr (WK > 1) {
+            lds_barrier();
 #pragma unroll
-        for (int s = 0; s < KSTEPS; ++s) {
-            const float v[8] = {raw[s][0][0] * sq, raw[s][0][1] * sq, raw[s][0][2] * sq, raw[s][0][3] * sq,
-                                raw[s][1][0] * sq, raw[s][1][1] * sq, raw[s][1][2] * sq, raw[s][1][3] * sq};
-            cut3x8(v, q3[s]);
+            for (int i = 0; i < KR; ++i)
+#pragma unroll
+                for (int k = 0; k < 3; ++k) q3[round * KR + i][k] = *(const bf16x8 *)(at + (i * 3 + k) * 1024);
         }
     }
+    if constexpr (F32 && WK > 1) lds_barrier();  // read before the tile comes in their place
+    if (in_tree) find_ancestors(parent, a.n, tree);
     // This lane's transposing V reads in a 16-position block: rows
     // 8 half + i / 4 (and + 4), dims 32 u + 16 ((lane / 16) % 2) + 4 (i % 4).
     const int vi = lane & 15, vrow = 8 * half + (vi >> 2);
@@ -464,8 +499,8 @@ void tree_attn_kernel(TreeArgs a, int S, int units, int unit) {
             if (t0 + p0 >= end) break;
             uint32_t vad[UT];
 #pragma unroll
-            for (int u = 0; u < UT; ++u) vad[u] = (vbase + b * TB + p0 * HD * 2) ^ (64 * u);
-            const int kat = kbase + b * TB + p0 * HD * 2;
+            for (int u = 0; u < UT; ++u) vad[u] = (vbase + b * 2 * TB + p0 * HD * 2) ^ (64 * u);
+            const int kat = kbase + b * 2 * TB + p0 * HD * 2;
             // BF16: every K fragment of the step in flight at once. (f32: three parts
             // of each would take the registers of the second wave at head_dim 64.)
             bf16x8 ka[F32 ? 1 : KSTEPS][PL];
