@@ -813,12 +813,33 @@ __global__ __launch_bounds__(kThreads) void tree_commit_kernel(CommitArgs a) {
 
 namespace {
 
-// Row waves of a block: one for up to 32 rows, else two or four, the fewer
-// where four would leave two of the last block without rows. f32: two or four.
+// Splits of whole tiles that a KV head's rows could use: a tile each, but up to two
+// BF16 tiles in one, which a block walks sooner than two blocks join (5 nodes on
+// 250, 14 / 2 heads of 64: 7.4 and 9.0 us; 24 on 120, 32 / 8 of 128: 10.4 and 11.2).
+size_t tree_wanted(const TreeJob &j) {
+    const size_t tile = j.g.kv_f32 ? tree_tile<float>() : tree_tile<uint16_t>();
+    const size_t tiles = (j.offset + j.n + tile - 1) / tile;
+    return !j.g.kv_f32 && tiles <= 2 ? 1 : tiles;
+}
+
+// Splits that one block a CU (f32 at head_dim 64: two) lets a KV head have, with wr
+// row waves a block.
+size_t tree_room(const TreeJob &j, int wr) {
+    const size_t rows = j.n * (size_t)(j.q_heads / j.g.kv_heads), rb = (rows + 32 * wr - 1) / (32 * wr);
+    const size_t slots = (j.g.kv_f32 && j.g.head_dim == 64 ? 2 : 1) * (size_t)std::max(device_cus(), 8);
+    return std::max<size_t>(std::max<size_t>(slots / 8 / rb, 1) * 8 / (size_t)j.g.kv_heads, 1);
+}
+
+// Row waves of a block. While every split wanted has a block of its own anyway, the
+// fewest that let it: short walks, and CUs that would stand idle otherwise (16
+// nodes on 700, 28 / 4 heads of 128: four waves 16.2 us, two 12.8, one 11.6; 32 on
+// 500, f32, four 21.7, two 17.7). Else one for up to 32 rows, two or four for more,
+// the fewer where four would leave two of the last block without rows.
 int tree_row_waves(const TreeJob &j) {
     const int rows = (int)j.n * (j.q_heads / j.g.kv_heads), waves = (rows + 31) / 32;
-    if (waves == 1 && !j.g.kv_f32) return 1;
-    return waves <= 2 || waves % 4 == 1 || waves % 4 == 2 ? 2 : 4;
+    for (int wr = j.g.kv_f32 ? 2 : 1; wr < 4; wr *= 2)  // f32: two or four
+        if (waves <= wr || tree_wanted(j) <= tree_room(j, wr)) return wr;
+    return waves % 4 == 1 || waves % 4 == 2 ? 2 : 4;
 }
 
 template <int HD, int WR, int WK, class KT>
@@ -862,16 +883,7 @@ int launch_tree_h(const TreeJob &j, const TreeArgs &a, int S, int units, int uni
 // head_dim 64: two), of a tile at least; at least 8 (split, KV head) pairs go to the
 // XCDs in turn, so that their number is brought down to a multiple of 8.
 int tree_attention_splits(const TreeJob &j) {
-    const int rows = (int)j.n * (j.q_heads / j.g.kv_heads), wr = tree_row_waves(j);
-    const size_t tile = j.g.kv_f32 ? tree_tile<float>() : tree_tile<uint16_t>();
-    const size_t tiles = (j.offset + j.n + tile - 1) / tile;
-    const size_t slots = (j.g.kv_f32 && j.g.head_dim == 64 ? 2 : 1) * (size_t)std::max(device_cus(), 8);
-    const size_t rb = (size_t)((rows + 32 * wr - 1) / (32 * wr)), kvh = (size_t)j.g.kv_heads;
-    const size_t pairs = std::max<size_t>(slots / 8 / rb, 1) * 8;
-    // One block walks two BF16 tiles sooner than two blocks join (5 nodes on 250,
-    // 14 / 2 heads of 64: 9.1 and 10.6 us; 24 on 120, 32 / 8 of 128: 15.9 and 17.1).
-    if (!j.g.kv_f32 && tiles <= 2) return 1;
-    return (int)std::min({std::max<size_t>(pairs / kvh, 1), tiles, (size_t)attention_max_splits()});
+    return (int)std::min({tree_wanted(j), tree_room(j, tree_row_waves(j)), (size_t)attention_max_splits()});
 }
 
 int launch_tree_attention(const TreeJob &j, hipStream_t s) {
