@@ -256,7 +256,7 @@ constexpr size_t tree_lds_bytes() { return tree_tile_lds<HD, KT>() + sizeof(Tree
 
 template <int HD, int WR, int WK, class KT>
 __global__ __launch_bounds__(64 * WR * WK) __attribute__((amdgpu_waves_per_eu(WR * WK / 4)))
-void tree_attn_kernel(TreeArgs a, int S, int units, int unit) {
+void tree_attn_kernel(TreeArgs a, int S) {
     constexpr bool F32 = sizeof(KT) == 4;
     constexpr int NW = WR * WK, T = tree_tile<KT>(), STEPS = T / (32 * WK);
     constexpr int KSTEPS = HD / 16, UT = HD / 32;
@@ -278,13 +278,13 @@ void tree_attn_kernel(TreeArgs a, int S, int units, int unit) {
     const int m0 = rb * 32 * WR, m = m0 + wr * 32 + n;
     const bool rvalid = m < M;
     const int node = rvalid ? m / G : 0, head = g * G + (rvalid ? m % G : 0);
-    // units / S runs of `unit` positions a split, the first ones one more. (Block-
-    // uniform, said to the compiler: the quotients come from vector registers.)
-    const int each = units / S, extra = units % S;
+    // A run of tiles a split, the first ones one more. (Block-uniform, said to the
+    // compiler: the quotients come from vector registers.)
+    const int tiles = (a.offset + a.n - 1) / T + 1, each = tiles / S, extra = tiles % S;
     const int first = split * each + min(split, extra);
-    const int start = __builtin_amdgcn_readfirstlane(first * unit);
+    const int start = __builtin_amdgcn_readfirstlane(first * T);
     const int end = __builtin_amdgcn_readfirstlane(
-        (int)min((unsigned)(first + each + (split < extra)) * unit, (unsigned)(a.offset + (min(M, m0 + 32 * WR) - 1) / G + 1)));
+        (int)min((unsigned)(first + each + (split < extra)) * T, (unsigned)(a.offset + (min(M, m0 + 32 * WR) - 1) / G + 1)));
     const size_t at_part = ((size_t)node * a.q_heads + head) * S + split;
     if (start >= end) {  // no row of the block reaches the split
         if (rvalid && wk == 0 && half == 0) a.ml[at_part] = make_float2(-INFINITY, 0.f);
@@ -409,12 +409,10 @@ void tree_attn_kernel(TreeArgs a, int S, int units, int unit) {
     // What the tile's copies would hold up is asked for before them: the parents,
     // and the queries. The key waves of a row wave load and cut a part of its
     // fragments each (cutting all of them takes a wave 0.8 us) and hand them on in
-    // LDS, where the first tile does not come: f32 the tile's place itself, BF16
-    // the second tile's, in as many rounds as it takes.
+    // LDS, where the first tile does not come: BF16 in the second tile's place, f32
+    // in its own.
     constexpr int OWN = KSTEPS / WK;
-    constexpr int ROUNDS = WK == 1 ? 1 : (WR * KSTEPS * 3072 + (F32 ? 6 : 2) * TB - 1) / ((F32 ? 6 : 2) * TB);
-    constexpr int KR = KSTEPS / ROUNDS;
-    static_assert(KR % WK == 0, "a wave has a step of every round");
+    static_assert(WK == 1 || WR * KSTEPS * 3072 <= (F32 ? 6 : 2) * TB, "room for the fragments");
     const int parent = in_tree && (int)threadIdx.x < a.n ? a.parents[threadIdx.x] : -1;
     f32x4 raw[OWN][2];
     {
@@ -436,28 +434,24 @@ void tree_attn_kernel(TreeArgs a, int S, int units, int unit) {
 
     bf16x8 q3[KSTEPS][3];
     const float sq = rvalid ? (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f : 0.f;  // (no query: scores not used)
+    uint8_t *at = smem + (F32 ? 0 : 2 * TB) + wr * KSTEPS * 3072 + lane * 16;
 #pragma unroll
-    for (int round = 0; round < ROUNDS; ++round) {
-        uint8_t *at = smem + (F32 ? 0 : 2 * TB) + wr * KR * 3072 + lane * 16;
-        if (round) lds_barrier();  // the last one's are read
+    for (int i = 0; i < OWN; ++i) {
+        const float v[8] = {raw[i][0][0] * sq, raw[i][0][1] * sq, raw[i][0][2] * sq, raw[i][0][3] * sq,
+                            raw[i][1][0] * sq, raw[i][1][1] * sq, raw[i][1][2] * sq, raw[i][1][3] * sq};
+        bf16x8 w[3];
+        cut3x8(v, w);
 #pragma unroll
-        for (int i = round * KR / WK; i < (round + 1) * KR / WK; ++i) {
-            const float v[8] = {raw[i][0][0] * sq, raw[i][0][1] * sq, raw[i][0][2] * sq, raw[i][0][3] * sq,
-                                raw[i][1][0] * sq, raw[i][1][1] * sq, raw[i][1][2] * sq, raw[i][1][3] * sq};
-            bf16x8 w[3];
-            cut3x8(v, w);
+        for (int k = 0; k < 3; ++k)
+            if constexpr (WK == 1) q3[i][k] = w[k];
+            else *(bf16x8 *)(at + ((i * WK + wk) * 3 + k) * 1024) = w[k];
+    }
+    if constexpr (WK > 1) {
+        lds_barrier();
 #pragma unroll
-            for (int k = 0; k < 3; ++k)
-                if constexpr (WK == 1) q3[i][k] = w[k];
-                else *(bf16x8 *)(at + ((i * WK + wk - round * KR) * 3 + k) * 1024) = w[k];
-        }
-        if constexpr (WK > 1) {
-            lds_barrier();
+        for (int i = 0; i < KSTEPS; ++i)
 #pragma unroll
-            for (int i = 0; i < KR; ++i)
-#pragma unroll
-                for (int k = 0; k < 3; ++k) q3[round * KR + i][k] = *(const bf16x8 *)(at + (i * 3 + k) * 1024);
-        }
+            for (int k = 0; k < 3; ++k) q3[i][k] = *(const bf16x8 *)(at + (i * 3 + k) * 1024);
     }
     if constexpr (F32 && WK > 1) lds_barrier();  // read before the tile comes in their place
     if (in_tree) find_ancestors(parent, a.n, tree);
@@ -830,43 +824,50 @@ size_t tree_room(const TreeJob &j, int wr) {
     return std::max<size_t>(std::max<size_t>(slots / 8 / rb, 1) * 8 / (size_t)j.g.kv_heads, 1);
 }
 
-// Row waves of a block. While every split wanted has a block of its own anyway, the
-// fewest that let it: short walks, and CUs that would stand idle otherwise (16
-// nodes on 700, 28 / 4 heads of 128: four waves 16.2 us, two 12.8, one 11.6; 32 on
-// 500, f32, four 21.7, two 17.7). Else one for up to 32 rows, two or four for more,
-// the fewer where four would leave two of the last block without rows.
+// Row waves of a block: one for up to 32 rows, two for more. While every split
+// wanted has a block of its own anyway, the fewest that let it: short walks, and CUs
+// that would stand idle otherwise (16 nodes on 700, 28 / 4 heads of 128: two 12.8 us,
+// one 11.6; 32 on 500, f32, four 21.7, two 17.7). Twice as many with half the key
+// waves halve the tiles' traffic and double the partials': over BF16 that never
+// paid (64 nodes on 16k, 32 / 8 heads of 128: four 53.9 us, two 51.4; 18 on 16k,
+// 28 / 4: 27.6 and 22.3). f32 tiles cost their staging too: four at head_dim 128
+// (128 on 8k, 32 / 8: 61.3 us, two 68.2; head_dim 64, 256 on 8k, 14 / 2: 34.6 and
+// 33.2), unless they would leave two of the last block without rows.
 int tree_row_waves(const TreeJob &j) {
     const int rows = (int)j.n * (j.q_heads / j.g.kv_heads), waves = (rows + 31) / 32;
-    for (int wr = j.g.kv_f32 ? 2 : 1; wr < 4; wr *= 2)  // f32: two or four
-        if (waves <= wr || tree_wanted(j) <= tree_room(j, wr)) return wr;
-    return waves % 4 == 1 || waves % 4 == 2 ? 2 : 4;
+    if (!j.g.kv_f32) return waves == 1 || tree_wanted(j) <= tree_room(j, 1) ? 1 : 2;
+    const bool two = waves <= 2 || waves % 4 == 1 || waves % 4 == 2 || tree_wanted(j) <= tree_room(j, 2);
+    return two || j.g.head_dim == 64 ? 2 : 4;
 }
 
 template <int HD, int WR, int WK, class KT>
-int launch_tree_blocks(const TreeArgs &a, int S, int units, int unit, hipStream_t s) {
+int launch_tree_blocks(const TreeArgs &a, int S, hipStream_t s) {
     constexpr size_t lds = tree_lds_bytes<HD, KT>();
     static std::atomic<uint64_t> lds_set{0};
     CHIP_TRY(allow_dynamic_lds((const void *)tree_attn_kernel<HD, WR, WK, KT>, lds, lds_set));
     const int rb = (a.n * (a.q_heads / a.kv_heads) + 32 * WR - 1) / (32 * WR);
     const size_t blocks = ((size_t)S * a.kv_heads + 7) / 8 * 8 * (size_t)rb;
     if (blocks > (size_t)INT32_MAX) return fail("HIP backend: tree attention grid out of range.");
-    hipLaunchKernelGGL((tree_attn_kernel<HD, WR, WK, KT>), dim3((unsigned)blocks), dim3(64 * WR * WK), lds, s, a, S,
-                       units, unit);
+    hipLaunchKernelGGL((tree_attn_kernel<HD, WR, WK, KT>), dim3((unsigned)blocks), dim3(64 * WR * WK), lds, s, a, S);
     CHIP_CHECK(hipGetLastError());
     return 0;
 }
 
 template <int HD>
-int launch_tree_h(const TreeJob &j, const TreeArgs &a, int S, int units, int unit, hipStream_t s) {
+int launch_tree_rows(const TreeJob &j, const TreeArgs &a, int S, hipStream_t s) {
     const int wr = tree_row_waves(j);
-    if (j.g.kv_f32) {
-        if (wr == 2) CHIP_TRY((launch_tree_blocks<HD, 2, 2, float>(a, S, units, unit, s)));
-        else CHIP_TRY((launch_tree_blocks<HD, 4, 1, float>(a, S, units, unit, s)));
-    } else {
-        if (wr == 1) CHIP_TRY((launch_tree_blocks<HD, 1, 4, uint16_t>(a, S, units, unit, s)));
-        else if (wr == 2) CHIP_TRY((launch_tree_blocks<HD, 2, 4, uint16_t>(a, S, units, unit, s)));
-        else CHIP_TRY((launch_tree_blocks<HD, 4, 2, uint16_t>(a, S, units, unit, s)));
+    if (!j.g.kv_f32) {
+        if (wr == 1) return launch_tree_blocks<HD, 1, 4, uint16_t>(a, S, s);
+        return launch_tree_blocks<HD, 2, 4, uint16_t>(a, S, s);
     }
+    if constexpr (HD == 128)
+        if (wr == 4) return launch_tree_blocks<HD, 4, 1, float>(a, S, s);
+    return launch_tree_blocks<HD, 2, 2, float>(a, S, s);
+}
+
+template <int HD>
+int launch_tree_h(const TreeJob &j, const TreeArgs &a, int S, hipStream_t s) {
+    CHIP_TRY(launch_tree_rows<HD>(j, a, S, s));
     if (S == 1) return 0;
     const int items = (int)j.n * j.q_heads;
     if (S > 16)
@@ -894,13 +895,7 @@ int launch_tree_attention(const TreeJob &j, hipStream_t s) {
     int S = tree_attention_splits(j);
     const size_t split_floats = attention_part_floats(j.n, j.q_heads, 1, j.g.head_dim);
     if (S > 1) S = (int)std::min<size_t>((size_t)S, std::max<size_t>(j.part ? j.part_floats / split_floats : 1, 1));
-    // Splits of whole tiles, or of half ones where that makes the longest shorter
-    // (64 nodes on 16k, 9 or 8.5 tiles: 57.2 -> 55.4 us; 256 on 4k, 9 either way:
-    // 55.6, with half tiles 57.0).
-    const int tile = j.g.kv_f32 ? tree_tile<float>() : tree_tile<uint16_t>(), items = (int)j.n * j.q_heads;
-    auto units_of = [&](int unit) { return (int)((j.offset + j.n - 1) / (size_t)unit) + 1; };
-    auto longest = [&](int unit) { return (long)((units_of(unit) + S - 1) / S) * unit; };
-    const int unit = longest(64) < longest(tile) ? 64 : tile, units = units_of(unit);
+    const int items = (int)j.n * j.q_heads;
     TreeArgs a{};
     a.q = j.q;
     a.k = j.k;
@@ -917,8 +912,8 @@ int launch_tree_attention(const TreeJob &j, hipStream_t s) {
     a.q_heads = j.q_heads;
     a.offset = (int)j.offset;
     a.n = (int)j.n;
-    if (j.g.head_dim == 64) return launch_tree_h<64>(j, a, S, units, unit, s);
-    return launch_tree_h<128>(j, a, S, units, unit, s);
+    if (j.g.head_dim == 64) return launch_tree_h<64>(j, a, S, s);
+    return launch_tree_h<128>(j, a, S, s);
 }
 
 int launch_tree_commit(const KvLayer *layers, const int32_t *const *page_tables, size_t views, const KvGeom &g,
