@@ -414,6 +414,13 @@ int cheetah_hip_tree_commit(const cheetah_hip_kv_view *views, size_t nviews, uin
         if (views[i].page_size != views[0].page_size || views[i].kv_heads != views[0].kv_heads ||
             views[i].head_dim != views[0].head_dim)
             return fail("HIP backend: tree commit needs views of one geometry.");
+        // Moved by two blocks at once, a row could be read after it was replaced.
+        bool twice = views[i].k_pages == views[i].v_pages;
+        for (size_t h = 0; h < i; ++h)
+            twice |= views[h].page_table == views[i].page_table &&
+                     (views[h].k_pages == views[i].k_pages || views[h].v_pages == views[i].v_pages ||
+                      views[h].k_pages == views[i].v_pages || views[h].v_pages == views[i].k_pages);
+        if (twice) return fail("HIP backend: tree commit with a cache listed twice.");
     }
     for (size_t j = 0; j < count; ++j)
         if (nodes[j] >= CHEETAH_HIP_MAX_TREE_NODES || (j && nodes[j] <= nodes[j - 1]))

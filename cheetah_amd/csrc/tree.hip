@@ -244,6 +244,14 @@ __device__ __forceinline__ void read_vt2(const uint32_t (&addr)[HD / 32], bf16x8
 // Splits are runs of positions, joined by tree_merge_kernel. Blocks with
 // the same (split, KV head) and other rows are 8 apart, on one XCD: they read
 // the same tiles through its L2.
+//
+// Bound, long contexts: the matrix cores. 64 nodes on 16k (32 / 8 heads of 128)
+// take 51.5 us for 17.2 Gflop, 51.5 of them executed, 1.2 PFLOP/s in the loop,
+// what a large BF16 matrix product reaches (1.21). Around the loop's 43: 2.7 before
+// the first product, 1.2 for the key waves' join, 0.8 to write the partials, 2.5 a
+// launch, 4 the merge. Priorities or a late start for half of the waves change
+// nothing. Short contexts: those steps. 16 nodes on 2k 14.7 us, its tile 2.2 of
+// them; 5 on 60 (14 / 2 heads of 64) 6.7, one launch.
 // ---------------------------------------------------------------------------
 template <class KT>
 constexpr int tree_tile() { return sizeof(KT) == 2 ? 128 : 64; }
@@ -771,7 +779,8 @@ static_assert(sizeof(CommitArgs) <= 4096, "a launch's arguments");
 // before any of them is written, and a later batch's sources are past everything
 // an earlier one wrote. Bound: three dependent round trips to memory, the page
 // table's, the reads' and the writes' (a thread that walked the branch down its
-// own column took one for each eight rows: 40 rows of 32 f32 caches 21.3 us).
+// own column took one for each eight rows: 40 rows of 32 f32 caches 21.3 us, so
+// 6.4; 3 rows of 24 BF16 caches 4.9, a launch).
 constexpr int kMoves = 8;
 __global__ __launch_bounds__(kThreads) void tree_commit_kernel(CommitArgs a) {
     __shared__ size_t row[2][kMaxTreeNodes];  // byte offsets of the sources, the destinations

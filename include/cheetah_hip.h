@@ -243,15 +243,17 @@ int cheetah_hip_decode_greedy(cheetah_hip_model *m, uint32_t token, size_t offse
  *     commit_tree or until anything else runs on this instance or clears or
  *     restores its cache, which drops them.
  *   commit_tree: keeps a branch of that tree, nodes[count] from a child of the
- *     cached text to any node, each followed by a child of it; the cache is then
- *     as if the branch's tokens had been run alone. count 0 drops the tree.
+ *     cached text to any node, each followed by a child of it; the cache then
+ *     holds the branch's tokens, as if they had been run alone (up to the
+ *     rounding of a chunk's products). count 0 drops the tree.
  *   verify_tree: forward_tree and commit_tree in one call, greedily. Node 0 is
  *     the only root: the last token sampled, not yet in the cache. From it the
  *     walk goes to the child whose token is the argmax while there is one (the
  *     first such child). accepted[n] receives the walk's nodes, *count (at least
  *     1) their number, *next_token the argmax behind the last of them: what
- *     `count` steps of greedy decoding would have sampled. The cache then holds
- *     the accepted tokens. */
+ *     `count` steps of greedy decoding would have sampled (but for near ties: a
+ *     tree's products are a chunk's, which round otherwise than a decode step's).
+ *     The cache then holds the accepted tokens. */
 int cheetah_hip_forward_tree(cheetah_hip_model *m, const uint32_t *tokens, const int32_t *parents, size_t n,
                              size_t offset, uint32_t *next_tokens, float *logits_out);
 int cheetah_hip_commit_tree(cheetah_hip_model *m, const uint32_t *nodes, size_t count);

@@ -20,7 +20,7 @@ def refused(hip, rc, text):
 
 
 def view(hip, **kw):
-    a = dict(k=D, v=D, table=D, page=64, kvh=2, hd=64)
+    a = dict(k=D, v=2 * D, table=3 * D, page=64, kvh=2, hd=64)
     a.update(kw)
     return hip.KvView(a["k"], a["v"], a["table"], a["page"], a["kvh"], a["hd"])
 
@@ -68,6 +68,19 @@ def test_tree_commit_refuses_views(hip):
     refused(hip, call((hip.KvView * 1)(view(hip, hd=32)), 1, 0, 0, nodes, 2), "head_dim")
     for other in (dict(page=128), dict(kvh=4), dict(hd=128)):
         refused(hip, call((hip.KvView * 2)(view(hip), view(hip, **other)), 2, 0, 0, nodes, 2), "one geometry")
+
+
+@pytest.mark.parametrize("other", [dict(), dict(v=5 * D), dict(k=5 * D), dict(k=2 * D, v=5 * D), dict(k=5 * D, v=D)])
+def test_tree_commit_refuses_a_cache_listed_twice(hip, other):
+    """Two views that share a pool and its page table, or one whose K and V are
+    the same pool; a pool with another page table (another sequence) may come."""
+    call, nodes = hip.lib().cheetah_hip_tree_commit, (ctypes.c_uint32 * 2)(0, 2)
+    refused(hip, call((hip.KvView * 3)(view(hip), view(hip, k=7 * D, v=8 * D), view(hip, **other)), 3, 0, 0, nodes, 2),
+            "listed twice")
+    refused(hip, call((hip.KvView * 1)(view(hip, v=D)), 1, 0, 0, nodes, 2), "listed twice")
+    if not hip._initialized:  # (it would run)
+        two = (hip.KvView * 2)(view(hip), view(hip, table=6 * D, **other))
+        refused(hip, call(two, 2, 0, 0, nodes, 2), "not initialized")
 
 
 @pytest.mark.parametrize("change,text", [
