@@ -419,8 +419,8 @@ void tree_attn_kernel(TreeArgs a, int S) {
     // fragments each (cutting all of them takes a wave 0.8 us) and hand them on in
     // LDS, where the first tile does not come: BF16 in the second tile's place, f32
     // in its own.
-    constexpr int OWN = KSTEPS / WK;
-    static_assert(WK == 1 || WR * KSTEPS * 3072 <= (F32 ? 6 : 2) * TB, "room for the fragments");
+    constexpr int OWN = KSTEPS / WK, kFragments = 3 * 1024;  // a step's three parts, 16 bytes a lane
+    static_assert(WK == 1 || WR * KSTEPS * kFragments <= (F32 ? 6 : 2) * TB, "room for the fragments");
     const int parent = in_tree && (int)threadIdx.x < a.n ? a.parents[threadIdx.x] : -1;
     f32x4 raw[OWN][2];
     {
@@ -442,7 +442,7 @@ void tree_attn_kernel(TreeArgs a, int S) {
 
     bf16x8 q3[KSTEPS][3];
     const float sq = rvalid ? (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f : 0.f;  // (no query: scores not used)
-    uint8_t *at = smem + (F32 ? 0 : 2 * TB) + wr * KSTEPS * 3072 + lane * 16;
+    uint8_t *at = smem + (F32 ? 0 : 2 * TB) + wr * KSTEPS * kFragments + lane * 16;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
         const float v[8] = {raw[i][0][0] * sq, raw[i][0][1] * sq, raw[i][0][2] * sq, raw[i][0][3] * sq,

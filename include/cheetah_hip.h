@@ -147,8 +147,8 @@ int cheetah_hip_tree_attention(const float *q, const cheetah_hip_kv_view *kv, ui
  * K/V rows of positions offset + nodes[j] move to offset + j, j = 0 .. count-1.
  * nodes (host) is strictly increasing and below CHEETAH_HIP_MAX_TREE_NODES: a
  * root and its descendants in order. The views (host array) may have page
- * tables of their own but one page size, KV head count and head_dim, and no
- * cache may be listed twice. Rows past the branch are left as they are. */
+ * tables of their own but one page size, KV head count and head_dim; a cache
+ * listed twice (a pool with the same page table) is refused. Rows past the branch are left as they are. */
 int cheetah_hip_tree_commit(const cheetah_hip_kv_view *views, size_t nviews, uint32_t kv_format, size_t offset,
                             const uint32_t *nodes, size_t count);
 
