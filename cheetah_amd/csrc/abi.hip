@@ -386,7 +386,7 @@ int cheetah_hip_tree_attention(const float *q, const cheetah_hip_kv_view *kv, ui
     if (q_heads == 0 || q_heads > 65535 || q_heads % kv->kv_heads)
         return fail("HIP backend: q_heads must be a multiple of kv_heads.");
     if (q_heads / kv->kv_heads > 8) return fail("HIP backend: attention supports 1..8 query heads per KV head.");
-    if (offset > (size_t)INT32_MAX - n) return fail("HIP backend: tree position out of range.");
+    if (offset > kMaxTreePositions - n) return fail("HIP backend: tree position out of range.");
     if (((uintptr_t)q | (uintptr_t)out) % 16 || (uintptr_t)parents % 4)
         return fail("HIP backend: tree attention needs 16-byte aligned q and out, 4-byte aligned parents.");
     CHIP_TRY(ensure_ready());
@@ -426,7 +426,7 @@ int cheetah_hip_tree_commit(const cheetah_hip_kv_view *views, size_t nviews, uin
         if (nodes[j] >= CHEETAH_HIP_MAX_TREE_NODES || (j && nodes[j] <= nodes[j - 1]))
             return fail("HIP backend: a branch is strictly increasing nodes below " +
                         std::to_string(CHEETAH_HIP_MAX_TREE_NODES) + ".");
-    if (offset > (size_t)INT32_MAX - CHEETAH_HIP_MAX_TREE_NODES)
+    if (offset > kMaxTreePositions - CHEETAH_HIP_MAX_TREE_NODES)
         return fail("HIP backend: tree position out of range.");
     CHIP_TRY(ensure_ready());
     const KvGeom g{nullptr, (int)views[0].page_size, (int)views[0].kv_heads, (int)views[0].head_dim, (int)kv_format};

@@ -231,6 +231,9 @@ int attention_prefill_span(size_t kv_capacity, bool kv_f32);
 // Drafted tokens (tree.hip).
 // ---------------------------------------------------------------------------
 constexpr int kMaxTreeNodes = 256;  // CHEETAH_HIP_MAX_TREE_NODES
+// Positions of a prefix and its tree: the kernel's tile bounds behind the last one
+// stay below 2^31.
+constexpr size_t kMaxTreePositions = (size_t)INT32_MAX - 1023;
 // Views a launch of the commit moves (its arguments hold them).
 constexpr int kCommitViews = 128;
 

@@ -899,7 +899,7 @@ int tree_attention_splits(const TreeJob &j) {
 int launch_tree_attention(const TreeJob &j, hipStream_t s) {
     if (!j.q || (!j.out && !j.out_hi) || !j.out_hi != !j.out_lo || !j.k || !j.v || !j.g.page_table || !j.parents)
         return fail("HIP backend: tree attention is missing a buffer.");
-    if (j.n == 0 || j.n > (size_t)kMaxTreeNodes || j.offset > (size_t)INT32_MAX - j.n)
+    if (j.n == 0 || j.n > (size_t)kMaxTreeNodes || j.offset > kMaxTreePositions - j.n)
         return fail("HIP backend: tree attention shape out of range.");
     int S = tree_attention_splits(j);
     const size_t split_floats = attention_part_floats(j.n, j.q_heads, 1, j.g.head_dim);

@@ -30,7 +30,7 @@ def view(hip, **kw):
     (dict(n=0), "1 to 256 nodes"), (dict(n=257), "1 to 256 nodes"), (dict(n=1 << 40), "1 to 256 nodes"),
     (dict(fmt=2), "kv_format"), (dict(q_heads=0), "multiple of kv_heads"), (dict(q_heads=3), "multiple of kv_heads"),
     (dict(q_heads=18), "1..8 query heads"), (dict(q_heads=1 << 31), "multiple of kv_heads"),
-    (dict(offset=2**31 - 5), "position out of range"), (dict(offset=2**64 - 1), "position out of range"),
+    (dict(offset=2**31 - 5), "position out of range"), (dict(offset=2**31 - 1024), "position out of range"), (dict(offset=2**64 - 1), "position out of range"),
     (dict(q=D + 4), "aligned"), (dict(out=D + 8), "aligned"), (dict(parents=D + 2), "aligned"),
     (dict(view=dict(k=None)), "null cache"), (dict(view=dict(v=None)), "null cache"),
     (dict(view=dict(table=None)), "null cache"), (dict(view=dict(kvh=0)), "out of range"),

@@ -185,6 +185,42 @@ def test_rows_past_4_gib(hip):
            tops.download(np.float32).reshape(2, 5)), np.stack(rows), tokens, 5)
 
 
+@pytest.mark.parametrize("fmt", ["f32", "bf16"])
+def test_rows_between_one_segment_and_many(hip, fmt):
+    """Row counts where a row's segments go from many to two to one, in turn on
+    one thread's workspace, which grows and is used again by fewer rows."""
+    rng = np.random.default_rng(14)
+    x, values = logits(rng, 600, 20011, 20011, fmt)
+    tokens = rng.integers(0, 20011, 600).astype(np.uint32)
+    for rows in (2, 256, 1, 128, 600, 257, 200, 3, 255, 64, 2):
+        check(hip.logprobs(x[:rows], tokens[:rows], 7), values[:rows], tokens[:rows], 7)
+
+
+def test_threads_call_at_once(hip):
+    """Each thread's segments are counted in a workspace of its own."""
+    import threading
+
+    rng = np.random.default_rng(15)
+    cases = []
+    for i in range(4):
+        x, values = logits(rng, 3 + 40 * i, 30011, 30011, "f32")
+        cases.append((x, values, rng.integers(0, 30011, len(x)).astype(np.uint32)))
+    got = [[] for _ in cases]
+
+    def run(i):
+        for _ in range(5):
+            got[i].append(hip.logprobs(cases[i][0], cases[i][2], 9))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for results, (_, values, tokens) in zip(got, cases):
+        for r in results:
+            check(r, values, tokens, 9)
+
+
 def test_the_same_bits_again(hip):
     rng = np.random.default_rng(12)
     x, _ = logits(rng, 5, 100003, 100003, "f32")

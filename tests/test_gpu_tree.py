@@ -9,9 +9,10 @@ from cheetah_amd import synth
 
 pytestmark = pytest.mark.gpu
 
-# Queries and probabilities are two BF16 halves over a BF16 cache (2^-17 of a
-# value is left out, in products whose signs vary), f32 values over an f32 one:
-# 2e-5 of the largest output.
+# Every product is as exact as an f32 one (three BF16 parts of queries and
+# probabilities, and of an f32 cache), sums are f32: of 6,000 keys' weights at most
+# 6,000 roundings of 2^-25 at random, 5e-6 of the largest output at two deviations;
+# exponentials add 2^-22. 2e-5.
 TOL = 2e-5
 
 
@@ -202,6 +203,22 @@ def test_pools_past_4_gib(hip, kv, page_elems):
     hip.check(hip.lib().cheetah_hip_download(back.ctypes.data, pools[0].ptr + far * page_elems * elem, back.nbytes))
     a, b = (back[table[p // 64], :, p % 64] for p in (offset + 1, offset + 4))
     assert np.array_equal(a, b) and np.array_equal(b, kp[table[1], :, (offset + 4) % 64])
+
+
+@pytest.mark.parametrize("kv", ["bf16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,offset", [(140, 4200), (130, 4096 - 64)])
+def test_a_split_of_many_pages(hip, n, offset, hd, kv):
+    """64 query heads over 8: so many row blocks that a KV head's keys are one
+    split, whose page entries are looked up 64 at a time. One KV head's queries
+    are compared."""
+    rng, q, k, v, (kp, vp, table) = case(n + hd, 64, 8, hd, n, offset, kv)
+    parents = ref.parents_of("random", n, rng)
+    got = hip.tree_attention(q, kp, vp, table, 64, parents, offset)
+    assert np.isfinite(got).all()
+    head = slice(40 * hd, 48 * hd)
+    want = ref.attention64(np.ascontiguousarray(q[:, head]), k[:, 5:6], v[:, 5:6], 8, parents, offset)
+    assert rel_err(got[:, head], want) < TOL
 
 
 # ---------------------------------------------------------------------------
