@@ -14,15 +14,15 @@
 // rows have one segment each; few rows have many, whose results go through memory
 // to the row's last block, which joins them in the same launch.
 //
-// Bound: 512 f32 rows of 152064 (311 MB) with 5 alternatives take 60.7 us, 5.13
-// TB/s, a large copy's rate; BF16 rows take 0.86 of the time (the exponentials then
-// count: 16 of them a thread and chunk). Fewer rows are bound by the steps before
-// and behind the loop, each a memory or LDS round trip: of 64 rows' 20.4 us with 20
-// alternatives the loop ends at 13, the segment's sums and picks are in memory at
-// 14.6, counted at 15.2, read by the last block at 15.6, ranked at 17.6. As two
-// launches these 64 rows took 23.4 us, one row 11.6 (11.6 in one). A release
+// Bound: 512 f32 rows of 151936 (311 MB) with one alternative take 57.4 us, 5.42
+// TB/s, above a large copy's rate (5.16, read and write); BF16 rows 0.79 of the time
+// (the exponentials then count: 16 of them a thread and chunk). Fewer rows are bound
+// by the steps before and behind the loop, each a memory or LDS round trip: of 64
+// rows' 20.1 us with 20 alternatives the loop ends at 13, the segment's sums and
+// picks are in memory and counted at 14.6, read by the last block at 15.3, ranked at
+// 17.5. As two launches these 64 rows took 3 us more, one row the same. A release
 // fence in place of the write-through stores (it writes the whole L2 back) made
-// them 29.6 and 12.2.
+// them 29.6 for then 23.4.
 #include <algorithm>
 #include <type_traits>
 
@@ -181,6 +181,17 @@ struct Best {
     int hist[256], wave_total[kWaves], found[3];
     int count;  // keys held, the best among them; past kRoom: some had no room
 };
+
+// n places for the wave's keys (the same n in its lanes, all of which call).
+__device__ __forceinline__ int best_take(Best &b, int n) {
+    int k = 0;
+    if ((threadIdx.x & 63) == 0) k = atomicAdd(&b.count, n);
+    return __builtin_amdgcn_readfirstlane(k);
+}
+// How many of the lanes in m are below this one.
+__device__ __forceinline__ int lanes_below(uint64_t m) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
 
 // Sorts the keys held and keeps the first `top`. Every wave takes all the keys, R a
 // lane, and a quarter of them to compare with, eight reads in flight; a key's rank
@@ -411,8 +422,14 @@ __device__ __forceinline__ void join_row(const LogprobArgs &a, Best &best, const
     if (lane + 64 < a.segs) s2 = agent_load(a.sums + row * a.segs + lane + 64);
     const int n = a.segs * a.top;
     const Picks src{a.picks + row * n, a.segs, a.top, (n + kThreads - 1) / kThreads};
+    constexpr int HELD = 4;  // picks a thread keeps from the first look at them
+    uint64_t picks[HELD];
+#pragma unroll
+    for (int v = 0; v < HELD; ++v) picks[v] = src.load(v);
     float most = -INFINITY;
-    for (int v = 0; v < src.vectors; ++v) {
+#pragma unroll
+    for (int v = 0; v < HELD; ++v) most = fmaxf(most, picks[v] ? key_value(picks[v]) : -INFINITY);
+    for (int v = HELD; v < src.vectors; ++v) {
         const uint64_t k = src.load(v);
         most = fmaxf(most, k ? key_value(k) : -INFINITY);
     }
@@ -429,13 +446,15 @@ __device__ __forceinline__ void join_row(const LogprobArgs &a, Best &best, const
     s = wave_join(s, m);
     if (a.top) {
         const float from = n <= kThreads ? -INFINITY : best_bound(best, a.top, most);
-        for (int v = 0; v < src.vectors; ++v) {
-            const uint64_t k = src.load(v);
-            if (k && key_value(k) >= from) {
-                const int i = atomicAdd(&best.count, 1);
-                if (i < kRoom) best.key[i] = k;
-            }
-        }
+        auto append = [&](uint64_t k) {
+            const uint64_t m = __ballot(k && key_value(k) >= from);
+            if (!m) return;
+            const int place = best_take(best, __builtin_popcountll(m)) + lanes_below(m);
+            if (k && key_value(k) >= from && place < kRoom) best.key[place] = k;
+        };
+#pragma unroll
+        for (int v = 0; v < HELD; ++v) append(picks[v]);
+        for (int v = HELD; v < src.vectors; ++v) append(src.load(v));
         lds_barrier();
         const bool many = best.count > kRoom;
         lds_barrier();
@@ -478,12 +497,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
     lds_barrier();
     Sums s{0.0, 0.0, -INFINITY, 0};
     // A logit above `last` may be among the best. Waves hand theirs over as they
-    // go; the block looks at them after the first chunk and every kSettle-th, and
-    // takes the chunks since (from `since`) again where they had no room.
-    constexpr int kSettle = 4;
+    // go; the block looks at them after 1, 2, 4, 8, .. chunks, between which as many
+    // more as `top` are to be expected, and takes the chunks since (from `since`)
+    // again where they had no room. (A look every fourth chunk, kept where 64 had
+    // come: 512 rows of 151936 with one alternative 59.9 us, so 57.5; BF16 53.9, so
+    // 45.5; f32 with 64 78.0, so 72.3.)
     float last = -INFINITY;
     unsigned since = begin;
-    int held = 0, chunk = 0;
+    int held = 0, chunk = 0, look = 0;
     for (unsigned e0 = begin; e0 < end; e0 += CHUNK, ++chunk) {
         float x[PER];
 #pragma unroll
@@ -520,19 +541,23 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
         if (!a.top) continue;
         float above = last;
         if (chunk == 0) above = just_below(best_bound(best, a.top, most));  // all of them would be too many
-        if (most > above) {
+        if (__any(most > above)) {
+            // A wave's candidates in one run of places: logit by logit, lane by lane.
             int n = 0;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) n += x[i] > above;
-            int k = atomicAdd(&best.count, n);
+            for (int i = 0; i < PER; ++i) n += __builtin_popcountll(__ballot(x[i] > above));
+            int k = best_take(best, n);
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (x[i] > above) {
-                    if (k < kRoom) best.key[k] = key_of(x[i], at(i) - head);
-                    ++k;
-                }
+            for (int i = 0; i < PER; ++i) {
+                const uint64_t m = __ballot(x[i] > above);
+                if (!m) continue;
+                const int place = k + lanes_below(m);
+                if (x[i] > above && place < kRoom) best.key[place] = key_of(x[i], at(i) - head);
+                k += __builtin_popcountll(m);
+            }
         }
-        if (chunk % kSettle == 0 || e0 + CHUNK >= end) {
+        if (chunk == look || e0 + CHUNK >= end) {
+            look = 2 * chunk + 1;
             lds_barrier();
             const int n = best.count;
             lds_barrier();  // the same in every wave, before one goes on
@@ -544,7 +569,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
                 const Logits<T> src{from, since, head, upto, last_load, last, (int)((upto - since + kThreads * VE - 1) / (kThreads * VE))};
                 best_select(best, a.top, src);
             }
-            if (n >= a.top + 64 || chunk == 0 || e0 + CHUNK >= end) {
+            if (n > held || e0 + CHUNK >= end) {
                 held = best_settle(best, a.top, last);
                 since = e0 + CHUNK;
             }
