@@ -305,6 +305,16 @@ def test_refusals_leave_the_model_as_it_was(hip):
         g.forward_tree([1], [-1], 128)
 
 
+def test_arrays_of_other_lengths_are_refused(hip):
+    g = model(hip, configs.TINY_QWEN2)
+    g.forward([1, 2, 3], 0)
+    for call in (lambda: g.forward_tree([1, 2], [-1], 3), lambda: g.verify_tree([1], [-1, 0], 3),
+                 lambda: g.forward_logprobs([1, 2], 3, targets=[1])):
+        with pytest.raises(ValueError, match="one (parent|target) a token"):
+            call()
+    assert g.kv_len() == 3
+
+
 def test_the_pool_runs_out_under_a_tree(hip):
     """A clone holds the pages that a tree would need: refused, nothing lost."""
     shape = configs.TINY_LLAMA
