@@ -182,6 +182,18 @@ __device__ __forceinline__ void cut3x8(const float (&v)[8], bf16x8 (&out)[3]) {
     for (int k = 0; k < 3; ++k) out[k] = __builtin_bit_cast(bf16x8, w[k]);
 }
 
+// A value that is to be there at this point, in vector or in accumulation registers.
+__device__ __forceinline__ void pin_v(bf16x8 &x) {
+    u32x4 w = __builtin_bit_cast(u32x4, x);
+    asm volatile("" : "+v"(w));
+    x = __builtin_bit_cast(bf16x8, w);
+}
+__device__ __forceinline__ void pin_a(bf16x8 &x) {
+    u32x4 w = __builtin_bit_cast(u32x4, x);
+    asm volatile("" : "+a"(w));
+    x = __builtin_bit_cast(bf16x8, w);
+}
+
 // read_vt of two blocks of 16 positions, OFF and OFF + 16 rows, in one wait.
 template <int HD>
 __device__ __forceinline__ void read_vt2(const uint32_t (&addr)[HD / 32], bf16x8 (&v0)[HD / 32], bf16x8 (&v1)[HD / 32]) {
@@ -225,8 +237,8 @@ __device__ __forceinline__ void read_vt2(const uint32_t (&addr)[HD / 32], bf16x8
 // ---------------------------------------------------------------------------
 // On the matrix cores. The M = n G rows (node, head of the group) of a KV head
 // are cut into waves of 32 and blocks of WR row waves; the WK key waves of a
-// row wave take 32-position steps of the block's tiles in turn and are joined
-// at the end. Per step, as attn_prefill_kernel's:
+// row wave take 32 positions each of the block's tiles and are joined at the end.
+// Per tile, as attn_prefill_kernel's:
 //   S^T = K Q^T     K rows from LDS, Q^T in registers
 //   O^T += V^T P^T  V read transposed, P^T as the scores' registers lie
 // Q (scaled by log2(e) / sqrt(HD)) and P are three BF16 parts each, all 24 bits
@@ -236,10 +248,13 @@ __device__ __forceinline__ void read_vt2(const uint32_t (&addr)[HD / 32], bf16x8
 // the nine part products are taken (attn_prefill_f32_kernel's).
 //
 // BF16 tiles of 128 positions go global to LDS, the next one while the current
-// one computes; f32 tiles of 64 wait in registers and are split while staged.
-// Two waves a SIMD, one's softmax beside the other's products, in one block:
-// two blocks of four waves a CU ran at the pace of their ages, and the younger
-// alone at the end.
+// one computes; two waves a SIMD, one's softmax beside the other's products, in one
+// block: two blocks of four waves a CU ran at the pace of their ages, and the younger
+// alone at the end. f32 tiles of 64 come in registers, two ahead: while the scores
+// are multiplied the next one is cut into its parts, which take the keys' place in
+// LDS when those are read (200 nodes on 2,000, 32 / 8 heads of 128: 90 us when a tile
+// was cut between two others, so 79; its products alone would take 34).
+// The queries then sit in accumulation registers, which products read as well.
 //
 // Splits are runs of positions, joined by tree_merge_kernel. Blocks with
 // the same (split, KV head) and other rows are 8 apart, on one XCD: they read
@@ -256,22 +271,24 @@ __device__ __forceinline__ void read_vt2(const uint32_t (&addr)[HD / 32], bf16x8
 template <class KT>
 constexpr int tree_tile() { return sizeof(KT) == 2 ? 128 : 64; }
 template <int HD, class KT>
-constexpr size_t tree_tile_lds() {  // two BF16 tiles, or one of three parts
-    return sizeof(KT) == 2 ? (size_t)4 * tree_tile<KT>() * HD * 2 : (size_t)6 * tree_tile<KT>() * HD * 2;
+constexpr size_t tree_tile_lds() {  // two BF16 tiles; K of three parts and V, at head_dim 128 two of it
+    return (size_t)(sizeof(KT) == 2 ? 4 : HD == 128 ? 9 : 6) * tree_tile<KT>() * HD * 2;
 }
 template <int HD, class KT>
 constexpr size_t tree_lds_bytes() { return tree_tile_lds<HD, KT>() + sizeof(TreeLds); }
 
 template <int HD, int WR, int WK, class KT>
-__global__ __launch_bounds__(64 * WR * WK) __attribute__((amdgpu_waves_per_eu(WR * WK / 4)))
+__global__ __launch_bounds__(64 * WR * WK) __attribute__((amdgpu_waves_per_eu(sizeof(KT) == 4 && HD == 64 ? 2 : WR * WK / 4)))
 void tree_attn_kernel(TreeArgs a, int S) {
     constexpr bool F32 = sizeof(KT) == 4;
-    constexpr int NW = WR * WK, T = tree_tile<KT>(), STEPS = T / (32 * WK);
+    constexpr int NW = WR * WK, T = tree_tile<KT>();
+    static_assert(WK > 1 && T == 32 * WK, "32 positions of a tile for each key wave");
     constexpr int KSTEPS = HD / 16, UT = HD / 32;
     constexpr int CPR = HD / 8;       // 16-byte chunks per LDS row
     constexpr int HC = HD / 8 / NW;   // BF16: a wave's copies for 64 positions; f32: a thread's 8-dim units of a tile
     constexpr int PL = F32 ? 3 : 1;   // parts (planes) of K and V
     constexpr int TB = T * HD * 2;    // bytes of a tile's plane
+    constexpr bool V2 = F32 && HD == 128;  // the next tile's V has a place of its own
     extern __shared__ __attribute__((aligned(256))) uint8_t smem[];
     uint8_t *ks = smem, *vs = smem + PL * TB;  // the second BF16 tile, 2 TB on
     TreeLds &tree = *(TreeLds *)(smem + tree_tile_lds<HD, KT>());
@@ -367,7 +384,7 @@ void tree_attn_kernel(TreeArgs a, int S) {
     // of 0 does not clear a NaN), and so do those with an infinity or NaN (f32:
     // or a value that weights of up to 2^8 take past the largest number), whose
     // position is marked. BF16: in a landed tile that reaches the tree, a row by
-    // the wave that copied it. f32: while a tile is staged.
+    // the wave that copied it. f32: when its parts are stored.
     auto mark = [&](int p) {
         const int x = p - a.offset;
         if (x < 0) tree.sick_prefix = 1;
@@ -389,28 +406,49 @@ void tree_attn_kernel(TreeArgs a, int S) {
             if (bad) *at = u32x4{0u, 0u, 0u, 0u};
         }
     };
-    auto stage = [&](int t0) {
+    // f32: unit c of the next tile, cut into its parts while the matrix cores work
+    // on the current one; then all of them into the tile's place.
+    bf16x8 kp[F32 ? HC : 1][3], vp[F32 ? HC : 1][3];
+    uint32_t vmost[F32 ? HC : 1];  // largest magnitude of a unit's V, as bits
+    auto cut_unit = [&](int c) {
+        const float kv[8] = {kr[c][0][0], kr[c][0][1], kr[c][0][2], kr[c][0][3],
+                             kr[c][1][0], kr[c][1][1], kr[c][1][2], kr[c][1][3]};
+        const float vv[8] = {vr[c][0][0], vr[c][0][1], vr[c][0][2], vr[c][0][3],
+                             vr[c][1][0], vr[c][1][1], vr[c][1][2], vr[c][1][3]};
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(vv[i]) & 0x7FFFFFFFu);
+        vmost[c] = most;
+        cut3x8(kv, kp[c]);
+        cut3x8(vv, vp[c]);
+        if constexpr (HD == 128)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {  // here, not where they are stored
+                pin_v(kp[c][k]);
+                pin_v(vp[c][k]);
+            }
+    };
+    auto store_k = [&]() {
 #pragma unroll
         for (int c = 0; c < (F32 ? HC : 0); ++c) {
-            const int idx = (int)threadIdx.x + 64 * NW * c, r = idx / CPR, ch = idx % CPR, kr_ = krow_of(r);
-            const float kv[8] = {kr[c][0][0], kr[c][0][1], kr[c][0][2], kr[c][0][3],
-                                 kr[c][1][0], kr[c][1][1], kr[c][1][2], kr[c][1][3]};
-            float vv[8] = {vr[c][0][0], vr[c][0][1], vr[c][0][2], vr[c][0][3],
-                           vr[c][1][0], vr[c][1][1], vr[c][1][2], vr[c][1][3]};
-            bool fine = true;
+            const int idx = (int)threadIdx.x + 64 * NW * c, ch = idx % CPR, kr_ = krow_of(idx / CPR);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) fine = fine && fabsf(vv[i]) < 0x1p119f;
-            const bool past = t0 + r >= end;
-            if (!fine && !past) mark(t0 + r);
+            for (int k = 0; k < 3; ++k) *(bf16x8 *)(ks + k * TB + kr_ * HD * 2 + 16 * (ch ^ (kr_ % CPR))) = kp[c][k];
+        }
+    };
+    auto store_v = [&](int t0, int b) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) vv[i] = fine && !past ? vv[i] : 0.f;
-            bf16x8 w[3];
-            cut3x8(kv, w);
+        for (int c = 0; c < (F32 ? HC : 0); ++c) {
+            const int idx = (int)threadIdx.x + 64 * NW * c, r = idx / CPR, ch = idx % CPR;
+            const bool past = t0 + r >= end, sick = vmost[c] >= 0x7B000000u;  // 2^119 on
+            if (__any(past || sick)) {
+                if (sick && !past) mark(t0 + r);
 #pragma unroll
-            for (int k = 0; k < 3; ++k) *(bf16x8 *)(ks + k * TB + kr_ * HD * 2 + 16 * (ch ^ (kr_ % CPR))) = w[k];
-            cut3x8(vv, w);
+                for (int k = 0; k < 3; ++k)
+                    if (past || sick) vp[c][k] = bf16x8{};
+            }
 #pragma unroll
-            for (int k = 0; k < 3; ++k) *(bf16x8 *)(vs + k * TB + r * HD * 2 + 16 * (ch ^ vseg<HD>(r))) = w[k];
+            for (int k = 0; k < 3; ++k) *(bf16x8 *)(vs + (3 * b + k) * TB + r * HD * 2 + 16 * (ch ^ vseg<HD>(r))) = vp[c][k];
         }
     };
 
@@ -420,7 +458,7 @@ void tree_attn_kernel(TreeArgs a, int S) {
     // LDS, where the first tile does not come: BF16 in the second tile's place, f32
     // in its own.
     constexpr int OWN = KSTEPS / WK, kFragments = 3 * 1024;  // a step's three parts, 16 bytes a lane
-    static_assert(WK == 1 || WR * KSTEPS * kFragments <= (F32 ? 6 : 2) * TB, "room for the fragments");
+    static_assert(WR * KSTEPS * kFragments <= (F32 ? 6 : 2) * TB, "room for the fragments");
     const int parent = in_tree && (int)threadIdx.x < a.n ? a.parents[threadIdx.x] : -1;
     f32x4 raw[OWN][2];
     {
@@ -451,17 +489,19 @@ void tree_attn_kernel(TreeArgs a, int S) {
         cut3x8(v, w);
 #pragma unroll
         for (int k = 0; k < 3; ++k)
-            if constexpr (WK == 1) q3[i][k] = w[k];
-            else *(bf16x8 *)(at + ((i * WK + wk) * 3 + k) * 1024) = w[k];
+            *(bf16x8 *)(at + ((i * WK + wk) * 3 + k) * 1024) = w[k];
     }
-    if constexpr (WK > 1) {
-        lds_barrier();
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < KSTEPS; ++i)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) q3[i][k] = *(const bf16x8 *)(at + (i * 3 + k) * 1024);
+    if constexpr (F32 && HD == 128)
 #pragma unroll
         for (int i = 0; i < KSTEPS; ++i)
 #pragma unroll
-            for (int k = 0; k < 3; ++k) q3[i][k] = *(const bf16x8 *)(at + (i * 3 + k) * 1024);
-    }
-    if constexpr (F32 && WK > 1) lds_barrier();  // read before the tile comes in their place
+            for (int k = 0; k < 3; ++k) pin_a(q3[i][k]);
+    if constexpr (F32) lds_barrier();  // read before the tile comes in their place
     if (in_tree) find_ancestors(parent, a.n, tree);
     // This lane's transposing V reads in a 16-position block: rows
     // 8 half + i / 4 (and + 4), dims 32 u + 16 ((lane / 16) % 2) + 4 (i % 4).
@@ -482,27 +522,32 @@ void tree_attn_kernel(TreeArgs a, int S) {
             __syncthreads();  // the marks start at none
             clean_v(start, 0);
         }
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int c = 0; c < HC; ++c) cut_unit(c);
+        if (start + T < end) {
+            fetch(start + T, 0);
+            next_pages(start + 2 * T);
+        }
+        lds_barrier();
+        store_k();
+        store_v(start, 0);
+        lds_barrier();
     }
-    __syncthreads();
     int b = 0;
     for (int t0 = start; t0 < end; t0 += T) {
         const bool more = t0 + T < end;
-        if constexpr (F32) {
-            stage(t0);
-            __syncthreads();
-        }
-        if (more) {
+        if (!F32 && more) {
             fetch(t0 + T, b ^ 1);
             next_pages(t0 + 2 * T);
         }
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-            const int p0 = 32 * (st * WK + wk);
-            if (t0 + p0 >= end) break;
+        const int p0 = 32 * wk;
+        if (t0 + p0 < end) {  // a tile with another behind it is full
             uint32_t vad[UT];
 #pragma unroll
-            for (int u = 0; u < UT; ++u) vad[u] = (vbase + b * 2 * TB + p0 * HD * 2) ^ (64 * u);
-            const int kat = kbase + b * 2 * TB + p0 * HD * 2;
+            for (int u = 0; u < UT; ++u) vad[u] = (vbase + b * (F32 ? 3 : 2) * TB + p0 * HD * 2) ^ (64 * u);
+            const int kat = kbase + (F32 ? 0 : b * 2 * TB) + p0 * HD * 2;
             // BF16: every K fragment of the step in flight at once. (f32: three parts
             // of each would take the registers of the second wave at head_dim 64.)
             bf16x8 ka[F32 ? 1 : KSTEPS][PL];
@@ -530,11 +575,24 @@ void tree_attn_kernel(TreeArgs a, int S) {
                 if constexpr (F32) slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[1], q3[s][0], slow, 0, 0, 0);
                 slow = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], q3[s][1], slow, 0, 0, 0);
                 sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], q3[s][0], sacc, 0, 0, 0);
+                if constexpr (F32) {
+                    constexpr int EVERY = KSTEPS / HC;  // k-steps a unit of the next tile
+                    if (s % EVERY == EVERY - 1) cut_unit(s / EVERY);
+                }
+            }
+            if (F32 && more) {
+                lds_barrier();  // the tile's keys are read
+                store_k();
+                if constexpr (V2) store_v(t0 + T, b ^ 1);
+                if (t0 + 2 * T < end) {
+                    fetch(t0 + 2 * T, 0);
+                    next_pages(t0 + 3 * T);
+                }
             }
             if constexpr (F32) sacc += small;
             // The step's V^T fragments, while the score products drain.
-            bf16x8 va[F32 ? 1 : 2][PL][UT];
-            if constexpr (!F32) read_vt2<HD>(vad, va[0][0], va[F32 ? 0 : 1][0]);
+            bf16x8 va[2][UT];
+            if constexpr (!F32) read_vt2<HD>(vad, va[0], va[1]);
             // Register r holds position 8 half + (r & 3) + (r & 4) + 2 (r & 8) of the step.
             const int x0 = t0 + p0 - a.offset;  // node of the step's first position
             if (x0 + 32 > 0) {
@@ -592,7 +650,7 @@ void tree_attn_kernel(TreeArgs a, int S) {
                         oacc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[u], p, oacc[u], 0, 0, 0);
                 };
                 if constexpr (F32) {
-                    auto &v = va[0];
+                    bf16x8 v[3][UT];
                     read_vt<HD, s2 * 16 * HD * 2>(vad, v[0]);
                     read_vt<HD, TB + s2 * 16 * HD * 2>(vad, v[1]);
                     read_vt<HD, 2 * TB + s2 * 16 * HD * 2>(vad, v[2]);
@@ -603,9 +661,9 @@ void tree_attn_kernel(TreeArgs a, int S) {
                     product(v[0], p3[1]);
                     product(v[0], p3[0]);
                 } else {
-                    product(va[s2][0], p3[2]);
-                    product(va[s2][0], p3[1]);
-                    product(va[s2][0], p3[0]);
+                    product(va[s2], p3[2]);
+                    product(va[s2], p3[1]);
+                    product(va[s2], p3[0]);
                 }
             };
             mix(std::integral_constant<int, 0>{});
@@ -615,15 +673,23 @@ void tree_attn_kernel(TreeArgs a, int S) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             if (more && t0 + 2 * T > a.offset) clean_v(t0 + T, b ^ 1);
             b ^= 1;
+            __syncthreads();
+        } else {
+            lds_barrier();
+            if (V2) {
+                b ^= 1;
+            } else if (more) {
+                store_v(t0 + T, 0);
+                lds_barrier();
+            }
         }
-        __syncthreads();
     }
 
     l += __shfl_xor(l, 32, 64);
     // The key waves of a row join in LDS, in the tiles' place: each leaves the
     // blocks of 32 dims that others own (block u: wave u % WK) and adds up its own,
     // in wave order. Rows padded by 16 bytes, off each other's banks.
-    if constexpr (WK > 1) {
+    {
         constexpr int LD = 32 + 4;
         static_assert((size_t)WR * UT * (WK - 1) * 32 * LD * 4 + (size_t)NW * 32 * 8 <= tree_tile_lds<HD, KT>(),
                       "joined in the tiles' LDS");
@@ -833,20 +899,16 @@ size_t tree_room(const TreeJob &j, int wr) {
     return std::max<size_t>(std::max<size_t>(slots / 8 / rb, 1) * 8 / (size_t)j.g.kv_heads, 1);
 }
 
-// Row waves of a block: one for up to 32 rows, two for more. While every split
-// wanted has a block of its own anyway, the fewest that let it: short walks, and CUs
-// that would stand idle otherwise (16 nodes on 700, 28 / 4 heads of 128: two 12.8 us,
-// one 11.6; 32 on 500, f32, four 21.7, two 17.7). Twice as many with half the key
-// waves halve the tiles' traffic and double the partials': over BF16 that never
-// paid (64 nodes on 16k, 32 / 8 heads of 128: four 53.9 us, two 51.4; 18 on 16k,
-// 28 / 4: 27.6 and 22.3). f32 tiles cost their staging too: four at head_dim 128
-// (128 on 8k, 32 / 8: 61.3 us, two 68.2; head_dim 64, 256 on 8k, 14 / 2: 34.6 and
-// 33.2), unless they would leave two of the last block without rows.
+// Row waves of a block: two; over a BF16 cache one for up to 32 rows, and while every
+// split wanted then has a block of its own anyway: short walks, and CUs that would
+// stand idle otherwise (16 nodes on 700, 28 / 4 heads of 128: two 12.8 us, one 11.6).
+// Four with half the key waves halve the tiles' traffic and double the partials':
+// 64 nodes on 16k, 32 / 8 heads of 128, 53.9 us, with two 51.4; 18 on 16k, 28 / 4, 27.6
+// and 22.3; f32, 18 on 6k, 30.3 and 25.8 (128 on 3k, 32 / 8, 58.6 and 60.8).
 int tree_row_waves(const TreeJob &j) {
-    const int rows = (int)j.n * (j.q_heads / j.g.kv_heads), waves = (rows + 31) / 32;
-    if (!j.g.kv_f32) return waves == 1 || tree_wanted(j) <= tree_room(j, 1) ? 1 : 2;
-    const bool two = waves <= 2 || waves % 4 == 1 || waves % 4 == 2 || tree_wanted(j) <= tree_room(j, 2);
-    return two || j.g.head_dim == 64 ? 2 : 4;
+    if (j.g.kv_f32) return 2;
+    const size_t rows = j.n * (size_t)(j.q_heads / j.g.kv_heads);
+    return rows <= 32 || tree_wanted(j) <= tree_room(j, 1) ? 1 : 2;
 }
 
 template <int HD, int WR, int WK, class KT>
@@ -864,14 +926,9 @@ int launch_tree_blocks(const TreeArgs &a, int S, hipStream_t s) {
 
 template <int HD>
 int launch_tree_rows(const TreeJob &j, const TreeArgs &a, int S, hipStream_t s) {
-    const int wr = tree_row_waves(j);
-    if (!j.g.kv_f32) {
-        if (wr == 1) return launch_tree_blocks<HD, 1, 4, uint16_t>(a, S, s);
-        return launch_tree_blocks<HD, 2, 4, uint16_t>(a, S, s);
-    }
-    if constexpr (HD == 128)
-        if (wr == 4) return launch_tree_blocks<HD, 4, 1, float>(a, S, s);
-    return launch_tree_blocks<HD, 2, 2, float>(a, S, s);
+    if (j.g.kv_f32) return launch_tree_blocks<HD, 2, 2, float>(a, S, s);
+    if (tree_row_waves(j) == 1) return launch_tree_blocks<HD, 1, 4, uint16_t>(a, S, s);
+    return launch_tree_blocks<HD, 2, 4, uint16_t>(a, S, s);
 }
 
 template <int HD>
