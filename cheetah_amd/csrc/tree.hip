@@ -58,7 +58,6 @@ struct TreeLds {
     uint64_t anc[kMaxTreeNodes][kAncWords];
     uint64_t sick[kAncWords];  // nodes with an infinity or NaN in V
     uint32_t odd[4];           // a row wave's rows to compute again
-    int sick_prefix;           // an infinity or NaN in the prefix's V (f32)
     int32_t pages[64];         // the split's first page table entries
     int16_t up[kMaxTreeNodes];
 };
@@ -109,9 +108,10 @@ __device__ __forceinline__ float kv_value(const float *p) { return *p; }
 
 // One row over positions [start, end) in plain f32 products, a wave per row and
 // a lane per HD / 64 dims: the rare rows that the matrix cores' parts do not
-// carry. They see an infinity or NaN in a tree node's V (or anywhere in an f32
-// cache), which 0 x V would spread over the tile's rows, or their weight sum is
-// NaN, where a score of -inf has to weigh nothing. A NaN sum ends the row.
+// carry. They see an infinity or NaN in a tree node's V, which 0 x V would spread
+// over the tile's rows and which is cleared there; or an output is not finite,
+// where a weight's part of 0 has met an infinity in the prefix; or their weight sum
+// is NaN, where a score of -inf has to weigh nothing. A NaN sum ends the row.
 template <int HD, class KT>
 __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int head, int g, int start, int end, int S,
                           int split) {
@@ -381,14 +381,13 @@ void tree_attn_kernel(TreeArgs a, int S) {
         }
     };
     // V rows past the block's rows become zeros (unwritten memory: a probability
-    // of 0 does not clear a NaN), and so do those with an infinity or NaN (f32:
-    // or a value that weights of up to 2^8 take past the largest number), whose
-    // position is marked. BF16: in a landed tile that reaches the tree, a row by
-    // the wave that copied it. f32: when its parts are stored.
+    // of 0 does not clear a NaN), and so do nodes' with an infinity or NaN, which
+    // are marked. (The prefix's reach every row; they show in the result.) BF16: in
+    // a landed tile that reaches the tree, a row by the wave that copied it. f32:
+    // when its parts are stored.
     auto mark = [&](int p) {
         const int x = p - a.offset;
-        if (x < 0) tree.sick_prefix = 1;
-        else atomicOr((unsigned long long *)&tree.sick[x >> 6], 1ull << (x & 63));
+        atomicOr((unsigned long long *)&tree.sick[x >> 6], 1ull << (x & 63));
     };
     auto clean_v = [&](int t0, int b) {
         for (int c = 0; c < HC * T / 64; ++c) {
@@ -440,7 +439,7 @@ void tree_attn_kernel(TreeArgs a, int S) {
 #pragma unroll
         for (int c = 0; c < (F32 ? HC : 0); ++c) {
             const int idx = (int)threadIdx.x + 64 * NW * c, r = idx / CPR, ch = idx % CPR;
-            const bool past = t0 + r >= end, sick = vmost[c] >= 0x7B000000u;  // 2^119 on
+            const bool past = t0 + r >= end, sick = t0 + r >= a.offset && vmost[c] >= 0x7F800000u;
             if (__any(past || sick)) {
                 if (sick && !past) mark(t0 + r);
 #pragma unroll
@@ -471,7 +470,6 @@ void tree_attn_kernel(TreeArgs a, int S) {
     }
     if (wave == 0) tree.pages[lane] = held;
     if (threadIdx.x < 4) tree.odd[threadIdx.x] = 0;
-    if (threadIdx.x == 0) tree.sick_prefix = 0;
     lds_barrier();
     held = tree.pages[lane];
     next_pages(start);
@@ -737,13 +735,19 @@ void tree_attn_kernel(TreeArgs a, int S) {
             }
     }
     if (rvalid) {
-        bool odd = l != l || (F32 && tree.sick_prefix);
+        float zero = 0.f;  // NaN with a value that is not finite
+#pragma unroll
+        for (int u = 0; u < UT; ++u)
+            if (u % WK == wk)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) zero = fmaf(oacc[u][r], 0.f, zero);
+        bool odd = l != l || zero != zero;
         if (in_tree)
 #pragma unroll
             for (int k = 0; k < kAncWords; ++k) odd |= (tree.anc[node][k] & tree.sick[k]) != 0;
         const float inv = 1.0f / l;
         if (odd) {
-            if (wk == 0 && half == 0) atomicOr(&tree.odd[wr], 1u << n);
+            atomicOr(&tree.odd[wr], 1u << n);
         } else {
             const size_t ob = ((size_t)node * a.q_heads + head) * HD + 4 * half;
 #pragma unroll
@@ -758,6 +762,14 @@ void tree_attn_kernel(TreeArgs a, int S) {
             if (S > 1 && wk == 0 && half == 0) a.ml[at_part] = make_float2(m2, l);
         }
     }
+    __syncthreads();
+    uint32_t odd_rows = 0;
+#pragma unroll
+    for (int w = 0; w < WR; ++w) odd_rows |= tree.odd[w];
+    if (odd_rows == 0) return;
+    // Waves whose share of such a row was finite have written it: before it is
+    // written again.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 #pragma unroll 1
     for (int r = wave; r < 32 * WR; r += NW)
