@@ -110,8 +110,11 @@ __device__ __forceinline__ float kv_value(const float *p) { return *p; }
 // a lane per HD / 64 dims: the rare rows that the matrix cores' parts do not
 // carry. They see an infinity or NaN in a tree node's V, which 0 x V would spread
 // over the tile's rows and which is cleared there; or an output is not finite,
-// where a weight's part of 0 has met an infinity in the prefix; or their weight sum
-// is NaN, where a score of -inf has to weigh nothing. A NaN sum ends the row.
+// where a weight's part of 0 has met an infinity in the prefix, or weights of up to
+// 2^8 have taken a sum of large values past the largest number; or their weight sum
+// is NaN, where a score of -inf has to weigh nothing. A NaN sum ends the row. Where
+// a sum overflows with weights of at most 1 too, it is taken again of V / 2^32 (it
+// has fewer than 2^32 keys): the average itself is no larger than V.
 template <int HD, class KT>
 __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int head, int g, int start, int end, int S,
                           int split) {
@@ -119,27 +122,37 @@ __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int hea
     const int lane = threadIdx.x & 63;
     const size_t row = ((size_t)node * a.q_heads + head) * HD;
     const float scale = (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f;
-    float q[D], o[D], m = -INFINITY, l = 0.f;
+    float q[D], o[D], m, l;
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-        q[d] = a.q[row + lane + 64 * d];
-        o[d] = 0.f;
-    }
+    for (int d = 0; d < D; ++d) q[d] = a.q[row + lane + 64 * d];
+    int shift = 0;  // V / 2^shift
+    for (;;) {
+        const float vs = shift ? 0x1p-32f : 1.f;
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int d = 0; d < D; ++d) o[d] = 0.f;
 #pragma unroll 1
-    for (int p = start; p < end && l == l; ++p) {
-        const int x = p - a.offset;
-        if (x >= 0 && !(t.anc[node][x >> 6] >> (x & 63) & 1)) continue;
-        const size_t at = (((size_t)a.page_table[p / a.page_size] * a.kv_heads + g) * a.page_size + p % a.page_size) * HD;
-        float dot = 0.f;
+        for (int p = start; p < end && l == l; ++p) {
+            const int x = p - a.offset;
+            if (x >= 0 && !(t.anc[node][x >> 6] >> (x & 63) & 1)) continue;
+            const size_t at = (((size_t)a.page_table[p / a.page_size] * a.kv_heads + g) * a.page_size + p % a.page_size) * HD;
+            float dot = 0.f;
 #pragma unroll
-        for (int d = 0; d < D; ++d) dot = fmaf(q[d], kv_value((const KT *)a.k + at + lane + 64 * d), dot);
-        const float s = wave_sum(dot) * scale, mn = fmaxf(m, s);
-        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-        const float w = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - mn);
-        m = mn;
-        l = l * alpha + w;
+            for (int d = 0; d < D; ++d) dot = fmaf(q[d], kv_value((const KT *)a.k + at + lane + 64 * d), dot);
+            const float s = wave_sum(dot) * scale, mn = fmaxf(m, s);
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            const float w = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - mn);
+            m = mn;
+            l = l * alpha + w;
 #pragma unroll
-        for (int d = 0; d < D; ++d) o[d] = fmaf(w, kv_value((const KT *)a.v + at + lane + 64 * d), o[d] * alpha);
+            for (int d = 0; d < D; ++d) o[d] = fmaf(w, kv_value((const KT *)a.v + at + lane + 64 * d) * vs, o[d] * alpha);
+        }
+        float zero = 0.f;  // NaN with a value that is not finite
+#pragma unroll
+        for (int d = 0; d < D; ++d) zero = fmaf(o[d], 0.f, zero);
+        if (shift || l != l || !__any(zero != zero)) break;
+        shift = 32;
     }
     const size_t at = ((size_t)node * a.q_heads + head) * S + split;
 #pragma unroll
@@ -147,7 +160,7 @@ __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int hea
         if (S > 1) {
             a.part[at * HD + lane + 64 * d] = o[d];
         } else {
-            const float v = o[d] / l;
+            const float v = o[d] / l * (shift ? 0x1p32f : 1.f);
             if (a.out) a.out[row + lane + 64 * d] = v;
             if (a.out_hi) {
                 const __bf16 hb = (__bf16)v;
@@ -156,7 +169,9 @@ __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int hea
             }
         }
     }
-    if (S > 1 && lane == 0) a.ml[at] = make_float2(l == l ? m : INFINITY, l);  // a NaN row: no split outweighs it
+    // A NaN row: no split outweighs it. A scaled one: its sums are 2^-32 of theirs,
+    // about a maximum 2^32 higher.
+    if (S > 1 && lane == 0) a.ml[at] = make_float2(l == l ? m + (float)shift : INFINITY, shift ? l * 0x1p-32f : l);
 }
 
 // Eight values as three BF16 parts, each the top 8 bits of what the ones before
@@ -781,7 +796,10 @@ void tree_attn_kernel(TreeArgs a, int S) {
 
 // Joins the splits of one (row, head): W waves of a block each add up every
 // W-th split's values in order, then their sums in order. Every load of a batch
-// is in flight at once, the first batch beside the maxima.
+// is in flight at once, the first batch beside the maxima. The sums are taken of
+// 2^-7 of the values (at most 2^7 splits), so that they stay finite where each
+// split's are; a power of two rounds nothing.
+constexpr int kMergeSplits = 128;  // two a lane
 template <int HD, int W>
 __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a, int S, int items) {
     constexpr int D = HD / 64, B = 8;
@@ -805,6 +823,8 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a, int S,
     const float f0 = m0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
     const float f1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - M);
     const float L = wave_sum((f0 != 0.f ? f0 * x.y : 0.f) + (f1 != 0.f ? f1 * y.y : 0.f));
+    static_assert(kMergeSplits == 1 << 7, "the scale of the sums");
+    const float g0 = f0 * 0x1p-7f, g1 = f1 * 0x1p-7f;
     vec o = {};
     for (int s0 = w0; s0 < S; s0 += W * B) {
         if (s0 != w0) load(s0);
@@ -813,7 +833,7 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a, int S,
             // A split without a key of the row (and what a lane past S read) holds no
             // values; selected, not branched around: a load would sink into the branch.
             const int s = s0 + W * i;
-            const float f = s >= S ? 0.f : s < 64 ? lane_read(f0, s) : lane_read(f1, s - 64);
+            const float f = s >= S ? 0.f : s < 64 ? lane_read(g0, s) : lane_read(g1, s - 64);
 #pragma unroll
             for (int d = 0; d < D; ++d) o[d] = fmaf(f, f != 0.f ? v[i][d] : 0.f, o[d]);
         }
@@ -825,7 +845,7 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a, int S,
 #pragma unroll
         for (int w = 1; w < W; ++w) o += *(const vec *)&so[wave + w][D * lane];
     }
-    const float inv = 1.0f / L;
+    const float inv = 1.0f / L * 0x1p7f;
     const size_t at = (size_t)item * HD + D * lane;
 #pragma unroll
     for (int d = 0; d < D; ++d) {
@@ -962,7 +982,7 @@ int launch_tree_h(const TreeJob &j, const TreeArgs &a, int S, hipStream_t s) {
 // head_dim 64: two), of a tile at least; at least 8 (split, KV head) pairs go to the
 // XCDs in turn, so that their number is brought down to a multiple of 8.
 int tree_attention_splits(const TreeJob &j) {
-    return (int)std::min({tree_wanted(j), tree_room(j, tree_row_waves(j)), (size_t)attention_max_splits()});
+    return (int)std::min({tree_wanted(j), tree_room(j, tree_row_waves(j)), (size_t)attention_max_splits(), (size_t)kMergeSplits});
 }
 
 int launch_tree_attention(const TreeJob &j, hipStream_t s) {
