@@ -823,19 +823,21 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeArgs a, int S,
     const float f0 = m0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m0 - M);
     const float f1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - M);
     const float L = wave_sum((f0 != 0.f ? f0 * x.y : 0.f) + (f1 != 0.f ? f1 * y.y : 0.f));
+    // A split without a key of the row (and what a lane past S read) holds no values
+    // and is told apart by a factor of -1: one whose factor rounds to 0 holds them,
+    // and an infinity among them shows, as it does within a split.
     static_assert(kMergeSplits == 1 << 7, "the scale of the sums");
-    const float g0 = f0 * 0x1p-7f, g1 = f1 * 0x1p-7f;
+    const float g0 = m0 == -INFINITY ? -1.f : f0 * 0x1p-7f, g1 = m1 == -INFINITY ? -1.f : f1 * 0x1p-7f;
     vec o = {};
     for (int s0 = w0; s0 < S; s0 += W * B) {
         if (s0 != w0) load(s0);
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            // A split without a key of the row (and what a lane past S read) holds no
-            // values; selected, not branched around: a load would sink into the branch.
+            // Selected, not branched around: a load would sink into the branch.
             const int s = s0 + W * i;
-            const float f = s >= S ? 0.f : s < 64 ? lane_read(g0, s) : lane_read(g1, s - 64);
+            const float f = s >= S ? -1.f : s < 64 ? lane_read(g0, s) : lane_read(g1, s - 64);
 #pragma unroll
-            for (int d = 0; d < D; ++d) o[d] = fmaf(f, f != 0.f ? v[i][d] : 0.f, o[d]);
+            for (int d = 0; d < D; ++d) o[d] = fmaf(f, f == -1.f ? 0.f : v[i][d], o[d]);
         }
     }
     if constexpr (W > 1) {

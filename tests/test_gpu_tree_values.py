@@ -65,6 +65,22 @@ def test_an_infinity_in_the_prefix_shows(hip, n, offset, hd, kv):
 
 @pytest.mark.parametrize("kv", ["bf16", "f32"])
 @pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,offset", SHAPES)
+def test_an_infinity_of_no_weight_still_shows(hip, n, offset, hd, kv):
+    """Scores hundreds apart: the weight of the infinity's key rounds to 0 in
+    f32 for most rows, and 0 times infinity is NaN, in one split or many."""
+    rng, q, k, v, parents = case(n + hd + 1, n, offset, hd, kv)
+    q *= 60
+    d = 5
+    v[offset // 3, :, d] = np.inf
+    kp, vp, table = ref.paged(k, v, kv, rng)
+    got = hip.tree_attention(q, kp, vp, table, 8, parents, offset).reshape(n, 8, hd)
+    assert not np.isfinite(got[:, :, d]).any()
+    assert np.isfinite(np.delete(got, d, 2)).all()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("n,offset", SHAPES + [(12, 0)])
 @pytest.mark.parametrize("what", ["one", "120", "123", "126", "1e38", "most", "signs"])
 def test_large_finite_values_average(hip, what, n, offset, hd, kv):
