@@ -279,7 +279,8 @@ def attention(q: np.ndarray, kp: np.ndarray, vp: np.ndarray, table: np.ndarray, 
     noalloc: through cheetah_hip_attention_noalloc (fixed device scratch)."""
     _, kvh, ps, hd = kp.shape
     qd = DeviceBuffer.from_array(np.ascontiguousarray(q, np.float32))
-    kd, vd, td = DeviceBuffer.from_array(kp), DeviceBuffer.from_array(vp), DeviceBuffer.from_array(table)
+    kd, vd = DeviceBuffer.from_array(kp), DeviceBuffer.from_array(vp)
+    td = DeviceBuffer.from_array(np.ascontiguousarray(table, np.int32))
     od = DeviceBuffer(rows * q_heads * hd * 4)
     view = KvView(kd.ptr, vd.ptr, td.ptr, ps, kvh, hd)
     fn = lib().cheetah_hip_attention_noalloc if noalloc else lib().cheetah_hip_attention
@@ -303,7 +304,8 @@ def tree_attention(q: np.ndarray, kp: np.ndarray, vp: np.ndarray, table: np.ndar
     if table.size and not 0 <= int(table.min()) <= int(table.max()) < kp.shape[0]:
         raise ValueError("page table entry outside the pool")
     qd = DeviceBuffer.from_array(np.ascontiguousarray(q, np.float32))
-    kd, vd, td = DeviceBuffer.from_array(kp), DeviceBuffer.from_array(vp), DeviceBuffer.from_array(table)
+    kd, vd = DeviceBuffer.from_array(kp), DeviceBuffer.from_array(vp)
+    td = DeviceBuffer.from_array(np.ascontiguousarray(table, np.int32))
     pd, od = DeviceBuffer.from_array(parents), DeviceBuffer(max(n, 1) * q_heads * hd * 4)
     view = KvView(kd.ptr, vd.ptr, td.ptr, ps, kvh, hd)
     check(lib().cheetah_hip_tree_attention(qd.ptr, _c.byref(view), int(kp.dtype == np.float32), q_heads, pd.ptr, n,
