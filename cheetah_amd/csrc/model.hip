@@ -1251,6 +1251,15 @@ int validate_decode(const cheetah_hip_model *m, uint32_t token, size_t offset, s
     return 0;
 }
 
+// The decode step of one token at `offset` (positions reserved), its logits left in
+// m->logits. The persistent kernel's launch (*ran_fused) also samples, exports and
+// waits; the graph's is enqueued, with `sample` its argmax in next_dev.
+int run_step(cheetah_hip_model *m, uint32_t token, size_t offset, bool sample, bool want_logits, bool *ran_fused) {
+    CHIP_TRY(launch_set_step(m->step_dev, (int32_t)token, (int32_t)offset, m->stream));
+    *ran_fused = fused_fits(m, offset, 1);
+    return *ran_fused ? run_fused(m, offset, 1, want_logits) : launch_decode(m, offset, sample);
+}
+
 // Runs the forward and waits for it; leaves, with `sample`, the argmax in
 // words_host[0] and, with want_logits, the final logits in logits_host.
 int run_forward(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t offset, size_t chunk_rows,
@@ -1263,13 +1272,12 @@ int run_forward(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t o
     m->tree_n = 0;
     CHIP_TRY(reserve_positions(m, n));
     if (n == 1) {
-        CHIP_TRY(launch_set_step(m->step_dev, (int32_t)tokens[0], (int32_t)offset, m->stream));
-        if (fused_fits(m, offset, 1)) {
-            CHIP_TRY(run_fused(m, offset, 1, want_logits));
+        bool ran_fused = false;
+        CHIP_TRY(run_step(m, tokens[0], offset, sample, want_logits, &ran_fused));
+        if (ran_fused) {
             m->len = offset + 1;
             return 0;
         }
-        CHIP_TRY(launch_decode(m, offset, sample));
     } else {
         CHIP_CHECK(hipStreamSynchronize(m->stream));  // tokens_host reuse
         std::memcpy(m->tokens_host, tokens, n * sizeof(uint32_t));
@@ -1355,8 +1363,8 @@ int keep_branch(cheetah_hip_model *m, const uint32_t *nodes, size_t count) {
     return 0;
 }
 
-// Prefill that also scores every position (run_forward's chunks, the LM head
-// over all of their rows).
+// Forward that also scores every position: run_forward's chunks, the LM head over
+// all of their rows, or its decode step.
 int run_scored(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t offset, size_t chunk_rows,
                const uint32_t *targets, uint32_t top, float *logprobs, float *entropy, uint32_t *top_ids,
                float *top_logprobs) {
@@ -1376,7 +1384,7 @@ int run_scored(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t of
     // be bound by the matrix cores.
     const size_t V = C(m).vocab_size, group = std::min({n, chunk_rows, (size_t)256});
     m->tree_n = 0;
-    CHIP_TRY(grow(m, &m->row_logits, &m->row_logits_floats, group * V));
+    if (n > 1) CHIP_TRY(grow(m, &m->row_logits, &m->row_logits_floats, group * V));
     CHIP_TRY(grow(m, &m->score_dev, &m->score_words, n * (3 + 2 * (size_t)top)));
     size_t ws = 0;
     for (size_t r = 1; r <= group; ++r) ws = std::max(ws, logprobs_workspace_bytes(r, V, (int)top));
@@ -1385,34 +1393,44 @@ int run_scored(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t of
         CHIP_TRY(logprobs_workspace_clear(m->score_ws, m->stream));
     }
     CHIP_TRY(reserve_positions(m, n));
-    CHIP_CHECK(hipStreamSynchronize(m->stream));  // tokens_host reuse
-    std::memcpy(m->tokens_host, tokens, n * sizeof(uint32_t));
-    CHIP_CHECK(hipMemcpyAsync(m->tokens_dev, m->tokens_host, n * sizeof(uint32_t), hipMemcpyHostToDevice, m->stream));
     uint32_t *want = m->score_dev;
     float *lp = (float *)(want + n), *ent = lp + n;
     uint32_t *ids = (uint32_t *)(ent + n);
     float *tops = (float *)(ids + n * top);
     if (logprobs)
         CHIP_CHECK(hipMemcpyAsync(want, targets, n * sizeof(uint32_t), hipMemcpyHostToDevice, m->stream));
-    for (size_t start = 0; start < n; start += chunk_rows) {
-        const size_t rows = std::min(chunk_rows, n - start);
-        CHIP_TRY(enqueue_chunk(m, m->tokens_dev + start, rows, offset + start, false));
-        for (size_t r0 = 0; r0 < rows; r0 += group) {
-            const size_t at = start + r0;
-            LogprobJob j;
-            j.x = m->row_logits;
-            j.rows = std::min(group, rows - r0);
-            j.vocab = j.stride = V;
-            j.tokens = logprobs ? want + at : nullptr;
-            j.top = (int)top;
-            j.logprobs = logprobs ? lp + at : nullptr;
-            j.entropy = entropy ? ent + at : nullptr;
-            j.ids = top ? ids + at * top : nullptr;
-            j.tops = top ? tops + at * top : nullptr;
-            j.ws = m->score_ws;
-            j.ws_bytes = m->score_ws_bytes;
-            CHIP_TRY(enqueue_head_rows(m, r0, j.rows));
-            CHIP_TRY(launch_logprobs(j, m->stream));
+    auto score = [&](const float *x, size_t at, size_t rows) {
+        LogprobJob j;
+        j.x = x;
+        j.rows = rows;
+        j.vocab = j.stride = V;
+        j.tokens = logprobs ? want + at : nullptr;
+        j.top = (int)top;
+        j.logprobs = logprobs ? lp + at : nullptr;
+        j.entropy = entropy ? ent + at : nullptr;
+        j.ids = top ? ids + at * top : nullptr;
+        j.tops = top ? tops + at * top : nullptr;
+        j.ws = m->score_ws;
+        j.ws_bytes = m->score_ws_bytes;
+        return launch_logprobs(j, m->stream);
+    };
+    if (n == 1) {
+        bool ran_fused = false;
+        CHIP_TRY(run_step(m, tokens[0], offset, false, false, &ran_fused));
+        CHIP_TRY(score(m->logits, 0, 1));
+    } else {
+        CHIP_CHECK(hipStreamSynchronize(m->stream));  // tokens_host reuse
+        std::memcpy(m->tokens_host, tokens, n * sizeof(uint32_t));
+        CHIP_CHECK(hipMemcpyAsync(m->tokens_dev, m->tokens_host, n * sizeof(uint32_t), hipMemcpyHostToDevice,
+                                  m->stream));
+        for (size_t start = 0; start < n; start += chunk_rows) {
+            const size_t rows = std::min(chunk_rows, n - start);
+            CHIP_TRY(enqueue_chunk(m, m->tokens_dev + start, rows, offset + start, false));
+            for (size_t r0 = 0; r0 < rows; r0 += group) {
+                const size_t some = std::min(group, rows - r0);
+                CHIP_TRY(enqueue_head_rows(m, r0, some));
+                CHIP_TRY(score(m->row_logits, start + r0, some));
+            }
         }
     }
     auto get = [&](void *dst, const void *src, size_t words) -> int {

@@ -264,7 +264,8 @@ int cheetah_hip_verify_tree(cheetah_hip_model *m, const uint32_t *tokens, const 
  * log probabilities go to logprobs[n] (both may be NULL; for a text's own tokens
  * targets[i] = the token after tokens[i]; one past the vocabulary gives NaN),
  * entropy[n] may be NULL, top_ids and top_logprobs [n * top] are NULL when top
- * is 0. Chunks and cache as cheetah_hip_forward. */
+ * is 0. Chunks and cache as cheetah_hip_forward, bit for bit: one token is a
+ * decode step, and its scores are of that step's logits. */
 int cheetah_hip_forward_logprobs(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t offset,
                                  size_t chunk_rows, const uint32_t *targets, uint32_t top, float *logprobs,
                                  float *entropy, uint32_t *top_ids, float *top_logprobs);

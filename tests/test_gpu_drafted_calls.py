@@ -4,8 +4,11 @@ import numpy as np
 import pytest
 
 import tree_reference as ref
+from cheetah_amd import configs, synth
 
 pytestmark = pytest.mark.gpu
+
+SHAPES = [configs.TINY_QWEN2, configs.TINY_LLAMA]
 
 
 @pytest.fixture(scope="module")
@@ -31,3 +34,34 @@ def test_page_tables_of_other_types(hip, dtype, call):
         return hip.attention(q, kp, vp, t, 8, 8, 192)
 
     assert np.array_equal(run(table.astype(dtype)).view(np.uint32), run(table).view(np.uint32))
+
+
+@pytest.mark.parametrize("quant", [None, "q8"])
+@pytest.mark.parametrize("kv", ["bf16", "f32"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: s.name)
+def test_a_token_scored_alone_is_forwards_decode_step(hip, shape, kv, quant):
+    """Tokens scored one at a time, and a last one behind a chunk: the K/V rows of
+    forward bit for bit, and the scores of forward's own logits (f32 sums of up
+    to 16 terms a thread, 2^-22 + 17 * 2^-24 of them, and a rounding of results
+    below 32)."""
+    w = synth.make_weights(shape)
+    g, plain = (hip.HipForward(shape, w, quant=quant, kv_capacity=256, max_chunk_rows=64, kv=kv) for _ in "gp")
+    text = synth.make_tokens(shape.vocab_size, 45, seed=61)
+    for m in (g, plain):
+        m.forward(text[:40], 0)
+    for i in range(40, 44):
+        lp, ent, ids, tops = g.forward_logprobs(text[i:i + 1], i, targets=text[i + 1:i + 2], top=5)
+        x = plain.forward(text[i:i + 1], i).astype(np.float64)
+        lse = x.max() + np.log(np.exp(x - x.max()).sum())
+        order = np.argsort(-x, kind="stable")[:5]
+        assert np.array_equal(ids[0], order)
+        bar = 2.0**-22 + 17 * 2.0**-24 + 2.0**-20
+        assert abs(lp[0] - (x[text[i + 1]] - lse)) < bar
+        assert (np.abs(tops[0] - (x[order] - lse)) < bar).all()
+        p = np.exp(x - lse)
+        assert abs(ent[0] + (p * (x - lse)).sum()) < 2 * bar * (1 + ent[0])
+    assert g.kv_len() == 44
+    for layer in range(shape.num_layers):
+        for a, b in zip(g.kv_rows(layer, 0, 44), plain.kv_rows(layer, 0, 44)):
+            assert np.array_equal(np.asarray(a, np.float32).view(np.uint32), np.asarray(b, np.float32).view(np.uint32))
+    assert np.array_equal(g.forward(text[44:], 44).view(np.uint32), plain.forward(text[44:], 44).view(np.uint32))
