@@ -1390,7 +1390,10 @@ int run_scored(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t of
     for (size_t r = 1; r <= group; ++r) ws = std::max(ws, logprobs_workspace_bytes(r, V, (int)top));
     if (ws > m->score_ws_bytes) {
         CHIP_TRY(grow(m, &m->score_ws, &m->score_ws_bytes, ws));
-        CHIP_TRY(logprobs_workspace_clear(m->score_ws, m->stream));
+        if (logprobs_workspace_clear(m->score_ws, m->stream)) {
+            m->score_ws_bytes = 0;  // not usable: the next call takes a new one
+            return -1;
+        }
     }
     CHIP_TRY(reserve_positions(m, n));
     uint32_t *want = m->score_dev;
