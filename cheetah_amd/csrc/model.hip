@@ -248,11 +248,11 @@ struct cheetah_hip_model {
     float *row_logits = nullptr, *tree_part = nullptr;
     size_t row_logits_floats = 0, tree_part_floats = 0;
     // The tree whose nodes' K/V rows are at positions [len, len + tree_n); 0:
-    // none. Pinned staging and its device copy: tokens, parents, rotation
-    // positions, then the nodes' argmaxes (kMaxTreeNodes words each).
+    // none. Pinned staging and its device copy (of the first tree on): tokens,
+    // parents, rotation positions, then the nodes' argmaxes (kMaxTreeNodes words each).
     size_t tree_n = 0;
     int32_t *tree_host = nullptr, *tree_dev = nullptr;
-    void *row_scratch = nullptr;  // argmax over kMaxTreeNodes rows
+    uint8_t *row_scratch = nullptr;  // argmax over kMaxTreeNodes rows
     // Scored chunks: the targets and results of a call, the segments' sums.
     uint32_t *score_dev = nullptr;
     uint8_t *score_ws = nullptr;
@@ -730,10 +730,6 @@ int init_instance(cheetah_hip_model *m) {
     CHIP_CHECK(hipHostMalloc((void **)&m->logits_host, (size_t)c.vocab_size * sizeof(float), hipHostMallocDefault));
     CHIP_CHECK(hipHostGetDevicePointer((void **)&m->logits_out, m->logits_host, 0));
     m->page_host.assign(sh.num_pages, 0);
-    CHIP_CHECK(hipHostMalloc((void **)&m->tree_host, 4 * kMaxTreeNodes * sizeof(int32_t), hipHostMallocDefault));
-    CHIP_TRY(m->mem.alloc(&m->tree_dev, 4 * kMaxTreeNodes));
-    CHIP_TRY(m->mem.alloc(&scratch, argmax_scratch_bytes(kMaxTreeNodes)));
-    m->row_scratch = scratch;
     return init_fused(m);
 }
 
@@ -1298,6 +1294,15 @@ int run_forward(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t o
     return 0;
 }
 
+// The buffers of an instance that runs trees: most clones, one a generation, do not.
+int ensure_tree_buffers(cheetah_hip_model *m) {
+    if (!m->tree_dev) CHIP_TRY(m->mem.alloc(&m->tree_dev, 4 * kMaxTreeNodes));
+    if (!m->row_scratch) CHIP_TRY(m->mem.alloc(&m->row_scratch, argmax_scratch_bytes(kMaxTreeNodes)));
+    if (!m->tree_host)
+        CHIP_CHECK(hipHostMalloc((void **)&m->tree_host, 4 * kMaxTreeNodes * sizeof(int32_t), hipHostMallocDefault));
+    return 0;
+}
+
 // Runs a tree's nodes behind the cached positions and waits: their K/V rows
 // in slots [offset, offset + n), their logits in row_logits, with `sample` their
 // argmaxes in the fourth row of tree_host. The tree is then the pending one.
@@ -1314,6 +1319,7 @@ int run_tree(cheetah_hip_model *m, const uint32_t *tokens, const int32_t *parent
             return fail("HIP backend: a node's parent comes before it (-1: a child of the cached text).");
     CHIP_TRY(refresh_weights(m));
     m->tree_n = 0;
+    CHIP_TRY(ensure_tree_buffers(m));
     CHIP_TRY(grow(m, &m->row_logits, &m->row_logits_floats, n * C(m).vocab_size));
     CHIP_TRY(reserve_positions(m, n));
     CHIP_CHECK(hipStreamSynchronize(m->stream));  // tree_host reuse

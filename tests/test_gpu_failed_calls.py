@@ -107,3 +107,24 @@ assert memsets.value == before + 1
 assert all(p.tobytes() == q.tobytes() for p, q in zip(a, b))
 print("done")
 """)
+
+
+def test_a_clone_takes_no_buffers_of_trees(shim):
+    """They come with its first tree; a clone costs what it did without them:
+    pinned memory for its words, its tokens and its logits."""
+    run(shim, r"""
+before = host_allocs.value
+g = model.clone()
+assert host_allocs.value == before + 3
+first = g.forward_greedy(text, 0)
+g.decode_greedy(first, 30, 4)
+g.forward_logprobs(text[:2], 34)
+assert host_allocs.value == before + 3
+a = g.forward_tree([5, 6, 7], [-1, 0, 0], 36)
+assert host_allocs.value == before + 4
+assert g.forward_tree([5, 6, 7], [-1, 0, 0], 36).tolist() == a.tolist()
+g.commit_tree([0, 2])
+g.verify_tree([3, 4], [-1, 0], 38)
+assert host_allocs.value == before + 4
+print("done")
+""")
