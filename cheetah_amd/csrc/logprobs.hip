@@ -627,15 +627,29 @@ int logprob_segs(size_t rows, size_t vocab) {
     return (int)std::max<size_t>(std::min({want, most, (size_t)kMaxSegs}), 1);
 }
 
+// A launch has fewer than 2^32 threads: rows past that (in one segment each) take
+// another.
+constexpr size_t kLaunchRows = UINT32_MAX / kThreads;
 template <class T>
 int launch_logprobs_t(const LogprobJob &j, LogprobArgs &a, hipStream_t s) {
-    const size_t blocks = j.rows * (size_t)a.segs;
-    if (blocks > (size_t)INT32_MAX) return fail("HIP backend: logprobs grid out of range.");
-    if (a.seg <= (unsigned)(8 * kThreads))
-        hipLaunchKernelGGL((logprobs_kernel<T, 8>), dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
-    else
-        hipLaunchKernelGGL((logprobs_kernel<T, 16>), dim3((unsigned)blocks), dim3(kThreads), 0, s, a);
-    CHIP_CHECK(hipGetLastError());
+    for (size_t left = j.rows; left;) {
+        const size_t rows = std::min(left, kLaunchRows / (size_t)a.segs), top = (size_t)a.top;
+        const dim3 grid((unsigned)(rows * (size_t)a.segs));
+        if (a.seg <= (unsigned)(8 * kThreads))
+            hipLaunchKernelGGL((logprobs_kernel<T, 8>), grid, dim3(kThreads), 0, s, a);
+        else
+            hipLaunchKernelGGL((logprobs_kernel<T, 16>), grid, dim3(kThreads), 0, s, a);
+        CHIP_CHECK(hipGetLastError());
+        if (!(left -= rows)) break;
+        a.x = (const T *)a.x + rows * a.stride;
+        if (a.tokens) a.tokens += rows;
+        if (a.logprobs) a.logprobs += rows;
+        if (a.entropy) a.entropy += rows;
+        if (top) {
+            a.ids += rows * top;
+            a.tops += rows * top;
+        }
+    }
     return 0;
 }
 

@@ -65,3 +65,22 @@ def test_a_token_scored_alone_is_forwards_decode_step(hip, shape, kv, quant):
         for a, b in zip(g.kv_rows(layer, 0, 44), plain.kv_rows(layer, 0, 44)):
             assert np.array_equal(np.asarray(a, np.float32).view(np.uint32), np.asarray(b, np.float32).view(np.uint32))
     assert np.array_equal(g.forward(text[44:], 44).view(np.uint32), plain.forward(text[44:], 44).view(np.uint32))
+
+
+@pytest.mark.parametrize("top", [0, 1])
+def test_more_rows_than_a_launch_has_threads_for(hip, top):
+    """2^24 rows of 256 threads are 2^32."""
+    rows = 2**24 + 5
+    x = np.random.default_rng(5).standard_normal((rows, 2)).astype(np.float32)
+    tokens = (np.arange(rows) % 2).astype(np.uint32)
+    lp, ent, ids, tops = hip.logprobs(x, tokens, top)
+    d = x[:, 1].astype(np.float64) - x[:, 0]
+    # log p of the second of two, and of the first.
+    second, first = -np.logaddexp(0, -d), -np.logaddexp(0, d)
+    want = np.where(tokens == 1, second, first)
+    bar = 2.0**-21 + 2.0**-24 * np.abs(want)  # an exponential, two roundings; the result's own
+    assert (np.abs(lp - want) <= bar).all()
+    assert (np.abs(ent + np.exp(first) * first + np.exp(second) * second) <= 2.0**-20).all()
+    if top:
+        assert np.array_equal(ids[:, 0], (d > 0).astype(np.uint32))
+        assert (np.abs(tops[:, 0] - np.maximum(first, second)) <= 2.0**-21).all()
