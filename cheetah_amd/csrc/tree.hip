@@ -122,7 +122,7 @@ __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int hea
     const int lane = threadIdx.x & 63;
     const size_t row = ((size_t)node * a.q_heads + head) * HD;
     const float scale = (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f;
-    float q[D], o[D], m, l;
+    float q[D], o[D], seen[D], m, l;  // seen: NaN with an infinity or NaN in a key's V
 #pragma unroll
     for (int d = 0; d < D; ++d) q[d] = a.q[row + lane + 64 * d];
     int shift = 0;  // V / 2^shift
@@ -131,7 +131,7 @@ __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int hea
         m = -INFINITY;
         l = 0.f;
 #pragma unroll
-        for (int d = 0; d < D; ++d) o[d] = 0.f;
+        for (int d = 0; d < D; ++d) o[d] = seen[d] = 0.f;
 #pragma unroll 1
         for (int p = start; p < end && l == l; ++p) {
             const int x = p - a.offset;
@@ -146,12 +146,16 @@ __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int hea
             m = mn;
             l = l * alpha + w;
 #pragma unroll
-            for (int d = 0; d < D; ++d) o[d] = fmaf(w, kv_value((const KT *)a.v + at + lane + 64 * d) * vs, o[d] * alpha);
+            for (int d = 0; d < D; ++d) {
+                const float v = kv_value((const KT *)a.v + at + lane + 64 * d);
+                o[d] = fmaf(w, v * vs, o[d] * alpha);
+                seen[d] = fmaf(v, 0.f, seen[d]);
+            }
         }
-        float zero = 0.f;  // NaN with a value that is not finite
+        bool over = false;
 #pragma unroll
-        for (int d = 0; d < D; ++d) zero = fmaf(o[d], 0.f, zero);
-        if (shift || l != l || !__any(zero != zero)) break;
+        for (int d = 0; d < D; ++d) over |= seen[d] == 0.f && o[d] * 0.f != 0.f;
+        if (shift || l != l || !__any(over)) break;
         shift = 32;
     }
     const size_t at = ((size_t)node * a.q_heads + head) * S + split;
