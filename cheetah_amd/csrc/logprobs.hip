@@ -22,7 +22,7 @@
 // picks are in memory and counted at 14.6, read by the last block at 15.3, ranked at
 // 17.5. As two launches these 64 rows took 3 us more, one row the same. A release
 // fence in place of the write-through stores (it writes the whole L2 back) made
-// them 29.6 for then 23.4.
+// them 29.6 for 20.4 then.
 #include <algorithm>
 #include <type_traits>
 

@@ -135,7 +135,10 @@ int cheetah_hip_attention_noalloc(const float *q, const cheetah_hip_kv_view *kv,
  * earlier node; a value outside [0, i) makes node i a root. Node i's K/V row is
  * already in the cache, at position offset + i. Every node attends to the
  * positions [0, offset), its ancestors and itself: never to other branches or to
- * positions past the tree, whatever their rows hold (NaN, unwritten memory).
+ * positions past the tree, whatever their rows hold (NaN, unwritten memory). An
+ * infinity or NaN in a V row that a node does see shows in that element of its
+ * output (NaN where the row's weight rounds to 0); finite rows of any size average
+ * to finite outputs. Rows with such values are slow (computed key by key).
  * kv: the paged view of cheetah_hip_attention; kv_format 0 = BF16 pools, 1 =
  * f32 (k_pages / v_pages then point to f32 elements). Page size a multiple of
  * 64, head_dim 64 or 128, 1 to 8 query heads per KV head, 16-byte aligned
@@ -148,7 +151,8 @@ int cheetah_hip_tree_attention(const float *q, const cheetah_hip_kv_view *kv, ui
  * nodes (host) is strictly increasing and below CHEETAH_HIP_MAX_TREE_NODES: a
  * root and its descendants in order. The views (host array) may have page
  * tables of their own but one page size, KV head count and head_dim; a cache
- * listed twice (a pool with the same page table) is refused. Rows past the branch are left as they are. */
+ * listed twice (a pool with the same page table) is refused. Rows past the branch
+ * are left as they are. */
 int cheetah_hip_tree_commit(const cheetah_hip_kv_view *views, size_t nviews, uint32_t kv_format, size_t offset,
                             const uint32_t *nodes, size_t count);
 
