@@ -1265,8 +1265,8 @@ int run_forward(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t o
     CHIP_TRY(refresh_weights(m));
     if (chunk_rows == 0) chunk_rows = 256;
     chunk_rows = std::min(chunk_rows, m->sh->max_chunk);
-    m->tree_n = 0;
     CHIP_TRY(reserve_positions(m, n));
+    m->tree_n = 0;
     if (n == 1) {
         bool ran_fused = false;
         CHIP_TRY(run_step(m, tokens[0], offset, sample, want_logits, &ran_fused));
@@ -1318,10 +1318,10 @@ int run_tree(cheetah_hip_model *m, const uint32_t *tokens, const int32_t *parent
         if (parents[i] < -1 || parents[i] >= (long)i)
             return fail("HIP backend: a node's parent comes before it (-1: a child of the cached text).");
     CHIP_TRY(refresh_weights(m));
-    m->tree_n = 0;
     CHIP_TRY(ensure_tree_buffers(m));
     CHIP_TRY(grow(m, &m->row_logits, &m->row_logits_floats, n * C(m).vocab_size));
     CHIP_TRY(reserve_positions(m, n));
+    m->tree_n = 0;
     CHIP_CHECK(hipStreamSynchronize(m->stream));  // tree_host reuse
     constexpr size_t N = kMaxTreeNodes;
     int32_t *host = m->tree_host, *dev = m->tree_dev;
@@ -1389,7 +1389,6 @@ int run_scored(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t of
     // Rows whose logits are held at once: enough for the LM head's products to
     // be bound by the matrix cores.
     const size_t V = C(m).vocab_size, group = std::min({n, chunk_rows, (size_t)256});
-    m->tree_n = 0;
     if (n > 1) CHIP_TRY(grow(m, &m->row_logits, &m->row_logits_floats, group * V));
     CHIP_TRY(grow(m, &m->score_dev, &m->score_words, n * (3 + 2 * (size_t)top)));
     size_t ws = 0;
@@ -1402,6 +1401,7 @@ int run_scored(cheetah_hip_model *m, const uint32_t *tokens, size_t n, size_t of
         }
     }
     CHIP_TRY(reserve_positions(m, n));
+    m->tree_n = 0;
     uint32_t *want = m->score_dev;
     float *lp = (float *)(want + n), *ent = lp + n;
     uint32_t *ids = (uint32_t *)(ent + n);
@@ -1595,8 +1595,8 @@ int cheetah_hip_decode_greedy(cheetah_hip_model *m, uint32_t token, size_t offse
     if (!tokens_out) return fail("HIP backend: null tokens_out.");
     CHIP_TRY(validate_decode(m, token, offset, steps));
     CHIP_TRY(refresh_weights(m));
-    m->tree_n = 0;
     CHIP_TRY(reserve_positions(m, steps));
+    m->tree_n = 0;
     CHIP_TRY(launch_set_step(m->step_dev, (int32_t)token, (int32_t)offset, m->stream));
     if (fused_fits(m, offset, steps)) CHIP_TRY(run_fused(m, offset, steps));
     else
@@ -1665,8 +1665,8 @@ int cheetah_hip_time_decode(cheetah_hip_model *m, uint32_t token, size_t offset,
     if (steps == 0 || !ms_per_step) return fail("HIP backend: time_decode needs steps and an output.");
     CHIP_TRY(validate_decode(m, token, offset, steps));
     CHIP_TRY(refresh_weights(m));
-    m->tree_n = 0;
     CHIP_TRY(reserve_positions(m, steps));
+    m->tree_n = 0;
     CHIP_TRY(launch_set_step(m->step_dev, (int32_t)token, (int32_t)offset, m->stream));
     hipEvent_t e0, e1;
     CHIP_CHECK(hipEventCreate(&e0));

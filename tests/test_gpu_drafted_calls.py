@@ -84,3 +84,31 @@ def test_more_rows_than_a_launch_has_threads_for(hip, top):
     if top:
         assert np.array_equal(ids[:, 0], (d > 0).astype(np.uint32))
         assert (np.abs(tops[:, 0] - np.maximum(first, second)) <= 2.0**-21).all()
+
+
+def test_a_call_that_finds_no_pages_leaves_the_tree(hip):
+    """Refused calls run nothing: the tree that waits is still there to commit, as
+    if they had not been made."""
+    shape = configs.TINY_LLAMA
+    w = synth.make_weights(shape)
+    g = hip.HipForward(shape, w, kv_capacity=256, max_chunk_rows=64)
+    other = g.clone()
+    text = synth.make_tokens(shape.vocab_size, 128, seed=36)
+    other.forward(text, 0)  # half of the pages
+    g.forward(text[:120], 0)
+    parents = [-1, 0, 0, 1, 1, 3, 2, 6]
+    drafts = synth.make_tokens(shape.vocab_size, 8, seed=37)
+    g.forward_tree(drafts, parents, 120)
+    for call in (lambda: g.forward(text[:20], 120), lambda: g.forward_greedy(text[:20], 120),
+                 lambda: g.decode_greedy(1, 120, 20), lambda: g.time_decode(1, 120, 20),
+                 lambda: g.forward_tree([1] * 20, [-1] * 20, 120), lambda: g.verify_tree([1] * 20, [-1] + [0] * 19, 120),
+                 lambda: g.forward_logprobs(text[:20], 120)):
+        with pytest.raises(hip.HipError, match="pool exhausted"):
+            call()
+    g.commit_tree([0, 2, 6])
+    assert g.kv_len() == 123
+    plain = hip.HipForward(shape, w, kv_capacity=256, max_chunk_rows=64)
+    plain.forward(text[:120], 0)
+    plain.forward_tree(drafts, parents, 120)
+    plain.commit_tree([0, 2, 6])
+    assert np.array_equal(g.forward([5], 123).view(np.uint32), plain.forward([5], 123).view(np.uint32))
