@@ -7,6 +7,7 @@
 //   out[i, h] = sum_p w_p v[p, h / G],  w = softmax_p(q[i, h] . k[p, h / G] / sqrt(head_dim))
 // over p in [0, offset) and offset + a, a = i or an ancestor of i.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "attn_tiles.hpp"
@@ -176,8 +177,9 @@ __device__ void plain_row(const TreeArgs &a, const TreeLds &t, int node, int hea
         }
     }
     // A NaN row: no split outweighs it. A scaled one: its sums are 2^-32 of theirs,
-    // about a maximum 2^32 higher.
-    if (S > 1 && lane == 0) a.ml[at] = make_float2(l == l ? m + (float)shift : INFINITY, shift ? l * 0x1p-32f : l);
+    // about a maximum 2^32 higher. Scores of -inf only: not a split without a key.
+    if (S > 1 && lane == 0)
+        a.ml[at] = make_float2(l == l ? fmaxf(m + (float)shift, -FLT_MAX) : INFINITY, shift ? l * 0x1p-32f : l);
 }
 
 // Eight values as three BF16 parts, each the top 8 bits of what the ones before

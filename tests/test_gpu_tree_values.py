@@ -108,3 +108,24 @@ def test_large_finite_values_average(hip, what, n, offset, hd, kv):
     want, got = (t.astype(np.float64).reshape(n, 8, hd) for t in (want, got))
     for dims in (large, ~large):
         assert (np.abs(got - want)[..., dims] <= TOL * np.abs(v[..., dims]).max()).all()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,offset", SHAPES)
+def test_an_infinity_among_scores_of_minus_infinity_shows(hip, n, offset, hd, kv):
+    """A run of keys whose scores are all -inf, as long as a split: they weigh
+    nothing, and nothing times infinity is NaN."""
+    rng, q, k, v, parents = case(n + hd + 3, n, offset, hd, kv)
+    q.reshape(n, 8, hd)[:, :, 0] = 1.0
+    k[:min(offset - 30, 128), :, 0] = -np.inf
+    clean = ref.attention64(q, k, v, 8, parents, offset)
+    kp, vp, table = ref.paged(k, v, kv, rng)
+    got = hip.tree_attention(q, kp, vp, table, 8, parents, offset)
+    assert (np.abs(got - clean) <= TOL * np.abs(clean).max()).all()
+    v[20, :, 7] = np.inf
+    kp, vp, table = ref.paged(k, v, kv, rng)
+    got = hip.tree_attention(q, kp, vp, table, 8, parents, offset).reshape(n, 8, hd)
+    assert np.isnan(got[:, :, 7]).all()
+    clean = clean.reshape(n, 8, hd)
+    assert (np.abs(np.delete(got - clean, 7, 2)) <= TOL * np.abs(clean).max()).all()
