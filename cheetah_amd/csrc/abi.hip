@@ -443,6 +443,86 @@ int cheetah_hip_tree_commit(const cheetah_hip_kv_view *views, size_t nviews, uin
     return 0;
 }
 
+// What the calls over an 8-bit cache ask of its view.
+static int check_kv8_view(const cheetah_hip_kv8_view &kv, Kv8Cache &c) {
+    if (!kv.k_codes || !kv.v_codes || !kv.k_scales || !kv.v_scales || !kv.page_table)
+        return fail("HIP backend: 8-bit cache with a null pointer.");
+    if (kv.kv_heads == 0 || kv.kv_heads > 65535 || kv.page_size > INT32_MAX)
+        return fail("HIP backend: 8-bit cache geometry out of range.");
+    if (kv.page_size == 0 || kv.page_size % 64)
+        return fail("HIP backend: the KV page size must be a multiple of 64 positions.");
+    if (kv.head_dim != 64 && kv.head_dim != 128)
+        return fail("HIP backend: an 8-bit cache has head_dim 64 or 128.");
+    if (((uintptr_t)kv.k_codes | (uintptr_t)kv.v_codes) % 16 || (uintptr_t)kv.page_table % 4)
+        return fail("HIP backend: 8-bit cache with codes that are not 16-byte aligned (page table 4).");
+    if (kv.k_codes == kv.v_codes || kv.k_scales == kv.v_scales)
+        return fail("HIP backend: 8-bit cache whose K and V are the same pool.");
+    c = Kv8Cache{kv.k_codes, kv.v_codes, kv.k_scales, kv.v_scales,
+                 Kv8Geom{kv.page_table, (int)kv.page_size, (int)kv.kv_heads, (int)kv.head_dim}};
+    return 0;
+}
+
+int cheetah_hip_kv8_append(const void *k, const void *v, uint32_t row_format, size_t rows, size_t stride, size_t offset,
+                           const cheetah_hip_kv8_view *kv) {
+    if (!k || !v || !kv) return fail("HIP backend: 8-bit append with a null pointer.");
+    Kv8AppendJob j;
+    CHIP_TRY(check_kv8_view(*kv, j.kv));
+    if (row_format > 1) return fail("HIP backend: row_format must be 0 (BF16) or 1 (f32).");
+    if (rows == 0) return fail("HIP backend: 8-bit append needs at least one row.");
+    if (rows > kMaxKv8Positions || offset > kMaxKv8Positions - rows)
+        return fail("HIP backend: cache position out of range.");
+    if (stride < (size_t)kv->kv_heads * kv->head_dim || stride > (size_t)INT64_MAX / 4 / (rows + kKv8Block))
+        return fail("HIP backend: 8-bit append with a stride out of range.");
+    const size_t unit = row_format ? 4 : 2;
+    if (((uintptr_t)k | (uintptr_t)v) % unit) return fail("HIP backend: 8-bit append with misaligned rows.");
+    CHIP_TRY(ensure_ready());
+    j.k = k;
+    j.v = v;
+    j.f32 = row_format != 0;
+    j.rows = rows;
+    j.stride = stride;
+    j.offset = offset;
+    return launch_kv8_append(j, g_stream);
+}
+
+int cheetah_hip_kv8_read(const cheetah_hip_kv8_view *kv, size_t begin, size_t n, uint32_t row_format, void *k_out,
+                         void *v_out) {
+    if (!kv || !k_out || !v_out) return fail("HIP backend: 8-bit read with a null pointer.");
+    Kv8Cache c;
+    CHIP_TRY(check_kv8_view(*kv, c));
+    if (row_format > 1) return fail("HIP backend: row_format must be 0 (BF16) or 1 (f32).");
+    if (n == 0) return fail("HIP backend: 8-bit read needs at least one row.");
+    if (n > kMaxKv8Positions || begin > kMaxKv8Positions - n) return fail("HIP backend: cache position out of range.");
+    if (((uintptr_t)k_out | (uintptr_t)v_out) % 16) return fail("HIP backend: 8-bit read needs 16-byte aligned outputs.");
+    CHIP_TRY(ensure_ready());
+    return launch_kv8_read(c, begin, n, row_format != 0, k_out, v_out, g_stream);
+}
+
+int cheetah_hip_kv8_attention(const float *q, const cheetah_hip_kv8_view *kv, uint32_t q_heads, size_t rows,
+                              size_t offset, size_t window, size_t sinks, float *out) {
+    if (!q || !kv || !out) return fail("HIP backend: attention with a null pointer.");
+    Kv8AttnJob j;
+    CHIP_TRY(check_kv8_view(*kv, j.kv));
+    if (rows == 0) return fail("HIP backend: attention needs at least one query row.");
+    if (q_heads == 0 || q_heads > 65535 || q_heads % kv->kv_heads)
+        return fail("HIP backend: q_heads must be a multiple of kv_heads.");
+    if (q_heads / kv->kv_heads > 8) return fail("HIP backend: attention supports 1..8 query heads per KV head.");
+    if (rows > kMaxKv8Positions || offset > kMaxKv8Positions - rows)
+        return fail("HIP backend: cache position out of range.");
+    if (sinks && !window) return fail("HIP backend: sinks go with a window.");
+    if (((uintptr_t)q | (uintptr_t)out) % 16) return fail("HIP backend: attention needs 16-byte aligned q and out.");
+    CHIP_TRY(ensure_ready());
+    j.q = q;
+    j.out = out;
+    j.q_heads = (int)q_heads;
+    j.rows = rows;
+    j.offset = offset;
+    // A window or sinks past every position are as one that just reaches them.
+    j.window = std::min(window, kMaxKv8Positions);
+    j.sinks = std::min(sinks, kMaxKv8Positions);
+    return launch_kv8_attention(j, g_stream);
+}
+
 int cheetah_hip_logprobs(const void *logits, uint32_t logit_format, size_t rows, size_t vocab, size_t stride,
                          const uint32_t *tokens, uint32_t top, float *logprobs, float *entropy, uint32_t *top_ids,
                          float *top_logprobs) {

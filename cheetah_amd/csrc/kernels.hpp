@@ -262,6 +262,48 @@ int launch_tree_commit(const KvLayer *layers, const int32_t *const *page_tables,
                        size_t offset, const uint32_t *nodes, size_t count, hipStream_t s);
 
 // ---------------------------------------------------------------------------
+// The 8-bit paged K/V cache (kv8.hip): E4M3 codes, a power-of-two scale for each
+// kKv8Block positions of a KV head.
+// ---------------------------------------------------------------------------
+constexpr int kKv8Block = 32;
+// A call's positions end below this: tile bounds behind the last one stay below 2^31.
+constexpr size_t kMaxKv8Positions = (size_t)INT32_MAX - 1023;
+
+struct Kv8Geom {
+    const int32_t *page_table = nullptr;  // device
+    int page_size = 64;                   // a multiple of 64
+    int kv_heads = 0;
+    int head_dim = 0;  // 64 or 128
+};
+struct Kv8Cache {
+    uint8_t *k = nullptr, *v = nullptr;                // codes
+    uint8_t *k_scales = nullptr, *v_scales = nullptr;  // exponent + 127
+    Kv8Geom g;
+};
+// Rows of K and V (f32 or BF16, `stride` elements apart, kv_heads * head_dim
+// each) quantised into positions offset .. offset + rows - 1, or from *pos_dev on.
+struct Kv8AppendJob {
+    const void *k = nullptr, *v = nullptr;
+    bool f32 = true;
+    size_t stride = 0, rows = 0, offset = 0;
+    const int32_t *pos_dev = nullptr;
+    Kv8Cache kv;
+};
+int launch_kv8_append(const Kv8AppendJob &job, hipStream_t s);
+// Positions begin .. begin + n - 1 as rows of kv_heads * head_dim f32 or BF16 values.
+int launch_kv8_read(const Kv8Cache &kv, size_t begin, size_t n, bool f32, void *k_out, void *v_out, hipStream_t s);
+// Causal attention of `rows` rows from position `offset` on; window 0: over all
+// positions, else the last `window` of a row and the first `sinks`.
+struct Kv8AttnJob {
+    const float *q = nullptr;  // [rows][q_heads * head_dim]
+    float *out = nullptr;
+    Kv8Cache kv;
+    int q_heads = 0;
+    size_t rows = 0, offset = 0, window = 0, sinks = 0;
+};
+int launch_kv8_attention(const Kv8AttnJob &job, hipStream_t s);
+
+// ---------------------------------------------------------------------------
 // Log probabilities (logprobs.hip): rows of `vocab` logits, `stride` elements
 // apart, BF16 or f32. Null outputs are left out; ids / tops hold `top` a row.
 // ---------------------------------------------------------------------------

@@ -46,6 +46,14 @@ class KvView(_c.Structure):
                 ("kv_heads", _c.c_uint32), ("head_dim", _c.c_uint32)]
 
 
+KV8_BLOCK = 32  # CHEETAH_HIP_KV8_BLOCK
+
+
+class Kv8View(_c.Structure):
+    _fields_ = [("k_codes", _VP), ("v_codes", _VP), ("k_scales", _VP), ("v_scales", _VP), ("page_table", _VP),
+                ("page_size", _c.c_uint32), ("kv_heads", _c.c_uint32), ("head_dim", _c.c_uint32)]
+
+
 # name -> (restype, argtypes): every symbol include/cheetah_hip.h declares.
 SIGNATURES = {
     "cheetah_hip_init": (_c.c_int, [_c.c_int]),
@@ -74,6 +82,9 @@ SIGNATURES = {
     "cheetah_hip_attention_noalloc": (_c.c_int, [_VP, _c.POINTER(KvView), _c.c_uint32, _SZ, _SZ, _VP]),
     "cheetah_hip_tree_attention": (_c.c_int, [_VP, _c.POINTER(KvView), _c.c_uint32, _c.c_uint32, _VP, _SZ, _SZ, _VP]),
     "cheetah_hip_tree_commit": (_c.c_int, [_c.POINTER(KvView), _SZ, _c.c_uint32, _SZ, _U32P, _SZ]),
+    "cheetah_hip_kv8_append": (_c.c_int, [_VP, _VP, _c.c_uint32, _SZ, _SZ, _SZ, _c.POINTER(Kv8View)]),
+    "cheetah_hip_kv8_read": (_c.c_int, [_c.POINTER(Kv8View), _SZ, _SZ, _c.c_uint32, _VP, _VP]),
+    "cheetah_hip_kv8_attention": (_c.c_int, [_VP, _c.POINTER(Kv8View), _c.c_uint32, _SZ, _SZ, _SZ, _SZ, _VP]),
     "cheetah_hip_logprobs": (_c.c_int, [_VP, _c.c_uint32, _SZ, _SZ, _SZ, _VP, _c.c_uint32, _VP, _VP, _VP, _VP]),
     "cheetah_hip_model_create": (_VP, [_c.POINTER(Config), _c.c_uint32, _c.c_uint32, _SZ, _SZ]),
     "cheetah_hip_model_set_unit": (_c.c_int, [_VP, _c.c_char_p, _VP, _SZ, _c.c_uint32,
@@ -335,6 +346,81 @@ def tree_commit(caches, offset: int, nodes) -> list:
                                         nodes.ctypes.data_as(_U32P), nodes.size))
     return [(b[0].download(c[0].dtype, c[0].size).reshape(c[0].shape),
              b[1].download(c[1].dtype, c[1].size).reshape(c[1].shape)) for b, c in zip(held, caches)]
+
+
+class Kv8Cache:
+    """A paged 8-bit K/V cache on the device (E4M3 codes, a power-of-two scale
+    for each 32 positions of a KV head) of `positions` positions: append rows,
+    read them back, attend. table: int32 page table, pages in any order
+    (default: in order); pages: the pool's page count (default: the table's)."""
+
+    def __init__(self, positions: int, kv_heads: int, head_dim: int, page_size: int = 64, table=None, pages=None):
+        if page_size <= 0 or page_size % 64:
+            raise ValueError("the page size is a multiple of 64 positions")
+        if table is None:
+            table = np.arange(-(-positions // page_size))
+        table = np.ascontiguousarray(table, np.int32)
+        pages = max(int(table.max(initial=-1)) + 1, 1) if pages is None else pages
+        if table.size and int(table.max()) >= pages:
+            raise ValueError("page table entry outside the pool")
+        if positions > table.size * page_size:
+            raise ValueError("the page table ends before the cache's positions")
+        self.table, self.page_size, self.kv_heads, self.head_dim = table, page_size, kv_heads, head_dim
+        per = pages * kv_heads * page_size
+        self.codes_shape = (pages, kv_heads, page_size // KV8_BLOCK, KV8_BLOCK * head_dim)
+        # Unwritten memory: NaN codes.
+        self._codes = [DeviceBuffer.from_array(np.full(per * head_dim, 0x7F, np.uint8)) for _ in "kv"]
+        self._scales = [DeviceBuffer.from_array(np.zeros(per // KV8_BLOCK, np.uint8)) for _ in "kv"]
+        self._table = DeviceBuffer.from_array(table)
+        self.view = Kv8View(*(b.ptr for b in self._codes + self._scales), self._table.ptr, page_size, kv_heads,
+                            head_dim)
+
+    def _pages(self, positions) -> None:
+        pages = np.unique(np.asarray(positions, np.int64) // self.page_size)
+        if pages.size and (pages[0] < 0 or pages[-1] >= self.table.size):
+            raise ValueError("position outside the page table")
+        if (self.table[pages] < 0).any():
+            raise ValueError("page table entry outside the pool")
+
+    def append(self, k: np.ndarray, v: np.ndarray, offset: int) -> None:
+        """cheetah_hip_kv8_append of rows [n, kv_heads * head_dim], f32 or BF16
+        (uint16), at positions offset .. offset + n - 1."""
+        k, v = np.ascontiguousarray(k), np.ascontiguousarray(v)
+        if k.dtype != v.dtype or k.dtype not in (np.uint16, np.float32):
+            raise ValueError("rows must both be BF16 (uint16) or both f32")
+        width = self.kv_heads * self.head_dim
+        if k.shape != v.shape or k.size % width:
+            raise ValueError("rows of kv_heads * head_dim values")
+        n = k.size // width
+        self._pages(np.arange(offset // KV8_BLOCK * KV8_BLOCK, offset + n))
+        kd, vd = DeviceBuffer.from_array(k), DeviceBuffer.from_array(v)
+        check(lib().cheetah_hip_kv8_append(kd.ptr, vd.ptr, int(k.dtype == np.float32), n, width, offset,
+                                           _c.byref(self.view)))
+
+    def read(self, begin: int, n: int, bf16: bool = False):
+        """cheetah_hip_kv8_read: K and V of n positions as [n, kv_heads, head_dim]."""
+        dtype = np.uint16 if bf16 else np.float32
+        self._pages(np.arange(begin, begin + n))
+        out = [DeviceBuffer(max(n, 1) * self.kv_heads * self.head_dim * np.dtype(dtype).itemsize) for _ in "kv"]
+        check(lib().cheetah_hip_kv8_read(_c.byref(self.view), begin, n, int(not bf16), out[0].ptr, out[1].ptr))
+        shape = (n, self.kv_heads, self.head_dim)
+        return tuple(o.download(dtype, int(np.prod(shape))).reshape(shape) for o in out)
+
+    def attention(self, q: np.ndarray, q_heads: int, offset: int, window: int = 0, sinks: int = 0) -> np.ndarray:
+        """cheetah_hip_kv8_attention: q f32 [rows, q_heads * head_dim]."""
+        q = np.ascontiguousarray(q, np.float32).reshape(-1, q_heads * self.head_dim)
+        rows = q.shape[0]
+        first = max(offset + 1 - window, 0) if window else 0
+        self._pages(np.concatenate([np.arange(min(sinks, first)), np.arange(first, offset + rows)]))
+        qd, od = DeviceBuffer.from_array(q), DeviceBuffer(max(q.nbytes, 1))
+        check(lib().cheetah_hip_kv8_attention(qd.ptr, _c.byref(self.view), q_heads, rows, offset, window, sinks,
+                                              od.ptr))
+        return od.download(np.float32, q.size).reshape(q.shape)
+
+    def codes(self):
+        """The pools' bytes: (K codes, V codes, K scales, V scales)."""
+        return tuple(b.download(np.uint8).reshape(self.codes_shape) for b in self._codes) + tuple(
+            b.download(np.uint8).reshape(self.codes_shape[:3]) for b in self._scales)
 
 
 def logprobs(logits: np.ndarray, tokens=None, top: int = 0, vocab: int | None = None):

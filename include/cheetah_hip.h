@@ -156,6 +156,58 @@ int cheetah_hip_tree_attention(const float *q, const cheetah_hip_kv_view *kv, ui
 int cheetah_hip_tree_commit(const cheetah_hip_kv_view *views, size_t nviews, uint32_t kv_format, size_t offset,
                             const uint32_t *nodes, size_t count);
 
+/* ------------------------------------------------------------------------
+ * An 8-bit K/V cache, op level. No counterpart in the reference (its caches are
+ * f32). A cached value is an E4M3 code (sign, 4 bits of exponent, 3 of fraction,
+ * no infinities) times the scale of its block: CHEETAH_HIP_KV8_BLOCK consecutive
+ * positions of one KV head, K and V apart. A scale is 2^e, kept as the byte
+ * e + 127, e in [-117, 119]: every value is a normal f32 and an exact BF16 one.
+ *   codes  [pages][kv_heads][page_size / 32][32 * head_dim] bytes; a K block is
+ *          [head_dim / 32][32 positions][32 dims], a V block [head_dim][32 positions]
+ *   scales [pages][kv_heads][page_size / 32] bytes
+ * page_size is a multiple of 64, head_dim 64 or 128; codes are 16-byte aligned,
+ * the four pools do not overlap. page_table (device int32) maps logical pages;
+ * entries of pages that a call neither writes nor reads may hold anything.
+ * ---------------------------------------------------------------------- */
+#define CHEETAH_HIP_KV8_BLOCK 32
+typedef struct cheetah_hip_kv8_view {
+    uint8_t *k_codes;
+    uint8_t *v_codes;
+    uint8_t *k_scales;
+    uint8_t *v_scales;
+    const int32_t *page_table;
+    uint32_t page_size;
+    uint32_t kv_heads;
+    uint32_t head_dim;
+} cheetah_hip_kv8_view;
+/* Quantises `rows` K and V rows into positions offset .. offset + rows - 1. k, v:
+ * device rows of kv_heads * head_dim values, `stride` >= that many elements apart
+ * (k and v may point into packed projections), row_format 0 = BF16, 1 = f32. A
+ * block's scale is the least with |x| <= 448 * 2^e for its rows, codes round to
+ * nearest (ties to even). Rows of the block before `offset` keep their values; a
+ * scale that later rows raise rounds them again (only values below 2^-13 of the
+ * block's largest move, by at most 2^-16 of it), and it does not fall before the
+ * block's first position is written again. Rows behind the last new
+ * one keep their codes, not their values. An infinity or a NaN is kept as NaN and
+ * does not count for the scale; magnitudes past 448 * 2^119 become that. */
+int cheetah_hip_kv8_append(const void *k, const void *v, uint32_t row_format, size_t rows, size_t stride, size_t offset,
+                           const cheetah_hip_kv8_view *kv);
+/* The cached K and V rows of positions begin .. begin + n - 1 as [n][kv_heads *
+ * head_dim] values (device, 16-byte aligned), row_format 0 = BF16, 1 = f32; both
+ * exact. */
+int cheetah_hip_kv8_read(const cheetah_hip_kv8_view *kv, size_t begin, size_t n, uint32_t row_format, void *k_out,
+                         void *v_out);
+/* GQA causal attention over an 8-bit cache for `rows` query rows at positions
+ * offset .. offset + rows - 1 (their K/V already in the cache), q and out as
+ * cheetah_hip_attention's, 16-byte aligned. With window 0 row i sees the
+ * positions [0, offset + i]; with a window the last `window` of these and the
+ * first `sinks` positions (sinks is 0 without a window). 1 to 8 query heads per
+ * KV head. Positions that a row does not see do not count, whatever they hold
+ * (NaN, unwritten memory); a NaN in a row that it does see shows. Pages that no row
+ * sees are not read. */
+int cheetah_hip_kv8_attention(const float *q, const cheetah_hip_kv8_view *kv, uint32_t q_heads, size_t rows,
+                              size_t offset, size_t window, size_t sinks, float *out);
+
 /* Most alternatives a row of cheetah_hip_logprobs returns. */
 #define CHEETAH_HIP_MAX_TOP 64
 /* For each of `rows` rows of `vocab` logits (device, `stride` >= vocab elements
