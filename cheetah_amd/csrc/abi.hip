@@ -520,6 +520,8 @@ int cheetah_hip_kv8_attention(const float *q, const cheetah_hip_kv8_view *kv, ui
     // A window or sinks past every position are as one that just reaches them.
     j.window = std::min(window, kMaxKv8Positions);
     j.sinks = std::min(sinks, kMaxKv8Positions);
+    j.splits = kv8_attention_splits(j);
+    if (j.splits > 1) CHIP_TRY(attention_scratch(kv8_attention_part_floats(j, j.splits), &j.part, &j.part_floats));
     return launch_kv8_attention(j, g_stream);
 }
 

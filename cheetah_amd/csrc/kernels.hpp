@@ -300,7 +300,13 @@ struct Kv8AttnJob {
     Kv8Cache kv;
     int q_heads = 0;
     size_t rows = 0, offset = 0, window = 0, sinks = 0;
+    // Splits of the keys and their partials, kv8_attention_part_floats of them.
+    int splits = 1;
+    float *part = nullptr;
+    size_t part_floats = 0;
 };
+int kv8_attention_splits(const Kv8AttnJob &job);
+size_t kv8_attention_part_floats(const Kv8AttnJob &job, int splits);
 int launch_kv8_attention(const Kv8AttnJob &job, hipStream_t s);
 
 // ---------------------------------------------------------------------------

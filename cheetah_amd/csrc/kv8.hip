@@ -18,6 +18,7 @@
 // so that a lane's operand is 16 consecutive bytes of a 1 KB piece, and a wave's
 // load one piece.
 #include <algorithm>
+#include <atomic>
 
 #include "kernels.hpp"
 
@@ -271,6 +272,8 @@ struct Kv8AttnArgs {
     Kv8Geom g;
     int q_heads, rows, offset, window, sinks;
     float *out;
+    float *part;  // [row][head][split][HD]: weighted sums
+    float2 *ml;   // [row][head][split]: maximum (log2 units), weight sum
 };
 
 // The first position of the window of a row at `pos` (0 without one).
@@ -347,12 +350,449 @@ __device__ void plain_row(const Kv8AttnArgs &a, int row, int head, float *out) {
     }
 }
 
+// The blocks of positions that a range of rows sees, in order: the first `sink`
+// ones, then blocks from `first` on, `count` in all.
+struct Reach {
+    int sink, first, count;
+    __device__ int block(int i) const { return i < sink ? i : first + i - sink; }
+};
+__host__ __device__ __forceinline__ Reach reach_of(int pos_lo, int pos_hi, int window, int sinks) {
+    const int lo = window && pos_lo + 1 > window ? pos_lo + 1 - window : 0;
+    Reach r;
+    r.sink = ((sinks < lo ? sinks : lo) + kBlock - 1) / kBlock;
+    r.first = lo / kBlock > r.sink ? lo / kBlock : r.sink;
+    r.count = r.sink + pos_hi / kBlock + 1 - r.first;
+    return r;
+}
+
+// ---------------------------------------------------------------------------
+// On the matrix cores: v_mfma_f32_32x32x16_f16 over 32 "M rows" (query row x head
+// of the KV group) a wave and blocks of 32 positions,
+//   S^T = K Q^T     A = K: lane (n, h) takes the 16 dims 32 c + 16 h .. of position
+//                   kpos(n); B = the queries, in registers.
+//   O^T += V^T P^T  A = V^T: lane (n, h) takes positions 16 h .. + 15 of dim
+//                   32 u + n; B = the probabilities: with that kpos lane (m, h)
+//                   holds those of its row at positions 16 h .. + 15, where the
+//                   first product leaves them.
+// Codes are exact F16 numbers. Queries (by a power of two of their own a row, so
+// that they fill F16's range) and probabilities are two F16 parts, 22 bits. A
+// K scale multiplies the scores, a V scale comes with the conversion, relative
+// to one that the running sums carry (a power of two, changed without rounding).
+// ---------------------------------------------------------------------------
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ int kpos(int n) { return 16 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3); }
+
+// Eight codes times 2^k as F16.
+__device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b, float scale) {
+    f16x2 r[4];
+    r[0] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, false));
+    r[1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, true));
+    r[2] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, false));
+    r[3] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, true));
+    f16x8 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = r[i][0], v[2 * i + 1] = r[i][1];
+    return v;
+}
+// Two F16 parts of eight values.
+__device__ __forceinline__ void split_f16(const float (&x)[8], f16x8 &hi, f16x8 &lo) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        hi[i] = (_Float16)x[i];
+        lo[i] = (_Float16)(x[i] - (float)hi[i]);
+    }
+}
+
+// One row's output from the parts of its splits or key waves; not finite: again,
+// in plain products. A wave; v: HD / 64 consecutive dims a lane.
 template <int HD>
-__global__ __launch_bounds__(kThreads) void kv8_attn_plain_kernel(Kv8AttnArgs a) {
-    const long item = (long)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-    if (item >= (long)a.rows * a.q_heads) return;
-    const int row = (int)(item / a.q_heads), head = (int)(item % a.q_heads);
-    plain_row<HD>(a, row, head, a.out + (size_t)item * HD);
+__device__ __forceinline__ void finish_row(const Kv8AttnArgs &a, int row, int head, float (&v)[HD / 64]) {
+    float *out = a.out + ((size_t)row * a.q_heads + head) * HD;
+    const int lane = threadIdx.x & 63;
+    bool fine = true;
+#pragma unroll
+    for (int k = 0; k < HD / 64; ++k) fine = fine && fabsf(v[k]) < INFINITY;
+    if (__any(!fine)) {
+        plain_row<HD>(a, row, head, out);
+        return;
+    }
+    if constexpr (HD == 128) *(float2 *)(out + 2 * lane) = make_float2(v[0], v[1]);
+    else out[lane] = v[0];
+}
+
+constexpr int kWaves = 8;
+template <int HD>
+constexpr int kRowPad = HD + 4;  // floats of a row of outputs in LDS
+template <int HD, int WR>
+constexpr size_t kv8_attn_lds_bytes() {
+    constexpr size_t stage = WR == 1 ? 0 : 2 * (kWaves / WR) * 2 * kBlock * HD;
+    constexpr size_t join = kWaves * 32 * kRowPad<HD> * 4 + kWaves * 32 * 8;
+    return stage > join ? stage : join;
+}
+
+template <int HD, int WR>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))) void kv8_attn_kernel(Kv8AttnArgs a, int S) {
+    constexpr int WK = kWaves / WR, C = HD / 32;
+    constexpr bool DIRECT = WR == 1;    // no other wave reads this wave's blocks
+    constexpr int PIECES = 2 * C / WR;  // of a block, copied by a wave (1 KB each)
+    extern __shared__ __attribute__((aligned(256))) uint8_t smem[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wr = wave % WR, wk = wave / WR;
+    const int n = lane & 31, half = lane >> 5;
+    const int G = a.q_heads / a.g.kv_heads, M = a.rows * G, RB = (M + 32 * WR - 1) / (32 * WR);
+    // All row blocks of a KV head and split on one XCD.
+    const int pair = (int)blockIdx.x / (8 * RB) * 8 + (int)blockIdx.x % 8, rb = RB - 1 - (int)blockIdx.x / 8 % RB;
+    if (pair >= S * a.g.kv_heads) return;
+    const int g = pair % a.g.kv_heads, split = pair / a.g.kv_heads;
+    const int m0 = rb * 32 * WR, m = m0 + wr * 32 + n;
+    const bool rvalid = m < M;
+    const int row = rvalid ? m / G : 0, head = g * G + (rvalid ? m % G : 0);
+    const int pos = a.offset + row, lo = window_start(a, pos);
+    // Rows of the block and of the wave (uniform).
+    const int pos_lo = a.offset + m0 / G, pos_hi = a.offset + (min(M, m0 + 32 * WR) - 1) / G;
+    const int wave_lo = a.offset + min(m0 + wr * 32, M - 1) / G, wave_hi = a.offset + (min(M, m0 + wr * 32 + 32) - 1) / G;
+    const int seen_lo = window_start(a, pos_lo), wave_first = window_start(a, wave_hi);
+    const Reach reach = reach_of(pos_lo, pos_hi, a.window, a.sinks);
+    const int begin = (int)((long)reach.count * split / S), end = (int)((long)reach.count * (split + 1) / S);
+    const int steps = __builtin_amdgcn_readfirstlane((end - begin + WK - 1) / WK);  // of the longest key wave
+    const int mine = __builtin_amdgcn_readfirstlane(max(end - begin - wk + WK - 1, 0) / WK);
+
+    // Where this wave's next 64 blocks lie and their scales, a lane each.
+    int held_at = 0;
+    uint32_t held_k = 0, held_v = 0;
+    auto look_up = [&](int i0) {
+        const int i = min(i0 + lane, max(mine - 1, 0));
+        const int b = reach.block(min(begin + wk + i * WK, reach.count - 1));
+        const int per = a.g.page_size / kBlock;
+        const int page = a.g.page_table[b / per];
+        held_at = (page * a.g.kv_heads + g) * per + b % per;
+        held_k = a.k_scales[held_at];
+        held_v = a.v_scales[held_at];
+        asm volatile("" : "+v"(held_k), "+v"(held_v));  // waited for here
+    };
+    look_up(0);
+
+    // Queries: times log2(e) / sqrt(HD), each row by a power of two to 2^14 .. 2^15.
+    f16x8 qh[2 * C], ql[2 * C];
+    int q_exp;
+    {
+        const float sl2 = (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f;
+        const float *qp = a.q + ((size_t)row * a.q_heads + head) * HD + 16 * half;
+        f32x4 raw[C][4];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[c][i] = *(const f32x4 *)(qp + 32 * c + 4 * i);
+        float most = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    raw[c][i][e] = rvalid ? raw[c][i][e] * sl2 : 0.f;
+                    most = fmaxf(most, fabsf(raw[c][i][e]));
+                }
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        q_exp = min(max((int)(__float_as_uint(most) >> 23) - 127, -112), 127) - 14;
+        const float up = two_to(-q_exp);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = raw[c][2 * t + e / 4][e % 4] * up;
+                split_f16(x, qh[2 * c + t], ql[2 * c + t]);
+            }
+    }
+
+    f32x16 o[C];
+#pragma unroll
+    for (int u = 0; u < C; ++u) o[u] = f32x16{};
+    float m2 = -INFINITY, l = 0.f;
+    int v_exp = 0;  // o is in units of 2^v_exp
+
+    const int koff = kpos(n) * 32 + 16 * half, voff = n * kBlock + 16 * half;
+    constexpr int BB = kBlock * HD;  // bytes of a block of K or V
+    u32x4 kr[DIRECT ? C : 1], vr[DIRECT ? C : 1];
+    auto load_k = [&](size_t at) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) kr[DIRECT ? c : 0] = *(const u32x4 *)(a.k + at * BB + 1024 * c + koff);
+    };
+    auto load_v = [&](size_t at) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) vr[DIRECT ? c : 0] = *(const u32x4 *)(a.v + at * BB + 1024 * c + voff);
+    };
+    // A block's pieces to LDS, each lane's own 16 bytes at 16 lane: [K pieces | V pieces].
+    auto copy = [&](size_t at, int buf) {
+        uint8_t *to = smem + (buf * WK + wk) * 2 * BB;
+        const __amdgpu_buffer_rsrc_t rk =
+            __builtin_amdgcn_make_buffer_rsrc((void *)(a.k + at * BB), (short)0, BB, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rv =
+            __builtin_amdgcn_make_buffer_rsrc((void *)(a.v + at * BB), (short)0, BB, 0x00020000);
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            const int c = wr * PIECES + j;  // uniform
+            if (c < C) buf_to_lds<16>(rk, to + 1024 * c, koff, 1024 * c);
+            else buf_to_lds<16>(rv, to + 1024 * c, voff, 1024 * (c - C));
+        }
+    };
+    auto at_of = [&](int i) { return (size_t)(uint32_t)__builtin_amdgcn_readlane(held_at, i & 63); };
+    if (mine > 0) {
+        if constexpr (DIRECT) load_k(at_of(0)), load_v(at_of(0));
+        else copy(at_of(0), 0);
+    }
+    for (int i = 0; i < steps; ++i) {
+        const int buf = i & 1;
+        const bool here = i < mine, more = i + 1 < mine;
+        const int e_k = (int)__builtin_amdgcn_readlane(held_k, i & 63) - 127;
+        const int e_v = (int)__builtin_amdgcn_readlane(held_v, i & 63) - 127;
+        if (more && ((i + 1) & 63) == 0) look_up(i + 1);
+        const size_t at_next = at_of(i + 1);
+        if constexpr (!DIRECT) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (more) copy(at_next, buf ^ 1);
+        }
+        if (!here) continue;
+        const uint8_t *from = smem + (buf * WK + wk) * 2 * BB + 16 * lane;
+        f32x16 s = f32x16{};
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            u32x4 w;
+            if constexpr (DIRECT) w = kr[c];
+            else w = *(const u32x4 *)(from + 1024 * c);
+            const f16x8 k0 = codes_f16(w[0], w[1], 1.f), k1 = codes_f16(w[2], w[3], 1.f);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[2 * c], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[2 * c], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[2 * c + 1], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[2 * c + 1], s, 0, 0, 0);
+        }
+        if constexpr (DIRECT) {
+            if (more) load_k(at_next);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const int p0 = reach.block(begin + wk + i * WK) * kBlock;
+        // Masks, where a row of the wave does not see all of the block.
+        if (p0 + kBlock - 1 > wave_lo || (p0 < wave_first && p0 + kBlock > a.sinks)) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int p = p0 + 16 * half + r;
+                if (p > pos || (p < lo && p >= a.sinks)) s[r] = -INFINITY;
+            }
+        }
+        const float fs = ldexpf(1.f, max(q_exp + e_k, -126));
+        float tmax = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, s[r]);
+        tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64)) * fs;
+        // Exponentials against a maximum that is raised when a score exceeds it by
+        // more than 8 (so p <= 2^8); the running sums are rescaled only then.
+        const bool raise = tmax > m2 + 8.0f;
+        if (__any(raise)) {
+            const float mnew = raise ? tmax : m2;
+            const float alpha = raise ? __builtin_amdgcn_exp2f(m2 - mnew) : 1.f;
+            l *= alpha;
+#pragma unroll
+            for (int u = 0; u < C; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[u][r] *= alpha;
+            m2 = mnew;
+        }
+        const float mref = m2 == -INFINITY ? 0.f : m2;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], fs, -mref));
+            l += s[r];
+        }
+        f16x8 ph[2], pl[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = s[8 * t + e];
+            split_f16(x, ph[t], pl[t]);
+        }
+        // V under 2^(e_v - v_exp): exact in F16 for differences of -15 .. 7.
+        if (i == 0) v_exp = e_v;
+        if (e_v - v_exp > 7 || e_v - v_exp < -15) {
+            // Steps that could lose the sums' values: the rows are computed again.
+            if (abs(e_v - v_exp) > 100) l = NAN;
+#pragma unroll
+            for (int u = 0; u < C; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[u][r] = ldexpf(o[u][r], v_exp - e_v);
+            v_exp = e_v;
+        }
+        const float vs = two_to(e_v - v_exp);
+        // Positions that no row of the block sees may hold anything: zeros.
+        const bool v_edge = p0 + kBlock - 1 > pos_hi || (p0 < seen_lo && p0 + kBlock > a.sinks);
+#pragma unroll
+        for (int u = 0; u < C; ++u) {
+            u32x4 w;
+            if constexpr (DIRECT) w = vr[u];
+            else w = *(const u32x4 *)(from + BB + 1024 * u);
+            if (v_edge) {
+#pragma unroll
+                for (int b = 0; b < 16; ++b) {
+                    const int p = p0 + 16 * half + b;
+                    if (p > pos_hi || (p < seen_lo && p >= a.sinks)) w[b / 4] &= ~(0xFFu << (8 * (b % 4)));
+                }
+            }
+            const f16x8 v0 = codes_f16(w[0], w[1], vs), v1 = codes_f16(w[2], w[3], vs);
+            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, ph[0], o[u], 0, 0, 0);
+            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pl[0], o[u], 0, 0, 0);
+            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, ph[1], o[u], 0, 0, 0);
+            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pl[1], o[u], 0, 0, 0);
+        }
+        if constexpr (DIRECT) {
+            if (more) load_v(at_next);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // The key waves' parts meet in LDS.
+    l += __shfl_xor(l, 32, 64);
+    __syncthreads();  // the tiles' last reads are done
+    float *so = (float *)smem + (size_t)wave * 32 * kRowPad<HD>;
+    float2 *sml = (float2 *)(smem + (size_t)kWaves * 32 * kRowPad<HD> * 4);
+    if (rvalid) {
+#pragma unroll
+        for (int u = 0; u < C; ++u)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = ldexpf(o[u][4 * q + e], v_exp);
+                *(f32x4 *)(so + n * kRowPad<HD> + 32 * u + 8 * q + 4 * half) = v;
+            }
+        if (half == 0) sml[wave * 32 + n] = make_float2(m2, l);
+    }
+    __syncthreads();
+    constexpr int D = HD / 64;
+    for (int r = wave; r < 32 * WR && m0 + r < M; r += kWaves) {
+        float2 ml[WK];
+        float top = -INFINITY, sum = 0.f, v[D];
+#pragma unroll
+        for (int k = 0; k < WK; ++k) {
+            ml[k] = sml[(k * WR + r / 32) * 32 + r % 32];
+            top = fmaxf(top, ml[k].x);
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d) v[d] = 0.f;
+#pragma unroll
+        for (int k = 0; k < WK; ++k) {
+            if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;  // saw nothing (uniform)
+            const float w = __builtin_amdgcn_exp2f(ml[k].x - top);
+            sum = fmaf(w, ml[k].y, sum);
+            const float *p = (const float *)smem + ((size_t)(k * WR + r / 32) * 32 + r % 32) * kRowPad<HD> + D * lane;
+#pragma unroll
+            for (int d = 0; d < D; ++d) v[d] = fmaf(w, p[d], v[d]);
+        }
+        const int orow = (m0 + r) / G, ohead = g * G + (m0 + r) % G;
+        if (S == 1) {
+            const float inv = 1.0f / sum;
+#pragma unroll
+            for (int d = 0; d < D; ++d) v[d] *= inv;
+            finish_row<HD>(a, orow, ohead, v);
+        } else {
+            const size_t at = ((size_t)orow * a.q_heads + ohead) * S + split;
+            if constexpr (D == 2) *(float2 *)(a.part + at * HD + 2 * lane) = make_float2(v[0], v[1]);
+            else a.part[at * HD + lane] = v[0];
+            if (lane == 0) a.ml[at] = make_float2(top, sum);
+        }
+    }
+}
+
+// The splits of a row and head, joined by W waves (each takes every W-th).
+constexpr int kMaxSplits = 128;
+template <int HD, int W>
+__global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a, int S) {
+    constexpr int D = HD / 64, I = 4 / W;  // items a block
+    __shared__ float s_o[4][HD];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w0 = wave % W;
+    const long item = (long)blockIdx.x * I + wave / W;
+    const bool valid = item < (long)a.rows * a.q_heads;
+    float v[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) v[d] = 0.f;
+    if (valid) {
+        const float2 *ml = a.ml + item * S;
+        const float2 x = lane < S ? ml[lane] : make_float2(-INFINITY, 0.f);
+        const float2 y = lane + 64 < S ? ml[lane + 64] : make_float2(-INFINITY, 0.f);
+        const float top = wave_max(fmaxf(x.x, y.x));
+        // A split that saw nothing counts nothing; a NaN sum shows.
+        const float wx = x.x == -INFINITY && x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
+        const float wy = y.x == -INFINITY && y.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(y.x - top);
+        const float inv = 1.0f / wave_sum(wx * x.y + wy * y.y);
+        const float *part = a.part + item * S * HD + D * lane;
+        constexpr int B = 8;
+        for (int s0 = w0; s0 < S; s0 += B * W) {
+            float p[B][D];
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const float *q = part + (size_t)min(s0 + b * W, S - 1) * HD;
+                if constexpr (D == 2) {
+                    const float2 t = *(const float2 *)q;
+                    p[b][0] = t.x, p[b][D - 1] = t.y;
+                } else {
+                    p[b][0] = *q;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int s = s0 + b * W;
+                if (s >= S) break;
+                const float w = __shfl(s < 64 ? wx : wy, s & 63, 64);
+                if (w != 0.f) {  // (NaN too)
+#pragma unroll
+                    for (int d = 0; d < D; ++d) v[d] = fmaf(w, p[b][d], v[d]);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d) v[d] *= inv;
+    }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) s_o[wave][D * lane + d] = v[d];
+        __syncthreads();
+        if (w0 != 0) return;
+#pragma unroll
+        for (int k = 1; k < W; ++k)
+#pragma unroll
+            for (int d = 0; d < D; ++d) v[d] += s_o[wave + k][D * lane + d];
+    }
+    if (valid) finish_row<HD>(a, (int)(item / a.q_heads), (int)(item % a.q_heads), v);
+}
+
+template <int HD, int WR>
+int launch_attn_blocks(const Kv8AttnArgs &a, int S, hipStream_t s) {
+    constexpr size_t lds = kv8_attn_lds_bytes<HD, WR>();
+    static std::atomic<uint64_t> lds_set{0};
+    CHIP_TRY(allow_dynamic_lds((const void *)kv8_attn_kernel<HD, WR>, lds, lds_set));
+    const long M = (long)a.rows * (a.q_heads / a.g.kv_heads), RB = (M + 32 * WR - 1) / (32 * WR);
+    const long pairs = ((long)S * a.g.kv_heads + 7) / 8 * 8;
+    hipLaunchKernelGGL((kv8_attn_kernel<HD, WR>), dim3((unsigned)(pairs * RB)), dim3(64 * kWaves), lds, s, a, S);
+    CHIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+template <int HD>
+int launch_attn(const Kv8AttnArgs &a, int wr, int S, hipStream_t s) {
+    if (wr == 1) CHIP_TRY((launch_attn_blocks<HD, 1>(a, S, s)));
+    else if (wr == 2) CHIP_TRY((launch_attn_blocks<HD, 2>(a, S, s)));
+    else CHIP_TRY((launch_attn_blocks<HD, 4>(a, S, s)));
+    if (S == 1) return 0;
+    const long items = (long)a.rows * a.q_heads;
+    if (S >= 16) hipLaunchKernelGGL((kv8_merge_kernel<HD, 4>), dim3((unsigned)items), dim3(256), 0, s, a, S);
+    else hipLaunchKernelGGL((kv8_merge_kernel<HD, 1>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, s, a, S);
+    CHIP_CHECK(hipGetLastError());
+    return 0;
 }
 
 template <int HD, class T>
@@ -405,7 +845,35 @@ int launch_kv8_read(const Kv8Cache &kv, size_t begin, size_t n, bool f32, void *
     return 0;
 }
 
+// Row waves of a block: as many as there are rows of 32 (query row x head of the
+// group), at most four. The other waves of eight split the keys.
+static int row_waves(const Kv8AttnJob &j) {
+    const size_t M = j.rows * (size_t)(j.q_heads / j.kv.g.kv_heads);
+    return M <= 32 ? 1 : M <= 64 ? 2 : 4;
+}
+
+// A block per CU, and no split without a block of positions for each key wave.
+int kv8_attention_splits(const Kv8AttnJob &j) {
+    const int wr = row_waves(j), wk = kWaves / wr;
+    const size_t M = j.rows * (size_t)(j.q_heads / j.kv.g.kv_heads);
+    const size_t blocks = (M + 32 * wr - 1) / (32 * wr) * (size_t)j.kv.g.kv_heads;
+    const int last = (int)(j.offset + j.rows - 1);
+    const int first = std::max(last + 1 - (int)std::min<size_t>(j.rows, 32 * wr), 0);
+    const size_t reach = (size_t)reach_of(first, last, (int)j.window, (int)j.sinks).count;
+    const size_t most = std::min<size_t>(kMaxSplits, (reach + wk - 1) / wk);
+    return (int)std::max<size_t>(1, std::min(most, (size_t)device_cus() / std::max<size_t>(blocks, 1)));
+}
+
+size_t kv8_attention_part_floats(const Kv8AttnJob &j, int splits) {
+    return splits <= 1 ? 0 : j.rows * (size_t)j.q_heads * splits * (j.kv.g.head_dim + 2);
+}
+
 int launch_kv8_attention(const Kv8AttnJob &j, hipStream_t s) {
+    const int S = std::max(1, j.splits), wr = row_waves(j);
+    if (S > kMaxSplits || j.part_floats < kv8_attention_part_floats(j, S))
+        return fail("HIP backend: 8-bit attention partial buffer too small.");
+    const size_t items = j.rows * (size_t)j.q_heads;
+    if (items / j.kv.g.kv_heads > (size_t)INT32_MAX - 256) return fail("HIP backend: attention with too many rows.");
     Kv8AttnArgs a;
     a.q = j.q;
     a.k = j.kv.k, a.v = j.kv.v, a.k_scales = j.kv.k_scales, a.v_scales = j.kv.v_scales;
@@ -413,11 +881,9 @@ int launch_kv8_attention(const Kv8AttnJob &j, hipStream_t s) {
     a.q_heads = j.q_heads;
     a.rows = (int)j.rows, a.offset = (int)j.offset, a.window = (int)j.window, a.sinks = (int)j.sinks;
     a.out = j.out;
-    const dim3 grid((unsigned)((j.rows * j.q_heads + 3) / 4));
-    if (j.kv.g.head_dim == 64) hipLaunchKernelGGL((kv8_attn_plain_kernel<64>), grid, dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL((kv8_attn_plain_kernel<128>), grid, dim3(kThreads), 0, s, a);
-    CHIP_CHECK(hipGetLastError());
-    return 0;
+    a.part = j.part;
+    a.ml = (float2 *)(j.part + items * (size_t)S * j.kv.g.head_dim);
+    return j.kv.g.head_dim == 64 ? launch_attn<64>(a, wr, S, s) : launch_attn<128>(a, wr, S, s);
 }
 
 }  // namespace chip
