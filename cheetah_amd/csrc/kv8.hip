@@ -283,11 +283,18 @@ __device__ __forceinline__ int window_start(const Kv8AttnArgs &a, int pos) {
 
 // One row and head in plain f32 products, a wave: the maximum and the weight sum,
 // then the values under finished weights, so that finite values average to a
-// finite output and an infinity or a NaN in a value that the row sees shows.
+// finite output and an infinity or a NaN in a value that the row sees shows. A
+// call, so that it takes no registers of the loops it is behind, and one that gets
+// the kernel's arguments where they are, so that it needs no stack (kernels with
+// one start some 5 us later).
+typedef const __attribute__((address_space(4))) Kv8AttnArgs *Kv8KernArgs;
+__device__ __forceinline__ Kv8KernArgs kernel_args() { return (Kv8KernArgs)__builtin_amdgcn_kernarg_segment_ptr(); }
 template <int HD>
-__device__ void plain_row(const Kv8AttnArgs &a, int row, int head, float *out) {
+__device__ __attribute__((noinline)) void plain_row(Kv8KernArgs args, int row, int head) {
+    const Kv8AttnArgs a = *(const Kv8AttnArgs *)args;
     constexpr int C = HD / 32;
     const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
+    float *out = a.out + ((size_t)row * a.q_heads + head) * HD;
     const int g = head / (a.q_heads / a.g.kv_heads), pos = a.offset + row;
     const int lo = window_start(a, pos), sinks = a.window ? min(a.sinks, lo) : 0;
     const float sl2 = (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f;
@@ -325,19 +332,21 @@ __device__ void plain_row(const Kv8AttnArgs &a, int row, int head, float *out) {
             } else {
                 const float w = seen ? __builtin_amdgcn_exp2f(s - m) / l : 0.f;
                 const float scale = two_to((int)a.v_scales[at.scale] - 127);
+#pragma unroll 1
+                for (int j = 16 * half; j < 16 * half + 16; j += 4) {
+                    float wj[4];
+                    bool there[4];
 #pragma unroll
-                for (int u = 0; u < C; ++u) {
-                    const u32x4 c = *(const u32x4 *)(a.v + at.codes + (32 * u + n) * kBlock + 16 * half);
+                    for (int e = 0; e < 4; ++e) {
+                        const int pj = b * kBlock + j + e;
+                        wj[e] = __shfl(w, j + e, 64);
+                        there[e] = pj <= pos && (pj >= lo || pj < sinks);
+                    }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 x = code_values(c[i]) * scale;
+                    for (int u = 0; u < C; ++u) {
+                        const f32x4 x = code_values(*(const uint32_t *)(a.v + at.codes + (32 * u + n) * kBlock + j)) * scale;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int j = 16 * half + 4 * i + e;
-                            const float wj = __shfl(w, j, 64);
-                            const int pj = b * kBlock + j;
-                            if (pj <= pos && (pj >= lo || pj < sinks)) o[u] = fmaf(wj, x[e], o[u]);
-                        }
+                        for (int e = 0; e < 4; ++e) o[u] = there[e] ? fmaf(wj[e], x[e], o[u]) : o[u];
                     }
                 }
             }
@@ -406,21 +415,11 @@ __device__ __forceinline__ void split_f16(const float (&x)[8], f16x8 &hi, f16x8 
     }
 }
 
-// One row's output from the parts of its splits or key waves; not finite: again,
-// in plain products. A wave; v: HD / 64 consecutive dims a lane.
-template <int HD>
-__device__ __forceinline__ void finish_row(const Kv8AttnArgs &a, int row, int head, float (&v)[HD / 64]) {
-    float *out = a.out + ((size_t)row * a.q_heads + head) * HD;
-    const int lane = threadIdx.x & 63;
-    bool fine = true;
-#pragma unroll
-    for (int k = 0; k < HD / 64; ++k) fine = fine && fabsf(v[k]) < INFINITY;
-    if (__any(!fine)) {
-        plain_row<HD>(a, row, head, out);
-        return;
-    }
-    if constexpr (HD == 128) *(float2 *)(out + 2 * lane) = make_float2(v[0], v[1]);
-    else out[lane] = v[0];
+// Which of the positions base .. base + 15 lie at or below `last` and at or above
+// `first` or below `sinks`, a bit each.
+__device__ __forceinline__ uint32_t seen_bits(int base, int last, int first, int sinks) {
+    auto below = [](int n) { return 0xFFFFu >> (16 - min(max(n, 0), 16)); };  // the first n
+    return below(last - base + 1) & (~below(first - base) | below(sinks - base));
 }
 
 constexpr int kWaves = 8;
@@ -429,8 +428,8 @@ constexpr int kRowPad = HD + 4;  // floats of a row of outputs in LDS
 template <int HD, int WR>
 constexpr size_t kv8_attn_lds_bytes() {
     constexpr size_t stage = WR == 1 ? 0 : 2 * (kWaves / WR) * 2 * kBlock * HD;
-    constexpr size_t join = kWaves * 32 * kRowPad<HD> * 4 + kWaves * 32 * 8;
-    return stage > join ? stage : join;
+    constexpr size_t join = kWaves * 32 * kRowPad<HD> * 4;
+    return (stage > join ? stage : join) + kWaves * 32 * 8 + 16;
 }
 
 template <int HD, int WR>
@@ -438,28 +437,37 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     constexpr int WK = kWaves / WR, C = HD / 32;
     constexpr bool DIRECT = WR == 1;    // no other wave reads this wave's blocks
     constexpr int PIECES = 2 * C / WR;  // of a block, copied by a wave (1 KB each)
+    constexpr int BB = kBlock * HD;     // bytes of a block of K or V
     extern __shared__ __attribute__((aligned(256))) uint8_t smem[];
+    float2 *sml = (float2 *)(smem + kv8_attn_lds_bytes<HD, WR>() - kWaves * 32 * 8 - 16);
+    int *odd = (int *)(sml + kWaves * 32);  // a row wave's rows to compute again
+    auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wave = uniform((int)(threadIdx.x >> 6));
     const int wr = wave % WR, wk = wave / WR;
     const int n = lane & 31, half = lane >> 5;
     const int G = a.q_heads / a.g.kv_heads, M = a.rows * G, RB = (M + 32 * WR - 1) / (32 * WR);
-    // All row blocks of a KV head and split on one XCD.
-    const int pair = (int)blockIdx.x / (8 * RB) * 8 + (int)blockIdx.x % 8, rb = RB - 1 - (int)blockIdx.x / 8 % RB;
-    if (pair >= S * a.g.kv_heads) return;
-    const int g = pair % a.g.kv_heads, split = pair / a.g.kv_heads;
+    // Blocks b, b + 8, .. run on one XCD: each takes a run of (KV head, split, row
+    // block), so that few of them read a cache's block. Rows that see the most and
+    // the fewest positions alternate.
+    const int total = RB * S * a.g.kv_heads, run = (total + 7) / 8;
+    const int work = (int)blockIdx.x % 8 * run + (int)blockIdx.x / 8;
+    if (work >= total) return;
+    const int pair = work / RB, turn = work % RB, rb = uniform(turn & 1 ? turn / 2 : RB - 1 - turn / 2);
+    const int g = uniform(pair % a.g.kv_heads), split = uniform(pair / a.g.kv_heads);
     const int m0 = rb * 32 * WR, m = m0 + wr * 32 + n;
     const bool rvalid = m < M;
     const int row = rvalid ? m / G : 0, head = g * G + (rvalid ? m % G : 0);
     const int pos = a.offset + row, lo = window_start(a, pos);
-    // Rows of the block and of the wave (uniform).
-    const int pos_lo = a.offset + m0 / G, pos_hi = a.offset + (min(M, m0 + 32 * WR) - 1) / G;
-    const int wave_lo = a.offset + min(m0 + wr * 32, M - 1) / G, wave_hi = a.offset + (min(M, m0 + wr * 32 + 32) - 1) / G;
+    // Rows of the block and of the wave.
+    const int pos_lo = uniform(a.offset + m0 / G), pos_hi = uniform(a.offset + (min(M, m0 + 32 * WR) - 1) / G);
+    const int wave_lo = uniform(a.offset + min(m0 + wr * 32, M - 1) / G);
+    const int wave_hi = uniform(a.offset + (min(M, m0 + wr * 32 + 32) - 1) / G);
     const int seen_lo = window_start(a, pos_lo), wave_first = window_start(a, wave_hi);
     const Reach reach = reach_of(pos_lo, pos_hi, a.window, a.sinks);
-    const int begin = (int)((long)reach.count * split / S), end = (int)((long)reach.count * (split + 1) / S);
-    const int steps = __builtin_amdgcn_readfirstlane((end - begin + WK - 1) / WK);  // of the longest key wave
-    const int mine = __builtin_amdgcn_readfirstlane(max(end - begin - wk + WK - 1, 0) / WK);
+    const int begin = uniform((int)((long)reach.count * split / S)), end = uniform((int)((long)reach.count * (split + 1) / S));
+    const int steps = (end - begin + WK - 1) / WK;  // of the longest key wave
+    const int mine = max(end - begin - wk + WK - 1, 0) / WK;
 
     // Where this wave's next 64 blocks lie and their scales, a lane each.
     int held_at = 0;
@@ -470,13 +478,48 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         const int per = a.g.page_size / kBlock;
         const int page = a.g.page_table[b / per];
         held_at = (page * a.g.kv_heads + g) * per + b % per;
+    };
+    auto look_up_scales = [&]() {
         held_k = a.k_scales[held_at];
         held_v = a.v_scales[held_at];
-        asm volatile("" : "+v"(held_k), "+v"(held_v));  // waited for here
     };
-    look_up(0);
+    // Waited for here, not at every use.
+    auto landed = [&]() { asm volatile("" : "+v"(held_k), "+v"(held_v)); };
+    auto at_of = [&](int i) { return (size_t)(uint32_t)__builtin_amdgcn_readlane(held_at, i & 63); };
+
+    const int koff = kpos(n) * 32 + 16 * half, voff = n * kBlock + 16 * half;
+    u32x4 kr[C], vr[C];
+    auto load_k = [&](size_t at) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) kr[c] = *(const u32x4 *)(a.k + at * BB + 1024 * c + koff);
+    };
+    auto load_v = [&](size_t at) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) vr[c] = *(const u32x4 *)(a.v + at * BB + 1024 * c + voff);
+    };
+    // A block's pieces to LDS, each lane's own 16 bytes at 16 lane: [K pieces | V pieces].
+    auto copy = [&](size_t at, int buf) {
+        uint8_t *to = smem + (buf * WK + wk) * 2 * BB;
+        const __amdgpu_buffer_rsrc_t rk =
+            __builtin_amdgcn_make_buffer_rsrc((void *)(a.k + at * BB), (short)0, BB, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rv =
+            __builtin_amdgcn_make_buffer_rsrc((void *)(a.v + at * BB), (short)0, BB, 0x00020000);
+#pragma unroll
+        for (int j = 0; j < PIECES / 2; ++j) {
+            const int c = wr * (PIECES / 2) + j;
+            buf_to_lds<16>(rk, to + 1024 * c, koff, 1024 * c);
+            buf_to_lds<16>(rv, to + BB + 1024 * c, voff, 1024 * c);
+        }
+        if constexpr (PIECES == 1) {  // K by the first half of the waves, V by the others
+            const int c = wr % C;
+            if (wr < C) buf_to_lds<16>(rk, to + 1024 * c, koff, 1024 * c);
+            else buf_to_lds<16>(rv, to + BB + 1024 * c, voff, 1024 * c);
+        }
+    };
 
     // Queries: times log2(e) / sqrt(HD), each row by a power of two to 2^14 .. 2^15.
+    // (Every load of the start is in flight at once.)
+    look_up(0);
     f16x8 qh[2 * C], ql[2 * C];
     int q_exp;
     {
@@ -487,6 +530,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i) raw[c][i] = *(const f32x4 *)(qp + 32 * c + 4 * i);
+        __builtin_amdgcn_sched_barrier(0);
+        look_up_scales();
+        if (mine > 0) {
+            if constexpr (DIRECT) load_k(at_of(0)), load_v(at_of(0));
+            else copy(at_of(0), 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         float most = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c)
@@ -510,49 +560,19 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                 split_f16(x, qh[2 * c + t], ql[2 * c + t]);
             }
     }
+    landed();
 
     f32x16 o[C];
 #pragma unroll
     for (int u = 0; u < C; ++u) o[u] = f32x16{};
     float m2 = -INFINITY, l = 0.f;
     int v_exp = 0;  // o is in units of 2^v_exp
-
-    const int koff = kpos(n) * 32 + 16 * half, voff = n * kBlock + 16 * half;
-    constexpr int BB = kBlock * HD;  // bytes of a block of K or V
-    u32x4 kr[DIRECT ? C : 1], vr[DIRECT ? C : 1];
-    auto load_k = [&](size_t at) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) kr[DIRECT ? c : 0] = *(const u32x4 *)(a.k + at * BB + 1024 * c + koff);
-    };
-    auto load_v = [&](size_t at) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) vr[DIRECT ? c : 0] = *(const u32x4 *)(a.v + at * BB + 1024 * c + voff);
-    };
-    // A block's pieces to LDS, each lane's own 16 bytes at 16 lane: [K pieces | V pieces].
-    auto copy = [&](size_t at, int buf) {
-        uint8_t *to = smem + (buf * WK + wk) * 2 * BB;
-        const __amdgpu_buffer_rsrc_t rk =
-            __builtin_amdgcn_make_buffer_rsrc((void *)(a.k + at * BB), (short)0, BB, 0x00020000);
-        const __amdgpu_buffer_rsrc_t rv =
-            __builtin_amdgcn_make_buffer_rsrc((void *)(a.v + at * BB), (short)0, BB, 0x00020000);
-#pragma unroll
-        for (int j = 0; j < PIECES; ++j) {
-            const int c = wr * PIECES + j;  // uniform
-            if (c < C) buf_to_lds<16>(rk, to + 1024 * c, koff, 1024 * c);
-            else buf_to_lds<16>(rv, to + 1024 * c, voff, 1024 * (c - C));
-        }
-    };
-    auto at_of = [&](int i) { return (size_t)(uint32_t)__builtin_amdgcn_readlane(held_at, i & 63); };
-    if (mine > 0) {
-        if constexpr (DIRECT) load_k(at_of(0)), load_v(at_of(0));
-        else copy(at_of(0), 0);
-    }
     for (int i = 0; i < steps; ++i) {
         const int buf = i & 1;
         const bool here = i < mine, more = i + 1 < mine;
         const int e_k = (int)__builtin_amdgcn_readlane(held_k, i & 63) - 127;
         const int e_v = (int)__builtin_amdgcn_readlane(held_v, i & 63) - 127;
-        if (more && ((i + 1) & 63) == 0) look_up(i + 1);
+        if (more && ((i + 1) & 63) == 0) look_up(i + 1), look_up_scales(), landed();
         const size_t at_next = at_of(i + 1);
         if constexpr (!DIRECT) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -561,13 +581,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         }
         if (!here) continue;
         const uint8_t *from = smem + (buf * WK + wk) * 2 * BB + 16 * lane;
+        if constexpr (!DIRECT) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) kr[c] = *(const u32x4 *)(from + 1024 * c);
+        }
         f32x16 s = f32x16{};
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            u32x4 w;
-            if constexpr (DIRECT) w = kr[c];
-            else w = *(const u32x4 *)(from + 1024 * c);
-            const f16x8 k0 = codes_f16(w[0], w[1], 1.f), k1 = codes_f16(w[2], w[3], 1.f);
+            const f16x8 k0 = codes_f16(kr[c][0], kr[c][1], 1.f), k1 = codes_f16(kr[c][2], kr[c][3], 1.f);
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[2 * c], s, 0, 0, 0);
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[2 * c], s, 0, 0, 0);
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[2 * c + 1], s, 0, 0, 0);
@@ -575,16 +596,17 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         }
         if constexpr (DIRECT) {
             if (more) load_k(at_next);
-            __builtin_amdgcn_sched_barrier(0);
+        } else {
+#pragma unroll
+            for (int u = 0; u < C; ++u) vr[u] = *(const u32x4 *)(from + BB + 1024 * u);
         }
+        __builtin_amdgcn_sched_barrier(0);
         const int p0 = reach.block(begin + wk + i * WK) * kBlock;
         // Masks, where a row of the wave does not see all of the block.
         if (p0 + kBlock - 1 > wave_lo || (p0 < wave_first && p0 + kBlock > a.sinks)) {
+            const uint32_t bits = seen_bits(p0 + 16 * half, pos, lo, a.sinks);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int p = p0 + 16 * half + r;
-                if (p > pos || (p < lo && p >= a.sinks)) s[r] = -INFINITY;
-            }
+            for (int r = 0; r < 16; ++r) s[r] = bits >> r & 1 ? s[r] : -INFINITY;
         }
         const float fs = ldexpf(1.f, max(q_exp + e_k, -126));
         float tmax = s[0];
@@ -631,20 +653,18 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         }
         const float vs = two_to(e_v - v_exp);
         // Positions that no row of the block sees may hold anything: zeros.
-        const bool v_edge = p0 + kBlock - 1 > pos_hi || (p0 < seen_lo && p0 + kBlock > a.sinks);
+        if (p0 + kBlock - 1 > pos_hi || (p0 < seen_lo && p0 + kBlock > a.sinks)) {
+            const uint32_t bits = seen_bits(p0 + 16 * half, pos_hi, seen_lo, a.sinks);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t bytes = ((bits >> (4 * j) & 15) * 0x204081u & 0x01010101u) * 0xFFu;
+#pragma unroll
+                for (int u = 0; u < C; ++u) vr[u][j] &= bytes;
+            }
+        }
 #pragma unroll
         for (int u = 0; u < C; ++u) {
-            u32x4 w;
-            if constexpr (DIRECT) w = vr[u];
-            else w = *(const u32x4 *)(from + BB + 1024 * u);
-            if (v_edge) {
-#pragma unroll
-                for (int b = 0; b < 16; ++b) {
-                    const int p = p0 + 16 * half + b;
-                    if (p > pos_hi || (p < seen_lo && p >= a.sinks)) w[b / 4] &= ~(0xFFu << (8 * (b % 4)));
-                }
-            }
-            const f16x8 v0 = codes_f16(w[0], w[1], vs), v1 = codes_f16(w[2], w[3], vs);
+            const f16x8 v0 = codes_f16(vr[u][0], vr[u][1], vs), v1 = codes_f16(vr[u][2], vr[u][3], vs);
             o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, ph[0], o[u], 0, 0, 0);
             o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pl[0], o[u], 0, 0, 0);
             o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, ph[1], o[u], 0, 0, 0);
@@ -655,12 +675,12 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    // The key waves' parts meet in LDS.
+    // The key waves' parts meet in LDS: sums, then a factor for each row and wave.
     l += __shfl_xor(l, 32, 64);
     __syncthreads();  // the tiles' last reads are done
-    float *so = (float *)smem + (size_t)wave * 32 * kRowPad<HD>;
-    float2 *sml = (float2 *)(smem + (size_t)kWaves * 32 * kRowPad<HD> * 4);
+    const int held_rows = min(32 * WR, M - m0);
     if (rvalid) {
+        float *so = (float *)smem + ((size_t)wave * 32 + n) * kRowPad<HD>;
 #pragma unroll
         for (int u = 0; u < C; ++u)
 #pragma unroll
@@ -668,48 +688,61 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                 f32x4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = ldexpf(o[u][4 * q + e], v_exp);
-                *(f32x4 *)(so + n * kRowPad<HD> + 32 * u + 8 * q + 4 * half) = v;
+                *(f32x4 *)(so + 32 * u + 8 * q + 4 * half) = v;
             }
         if (half == 0) sml[wave * 32 + n] = make_float2(m2, l);
     }
+    if (threadIdx.x < 4) odd[threadIdx.x] = 0;
     __syncthreads();
-    constexpr int D = HD / 64;
-    for (int r = wave; r < 32 * WR && m0 + r < M; r += kWaves) {
+    const int r = (int)threadIdx.x;
+    if (r < held_rows) {
         float2 ml[WK];
-        float top = -INFINITY, sum = 0.f, v[D];
+        float top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int k = 0; k < WK; ++k) {
             ml[k] = sml[(k * WR + r / 32) * 32 + r % 32];
             top = fmaxf(top, ml[k].x);
         }
 #pragma unroll
-        for (int d = 0; d < D; ++d) v[d] = 0.f;
+        for (int k = 0; k < WK; ++k) {  // (a wave that saw nothing counts nothing; a NaN sum shows)
+            const float w = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[k].x - top);
+            sum += w != 0.f || ml[k].y != ml[k].y ? w * ml[k].y : 0.f;
+            ml[k].x = w;
+        }
+        const float inv = S == 1 ? 1.0f / sum : 1.f;
+#pragma unroll
+        for (int k = 0; k < WK; ++k) sml[(k * WR + r / 32) * 32 + r % 32].x = ml[k].x * inv;
+        if (S > 1) a.ml[((size_t)((m0 + r) / G) * a.q_heads + g * G + (m0 + r) % G) * S + split] = make_float2(top, sum);
+    }
+    __syncthreads();
+    for (int u = (int)threadIdx.x; u < held_rows * (HD / 4); u += 64 * kWaves) {
+        const int r = u / (HD / 4), d = u % (HD / 4) * 4;
+        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < WK; ++k) {
-            if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;  // saw nothing (uniform)
-            const float w = __builtin_amdgcn_exp2f(ml[k].x - top);
-            sum = fmaf(w, ml[k].y, sum);
-            const float *p = (const float *)smem + ((size_t)(k * WR + r / 32) * 32 + r % 32) * kRowPad<HD> + D * lane;
+            const int at = (k * WR + r / 32) * 32 + r % 32;
+            const float w = sml[at].x;
+            const f32x4 p = *(const f32x4 *)((const float *)smem + (size_t)at * kRowPad<HD> + d);
 #pragma unroll
-            for (int d = 0; d < D; ++d) v[d] = fmaf(w, p[d], v[d]);
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(w, p[e], v[e]);
         }
-        const int orow = (m0 + r) / G, ohead = g * G + (m0 + r) % G;
+        const size_t item = (size_t)((m0 + r) / G) * a.q_heads + g * G + (m0 + r) % G;
         if (S == 1) {
-            const float inv = 1.0f / sum;
-#pragma unroll
-            for (int d = 0; d < D; ++d) v[d] *= inv;
-            finish_row<HD>(a, orow, ohead, v);
+            *(f32x4 *)(a.out + item * HD + d) = v;
+            if (!(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY))
+                atomicOr(&odd[r / 32], 1 << (r % 32));
         } else {
-            const size_t at = ((size_t)orow * a.q_heads + ohead) * S + split;
-            if constexpr (D == 2) *(float2 *)(a.part + at * HD + 2 * lane) = make_float2(v[0], v[1]);
-            else a.part[at * HD + lane] = v[0];
-            if (lane == 0) a.ml[at] = make_float2(top, sum);
+            *(f32x4 *)(a.part + (item * S + split) * HD + d) = v;
         }
     }
+    if (S > 1) return;
+    __syncthreads();
+    for (int r = wave; r < held_rows; r += kWaves)
+        if (uniform(odd[r / 32]) >> (r % 32) & 1) plain_row<HD>(kernel_args(), (m0 + r) / G, g * G + (m0 + r) % G);
 }
 
-// The splits of a row and head, joined by W waves (each takes every W-th).
 constexpr int kMaxSplits = 128;
+// The splits of a row and head, joined by W waves (each takes every W-th).
 template <int HD, int W>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a, int S) {
     constexpr int D = HD / 64, I = 4 / W;  // items a block
@@ -767,7 +800,16 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a, int S) {
 #pragma unroll
             for (int d = 0; d < D; ++d) v[d] += s_o[wave + k][D * lane + d];
     }
-    if (valid) finish_row<HD>(a, (int)(item / a.q_heads), (int)(item % a.q_heads), v);
+    if (!valid) return;
+    float *out = a.out + item * HD + D * lane;
+    bool fine = fabsf(v[0]) < INFINITY;
+    if constexpr (D == 2) {
+        fine = fine && fabsf(v[1]) < INFINITY;
+        *(float2 *)out = make_float2(v[0], v[1]);
+    } else {
+        *out = v[0];
+    }
+    if (__any(!fine)) plain_row<HD>(kernel_args(), (int)(item / a.q_heads), (int)(item % a.q_heads));
 }
 
 template <int HD, int WR>
@@ -776,8 +818,8 @@ int launch_attn_blocks(const Kv8AttnArgs &a, int S, hipStream_t s) {
     static std::atomic<uint64_t> lds_set{0};
     CHIP_TRY(allow_dynamic_lds((const void *)kv8_attn_kernel<HD, WR>, lds, lds_set));
     const long M = (long)a.rows * (a.q_heads / a.g.kv_heads), RB = (M + 32 * WR - 1) / (32 * WR);
-    const long pairs = ((long)S * a.g.kv_heads + 7) / 8 * 8;
-    hipLaunchKernelGGL((kv8_attn_kernel<HD, WR>), dim3((unsigned)(pairs * RB)), dim3(64 * kWaves), lds, s, a, S);
+    const long blocks = (RB * S * a.g.kv_heads + 7) / 8 * 8;
+    hipLaunchKernelGGL((kv8_attn_kernel<HD, WR>), dim3((unsigned)blocks), dim3(64 * kWaves), lds, s, a, S);
     CHIP_CHECK(hipGetLastError());
     return 0;
 }
