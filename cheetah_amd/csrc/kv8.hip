@@ -19,6 +19,7 @@
 // load one piece.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kernels.hpp"
 
@@ -29,6 +30,9 @@ constexpr int kThreads = 256;
 constexpr int kBlock = kKv8Block;
 constexpr int kScaleLeast = -117, kScaleMost = 119;
 constexpr uint32_t kNanCode = 0x7F;
+
+// Block barrier that waits for LDS only: loads stay in flight across it.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // 2^e, e in [-126, 127].
 __device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127) << 23); }
@@ -394,25 +398,29 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ int kpos(int n) { return 16 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3); }
 
-// Eight codes times 2^k as F16.
-__device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b, float scale) {
-    f16x2 r[4];
-    r[0] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, false));
-    r[1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, true));
-    r[2] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, false));
-    r[3] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, true));
-    f16x8 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = r[i][0], v[2 * i + 1] = r[i][1];
-    return v;
+// Four codes times 2^k as F16, and eight.
+__device__ __forceinline__ uint2 codes_f16x4(uint32_t w, float scale) {
+    return make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true)));
 }
-// Two F16 parts of eight values.
-__device__ __forceinline__ void split_f16(const float (&x)[8], f16x8 &hi, f16x8 &lo) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        hi[i] = (_Float16)x[i];
-        lo[i] = (_Float16)(x[i] - (float)hi[i]);
-    }
+__device__ __forceinline__ f16x8 operand(uint2 a, uint2 b) {
+    return __builtin_bit_cast(f16x8, u32x4{a.x, a.y, b.x, b.y});
+}
+__device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b, float scale) {
+    return operand(codes_f16x4(a, scale), codes_f16x4(b, scale));
+}
+// The larger of a lane's value and that of the lane 32 away.
+__device__ __forceinline__ float max_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// Two values' F16 parts: the first 11 bits of each (cut off, so that the subtraction
+// takes no conversion back) and the rest, rounded. Below F16's normal numbers both
+// round at 2^-25.
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const float ha = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), hb = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+    hi = __builtin_bit_cast(uint32_t, f16x2{(_Float16)ha, (_Float16)hb});
+    lo = __builtin_bit_cast(uint32_t, f16x2{(_Float16)(a - ha), (_Float16)(b - hb)});
 }
 
 // Which of the positions base .. base + 15 lie at or below `last` and at or above
@@ -425,11 +433,15 @@ __device__ __forceinline__ uint32_t seen_bits(int base, int last, int first, int
 constexpr int kWaves = 8;
 template <int HD>
 constexpr int kRowPad = HD + 4;  // floats of a row of outputs in LDS
+constexpr size_t kStage = 96 * 1024;   // LDS of three tiles
+template <int HD>
+constexpr int kQRow = HD * 4 + 16;     // bytes of a query row's parts in LDS: high, low, padding
 template <int HD, int WR>
 constexpr size_t kv8_attn_lds_bytes() {
-    constexpr size_t stage = WR == 1 ? 0 : 2 * (kWaves / WR) * 2 * kBlock * HD;
-    constexpr size_t join = kWaves * 32 * kRowPad<HD> * 4;
-    return (stage > join ? stage : join) + kWaves * 32 * 8 + 16;
+    constexpr size_t stage = WR == 1 ? 0 : kStage, join = kWaves * 32 * kRowPad<HD> * 4;
+    constexpr size_t queries = stage / 3 * 2 + 32 * WR * kQRow<HD>;  // in the third tile's place and behind
+    constexpr size_t most = stage > join ? stage : join;
+    return (most > queries ? most : queries) + kWaves * 32 * 8 + 16;
 }
 
 template <int HD, int WR>
@@ -438,6 +450,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     constexpr bool DIRECT = WR == 1;    // no other wave reads this wave's blocks
     constexpr int PIECES = 2 * C / WR;  // of a block, copied by a wave (1 KB each)
     constexpr int BB = kBlock * HD;     // bytes of a block of K or V
+    constexpr int NB = DIRECT ? 1 : (int)kStage / (3 * WK * 2 * BB);  // a key wave's blocks of a tile
     extern __shared__ __attribute__((aligned(256))) uint8_t smem[];
     float2 *sml = (float2 *)(smem + kv8_attn_lds_bytes<HD, WR>() - kWaves * 32 * 8 - 16);
     int *odd = (int *)(sml + kWaves * 32);  // a row wave's rows to compute again
@@ -457,8 +470,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     const int g = uniform(pair % a.g.kv_heads), split = uniform(pair / a.g.kv_heads);
     const int m0 = rb * 32 * WR, m = m0 + wr * 32 + n;
     const bool rvalid = m < M;
-    const int row = rvalid ? m / G : 0, head = g * G + (rvalid ? m % G : 0);
-    const int pos = a.offset + row, lo = window_start(a, pos);
+    const int pos = a.offset + (rvalid ? m / G : 0), lo = window_start(a, pos);
     // Rows of the block and of the wave.
     const int pos_lo = uniform(a.offset + m0 / G), pos_hi = uniform(a.offset + (min(M, m0 + 32 * WR) - 1) / G);
     const int wave_lo = uniform(a.offset + min(m0 + wr * 32, M - 1) / G);
@@ -498,8 +510,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         for (int c = 0; c < C; ++c) vr[c] = *(const u32x4 *)(a.v + at * BB + 1024 * c + voff);
     };
     // A block's pieces to LDS, each lane's own 16 bytes at 16 lane: [K pieces | V pieces].
-    auto copy = [&](size_t at, int buf) {
-        uint8_t *to = smem + (buf * WK + wk) * 2 * BB;
+    auto copy = [&](size_t at, int i) {
+        uint8_t *to = smem + (i % (3 * NB) * WK + wk) * 2 * BB;
         const __amdgpu_buffer_rsrc_t rk =
             __builtin_amdgcn_make_buffer_rsrc((void *)(a.k + at * BB), (short)0, BB, 0x00020000);
         const __amdgpu_buffer_rsrc_t rv =
@@ -517,75 +529,83 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         }
     };
 
-    // Queries: times log2(e) / sqrt(HD), each row by a power of two to 2^14 .. 2^15.
-    // (Every load of the start is in flight at once.)
+    // The start: page entries, queries, the first blocks and their scales, every load
+    // in flight before the first is waited for. Queries come in whole rows, times
+    // log2(e) / sqrt(HD) and by a power of two of each row's own to 2^14 .. 2^15, and
+    // reach the matrix operands by way of LDS (from memory an operand is 16 bytes of
+    // each of 32 rows a load: 4 us for the eight waves).
     look_up(0);
-    f16x8 qh[2 * C], ql[2 * C];
-    int q_exp;
+    uint8_t *sq = smem + (DIRECT ? 0 : kStage / 3 * 2);
+    int *sq_exp = (int *)sml;
+    constexpr int LPR = HD / 4, RPI = 64 / LPR, QI = 4 * WR / RPI;  // lanes a row, rows a load, loads a wave
     {
-        const float sl2 = (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f;
-        const float *qp = a.q + ((size_t)row * a.q_heads + head) * HD + 16 * half;
-        f32x4 raw[C][4];
+        f32x4 raw[QI];
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) raw[c][i] = *(const f32x4 *)(qp + 32 * c + 4 * i);
-        __builtin_amdgcn_sched_barrier(0);
-        look_up_scales();
-        if (mine > 0) {
-            if constexpr (DIRECT) load_k(at_of(0)), load_v(at_of(0));
-            else copy(at_of(0), 0);
+        for (int j = 0; j < QI; ++j) {
+            const int r = m0 + (wave * QI + j) * RPI + lane / LPR, rr = min(r, M - 1);
+            raw[j] = *(const f32x4 *)(a.q + ((size_t)(rr / G) * a.q_heads + g * G + rr % G) * HD + lane % LPR * 4);
         }
         __builtin_amdgcn_sched_barrier(0);
-        float most = 0.f;
+        look_up_scales();
+        // (Counts known here, so that the queries are not waited for with the copies:
+        // behind the last block it is copied again.)
+        if constexpr (DIRECT) {
+            load_k(at_of(0)), load_v(at_of(0));
+        } else {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+            for (int i = 0; i < 2 * NB; ++i) copy(at_of(max(min(i, mine - 1), 0)), i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const float sl2 = (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < QI; ++j) {
+            const int r = (wave * QI + j) * RPI + lane / LPR;
+            f32x4 v = raw[j] * (m0 + r < M ? sl2 : 0.f);
+            float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    raw[c][i][e] = rvalid ? raw[c][i][e] * sl2 : 0.f;
-                    most = fmaxf(most, fabsf(raw[c][i][e]));
-                }
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
-        q_exp = min(max((int)(__float_as_uint(most) >> 23) - 127, -112), 127) - 14;
-        const float up = two_to(-q_exp);
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = raw[c][2 * t + e / 4][e % 4] * up;
-                split_f16(x, qh[2 * c + t], ql[2 * c + t]);
-            }
+            for (int d = 1; d < LPR; d <<= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
+            const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -112), 127) - 14;
+            v *= two_to(-e);
+            uint2 hi, lo;
+            split_f16(v[0], v[1], hi.x, lo.x);
+            split_f16(v[2], v[3], hi.y, lo.y);
+            *(uint2 *)(sq + r * kQRow<HD> + lane % LPR * 8) = hi;
+            *(uint2 *)(sq + r * kQRow<HD> + HD * 2 + lane % LPR * 8) = lo;
+            if (lane % LPR == 0) sq_exp[r] = e;
+        }
     }
     landed();
+    lds_barrier();
+    f16x8 qh[2 * C], ql[2 * C];
+    const int q_exp = sq_exp[wr * 32 + n];
+#pragma unroll
+    for (int k = 0; k < 2 * C; ++k) {
+        const uint8_t *from = sq + (wr * 32 + n) * kQRow<HD> + k / 2 * 64 + 32 * half + 16 * (k % 2);
+        qh[k] = *(const f16x8 *)from;
+        ql[k] = *(const f16x8 *)(from + HD * 2);
+    }
 
     f32x16 o[C];
 #pragma unroll
     for (int u = 0; u < C; ++u) o[u] = f32x16{};
     float m2 = -INFINITY, l = 0.f;
     int v_exp = 0;  // o is in units of 2^v_exp
-    for (int i = 0; i < steps; ++i) {
-        const int buf = i & 1;
-        const bool here = i < mine, more = i + 1 < mine;
-        const int e_k = (int)__builtin_amdgcn_readlane(held_k, i & 63) - 127;
-        const int e_v = (int)__builtin_amdgcn_readlane(held_v, i & 63) - 127;
-        if (more && ((i + 1) & 63) == 0) look_up(i + 1), look_up_scales(), landed();
-        const size_t at_next = at_of(i + 1);
-        if constexpr (!DIRECT) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (more) copy(at_next, buf ^ 1);
-        }
-        if (!here) continue;
-        const uint8_t *from = smem + (buf * WK + wk) * 2 * BB + 16 * lane;
+    uint32_t now_k = held_k, now_v = held_v, next_k = 0, next_v = 0;  // (the next ones are looked up a tile ahead)
+    auto lds_at = [&](int i) { return smem + (i % (3 * NB) * WK + wk) * 2 * BB + 16 * lane; };
+    auto read_k = [&](int i) {
         if constexpr (!DIRECT) {
 #pragma unroll
-            for (int c = 0; c < C; ++c) kr[c] = *(const u32x4 *)(from + 1024 * c);
+            for (int c = 0; c < C; ++c) kr[c] = *(const u32x4 *)(lds_at(i) + 1024 * c);
         }
-        f32x16 s = f32x16{};
+    };
+    auto read_v = [&](int i) {
+        if constexpr (!DIRECT) {
+#pragma unroll
+            for (int u = 0; u < C; ++u) vr[u] = *(const u32x4 *)(lds_at(i) + BB + 1024 * u);
+        }
+    };
+    auto scores = [&](f32x16 &s) {
+        s = f32x16{};
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const f16x8 k0 = codes_f16(kr[c][0], kr[c][1], 1.f), k1 = codes_f16(kr[c][2], kr[c][3], 1.f);
@@ -594,27 +614,28 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[2 * c + 1], s, 0, 0, 0);
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[2 * c + 1], s, 0, 0, 0);
         }
-        if constexpr (DIRECT) {
-            if (more) load_k(at_next);
-        } else {
-#pragma unroll
-            for (int u = 0; u < C; ++u) vr[u] = *(const u32x4 *)(from + BB + 1024 * u);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+    };
+    // Masks, where a row of the wave does not see all of block i.
+    auto mask = [&](int i, f32x16 &s) {
         const int p0 = reach.block(begin + wk + i * WK) * kBlock;
-        // Masks, where a row of the wave does not see all of the block.
         if (p0 + kBlock - 1 > wave_lo || (p0 < wave_first && p0 + kBlock > a.sinks)) {
             const uint32_t bits = seen_bits(p0 + 16 * half, pos, lo, a.sinks);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = bits >> r & 1 ? s[r] : -INFINITY;
         }
-        const float fs = ldexpf(1.f, max(q_exp + e_k, -126));
-        float tmax = s[0];
+    };
+    auto largest = [&](const f32x16 &s) {
+        float t = s[0];
 #pragma unroll
-        for (int r = 1; r < 16; ++r) tmax = fmaxf(tmax, s[r]);
-        tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64)) * fs;
-        // Exponentials against a maximum that is raised when a score exceeds it by
-        // more than 8 (so p <= 2^8); the running sums are rescaled only then.
+        for (int r = 1; r < 16; ++r) t = fmaxf(t, s[r]);
+        return max_halves(t);
+    };
+    auto scale_of = [&](int i) {  // of block i's scores
+        return ldexpf(1.f, max(q_exp + (int)__builtin_amdgcn_readlane(now_k, i & 63) - 127, -126));
+    };
+    // Exponentials against a maximum that is raised when a score exceeds it by more
+    // than 8 (so p <= 2^8); the running sums are rescaled only then.
+    auto raise_to = [&](float tmax) {
         const bool raise = tmax > m2 + 8.0f;
         if (__any(raise)) {
             const float mnew = raise ? tmax : m2;
@@ -626,21 +647,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                 for (int r = 0; r < 16; ++r) o[u][r] *= alpha;
             m2 = mnew;
         }
-        const float mref = m2 == -INFINITY ? 0.f : m2;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], fs, -mref));
-            l += s[r];
-        }
-        f16x8 ph[2], pl[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[8 * t + e];
-            split_f16(x, ph[t], pl[t]);
-        }
-        // V under 2^(e_v - v_exp): exact in F16 for differences of -15 .. 7.
+    };
+    f32x16 s;
+    float fs = 0.f;
+    auto reference = [&]() { return m2 == -INFINITY ? 0.f : m2; };
+    // V under 2^(e_v - v_exp): exact in F16 for differences of -15 .. 7. The factor of
+    // block i's codes.
+    auto value_scale = [&](int i) {
+        const int e_v = (int)__builtin_amdgcn_readlane(now_v, i & 63) - 127;
         if (i == 0) v_exp = e_v;
         if (e_v - v_exp > 7 || e_v - v_exp < -15) {
             // Steps that could lose the sums' values: the rows are computed again.
@@ -651,8 +665,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                 for (int r = 0; r < 16; ++r) o[u][r] = ldexpf(o[u][r], v_exp - e_v);
             v_exp = e_v;
         }
-        const float vs = two_to(e_v - v_exp);
-        // Positions that no row of the block sees may hold anything: zeros.
+        return two_to(e_v - v_exp);
+    };
+    // Positions that no row of the block sees may hold anything: zeros.
+    auto clear_v = [&](int i) {
+        const int p0 = reach.block(begin + wk + i * WK) * kBlock;
         if (p0 + kBlock - 1 > pos_hi || (p0 < seen_lo && p0 + kBlock > a.sinks)) {
             const uint32_t bits = seen_bits(p0 + 16 * half, pos_hi, seen_lo, a.sinks);
 #pragma unroll
@@ -662,17 +679,131 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                 for (int u = 0; u < C; ++u) vr[u][j] &= bytes;
             }
         }
-#pragma unroll
-        for (int u = 0; u < C; ++u) {
-            const f16x8 v0 = codes_f16(vr[u][0], vr[u][1], vs), v1 = codes_f16(vr[u][2], vr[u][3], vs);
-            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, ph[0], o[u], 0, 0, 0);
-            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pl[0], o[u], 0, 0, 0);
-            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, ph[1], o[u], 0, 0, 0);
-            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pl[1], o[u], 0, 0, 0);
+    };
+    // Probability r - 1 of a block from its score's exponential, in two F16 parts (a
+    // pair at a time), and the exponential of score r, so that none is waited for.
+    uint32_t ph[8], pl[8];
+    auto exponential = [&](int r, float mref) {
+        if (r < 16) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], fs, -mref));
+        if (r > 0) l += s[r - 1];
+        if (r > 0 && r % 2 == 0) {
+            split_f16(s[r - 2], s[r - 1], ph[r / 2 - 1], pl[r / 2 - 1]);
         }
-        if constexpr (DIRECT) {
-            if (more) load_v(at_next);
+    };
+    auto part = [&](const uint32_t (&p)[8], int k) {
+        return __builtin_bit_cast(f16x8, u32x4{p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]});
+    };
+    if constexpr (DIRECT) {
+        // No other wave waits for this one's blocks: the next block's loads are issued
+        // as soon as the registers are free.
+        for (int i = 0; i < mine; ++i) {
+            if (i > 0 && (i & 63) == 0) now_k = held_k, now_v = held_v;
+            if (((i + 1) & 63) == 0 && i + 1 < mine) look_up(i + 1), look_up_scales(), landed();
+            const size_t at_next = at_of(i + 1);
+            scores(s);
+            if (i + 1 < mine) load_k(at_next);
             __builtin_amdgcn_sched_barrier(0);
+            mask(i, s);
+            fs = scale_of(i);
+            raise_to(largest(s) * fs);
+            const float mref = reference();
+#pragma unroll
+            for (int r = 0; r <= 16; ++r) exponential(r, mref);
+            const float vs = value_scale(i);
+            clear_v(i);
+#pragma unroll
+            for (int u = 0; u < C; ++u) {
+                const f16x8 v0 = codes_f16(vr[u][0], vr[u][1], vs), v1 = codes_f16(vr[u][2], vr[u][3], vs);
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, part(ph, 0), o[u], 0, 0, 0);
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, part(pl, 0), o[u], 0, 0, 0);
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, part(ph, 1), o[u], 0, 0, 0);
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, part(pl, 1), o[u], 0, 0, 0);
+            }
+            if (i + 1 < mine) load_v(at_next);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+        // A block's exponentials are laid between the products of the next block's
+        // scores, and the next maxima between its own V products: a wave's vector
+        // instructions run while its matrix instructions do, and two waves of a SIMD that
+        // do the same thing at the same time do not overlap. K and V are read from LDS
+        // one phase before their use.
+        // The first tile has landed (copies end in order; one block a tile: the second too).
+        constexpr int LATER = NB == 1 ? 0 : NB * PIECES;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(LATER) : "memory");
+        if (NB == 1 && mine > 2) copy(at_of(2), 2);
+        if (mine > 0) {
+            read_k(0);
+            scores(s);
+            mask(0, s);
+            fs = scale_of(0);
+            raise_to(largest(s) * fs);
+            if (mine > 1) read_k(1);
+        }
+        constexpr int E = 4 / C;  // exponentials for a product
+        for (int i = 0; i < steps; ++i) {
+            f32x16 t = f32x16{};
+            float vs = 0.f;
+            if (i < mine) {
+                read_v(i);
+                const float mref = reference();
+                uint2 k4[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) k4[q] = codes_f16x4(kr[0][q], 1.f);
+                // (Behind the last block: scores of an earlier one, which nothing reads.)
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const f16x8 k0 = operand(k4[0], k4[1]), k1 = operand(k4[2], k4[3]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(q < 2 ? k0 : k1, q & 1 ? ql[2 * c + q / 2] : qh[2 * c + q / 2], t, 0,
+                                                                   0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (c + 1 < C) k4[q] = codes_f16x4(kr[c + 1][q], 1.f);
+#pragma unroll
+                        for (int x = 0; x < E; ++x) exponential((4 * c + q) * E + x, mref);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                exponential(16, mref);
+            }
+            // The tile of block i + 2: it has landed, and V of block i and all before is read
+            // by all; the tile after it takes the place of the one before the last.
+            const int ahead = i + 2 + NB;
+            if ((i + 2) % NB == 0 && i + 2 < steps) {
+                if ((ahead & 63) == 0 && ahead < mine) look_up(ahead), look_up_scales(), landed(), next_k = held_k, next_v = held_v;
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                for (int j = ahead; j < min(ahead + NB, mine); ++j) copy(at_of(j), j);
+            }
+            if (i >= mine) continue;
+            if (i + 2 < mine) read_k(i + 2);
+            vs = value_scale(i);
+            clear_v(i);
+            if (i + 1 < mine) mask(i + 1, t);
+            float tmax = t[0];
+            uint2 v4[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v4[q] = codes_f16x4(vr[0][q], vs);
+#pragma unroll
+            for (int u = 0; u < C; ++u) {
+                const f16x8 v0 = operand(v4[0], v4[1]), v1 = operand(v4[2], v4[3]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q < 2 ? v0 : v1, q & 1 ? part(pl, q / 2) : part(ph, q / 2), o[u], 0, 0,
+                                                                  0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (u + 1 < C) v4[q] = codes_f16x4(vr[u + 1][q], vs);
+#pragma unroll
+                    for (int x = 0; x < E; ++x) tmax = fmaxf(tmax, t[(4 * u + q) * E + x]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (i + 1 < mine) {
+                if (((i + 1) & 63) == 0) now_k = next_k, now_v = next_v;
+                fs = scale_of(i + 1);
+                raise_to(max_halves(tmax) * fs);
+            }
+            s = t;
         }
     }
     // The key waves' parts meet in LDS: sums, then a factor for each row and wave.
@@ -715,6 +846,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         if (S > 1) a.ml[((size_t)((m0 + r) / G) * a.q_heads + g * G + (m0 + r) % G) * S + split] = make_float2(top, sum);
     }
     __syncthreads();
+#pragma unroll 4
     for (int u = (int)threadIdx.x; u < held_rows * (HD / 4); u += 64 * kWaves) {
         const int r = u / (HD / 4), d = u % (HD / 4) * 4;
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -741,66 +873,66 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         if (uniform(odd[r / 32]) >> (r % 32) & 1) plain_row<HD>(kernel_args(), (m0 + r) / G, g * G + (m0 + r) % G);
 }
 
+// The splits of a row and head, joined by W waves (each takes every W-th); the
+// values are on their way while the weights are found.
 constexpr int kMaxSplits = 128;
-// The splits of a row and head, joined by W waves (each takes every W-th).
 template <int HD, int W>
-__global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a, int S) {
-    constexpr int D = HD / 64, I = 4 / W;  // items a block
-    __shared__ float s_o[4][HD];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w0 = wave % W;
-    const long item = (long)blockIdx.x * I + wave / W;
-    const bool valid = item < (long)a.rows * a.q_heads;
-    float v[D];
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(Kv8AttnArgs a, int S) {
+    constexpr int D = HD / 64, I = W == 1 ? 4 : 1, B = W == 1 ? 8 : kMaxSplits / W;  // items a block, splits at once
+    __shared__ float s_o[W == 1 ? 1 : W][HD];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w0 = W == 1 ? 0 : wave;
+    const long item = (long)blockIdx.x * I + (W == 1 ? wave : 0);
+    if (item >= (long)a.rows * a.q_heads) return;  // (a wave's own where W is 1)
+    const float2 *ml = a.ml + item * S;
+    const float *part = a.part + item * S * HD + D * lane;
+    float v[D], p[B][D];
 #pragma unroll
     for (int d = 0; d < D; ++d) v[d] = 0.f;
-    if (valid) {
-        const float2 *ml = a.ml + item * S;
-        const float2 x = lane < S ? ml[lane] : make_float2(-INFINITY, 0.f);
-        const float2 y = lane + 64 < S ? ml[lane + 64] : make_float2(-INFINITY, 0.f);
-        const float top = wave_max(fmaxf(x.x, y.x));
-        // A split that saw nothing counts nothing; a NaN sum shows.
-        const float wx = x.x == -INFINITY && x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
-        const float wy = y.x == -INFINITY && y.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(y.x - top);
-        const float inv = 1.0f / wave_sum(wx * x.y + wy * y.y);
-        const float *part = a.part + item * S * HD + D * lane;
-        constexpr int B = 8;
-        for (int s0 = w0; s0 < S; s0 += B * W) {
-            float p[B][D];
+    const float2 x = ml[min(lane, S - 1)], y = ml[min(lane + 64, S - 1)];
+    auto load = [&](int s0) {
 #pragma unroll
-            for (int b = 0; b < B; ++b) {
-                const float *q = part + (size_t)min(s0 + b * W, S - 1) * HD;
-                if constexpr (D == 2) {
-                    const float2 t = *(const float2 *)q;
-                    p[b][0] = t.x, p[b][D - 1] = t.y;
-                } else {
-                    p[b][0] = *q;
-                }
-            }
-#pragma unroll
-            for (int b = 0; b < B; ++b) {
-                const int s = s0 + b * W;
-                if (s >= S) break;
-                const float w = __shfl(s < 64 ? wx : wy, s & 63, 64);
-                if (w != 0.f) {  // (NaN too)
-#pragma unroll
-                    for (int d = 0; d < D; ++d) v[d] = fmaf(w, p[b][d], v[d]);
-                }
+        for (int b = 0; b < B; ++b) {
+            const float *q = part + (size_t)min(s0 + b * W, S - 1) * HD;
+            if constexpr (D == 2) {
+                const float2 t = *(const float2 *)q;
+                p[b][0] = t.x, p[b][D - 1] = t.y;
+            } else {
+                p[b][0] = *q;
             }
         }
+    };
+    load(w0);
+    const float top = wave_max(fmaxf(x.x, y.x));
+    // A split that saw nothing counts nothing; a NaN sum shows.
+    const float wx = lane >= S || (x.x == -INFINITY && x.y == 0.f) ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
+    const float wy = lane + 64 >= S || (y.x == -INFINITY && y.y == 0.f) ? 0.f : __builtin_amdgcn_exp2f(y.x - top);
+    const float sum = wave_sum((wx != 0.f || x.y != x.y ? wx * x.y : 0.f) + (wy != 0.f || y.y != y.y ? wy * y.y : 0.f));
+    for (int s0 = w0; s0 < S; s0 += B * W) {
+        if (s0 != w0) load(s0);
 #pragma unroll
-        for (int d = 0; d < D; ++d) v[d] *= inv;
+        for (int b = 0; b < B; ++b) {
+            const int s = s0 + b * W;
+            if (s >= S) break;
+            const float w = __shfl(s < 64 ? wx : wy, s & 63, 64);
+            if (w != 0.f) {  // (NaN too)
+#pragma unroll
+                for (int d = 0; d < D; ++d) v[d] = fmaf(w, p[b][d], v[d]);
+            }
+        }
     }
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int d = 0; d < D; ++d) v[d] *= inv;
     if constexpr (W > 1) {
 #pragma unroll
         for (int d = 0; d < D; ++d) s_o[wave][D * lane + d] = v[d];
         __syncthreads();
-        if (w0 != 0) return;
+        if (wave != 0) return;
 #pragma unroll
         for (int k = 1; k < W; ++k)
 #pragma unroll
-            for (int d = 0; d < D; ++d) v[d] += s_o[wave + k][D * lane + d];
+            for (int d = 0; d < D; ++d) v[d] += s_o[k][D * lane + d];
     }
-    if (!valid) return;
     float *out = a.out + item * HD + D * lane;
     bool fine = fabsf(v[0]) < INFINITY;
     if constexpr (D == 2) {
@@ -831,7 +963,7 @@ int launch_attn(const Kv8AttnArgs &a, int wr, int S, hipStream_t s) {
     else CHIP_TRY((launch_attn_blocks<HD, 4>(a, S, s)));
     if (S == 1) return 0;
     const long items = (long)a.rows * a.q_heads;
-    if (S >= 16) hipLaunchKernelGGL((kv8_merge_kernel<HD, 4>), dim3((unsigned)items), dim3(256), 0, s, a, S);
+    if (S > 8) hipLaunchKernelGGL((kv8_merge_kernel<HD, 8>), dim3((unsigned)items), dim3(512), 0, s, a, S);
     else hipLaunchKernelGGL((kv8_merge_kernel<HD, 1>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, s, a, S);
     CHIP_CHECK(hipGetLastError());
     return 0;
@@ -887,31 +1019,46 @@ int launch_kv8_read(const Kv8Cache &kv, size_t begin, size_t n, bool f32, void *
     return 0;
 }
 
-// Row waves of a block: as many as there are rows of 32 (query row x head of the
-// group), at most four. The other waves of eight split the keys.
-static int row_waves(const Kv8AttnJob &j) {
-    const size_t M = j.rows * (size_t)(j.q_heads / j.kv.g.kv_heads);
-    return M <= 32 ? 1 : M <= 64 ? 2 : 4;
+// How a call is cut: row waves of a block (the other waves of eight split its keys
+// in LDS) and splits of the keys (a block each, joined by a merge kernel). The
+// cheapest by an estimate, in us: 1.85 (half that at head_dim 64) for a wave's block
+// of positions at two waves a SIMD, 6 for the start and the end of a round of
+// blocks, 4.5 TB/s for a merge's partials and 3 for its launch. Blocks of one row
+// wave read K and V from the caches for every 32 rows, four row waves for 128:
+// ties go to more.
+struct Cut {
+    int wr, splits;
+};
+static Cut cut_of(const Kv8AttnJob &j) {
+    const size_t G = j.q_heads / j.kv.g.kv_heads, M = j.rows * G, kvh = j.kv.g.kv_heads, hd = j.kv.g.head_dim;
+    const size_t cus = (size_t)std::max(device_cus(), 1), tiles = (M + 31) / 32;
+    const int last = (int)(j.offset + j.rows - 1);
+    Cut best{1, 1};
+    double least = 0;
+    for (int wr = 4; wr >= 1; wr /= 2) {
+        if (wr > 1 && tiles <= (size_t)wr / 2) continue;  // row waves without rows
+        const size_t wk = kWaves / wr, blocks = (tiles + wr - 1) / wr * kvh;
+        const int first = std::max(last + 1 - (int)std::min<size_t>(j.rows, (32 * wr + G - 1) / G + 1), 0);
+        const size_t reach = (size_t)reach_of(first, last, (int)j.window, (int)j.sinks).count;
+        const size_t most = std::max<size_t>(1, std::min<size_t>(kMaxSplits, std::min((reach + wk - 1) / wk, cus / blocks)));
+        for (size_t S = 1; S <= most; S = S < most && S * 2 > most ? most : S * 2) {
+            const double rounds = (double)((blocks * S + cus - 1) / cus), steps = (double)((reach + S * wk - 1) / (S * wk));
+            double us = rounds * (6 + steps * (hd == 64 ? 0.95 : 1.85));
+            if (S > 1) us += 3 + 2.0 * (double)(j.rows * j.q_heads * S * hd * 4) / 4.5e6;
+            if (least == 0 || us < least) least = us, best = Cut{wr, (int)S};
+        }
+    }
+    return best;
 }
 
-// A block per CU, and no split without a block of positions for each key wave.
-int kv8_attention_splits(const Kv8AttnJob &j) {
-    const int wr = row_waves(j), wk = kWaves / wr;
-    const size_t M = j.rows * (size_t)(j.q_heads / j.kv.g.kv_heads);
-    const size_t blocks = (M + 32 * wr - 1) / (32 * wr) * (size_t)j.kv.g.kv_heads;
-    const int last = (int)(j.offset + j.rows - 1);
-    const int first = std::max(last + 1 - (int)std::min<size_t>(j.rows, 32 * wr), 0);
-    const size_t reach = (size_t)reach_of(first, last, (int)j.window, (int)j.sinks).count;
-    const size_t most = std::min<size_t>(kMaxSplits, (reach + wk - 1) / wk);
-    return (int)std::max<size_t>(1, std::min(most, (size_t)device_cus() / std::max<size_t>(blocks, 1)));
-}
+int kv8_attention_splits(const Kv8AttnJob &j) { return cut_of(j).splits; }
 
 size_t kv8_attention_part_floats(const Kv8AttnJob &j, int splits) {
     return splits <= 1 ? 0 : j.rows * (size_t)j.q_heads * splits * (j.kv.g.head_dim + 2);
 }
 
 int launch_kv8_attention(const Kv8AttnJob &j, hipStream_t s) {
-    const int S = std::max(1, j.splits), wr = row_waves(j);
+    const int S = std::max(1, j.splits), wr = cut_of(j).wr;
     if (S > kMaxSplits || j.part_floats < kv8_attention_part_floats(j, S))
         return fail("HIP backend: 8-bit attention partial buffer too small.");
     const size_t items = j.rows * (size_t)j.q_heads;
