@@ -286,6 +286,7 @@ struct Kv8AppendJob {
     const void *k = nullptr, *v = nullptr;
     bool f32 = true;
     size_t stride = 0, rows = 0, offset = 0;
+    size_t head_stride = 0;  // elements between a row's KV heads (0: head_dim)
     const int32_t *pos_dev = nullptr;
     Kv8Cache kv;
 };
@@ -300,6 +301,10 @@ struct Kv8AttnJob {
     Kv8Cache kv;
     int q_heads = 0;
     size_t rows = 0, offset = 0, window = 0, sinks = 0;
+    // One row: its position on the device (a captured decode step).
+    const int32_t *pos_dev = nullptr;
+    // Optional BF16 halves of out (as AttnJob's); out may then be null.
+    uint16_t *out_hi = nullptr, *out_lo = nullptr;
     // Splits of the keys and their partials, kv8_attention_part_floats of them.
     int splits = 1;
     float *part = nullptr;
@@ -307,6 +312,9 @@ struct Kv8AttnJob {
 };
 int kv8_attention_splits(const Kv8AttnJob &job);
 size_t kv8_attention_part_floats(const Kv8AttnJob &job, int splits);
+// At least as many for any call, and what a launch sets up once (before a capture).
+size_t kv8_attention_part_most(int head_dim);
+int kv8_attention_prepare(int head_dim);
 int launch_kv8_attention(const Kv8AttnJob &job, hipStream_t s);
 
 // ---------------------------------------------------------------------------

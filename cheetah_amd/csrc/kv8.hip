@@ -88,7 +88,7 @@ __device__ __forceinline__ int exponent_for(float most) {
 // ---------------------------------------------------------------------------
 struct AppendArgs {
     const void *x[2];  // K, V rows
-    long stride;
+    long stride, head_stride;
     uint8_t *codes[2], *scales[2];
     Kv8Geom g;
     const int32_t *pos_dev;  // the first row's position, where set
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
     const BlockAt at = block_at(a.g, page, (int)(first % a.g.page_size) / kBlock, head, HD);
     uint8_t *codes = (which ? a.codes[1] : a.codes[0]) + at.codes;
     uint8_t *scale = (which ? a.scales[1] : a.scales[0]) + at.scale;
-    const T *x = (const T *)(which ? a.x[1] : a.x[0]) + (first - offset) * a.stride + (size_t)head * HD;
+    const T *x = (const T *)(which ? a.x[1] : a.x[0]) + (first - offset) * a.stride + head * a.head_stride;
     const int e_old = keep ? (int)*scale - 127 : kScaleLeast;
 
     f32x4 v[U][2];
@@ -278,7 +278,39 @@ struct Kv8AttnArgs {
     float *out;
     float *part;  // [row][head][split][HD]: weighted sums
     float2 *ml;   // [row][head][split]: maximum (log2 units), weight sum
+    const int32_t *pos_dev;     // offset's word on the device (null: offset)
+    uint16_t *out_hi, *out_lo;  // BF16 halves of out (null: not written); out may then be null
 };
+
+__device__ __forceinline__ int first_pos(const Kv8AttnArgs &a) { return a.pos_dev ? *a.pos_dev : a.offset; }
+
+// N consecutive outputs from element i on, and their BF16 halves where asked for.
+template <int N>
+__device__ __forceinline__ void store_out(const Kv8AttnArgs &a, size_t i, const float (&v)[N]) {
+    if (a.out) {
+        if constexpr (N == 4) *(f32x4 *)(a.out + i) = f32x4{v[0], v[1], v[2], v[3]};
+        else if constexpr (N == 2) *(float2 *)(a.out + i) = make_float2(v[0], v[1]);
+        else a.out[i] = v[0];
+    }
+    if (!a.out_hi) return;
+    uint16_t h[4], l[4];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const __bf16 hb = (__bf16)v[k];
+        h[k] = __builtin_bit_cast(uint16_t, hb);
+        l[k] = __builtin_bit_cast(uint16_t, (__bf16)(v[k] - (float)hb));
+    }
+    if constexpr (N == 4) {
+        *(uint2 *)(a.out_hi + i) = make_uint2((uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16);
+        *(uint2 *)(a.out_lo + i) = make_uint2((uint32_t)l[0] | (uint32_t)l[1] << 16, (uint32_t)l[2] | (uint32_t)l[3] << 16);
+    } else if constexpr (N == 2) {
+        *(uint32_t *)(a.out_hi + i) = (uint32_t)h[0] | (uint32_t)h[1] << 16;
+        *(uint32_t *)(a.out_lo + i) = (uint32_t)l[0] | (uint32_t)l[1] << 16;
+    } else {
+        a.out_hi[i] = h[0];
+        a.out_lo[i] = l[0];
+    }
+}
 
 // The first position of the window of a row at `pos` (0 without one).
 __device__ __forceinline__ int window_start(const Kv8AttnArgs &a, int pos) {
@@ -298,8 +330,7 @@ __device__ __attribute__((noinline)) void plain_row(Kv8KernArgs args, int row, i
     const Kv8AttnArgs a = *(const Kv8AttnArgs *)args;
     constexpr int C = HD / 32;
     const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
-    float *out = a.out + ((size_t)row * a.q_heads + head) * HD;
-    const int g = head / (a.q_heads / a.g.kv_heads), pos = a.offset + row;
+    const int g = head / (a.q_heads / a.g.kv_heads), pos = first_pos(a) + row;
     const int lo = window_start(a, pos), sinks = a.window ? min(a.sinks, lo) : 0;
     const float sl2 = (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f;
     const float *q = a.q + ((size_t)row * a.q_heads + head) * HD + 16 * half;
@@ -358,8 +389,8 @@ __device__ __attribute__((noinline)) void plain_row(Kv8KernArgs args, int row, i
     }
 #pragma unroll
     for (int u = 0; u < C; ++u) {
-        const float v = o[u] + __shfl_xor(o[u], 32, 64);
-        if (half == 0) out[32 * u + n] = v;
+        const float v[1] = {o[u] + __shfl_xor(o[u], 32, 64)};
+        if (half == 0) store_out<1>(a, ((size_t)row * a.q_heads + head) * HD + 32 * u + n, v);
     }
 }
 
@@ -470,11 +501,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     const int g = uniform(pair % a.g.kv_heads), split = uniform(pair / a.g.kv_heads);
     const int m0 = rb * 32 * WR, m = m0 + wr * 32 + n;
     const bool rvalid = m < M;
-    const int pos = a.offset + (rvalid ? m / G : 0), lo = window_start(a, pos);
+    const int offset = uniform(first_pos(a)), pos = offset + (rvalid ? m / G : 0), lo = window_start(a, pos);
     // Rows of the block and of the wave.
-    const int pos_lo = uniform(a.offset + m0 / G), pos_hi = uniform(a.offset + (min(M, m0 + 32 * WR) - 1) / G);
-    const int wave_lo = uniform(a.offset + min(m0 + wr * 32, M - 1) / G);
-    const int wave_hi = uniform(a.offset + (min(M, m0 + wr * 32 + 32) - 1) / G);
+    const int pos_lo = uniform(offset + m0 / G), pos_hi = uniform(offset + (min(M, m0 + 32 * WR) - 1) / G);
+    const int wave_lo = uniform(offset + min(m0 + wr * 32, M - 1) / G);
+    const int wave_hi = uniform(offset + (min(M, m0 + wr * 32 + 32) - 1) / G);
     const int seen_lo = window_start(a, pos_lo), wave_first = window_start(a, wave_hi);
     const Reach reach = reach_of(pos_lo, pos_hi, a.window, a.sinks);
     const int begin = uniform((int)((long)reach.count * split / S)), end = uniform((int)((long)reach.count * (split + 1) / S));
@@ -860,7 +891,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         }
         const size_t item = (size_t)((m0 + r) / G) * a.q_heads + g * G + (m0 + r) % G;
         if (S == 1) {
-            *(f32x4 *)(a.out + item * HD + d) = v;
+            const float x[4] = {v[0], v[1], v[2], v[3]};
+            store_out<4>(a, item * HD + d, x);
             if (!(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY))
                 atomicOr(&odd[r / 32], 1 << (r % 32));
         } else {
@@ -933,22 +965,16 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(Kv8Att
 #pragma unroll
             for (int d = 0; d < D; ++d) v[d] += s_o[k][D * lane + d];
     }
-    float *out = a.out + item * HD + D * lane;
-    bool fine = fabsf(v[0]) < INFINITY;
-    if constexpr (D == 2) {
-        fine = fine && fabsf(v[1]) < INFINITY;
-        *(float2 *)out = make_float2(v[0], v[1]);
-    } else {
-        *out = v[0];
-    }
+    bool fine = true;
+#pragma unroll
+    for (int d = 0; d < D; ++d) fine = fine && fabsf(v[d]) < INFINITY;
+    store_out<D>(a, item * HD + D * lane, v);
     if (__any(!fine)) plain_row<HD>(kernel_args(), (int)(item / a.q_heads), (int)(item % a.q_heads));
 }
 
 template <int HD, int WR>
 int launch_attn_blocks(const Kv8AttnArgs &a, int S, hipStream_t s) {
     constexpr size_t lds = kv8_attn_lds_bytes<HD, WR>();
-    static std::atomic<uint64_t> lds_set{0};
-    CHIP_TRY(allow_dynamic_lds((const void *)kv8_attn_kernel<HD, WR>, lds, lds_set));
     const long M = (long)a.rows * (a.q_heads / a.g.kv_heads), RB = (M + 32 * WR - 1) / (32 * WR);
     const long blocks = (RB * S * a.g.kv_heads + 7) / 8 * 8;
     hipLaunchKernelGGL((kv8_attn_kernel<HD, WR>), dim3((unsigned)blocks), dim3(64 * kWaves), lds, s, a, S);
@@ -984,6 +1010,7 @@ int launch_kv8_append(const Kv8AppendJob &j, hipStream_t s) {
     AppendArgs a;
     a.x[0] = j.k, a.x[1] = j.v;
     a.stride = (long)j.stride;
+    a.head_stride = (long)(j.head_stride ? j.head_stride : (size_t)j.kv.g.head_dim);
     a.codes[0] = j.kv.k, a.codes[1] = j.kv.v, a.scales[0] = j.kv.k_scales, a.scales[1] = j.kv.v_scales;
     a.g = j.kv.g;
     a.pos_dev = j.pos_dev;
@@ -993,7 +1020,7 @@ int launch_kv8_append(const Kv8AppendJob &j, hipStream_t s) {
     const size_t blocks = j.pos_dev ? (j.rows + kBlock - 2) / kBlock + 1
                                     : (j.offset + j.rows - 1) / kBlock - j.offset / kBlock + 1;
     const size_t unit = j.f32 ? 4 : 2;
-    const bool vec = ((uintptr_t)j.k | (uintptr_t)j.v | (j.stride * unit)) % 16 == 0;
+    const bool vec = ((uintptr_t)j.k | (uintptr_t)j.v | (j.stride * unit) | (a.head_stride * unit)) % 16 == 0;
     const unsigned n = (unsigned)blocks;
     if (j.kv.g.head_dim == 64)
         return j.f32 ? launch_append<64, float>(j, a, vec, n, s) : launch_append<64, uint16_t>(j, a, vec, n, s);
@@ -1057,7 +1084,23 @@ size_t kv8_attention_part_floats(const Kv8AttnJob &j, int splits) {
     return splits <= 1 ? 0 : j.rows * (size_t)j.q_heads * splits * (j.kv.g.head_dim + 2);
 }
 
+// Partials of any call of a head size: its splits and row blocks are one block of at
+// most 128 rows (query row x head) a CU, or one split.
+size_t kv8_attention_part_most(int head_dim) { return (size_t)std::max(device_cus(), 1) * 128 * (head_dim + 2); }
+
+template <int HD>
+static int prepare() {
+    static std::atomic<uint64_t> set[3];
+    CHIP_TRY(allow_dynamic_lds((const void *)kv8_attn_kernel<HD, 1>, kv8_attn_lds_bytes<HD, 1>(), set[0]));
+    CHIP_TRY(allow_dynamic_lds((const void *)kv8_attn_kernel<HD, 2>, kv8_attn_lds_bytes<HD, 2>(), set[1]));
+    return allow_dynamic_lds((const void *)kv8_attn_kernel<HD, 4>, kv8_attn_lds_bytes<HD, 4>(), set[2]);
+}
+int kv8_attention_prepare(int head_dim) { return head_dim == 64 ? prepare<64>() : prepare<128>(); }
+
 int launch_kv8_attention(const Kv8AttnJob &j, hipStream_t s) {
+    CHIP_TRY(kv8_attention_prepare(j.kv.g.head_dim));
+    if (!j.out && !(j.out_hi && j.out_lo)) return fail("HIP backend: 8-bit attention without an output.");
+    if (j.pos_dev && j.rows != 1) return fail("HIP backend: a position on the device goes with one row.");
     const int S = std::max(1, j.splits), wr = cut_of(j).wr;
     if (S > kMaxSplits || j.part_floats < kv8_attention_part_floats(j, S))
         return fail("HIP backend: 8-bit attention partial buffer too small.");
@@ -1070,6 +1113,8 @@ int launch_kv8_attention(const Kv8AttnJob &j, hipStream_t s) {
     a.q_heads = j.q_heads;
     a.rows = (int)j.rows, a.offset = (int)j.offset, a.window = (int)j.window, a.sinks = (int)j.sinks;
     a.out = j.out;
+    a.out_hi = j.out_hi, a.out_lo = j.out_lo;
+    a.pos_dev = j.pos_dev;
     a.part = j.part;
     a.ml = (float2 *)(j.part + items * (size_t)S * j.kv.g.head_dim);
     return j.kv.g.head_dim == 64 ? launch_attn<64>(a, wr, S, s) : launch_attn<128>(a, wr, S, s);

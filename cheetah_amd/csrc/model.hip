@@ -11,7 +11,9 @@
 // layer for K and for V. A page id indexes every layer's pool; one page
 // table per model maps logical page -> physical page. Pages are refcounted
 // across a model, its clones and snapshots: a snapshot takes references, a
-// restore maps them, and the first write into a shared page copies it.
+// restore maps them, and the first write into a shared page copies it. f32 pages
+// are laid out alike; an 8-bit cache (kv8.hip) has blocks of codes and a scale for
+// each, and rotated rows reach it by way of a chunk of f32 rows.
 //
 // Decode (n == 1) is one captured hipGraph: embedding, 24-32 layers of
 // {QKV GEMV with fused RMSNorm + bias, RoPE + KV append, split-K attention,
@@ -87,6 +89,7 @@ struct Layer {
     float *o_bias = nullptr;    // f32 [hidden] or null
     uint16_t *ln1 = nullptr, *ln2 = nullptr;
     KvLayer kv;
+    uint8_t *k_scales = nullptr, *v_scales = nullptr;  // of an 8-bit cache
     // The persistent decode kernel's copy of down_proj, columns regrouped
     // per FFN block of the grid (fused_down_columns); built while down is
     // resident, freed when down is evicted to the host tier.
@@ -120,6 +123,7 @@ struct Shared {
     cheetah_hip_config cfg{};
     int quant = 0;  // 0, FMT_Q8, FMT_Q4
     int kv_f32 = 0;  // KV element type: 0 = BF16, 1 = f32
+    bool kv8 = false;  // or E4M3 codes with a scale for each block (kv8.hip)
     size_t kv_capacity = 0, max_chunk = 0;
     bool finalized = false;
     std::unordered_map<std::string, Staged> staged;
@@ -131,7 +135,8 @@ struct Shared {
     float *rope_cos = nullptr, *rope_sin = nullptr;
     int num_pages = 0;
     size_t page_elems = 0;  // elements of one page of one layer (K or V)
-    size_t page_bytes() const { return page_elems * (kv_f32 ? 4 : 2); }
+    size_t page_bytes() const { return page_elems * (kv8 ? 1 : kv_f32 ? 4 : 2); }
+    size_t page_scales() const { return (size_t)cfg.kv_heads * (kPageSize / kKv8Block); }
     std::mutex mu;
     std::vector<int> refs;
     std::vector<int> free_list;
@@ -203,6 +208,11 @@ struct cheetah_hip_model {
     // activations
     float *hidden = nullptr, *normed = nullptr, *qkv = nullptr, *qrot = nullptr, *attn = nullptr, *act = nullptr;
     float *logits = nullptr, *part = nullptr;
+    // 8-bit cache: a chunk's rotated K and V rows on their way to it, laid out as an
+    // f32 cache of one page ([kv_head][max_chunk][head_dim] each), and device words
+    // 0, 1, .. kv_capacity - 1, 0.
+    float *kv_rows = nullptr;
+    int32_t *row_pos = nullptr;
     size_t part_floats = 0;
     float *gemm_ws = nullptr;  // split-K chunk sums of the prefill GEMMs
     size_t gemm_ws_floats = 0;
@@ -454,6 +464,9 @@ int finalize(cheetah_hip_model *m) {
         CHIP_TRY(sh.mem.alloc(&v, sh.page_bytes() * sh.num_pages));
         L.kv.k = k;
         L.kv.v = v;
+        if (!sh.kv8) continue;
+        CHIP_TRY(sh.mem.alloc(&L.k_scales, sh.page_scales() * sh.num_pages));
+        CHIP_TRY(sh.mem.alloc(&L.v_scales, sh.page_scales() * sh.num_pages));
     }
     sh.refs.assign(sh.num_pages, 0);
     sh.free_list.clear();
@@ -518,7 +531,7 @@ int init_fused(cheetah_hip_model *m) {
     // The kernel addresses one layer's K (or V) pool with 30-bit element
     // indices.
     const bool small_pool = (size_t)sh.num_pages * c.kv_heads * kPageSize * c.head_dim < (size_t(1) << 30);
-    m->fused_ok = small_pool && fused_decode_supported(L0.qkv.fmt, (int)c.hidden_size, (int)c.q_heads,
+    m->fused_ok = !sh.kv8 && small_pool && fused_decode_supported(L0.qkv.fmt, (int)c.hidden_size, (int)c.q_heads,
                                                        (int)c.kv_heads, (int)c.head_dim, (int)c.intermediate_size,
                                                        al, m->fused_blocks);
     if (!m->fused_ok) return 0;
@@ -701,6 +714,15 @@ int init_instance(cheetah_hip_model *m) {
         sh.kv_capacity, attention_prefill_span(sh.kv_capacity, sh.kv_f32 != 0));
     const size_t part_rows = std::max(R * prefill_splits, (size_t)attention_max_splits());
     m->part_floats = part_rows * c.q_heads * (c.head_dim + 2);
+    if (sh.kv8) {
+        m->part_floats = kv8_attention_part_most((int)c.head_dim);
+        CHIP_TRY(kv8_attention_prepare((int)c.head_dim));
+        CHIP_TRY(m->mem.alloc(&m->kv_rows, 2 * R * kvd));
+        CHIP_TRY(m->mem.alloc(&m->row_pos, sh.kv_capacity + 1));
+        std::vector<int32_t> at(sh.kv_capacity + 1, 0);  // positions in order, then a 0
+        for (size_t i = 0; i < sh.kv_capacity; ++i) at[i] = (int32_t)i;
+        CHIP_CHECK(hipMemcpy(m->row_pos, at.data(), at.size() * sizeof(int32_t), hipMemcpyHostToDevice));
+    }
     CHIP_TRY(m->mem.alloc(&m->part, m->part_floats));
     {
         const size_t qd = sh.q_dim(), kvd = sh.kv_dim(), I = c.intermediate_size, H = c.hidden_size;
@@ -781,6 +803,11 @@ int reserve_positions(cheetah_hip_model *m, size_t n) {
                                               m->stream));
                     CHIP_CHECK(hipMemcpyAsync(v + (size_t)np * pb, v + (size_t)p * pb, pb, hipMemcpyDeviceToDevice,
                                               m->stream));
+                    if (!sh.kv8) continue;
+                    const size_t ps = sh.page_scales();
+                    for (uint8_t *x : {L.k_scales, L.v_scales})
+                        CHIP_CHECK(hipMemcpyAsync(x + (size_t)np * ps, x + (size_t)p * ps, ps, hipMemcpyDeviceToDevice,
+                                                  m->stream));
                 }
                 log.push_back({lp, p, np});
                 m->pages[lp] = np;
@@ -804,6 +831,54 @@ int reserve_positions(cheetah_hip_model *m, size_t n) {
 
 KvGeom geom(const cheetah_hip_model *m) {
     return KvGeom{m->page_dev, kPageSize, (int)C(m).kv_heads, (int)C(m).head_dim, m->sh->kv_f32};
+}
+
+// A layer's 8-bit cache.
+Kv8Cache kv8_cache(const cheetah_hip_model *m, const Layer &L) {
+    return Kv8Cache{(uint8_t *)L.kv.k, (uint8_t *)L.kv.v, L.k_scales, L.v_scales,
+                    Kv8Geom{m->page_dev, kPageSize, (int)C(m).kv_heads, (int)C(m).head_dim}};
+}
+
+// Attention of `rows` rows from position `pos` on over it (the window is the
+// model's own; L null: for the split count alone).
+Kv8AttnJob kv8_job(const cheetah_hip_model *m, const Layer *L, size_t rows, size_t pos) {
+    Kv8AttnJob j;
+    j.q = m->qrot;
+    j.kv = kv8_cache(m, L ? *L : m->sh->layers[0]);
+    j.q_heads = (int)C(m).q_heads;
+    j.rows = rows;
+    j.offset = pos;
+    j.window = C(m).sliding_window;
+    j.part = m->part;
+    j.part_floats = m->part_floats;
+    return j;
+}
+
+// RoPE on a chunk's packed rows, its K and V rows into the 8-bit cache of layer L
+// (launch_rope_append's arguments): rotated into kv_rows, then quantised. One row of
+// a captured step comes with its position on the device.
+int kv8_rope_append(cheetah_hip_model *m, const Layer &L, size_t rows, size_t pos, const int32_t *pos_dev,
+                    const float *ws = nullptr, int nchunks = 0, const float *sc = nullptr, const float *bias = nullptr) {
+    const Shared &sh = *m->sh;
+    const size_t R = sh.max_chunk, hd = C(m).head_dim, kvh = C(m).kv_heads;
+    KvLayer to;
+    to.k = m->kv_rows;
+    to.v = m->kv_rows + R * kvh * hd;
+    // One page of R positions, its table the last word of row_pos.
+    const KvGeom g{m->row_pos + sh.kv_capacity, (int)R, (int)kvh, (int)hd, 1};
+    CHIP_TRY(launch_rope_append(m->qkv, m->qrot, rows, (int)C(m).q_heads, g, to, sh.rope_cos, sh.rope_sin,
+                                (int)C(m).rotary_dim, 0, nullptr, m->stream, ws, nchunks, sc, bias,
+                                pos_dev ? pos_dev : m->row_pos + pos));
+    Kv8AppendJob a;
+    a.k = to.k;
+    a.v = to.v;
+    a.stride = hd;
+    a.head_stride = R * hd;
+    a.rows = rows;
+    a.offset = pos;
+    a.pos_dev = pos_dev;
+    a.kv = kv8_cache(m, L);
+    return launch_kv8_append(a, m->stream);
 }
 
 // Copies layer l's host-tier matrices into slot l % 2 on the feed stream,
@@ -884,6 +959,7 @@ int refresh_weights(cheetah_hip_model *m) {
 // Attention splits of a decode step over `ctx` keys (one captured graph per
 // split count).
 int decode_splits(const cheetah_hip_model *m, size_t ctx) {
+    if (m->sh->kv8) return kv8_attention_splits(kv8_job(m, nullptr, 1, ctx - 1));
     return attention_decode_splits(ctx, (int)m->sh->cfg.kv_heads, 1, m->sh->kv_f32 != 0,
                                    (int)m->sh->cfg.head_dim);
 }
@@ -908,32 +984,41 @@ int enqueue_decode(cheetah_hip_model *m, int splits, bool sample) {
         qkv.bias = L.qkv_bias;
         qkv.y = m->qkv;
         CHIP_TRY(launch_gemv(qkv, s));
-        // RoPE and the K/V append run inside the attention kernel where it
-        // can (one launch fewer per layer), else as their own kernel.
-        const bool fuse = attention_decode_fuses_rope(geom(m), (int)c.q_heads, (int)c.rotary_dim);
-        if (!fuse)
-            CHIP_TRY(launch_rope_append(m->qkv, m->qrot, 1, (int)c.q_heads, geom(m), L.kv, sh.rope_cos, sh.rope_sin,
-                                        (int)c.rotary_dim, 0, pos, s));
-        AttnJob aj;
-        if (fuse) {
-            aj.qkv = m->qkv;
-            aj.rope_cos = sh.rope_cos;
-            aj.rope_sin = sh.rope_sin;
-            aj.rotary_dim = (int)c.rotary_dim;
+        if (sh.kv8) {
+            CHIP_TRY(kv8_rope_append(m, L, 1, 0, pos));
+            Kv8AttnJob j = kv8_job(m, &L, 1, 0);
+            j.pos_dev = pos;
+            j.splits = splits;
+            j.out = m->attn;
+            CHIP_TRY(launch_kv8_attention(j, s));
         } else {
-            aj.q = m->qrot;
+            // RoPE and the K/V append run inside the attention kernel where it
+            // can (one launch fewer per layer), else as their own kernel.
+            const bool fuse = attention_decode_fuses_rope(geom(m), (int)c.q_heads, (int)c.rotary_dim);
+            if (!fuse)
+                CHIP_TRY(launch_rope_append(m->qkv, m->qrot, 1, (int)c.q_heads, geom(m), L.kv, sh.rope_cos, sh.rope_sin,
+                                            (int)c.rotary_dim, 0, pos, s));
+            AttnJob aj;
+            if (fuse) {
+                aj.qkv = m->qkv;
+                aj.rope_cos = sh.rope_cos;
+                aj.rope_sin = sh.rope_sin;
+                aj.rotary_dim = (int)c.rotary_dim;
+            } else {
+                aj.q = m->qrot;
+            }
+            aj.q_stride = sh.q_dim();
+            aj.out = m->attn;
+            aj.k = L.kv.k;
+            aj.v = L.kv.v;
+            aj.g = geom(m);
+            aj.q_heads = (int)c.q_heads;
+            aj.rows = 1;
+            aj.pos_dev = pos;
+            aj.splits = splits;
+            aj.part = m->part;
+            CHIP_TRY(launch_attention(aj, s));
         }
-        aj.q_stride = sh.q_dim();
-        aj.out = m->attn;
-        aj.k = L.kv.k;
-        aj.v = L.kv.v;
-        aj.g = geom(m);
-        aj.q_heads = (int)c.q_heads;
-        aj.rows = 1;
-        aj.pos_dev = pos;
-        aj.splits = splits;
-        aj.part = m->part;
-        CHIP_TRY(launch_attention(aj, s));
         GemvJob o;
         o.w = L.o;
         o.x = m->attn;
@@ -1069,7 +1154,10 @@ int enqueue_chunk(cheetah_hip_model *m, const uint32_t *tokens_dev, size_t rows,
         int qkv_chunks = 0;
         qkv.deferred = &qkv_chunks;
         CHIP_TRY(launch_gemm(qkv, s));
-        CHIP_TRY(launch_rope_append(m->qkv, m->qrot, rows, (int)c.q_heads, geom(m), L.kv, sh.rope_cos, sh.rope_sin,
+        if (sh.kv8)
+            CHIP_TRY(kv8_rope_append(m, L, rows, pos, nullptr, m->gemm_ws, qkv_chunks, L.qkv.scales(), L.qkv_bias));
+        else
+            CHIP_TRY(launch_rope_append(m->qkv, m->qrot, rows, (int)c.q_heads, geom(m), L.kv, sh.rope_cos, sh.rope_sin,
                                     (int)c.rotary_dim, pos, nullptr, s, m->gemm_ws, qkv_chunks, L.qkv.scales(),
                                     L.qkv_bias, tree ? tree->angles : nullptr));
         // Either attention writes the o_proj input halves itself.
@@ -1081,6 +1169,13 @@ int enqueue_chunk(cheetah_hip_model *m, const uint32_t *tokens_dev, size_t rows,
             tj.out_hi = m->xh;
             tj.out_lo = m->xl;
             CHIP_TRY(launch_tree_attention(tj, s));
+        } else if (sh.kv8) {
+            Kv8AttnJob j = kv8_job(m, &L, rows, pos);
+            j.splits = kv8_attention_splits(j);
+            j.out = attn;
+            j.out_hi = m->xh;
+            j.out_lo = m->xl;
+            CHIP_TRY(launch_kv8_attention(j, s));
         } else {
             AttnJob aj;
             aj.q = m->qrot;
@@ -1309,6 +1404,7 @@ int ensure_tree_buffers(cheetah_hip_model *m) {
 int run_tree(cheetah_hip_model *m, const uint32_t *tokens, const int32_t *parents, size_t n, size_t offset,
              bool sample) {
     CHIP_TRY(check_model(m));
+    if (m->sh->kv8) return fail("HIP backend: drafted tokens are not served over an 8-bit KV cache.");
     if (n > (size_t)kMaxTreeNodes || (n && n > m->sh->max_chunk))
         return fail("HIP backend: a tree has at most " + std::to_string(kMaxTreeNodes) +
                     " nodes, and at most the model's chunk rows.");
@@ -1506,8 +1602,9 @@ cheetah_hip_model *cheetah_hip_model_create(const cheetah_hip_config *cfg, uint3
         fail("HIP backend: only the qwen2 (0) and llama (1) families are served.");
         return nullptr;
     }
-    if (c.sliding_window != 0) {
-        fail("HIP backend: sliding-window attention is not served (qwen2 and llama resolve it to 0).");
+    if (c.sliding_window != 0 && kv_format != 2) {
+        fail("HIP backend: sliding-window attention is served over an 8-bit KV cache only (qwen2 and llama resolve it "
+             "to 0).");
         return nullptr;
     }
     if ((c.head_dim != 64 && c.head_dim != 128) || c.q_heads / c.kv_heads > 8 || c.rotary_dim % 2 ||
@@ -1523,15 +1620,16 @@ cheetah_hip_model *cheetah_hip_model_create(const cheetah_hip_config *cfg, uint3
         fail("HIP backend: quant_format must be 0 (stored), 4 (q8) or 5 (q4).");
         return nullptr;
     }
-    if (kv_format > 1) {
-        fail("HIP backend: kv_format must be 0 (BF16) or 1 (f32).");
+    if (kv_format > 2) {
+        fail("HIP backend: kv_format must be 0 (BF16), 1 (f32) or 2 (8 bits).");
         return nullptr;
     }
     auto *m = new cheetah_hip_model();
     m->sh = std::make_shared<Shared>();
     m->sh->cfg = c;
     m->sh->quant = (int)quant_format;
-    m->sh->kv_f32 = (int)kv_format;
+    m->sh->kv_f32 = kv_format == 1;
+    m->sh->kv8 = kv_format == 2;
     m->sh->kv_capacity = kv_capacity ? kv_capacity : 65536;
     m->sh->max_chunk = max_chunk_rows ? max_chunk_rows : 1024;
     return m;
@@ -1860,6 +1958,17 @@ int cheetah_hip_kv_download(const cheetah_hip_model *m, uint32_t layer, size_t p
     if (!k_out || !v_out) return fail("HIP backend: kv_download with a null output.");
     CHIP_CHECK(hipStreamSynchronize(m->stream));
     const size_t hd = c.head_dim, kvh = c.kv_heads, eb = sh.kv_f32 ? 4 : 2;
+    if (sh.kv8) {  // by way of the rows of a chunk
+        float *k = m->kv_rows, *v = m->kv_rows + sh.max_chunk * kvh * hd;
+        for (size_t at = 0; at < n; at += sh.max_chunk) {
+            const size_t some = std::min(sh.max_chunk, n - at), bytes = some * kvh * hd * sizeof(float);
+            CHIP_TRY(launch_kv8_read(kv8_cache(m, sh.layers[layer]), pos_begin + at, some, true, k, v, m->stream));
+            CHIP_CHECK(hipMemcpyAsync(k_out + at * kvh * hd, k, bytes, hipMemcpyDeviceToHost, m->stream));
+            CHIP_CHECK(hipMemcpyAsync(v_out + at * kvh * hd, v, bytes, hipMemcpyDeviceToHost, m->stream));
+            CHIP_CHECK(hipStreamSynchronize(m->stream));
+        }
+        return 0;
+    }
     const size_t pb = sh.page_bytes();
     std::vector<uint8_t> page(pb);
     const KvLayer &kv = sh.layers[layer].kv;

@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(HERE, "libcheetah_hip.so")
 
 FMT_BF16, FMT_Q8, FMT_Q4 = 1, 4, 5
 QUANT = {None: 0, "bf16": 0, "q8": FMT_Q8, "q4": FMT_Q4}
-KV_FORMATS = {"bf16": 0, "f32": 1}
+KV_FORMATS = {"bf16": 0, "f32": 1, "e4m3": 2}
 
 _c = ctypes
 _SZ = _c.c_size_t

@@ -242,7 +242,7 @@ typedef struct cheetah_hip_config {
     uint32_t intermediate_size;
     uint32_t vocab_size;
     uint32_t tie_word_embeddings;
-    uint32_t sliding_window; /* 0 = whole cache (the only value served) */
+    uint32_t sliding_window; /* 0 = whole cache; others with an 8-bit KV cache (kv_format 2) only */
     float rope_theta;
     float rms_eps;
 } cheetah_hip_config;
@@ -255,7 +255,10 @@ typedef struct cheetah_hip_snapshot cheetah_hip_snapshot;
  * projections only — embedding, head, norms and biases keep BF16,
  * ops.rs:1533-1537). kv_format: element type of the paged KV cache, 0 = BF16
  * (half the KV bytes), 1 = f32 (the reference's own cache precision,
- * ops.rs:995-999). kv_capacity: positions the KV pool holds across this
+ * ops.rs:995-999), 2 = 8 bits (a quarter; cheetah_hip_kv8_append's codes and
+ * scales: K and V are rounded, by up to 2^-4 of a value). Over an 8-bit cache a
+ * position's results depend, in their last bits, on how the text was cut into
+ * chunks, and drafted tokens are refused. kv_capacity: positions the KV pool holds across this
  * model, its clones and its snapshots (0 = 65536). max_chunk_rows: largest
  * prefill chunk (0 = 1024). */
 cheetah_hip_model *cheetah_hip_model_create(const cheetah_hip_config *cfg, uint32_t quant_format,
@@ -287,7 +290,7 @@ int cheetah_hip_forward_greedy(cheetah_hip_model *m, const uint32_t *tokens, siz
 int cheetah_hip_decode_greedy(cheetah_hip_model *m, uint32_t token, size_t offset, size_t steps,
                               uint32_t *tokens_out);
 /* Verification of drafted tokens (speculative decoding; no counterpart in the
- * reference). A tree of candidate tokens is run in one forward behind the
+ * reference; refused over an 8-bit KV cache). A tree of candidate tokens is run in one forward behind the
  * cached positions. tokens[n]; parents[n]: parents[i] in [-1, i), -1 for a child
  * of the cached text; n at most CHEETAH_HIP_MAX_TREE_NODES and max_chunk_rows.
  * Node i attends to the cache, its ancestors and itself, at position offset +
@@ -341,7 +344,8 @@ void cheetah_hip_snapshot_free(cheetah_hip_snapshot *s);
 /* Cached K and V rows of positions [pos_begin, pos_begin + n) of one layer,
  * written to host buffers of n * kv_heads * head_dim floats each in the
  * reference's per-layer cache layout [pos][kv_head][dim] (ops.rs:995-999,
- * the rows KvSnapshot carries, registry.rs:48-55). BF16 pages widen exactly.
+ * the rows KvSnapshot carries, registry.rs:48-55). BF16 and 8-bit pages widen
+ * exactly.
  * Waits for the model's queued work. */
 int cheetah_hip_kv_download(const cheetah_hip_model *m, uint32_t layer, size_t pos_begin, size_t n, float *k_out,
                             float *v_out);

@@ -101,3 +101,36 @@ def some_rows(rng, n, kvh, hd):
     k[..., 3::29] += 5
     v = (rng.standard_normal((n, kvh, hd)) * np.exp(0.8 * rng.standard_normal((n, 1, 1)))).astype(np.float32)
     return k, v
+
+
+def decoder64(shape, w, tokens, cache, window=0):
+    """The decoder's logits at every position of `tokens` in 64 bits, and each
+    layer's rotated K and V rows before they are quantised. cache(layer): the K and V
+    values [positions, kvh, hd] that attention reads; w: widened weights."""
+    n, hd = len(tokens), shape.head_dim
+    half = shape.rotary_dim // 2
+
+    def norm(x, gain):
+        return x / np.sqrt((x * x).mean(-1, keepdims=True) + shape.rms_eps) * gain
+
+    freq = np.float32(shape.rope_theta) ** (np.float32(-2) * np.arange(half, dtype=np.float32) / np.float32(2 * half))
+    angle = (np.arange(n, dtype=np.float32)[:, None] * freq.astype(np.float32)).astype(np.float64)[:, None]
+
+    def rotate(x):
+        a, b = x[..., :half], x[..., half:2 * half]
+        c, s = np.cos(angle), np.sin(angle)
+        return np.concatenate([a * c - b * s, b * c + a * s, x[..., 2 * half:]], -1)
+
+    x, rows = w["model.embed_tokens.weight"][tokens], []
+    for layer in range(shape.num_layers):
+        p = f"model.layers.{layer}."
+        h = norm(x, w[p + "input_layernorm.weight"])
+        q, k, v = (h @ w[p + f"self_attn.{c}_proj.weight"].T + w.get(p + f"self_attn.{c}_proj.bias", 0) for c in "qkv")
+        q = rotate(q.reshape(n, -1, hd)).reshape(n, -1)
+        rows.append((rotate(k.reshape(n, -1, hd)), v.reshape(n, -1, hd)))
+        x = x + attention64(q, *cache(layer), shape.q_heads, 0, window) @ w[p + "self_attn.o_proj.weight"].T
+        h = norm(x, w[p + "post_attention_layernorm.weight"])
+        g = h @ w[p + "mlp.gate_proj.weight"].T
+        x = x + (g / (1 + np.exp(-g)) * (h @ w[p + "mlp.up_proj.weight"].T)) @ w[p + "mlp.down_proj.weight"].T
+    x = norm(x, w["model.norm.weight"])
+    return x @ w["model.embed_tokens.weight" if shape.tie_word_embeddings else "lm_head.weight"].T, rows
