@@ -275,6 +275,7 @@ struct Kv8AttnArgs {
     const uint8_t *k, *v, *k_scales, *v_scales;
     Kv8Geom g;
     int q_heads, rows, offset, window, sinks;
+    uint32_t over_group;  // ceil(2^32 / G) for G > 1 query heads per KV head
     float *out;
     float *part;  // [row][head][split][HD]: weighted sums
     float2 *ml;   // [row][head][split]: maximum (log2 units), weight sum
@@ -490,7 +491,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     const int wave = uniform((int)(threadIdx.x >> 6));
     const int wr = wave % WR, wk = wave / WR;
     const int n = lane & 31, half = lane >> 5;
+    // Division by G: exact below 2^29 (the launch refuses more rows).
     const int G = a.q_heads / a.g.kv_heads, M = a.rows * G, RB = (M + 32 * WR - 1) / (32 * WR);
+    auto over_g = [&](int x) { return G == 1 ? x : (int)__umulhi((uint32_t)x, a.over_group); };
     // Blocks b, b + 8, .. run on one XCD: each takes a run of (KV head, split, row
     // block), so that few of them read a cache's block. Rows that see the most and
     // the fewest positions alternate.
@@ -501,14 +504,15 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     const int g = uniform(pair % a.g.kv_heads), split = uniform(pair / a.g.kv_heads);
     const int m0 = rb * 32 * WR, m = m0 + wr * 32 + n;
     const bool rvalid = m < M;
-    const int offset = uniform(first_pos(a)), pos = offset + (rvalid ? m / G : 0), lo = window_start(a, pos);
+    const int offset = uniform(first_pos(a)), pos = offset + (rvalid ? over_g(m) : 0), lo = window_start(a, pos);
     // Rows of the block and of the wave.
-    const int pos_lo = uniform(offset + m0 / G), pos_hi = uniform(offset + (min(M, m0 + 32 * WR) - 1) / G);
-    const int wave_lo = uniform(offset + min(m0 + wr * 32, M - 1) / G);
-    const int wave_hi = uniform(offset + (min(M, m0 + wr * 32 + 32) - 1) / G);
+    const int pos_lo = uniform(offset + over_g(m0)), pos_hi = uniform(offset + over_g(min(M, m0 + 32 * WR) - 1));
+    const int wave_lo = uniform(offset + over_g(min(m0 + wr * 32, M - 1)));
+    const int wave_hi = uniform(offset + over_g(min(M, m0 + wr * 32 + 32) - 1));
     const int seen_lo = window_start(a, pos_lo), wave_first = window_start(a, wave_hi);
     const Reach reach = reach_of(pos_lo, pos_hi, a.window, a.sinks);
-    const int begin = uniform((int)((long)reach.count * split / S)), end = uniform((int)((long)reach.count * (split + 1) / S));
+    const int each = reach.count / S, extra = reach.count % S;
+    const int begin = uniform(split * each + min(split, extra)), end = uniform(begin + each + (split < extra));
     const int steps = (end - begin + WK - 1) / WK;  // of the longest key wave
     const int mine = max(end - begin - wk + WK - 1, 0) / WK;
 
@@ -574,7 +578,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
         for (int j = 0; j < QI; ++j) {
             const int r = m0 + (wave * QI + j) * RPI + lane / LPR, rr = min(r, M - 1);
-            raw[j] = *(const f32x4 *)(a.q + ((size_t)(rr / G) * a.q_heads + g * G + rr % G) * HD + lane % LPR * 4);
+            raw[j] = *(const f32x4 *)(a.q + ((size_t)over_g(rr) * a.q_heads + g * G + rr - over_g(rr) * G) * HD + lane % LPR * 4);
         }
         __builtin_amdgcn_sched_barrier(0);
         look_up_scales();
@@ -856,6 +860,10 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     }
     if (threadIdx.x < 4) odd[threadIdx.x] = 0;
     __syncthreads();
+    auto item_of = [&](int r) {  // row and head of the block's row r
+        const int row = over_g(m0 + r);
+        return (size_t)row * a.q_heads + g * G + (m0 + r - row * G);
+    };
     const int r = (int)threadIdx.x;
     if (r < held_rows) {
         float2 ml[WK];
@@ -874,7 +882,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         const float inv = S == 1 ? 1.0f / sum : 1.f;
 #pragma unroll
         for (int k = 0; k < WK; ++k) sml[(k * WR + r / 32) * 32 + r % 32].x = ml[k].x * inv;
-        if (S > 1) a.ml[((size_t)((m0 + r) / G) * a.q_heads + g * G + (m0 + r) % G) * S + split] = make_float2(top, sum);
+        if (S > 1) a.ml[item_of(r) * S + split] = make_float2(top, sum);
     }
     __syncthreads();
 #pragma unroll 4
@@ -889,7 +897,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = fmaf(w, p[e], v[e]);
         }
-        const size_t item = (size_t)((m0 + r) / G) * a.q_heads + g * G + (m0 + r) % G;
+        const size_t item = item_of(r);
         if (S == 1) {
             const float x[4] = {v[0], v[1], v[2], v[3]};
             store_out<4>(a, item * HD + d, x);
@@ -902,7 +910,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     if (S > 1) return;
     __syncthreads();
     for (int r = wave; r < held_rows; r += kWaves)
-        if (uniform(odd[r / 32]) >> (r % 32) & 1) plain_row<HD>(kernel_args(), (m0 + r) / G, g * G + (m0 + r) % G);
+        if (uniform(odd[r / 32]) >> (r % 32) & 1)
+            plain_row<HD>(kernel_args(), over_g(m0 + r), g * G + (m0 + r - over_g(m0 + r) * G));
 }
 
 // The splits of a row and head, joined by W waves (each takes every W-th); the
@@ -1105,13 +1114,15 @@ int launch_kv8_attention(const Kv8AttnJob &j, hipStream_t s) {
     if (S > kMaxSplits || j.part_floats < kv8_attention_part_floats(j, S))
         return fail("HIP backend: 8-bit attention partial buffer too small.");
     const size_t items = j.rows * (size_t)j.q_heads;
-    if (items / j.kv.g.kv_heads > (size_t)INT32_MAX - 256) return fail("HIP backend: attention with too many rows.");
+    if (items / j.kv.g.kv_heads >= (size_t)1 << 29) return fail("HIP backend: attention with too many rows.");
     Kv8AttnArgs a;
     a.q = j.q;
     a.k = j.kv.k, a.v = j.kv.v, a.k_scales = j.kv.k_scales, a.v_scales = j.kv.v_scales;
     a.g = j.kv.g;
     a.q_heads = j.q_heads;
     a.rows = (int)j.rows, a.offset = (int)j.offset, a.window = (int)j.window, a.sinks = (int)j.sinks;
+    const uint64_t group = (uint64_t)(j.q_heads / j.kv.g.kv_heads);
+    a.over_group = group > 1 ? (uint32_t)(((1ull << 32) + group - 1) / group) : 0;
     a.out = j.out;
     a.out_hi = j.out_hi, a.out_lo = j.out_lo;
     a.pos_dev = j.pos_dev;
