@@ -865,9 +865,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             s = t;
         }
     }
-    // The key waves' parts meet in LDS: sums, then a factor for each row and wave.
+    // The key waves' parts meet in LDS: sums, then a factor for each row and wave. (In
+    // the tiles' place: their last reads are done, and copies that nothing reads.)
     l += __shfl_xor(l, 32, 64);
-    __syncthreads();  // the tiles' last reads are done
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
     const int held_rows = min(32 * WR, M - m0);
     if (rvalid) {
         float *so = (float *)smem + ((size_t)wave * 32 + n) * kRowPad<HD>;
@@ -978,11 +980,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void kv8_merge_kernel(Kv8Att
         for (int b = 0; b < B; ++b) {
             const int s = s0 + b * W;
             if (s >= S) break;
+            // (A weight of 0 too: a NaN among its values shows. Empty splits hold zeros.)
             const float w = __shfl(s < 64 ? wx : wy, s & 63, 64);
-            if (w != 0.f) {  // (NaN too)
 #pragma unroll
-                for (int d = 0; d < D; ++d) v[d] = fmaf(w, p[b][d], v[d]);
-            }
+            for (int d = 0; d < D; ++d) v[d] = fmaf(w, p[b][d], v[d]);
         }
     }
     const float inv = 1.0f / sum;
@@ -1140,7 +1141,7 @@ int launch_kv8_attention(const Kv8AttnJob &j, hipStream_t s) {
     if (S > kMaxSplits || j.part_floats < kv8_attention_part_floats(j, S))
         return fail("HIP backend: 8-bit attention partial buffer too small.");
     const size_t items = j.rows * (size_t)j.q_heads;
-    if (items / j.kv.g.kv_heads >= (size_t)1 << 29) return fail("HIP backend: attention with too many rows.");
+    if (items / j.kv.g.kv_heads >= (size_t)1 << 29 || items > (size_t)INT32_MAX) return fail("HIP backend: attention with too many rows.");
     Kv8AttnArgs a;
     a.q = j.q;
     a.k = j.kv.k, a.v = j.kv.v, a.k_scales = j.kv.k_scales, a.v_scales = j.kv.v_scales;

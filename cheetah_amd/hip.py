@@ -359,10 +359,11 @@ class Kv8Cache:
             raise ValueError("the page size is a multiple of 64 positions")
         if table is None:
             table = np.arange(-(-positions // page_size))
-        table = np.ascontiguousarray(table, np.int32)
+        table = np.asarray(table)
         pages = max(int(table.max(initial=-1)) + 1, 1) if pages is None else pages
-        if table.size and int(table.max()) >= pages:
+        if table.size and not -2**31 <= int(table.min()) <= int(table.max()) < pages:
             raise ValueError("page table entry outside the pool")
+        table = np.ascontiguousarray(table, np.int32)
         if positions > table.size * page_size:
             raise ValueError("the page table ends before the cache's positions")
         self.table, self.page_size, self.kv_heads, self.head_dim = table, page_size, kv_heads, head_dim
@@ -375,11 +376,11 @@ class Kv8Cache:
         self.view = Kv8View(*(b.ptr for b in self._codes + self._scales), self._table.ptr, page_size, kv_heads,
                             head_dim)
 
-    def _pages(self, positions) -> None:
-        pages = np.unique(np.asarray(positions, np.int64) // self.page_size)
-        if pages.size and (pages[0] < 0 or pages[-1] >= self.table.size):
+    def _listed(self, begin: int, end: int) -> None:
+        """Refuses positions begin .. end - 1 whose pages the table does not list."""
+        if begin < 0 or end > self.table.size * self.page_size:
             raise ValueError("position outside the page table")
-        if (self.table[pages] < 0).any():
+        if begin < end and (self.table[begin // self.page_size:-(-end // self.page_size)] < 0).any():
             raise ValueError("page table entry outside the pool")
 
     def append(self, k: np.ndarray, v: np.ndarray, offset: int) -> None:
@@ -392,7 +393,7 @@ class Kv8Cache:
         if k.shape != v.shape or k.size % width:
             raise ValueError("rows of kv_heads * head_dim values")
         n = k.size // width
-        self._pages(np.arange(offset // KV8_BLOCK * KV8_BLOCK, offset + n))
+        self._listed(offset // KV8_BLOCK * KV8_BLOCK, offset + n)
         kd, vd = DeviceBuffer.from_array(k), DeviceBuffer.from_array(v)
         check(lib().cheetah_hip_kv8_append(kd.ptr, vd.ptr, int(k.dtype == np.float32), n, width, offset,
                                            _c.byref(self.view)))
@@ -400,7 +401,7 @@ class Kv8Cache:
     def read(self, begin: int, n: int, bf16: bool = False):
         """cheetah_hip_kv8_read: K and V of n positions as [n, kv_heads, head_dim]."""
         dtype = np.uint16 if bf16 else np.float32
-        self._pages(np.arange(begin, begin + n))
+        self._listed(begin, begin + n)
         out = [DeviceBuffer(max(n, 1) * self.kv_heads * self.head_dim * np.dtype(dtype).itemsize) for _ in "kv"]
         check(lib().cheetah_hip_kv8_read(_c.byref(self.view), begin, n, int(not bf16), out[0].ptr, out[1].ptr))
         shape = (n, self.kv_heads, self.head_dim)
@@ -411,7 +412,8 @@ class Kv8Cache:
         q = np.ascontiguousarray(q, np.float32).reshape(-1, q_heads * self.head_dim)
         rows = q.shape[0]
         first = max(offset + 1 - window, 0) if window else 0
-        self._pages(np.concatenate([np.arange(min(sinks, first)), np.arange(first, offset + rows)]))
+        self._listed(0, min(sinks, first))
+        self._listed(first, offset + rows)
         qd, od = DeviceBuffer.from_array(q), DeviceBuffer(max(q.nbytes, 1))
         check(lib().cheetah_hip_kv8_attention(qd.ptr, _c.byref(self.view), q_heads, rows, offset, window, sinks,
                                               od.ptr))

@@ -207,3 +207,54 @@ def test_larger_pages(hip, page):
     q = rng.standard_normal((20, 8 * 128)).astype(np.float32)
     want = ref.attention64(q, *cpu.values(0, 797), 8, 777)
     assert rel_err(dev.attention(q, 8, 777), want) < TOL
+
+
+def test_pools_past_four_gigabytes(hip):
+    """Pages whose codes lie past 2^32 bytes (and, of V, past 2^31 from the first):
+    the values and outputs of a cache with small offsets."""
+    kvh, hd, pages, n = 8, 128, 70000, 300
+    table = np.array([69999, 3, 65541, 40000, 69001], np.int32)
+    codes = [hip.DeviceBuffer(pages * kvh * 64 * hd) for _ in "kv"]
+    scales = [hip.DeviceBuffer(pages * kvh * 2) for _ in "kv"]
+    t = hip.DeviceBuffer.from_array(table)
+    far = hip.Kv8Cache.__new__(hip.Kv8Cache)
+    far.table, far.page_size, far.kv_heads, far.head_dim = table, 64, kvh, hd
+    far.view = hip.Kv8View(*(b.ptr for b in codes + scales), t.ptr, 64, kvh, hd)
+    rng = np.random.default_rng(8)
+    near, cpu = make(hip, rng, n, kvh, hd), ref.Cache(n, kvh, hd)
+    for at, some in ((0, 170), (170, 1), (171, 129)):
+        k, v = ref.some_rows(rng, some, kvh, hd)
+        for cache in (far, near, cpu):
+            cache.append(k, v, at)
+    same(far, cpu, 0, n)
+    for rows in (1, 100):
+        q = rng.standard_normal((rows, 32 * hd)).astype(np.float32)
+        np.testing.assert_array_equal(far.attention(q, 32, n - rows), near.attention(q, 32, n - rows))
+
+
+def test_the_wrapper_refuses_positions_that_the_table_does_not_list(hip):
+    cache = hip.Kv8Cache(200, 1, 64, table=np.array([2, 0, -1, 1], np.int64), pages=3)
+    rows = np.zeros((10, 64), np.float32)
+    cache.append(rows, rows, 100)
+    for call in (lambda: cache.append(rows, rows, 120), lambda: cache.read(120, 10), lambda: cache.append(rows, rows, 250),
+                 lambda: cache.attention(rows, 1, 140), lambda: cache.attention(rows, 1, 2**40)):
+        with pytest.raises(ValueError, match="page table"):
+            call()
+    with pytest.raises(ValueError, match="outside the pool"):
+        hip.Kv8Cache(100, 1, 64, table=np.array([2**32, 1]), pages=3)
+
+
+@pytest.mark.parametrize("order", [[0, 1, 2], [2, 1, 0]])
+def test_calls_of_growing_and_shrinking_size_share_their_scratch(hip, order):
+    """Calls with many splits, few and none, back to back on one stream: each is
+    what it is alone, twice over."""
+    shapes = [(1, 6000, 4, 28), (70, 900, 8, 32), (3, 40, 1, 5)]
+    made = []
+    for rows, offset, kvh, qh in shapes:
+        rng, dev, _ = filled(hip, rows, offset + rows, kvh, 128)
+        q = rng.standard_normal((rows, qh * 128)).astype(np.float32)
+        made.append((dev, q, qh, offset, dev.attention(q, qh, offset)))
+    for _ in range(2):
+        for i in order:
+            dev, q, qh, offset, want = made[i]
+            np.testing.assert_array_equal(dev.attention(q, qh, offset), want)

@@ -160,3 +160,27 @@ def test_a_query_with_nan_or_infinity_is_nan_alone(hip):
     bad = np.zeros((20, 8), bool)
     bad[3, 2] = bad[7, 6] = True
     assert np.isnan(got[bad]).all() and rel_err(got[~bad], want[~bad]) < TOL
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,offset", SHAPES)
+def test_a_nan_whose_weight_rounds_to_zero_shows(hip, rows, offset, hd):
+    """The key of one position scores hundreds below the others for every row: its
+    weight is 0, in its own split too, and its NaN value shows all the same."""
+    rng = np.random.default_rng(rows + offset + hd)
+    k, v = ref.some_rows(rng, offset + rows, 1, hd)
+    at = offset // 3
+    k[:, :, 0] = 8
+    k[at] = 0
+    k[at, :, 0] = -300
+    v[at, 0, 5] = np.nan
+    q = rng.standard_normal((rows, 4 * hd)).astype(np.float32)
+    q.reshape(rows, 4, hd)[:, :, 0] = 30
+    dev, cpu = make(hip, rng, offset + rows, 1, hd), ref.Cache(offset + rows, 1, hd)
+    dev.append(k, v, 0)
+    cpu.append(k, np.nan_to_num(v), 0)
+    got = dev.attention(q, 4, offset).reshape(rows, 4, hd)
+    want = ref.attention64(q, *cpu.values(0, offset + rows), 4, offset).reshape(rows, 4, hd)
+    assert np.isnan(got[:, :, 5]).all()
+    clean = np.arange(hd) != 5
+    assert rel_err(got[:, :, clean], want[:, :, clean]) < 2 * TOL  # scores of 30 * 8 / 8 more, of 2^-21 each
