@@ -19,7 +19,6 @@
 // load one piece.
 #include <algorithm>
 #include <atomic>
-#include <type_traits>
 
 #include "kernels.hpp"
 
@@ -152,7 +151,7 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
         const BlockAt at = block_at(a.g, page, (int)(first % a.g.page_size) / kBlock, head, HD);
         codes = (which ? a.codes[1] : a.codes[0]) + at.codes;
         scale = (which ? a.scales[1] : a.scales[0]) + at.scale;
-        if (keep) e_old = (int)*scale - 127;
+        if (keep) e_old = min(max((int)*scale - 127, kScaleLeast), kScaleMost);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)

@@ -184,7 +184,8 @@ typedef struct cheetah_hip_kv8_view {
  * device rows of kv_heads * head_dim values, `stride` >= that many elements apart
  * (k and v may point into packed projections), row_format 0 = BF16, 1 = f32. A
  * block's scale is the least with |x| <= 448 * 2^e for its rows, codes round to
- * nearest (ties to even). Rows of the block before `offset` keep their values; a
+ * nearest (ties to even). Rows of the block before `offset` (written before, from
+ * its first on) keep their values; a
  * scale that later rows raise rounds them again (only values below 2^-13 of the
  * block's largest move, by at most 2^-16 of it), and it does not fall before the
  * block's first position is written again. Rows behind the last new

@@ -217,3 +217,12 @@ def test_the_last_position_of_the_capacity(hip):
     assert np.isfinite(k).all() and np.isfinite(v).all()
     with pytest.raises(hip.HipError, match="capacity"):
         g.forward([1], 130)
+
+
+def test_unknown_cache_formats_are_refused(hip):
+    import ctypes
+    cfg = hip.make_config(configs.TINY_QWEN2)
+    assert not hip.lib().cheetah_hip_model_create(ctypes.byref(cfg), 0, 3, 0, 0)
+    assert b"kv_format" in hip.lib().cheetah_hip_last_error()
+    with pytest.raises(ValueError, match="kv must be one of"):
+        hip.HipForward(configs.TINY_QWEN2, kv="e5m2")
