@@ -503,13 +503,17 @@ constexpr int kRowPad = HD + 4;  // floats of a row of outputs in LDS
 constexpr size_t kStage = 96 * 1024;   // LDS of three tiles
 template <int HD>
 constexpr int kQRow = HD * 4 + 16;     // bytes of a query row's parts in LDS: high, low, padding
+// A block's LDS: tiles, then the waves' sums in their place; query rows on their way
+// to the operands (of one row wave behind the sums, else in the third tile's place
+// and behind it); a word of each wave and row (maximum, weight sum, the sums' unit);
+// the query rows' exponents; rows to compute again.
 template <int HD, int WR>
-constexpr size_t kv8_attn_lds_bytes() {
-    constexpr size_t stage = WR == 1 ? 0 : kStage, join = kWaves * 32 * kRowPad<HD> * 4;
-    constexpr size_t queries = stage / 3 * 2 + 32 * WR * kQRow<HD>;  // in the third tile's place and behind
-    constexpr size_t most = stage > join ? stage : join;
-    return (most > queries ? most : queries) + kWaves * 32 * 8 + 16;
-}
+constexpr size_t kQueriesAt = WR == 1 ? kWaves * 32 * kRowPad<HD> * 4 : kStage / 3 * 2;
+template <int HD, int WR>
+constexpr size_t kWordsAt = std::max({WR == 1 ? (size_t)0 : kStage, (size_t)(kWaves * 32 * kRowPad<HD> * 4),
+                                      kQueriesAt<HD, WR> + 32 * WR * kQRow<HD>});
+template <int HD, int WR>
+constexpr size_t kv8_attn_lds_bytes() { return kWordsAt<HD, WR> + kWaves * 32 * 16 + 32 * WR * 4 + 16; }
 
 template <int HD, int WR>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))) void kv8_attn_kernel(Kv8AttnArgs a, int S) {
@@ -519,8 +523,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     constexpr int BB = kBlock * HD;     // bytes of a block of K or V
     constexpr int NB = DIRECT ? 1 : (int)kStage / (3 * WK * 2 * BB);  // a key wave's blocks of a tile
     extern __shared__ __attribute__((aligned(256))) uint8_t smem[];
-    float2 *sml = (float2 *)(smem + kv8_attn_lds_bytes<HD, WR>() - kWaves * 32 * 8 - 16);
-    int *odd = (int *)(sml + kWaves * 32);  // a row wave's rows to compute again
+    f32x4 *words = (f32x4 *)(smem + kWordsAt<HD, WR>);
+    int *sq_exp = (int *)(words + kWaves * 32);
+    int *odd = sq_exp + 32 * WR;  // a row wave's rows to compute again
     auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
     const int lane = threadIdx.x & 63;
     const int wave = uniform((int)(threadIdx.x >> 6));
@@ -605,8 +610,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     // reach the matrix operands by way of LDS (from memory an operand is 16 bytes of
     // each of 32 rows a load: 4 us for the eight waves).
     look_up(0);
-    uint8_t *sq = smem + (DIRECT ? 0 : kStage / 3 * 2);
-    int *sq_exp = (int *)sml;
+    uint8_t *sq = smem + kQueriesAt<HD, WR>;
     constexpr int LPR = HD / 4, RPI = 64 / LPR, QI = 4 * WR / RPI;  // lanes a row, rows a load, loads a wave
     {
         f32x4 raw[QI];
@@ -876,72 +880,83 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             s = t;
         }
     }
-    // The key waves' parts meet in LDS: sums, then a factor for each row and wave. (In
-    // the tiles' place: their last reads are done, and copies that nothing reads.)
+    // The key waves' parts meet in LDS. (In the tiles' place: their last reads are
+    // done, and copies that nothing reads.)
     l += __shfl_xor(l, 32, 64);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    if constexpr (!DIRECT) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
     const int held_rows = min(32 * WR, M - m0);
     if (rvalid) {
         float *so = (float *)smem + ((size_t)wave * 32 + n) * kRowPad<HD>;
 #pragma unroll
         for (int u = 0; u < C; ++u)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                f32x4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = ldexpf(o[u][4 * q + e], v_exp);
-                *(f32x4 *)(so + 32 * u + 8 * q + 4 * half) = v;
-            }
-        if (half == 0) sml[wave * 32 + n] = make_float2(m2, l);
+            for (int q = 0; q < 4; ++q)
+                *(f32x4 *)(so + 32 * u + 8 * q + 4 * half) =
+                    f32x4{o[u][4 * q], o[u][4 * q + 1], o[u][4 * q + 2], o[u][4 * q + 3]};
+        if (half == 0) words[wave * 32 + n] = f32x4{m2, l, two_to(v_exp), 0.f};
     }
-    if (threadIdx.x < 4) odd[threadIdx.x] = 0;
+    if (threadIdx.x < WR) odd[threadIdx.x] = 0;
     __syncthreads();
     auto item_of = [&](int r) {  // row and head of the block's row r
         const int row = over_g(m0 + r);
         return (size_t)row * a.q_heads + g * G + (m0 + r - row * G);
     };
-    const int r = (int)threadIdx.x;
-    if (r < held_rows) {
-        float2 ml[WK];
+    // The factors of a row's waves, with one split of its weight sum too. (A wave that
+    // saw nothing counts nothing; a NaN sum shows.)
+    auto factors = [&](int r, float (&f)[WK], bool to_part) {
+        f32x4 word[WK];
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int k = 0; k < WK; ++k) {
-            ml[k] = sml[(k * WR + r / 32) * 32 + r % 32];
-            top = fmaxf(top, ml[k].x);
+            word[k] = words[k * WR * 32 + r];
+            top = fmaxf(top, word[k][0]);
         }
-#pragma unroll
-        for (int k = 0; k < WK; ++k) {  // (a wave that saw nothing counts nothing; a NaN sum shows)
-            const float w = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[k].x - top);
-            sum += w != 0.f || ml[k].y != ml[k].y ? w * ml[k].y : 0.f;
-            ml[k].x = w;
-        }
-        const float inv = S == 1 ? 1.0f / sum : 1.f;
-#pragma unroll
-        for (int k = 0; k < WK; ++k) sml[(k * WR + r / 32) * 32 + r % 32].x = ml[k].x * inv;
-        if (S > 1) a.ml[item_of(r) * S + split] = make_float2(top, sum);
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (int u = (int)threadIdx.x; u < held_rows * (HD / 4); u += 64 * kWaves) {
-        const int r = u / (HD / 4), d = u % (HD / 4) * 4;
-        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < WK; ++k) {
-            const int at = (k * WR + r / 32) * 32 + r % 32;
-            const float w = sml[at].x;
+            const float m = word[k][0], w = m == -INFINITY && word[k][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);
+            sum += w != 0.f || word[k][1] != word[k][1] ? w * word[k][1] : 0.f;
+            f[k] = w * word[k][2];
+        }
+        if (to_part) a.ml[item_of(r) * S + split] = make_float2(top, sum);
+        const float inv = S == 1 ? 1.0f / sum : 1.f;
+#pragma unroll
+        for (int k = 0; k < WK; ++k) f[k] *= inv;
+    };
+    // A few rows: every thread finds its row's factors, a barrier less (6.6 -> 6.1 us for
+    // one token on 576). Many: a thread a row (1,000 windowed rows 42.7 -> 41.7).
+    if constexpr (WR > 1) {
+        const int r = (int)threadIdx.x;
+        if (r < held_rows) {
+            float f[WK];
+            factors(r, f, S > 1);
+#pragma unroll
+            for (int k = 0; k < WK; ++k) words[k * WR * 32 + r][0] = f[k];
+        }
+        __syncthreads();
+    }
+#pragma unroll WR
+    for (int u = (int)threadIdx.x; u < held_rows * (HD / 4); u += 64 * kWaves) {  // 4 dims of a row
+        const int r = u / (HD / 4), d = u % (HD / 4) * 4;
+        float f[WK], v[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (WR == 1) factors(r, f, S > 1 && d == 0);
+#pragma unroll
+        for (int k = 0; k < WK; ++k) {
+            const int at = k * WR * 32 + r;
+            if constexpr (WR > 1) f[k] = words[at][0];
             const f32x4 p = *(const f32x4 *)((const float *)smem + (size_t)at * kRowPad<HD> + d);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = fmaf(w, p[e], v[e]);
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(f[k], p[e], v[e]);
         }
         const size_t item = item_of(r);
         if (S == 1) {
-            const float x[4] = {v[0], v[1], v[2], v[3]};
-            store_out<4>(a, item * HD + d, x);
+            store_out<4>(a, item * HD + d, v);
             if (!(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY))
                 atomicOr(&odd[r / 32], 1 << (r % 32));
         } else {
-            *(f32x4 *)(a.part + (item * S + split) * HD + d) = v;
+            *(f32x4 *)(a.part + (item * S + split) * HD + d) = f32x4{v[0], v[1], v[2], v[3]};
         }
     }
     if (S > 1) return;
