@@ -848,7 +848,7 @@ Kv8AttnJob kv8_job(const cheetah_hip_model *m, const Layer *L, size_t rows, size
     j.q_heads = (int)C(m).q_heads;
     j.rows = rows;
     j.offset = pos;
-    j.window = C(m).sliding_window;
+    j.window = std::min<size_t>(C(m).sliding_window, kMaxKv8Positions);  // (past every position: all of them)
     j.part = m->part;
     j.part_floats = m->part_floats;
     return j;

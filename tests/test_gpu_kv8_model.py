@@ -135,6 +135,15 @@ def test_sliding_window(hip, window):
             hip.HipForward(shape, weights(shape)[0], kv=kv)
 
 
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31, 2**32 - 1])
+def test_a_window_past_every_position_is_none(hip, window):
+    shape = configs.TINY_LLAMA
+    g, plain = model(hip, shape.replace(sliding_window=window)), model(hip, shape)
+    tokens = synth.make_tokens(shape.vocab_size, 150)
+    np.testing.assert_array_equal(g.forward(tokens, 0), plain.forward(tokens, 0))
+    np.testing.assert_array_equal(g.forward([5], 150), plain.forward([5], 150))
+
+
 @pytest.mark.parametrize("at", [33, 64, 90])
 def test_snapshots_and_clones(hip, at):
     """A snapshot inside a block keeps its values and scales while the instance
