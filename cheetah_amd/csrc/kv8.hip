@@ -731,8 +731,20 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         const int e_v = (int)__builtin_amdgcn_readlane(now_v, i & 63) - 127;
         if (i == 0) v_exp = e_v;
         if (e_v - v_exp > 7 || e_v - v_exp < -15) {
-            // Steps that could lose the sums' values: the rows are computed again.
-            if (abs(e_v - v_exp) > 100) l = NAN;
+            // Steps that could lose the sums' values: the rows are computed again. (A block
+            // of zeros, whose scale is the least, and sums that are 0 lose nothing.)
+            if (abs(e_v - v_exp) > 100) {
+                uint32_t codes = 0, sums = 0;
+#pragma unroll
+                for (int u = 0; u < C; ++u) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) codes |= vr[u][j];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sums |= __float_as_uint(o[u][r]);
+                }
+                if (!__any(codes & 0x7F7F7F7Fu)) return 1.f;
+                if (__any(sums << 1)) l = NAN;
+            }
 #pragma unroll
             for (int u = 0; u < C; ++u)
 #pragma unroll
@@ -783,8 +795,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             const float mref = reference();
 #pragma unroll
             for (int r = 0; r <= 16; ++r) exponential(r, mref);
-            const float vs = value_scale(i);
             clear_v(i);
+            const float vs = value_scale(i);
 #pragma unroll
             for (int u = 0; u < C; ++u) {
                 const f16x8 v0 = codes_f16(vr[u][0], vr[u][1], vs), v1 = codes_f16(vr[u][2], vr[u][3], vs);
@@ -851,8 +863,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             }
             if (i >= mine) continue;
             if (i + 2 < mine) read_k(i + 2);
-            vs = value_scale(i);
             clear_v(i);
+            vs = value_scale(i);
             if (i + 1 < mine) mask(i + 1, t);
             float tmax = t[0];
             uint2 v4[4];
@@ -906,6 +918,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     };
     // The factors of a row's waves, with one split of its weight sum too. (A wave that
     // saw nothing counts nothing; a NaN sum shows.)
+    // The quotient comes last: with the least unit a factor divided by a large sum would
+    // be no normal number.
     auto factors = [&](int r, float (&f)[WK], bool to_part) {
         f32x4 word[WK];
         float top = -INFINITY, sum = 0.f;
@@ -921,9 +935,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             f[k] = w * word[k][2];
         }
         if (to_part) a.ml[item_of(r) * S + split] = make_float2(top, sum);
-        const float inv = S == 1 ? 1.0f / sum : 1.f;
-#pragma unroll
-        for (int k = 0; k < WK; ++k) f[k] *= inv;
+        return S == 1 ? 1.0f / sum : 1.f;
     };
     // A few rows: every thread finds its row's factors, a barrier less (6.6 -> 6.1 us for
     // one token on 576). Many: a thread a row (1,000 windowed rows 42.7 -> 41.7).
@@ -931,7 +943,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         const int r = (int)threadIdx.x;
         if (r < held_rows) {
             float f[WK];
-            factors(r, f, S > 1);
+            const float inv = factors(r, f, S > 1);
+            words[r][1] = inv;
 #pragma unroll
             for (int k = 0; k < WK; ++k) words[k * WR * 32 + r][0] = f[k];
         }
@@ -940,8 +953,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll WR
     for (int u = (int)threadIdx.x; u < held_rows * (HD / 4); u += 64 * kWaves) {  // 4 dims of a row
         const int r = u / (HD / 4), d = u % (HD / 4) * 4;
-        float f[WK], v[4] = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (WR == 1) factors(r, f, S > 1 && d == 0);
+        float f[WK], inv, v[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (WR == 1) inv = factors(r, f, S > 1 && d == 0);
+        else inv = words[r][1];
 #pragma unroll
         for (int k = 0; k < WK; ++k) {
             const int at = k * WR * 32 + r;
@@ -950,6 +964,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = fmaf(f[k], p[e], v[e]);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= inv;
         const size_t item = item_of(r);
         if (S == 1) {
             store_out<4>(a, item * HD + d, v);

@@ -121,6 +121,41 @@ def test_scales_far_apart(hip, rows, offset, hd, spread):
     assert off.max() < TOL
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,offset", SHAPES)
+@pytest.mark.parametrize("zero", ["first", "last", "every other", "all"])
+def test_blocks_of_zeros(hip, rows, offset, hd, zero):
+    """A block of zeros has the least scale, far from the others'."""
+    rng = np.random.default_rng(rows + offset)
+    total = offset + rows
+    k, v = ref.some_rows(rng, total, 2, hd)
+    block = np.arange(total) // 32
+    at = {"first": block < 9, "last": block >= block[-1] - 1, "every other": block % 2 == 1, "all": block >= 0}[zero]
+    v[at] = 0
+    dev, cpu = make(hip, rng, total, 2, hd), ref.Cache(total, 2, hd)
+    dev.append(k, v, 0)
+    cpu.append(k, v, 0)
+    q = rng.standard_normal((rows, 8 * hd)).astype(np.float32)
+    want = ref.attention64(q, *cpu.values(0, total), 8, offset)
+    assert np.abs(dev.attention(q, 8, offset) - want).max() <= TOL * np.abs(want).max()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows,offset", [(1, 40000), (200, 20000)])
+def test_the_least_scale_under_many_positions(hip, rows, offset, hd):
+    """Weights' sums of 2^15 and values of the least scale: quotients keep their
+    bits (2^-110 or so, while a unit over the sum is no normal number)."""
+    rng = np.random.default_rng(rows + offset)
+    k, v = ref.some_rows(rng, offset + rows, 1, hd)
+    v = (2.0 ** -110 * rng.uniform(0.5, 1.0, v.shape)).astype(np.float32)
+    dev, cpu = make(hip, rng, offset + rows, 1, hd), ref.Cache(offset + rows, 1, hd)
+    dev.append(k, v, 0)
+    cpu.append(k, v, 0)
+    q = (2.0 ** -8 * rng.standard_normal((rows, 4 * hd))).astype(np.float32)
+    want = ref.attention64(q, *cpu.values(0, offset + rows), 4, offset)
+    assert rel_err(dev.attention(q, 4, offset), want) < TOL
+
+
 @pytest.mark.parametrize("rows,offset", [(1, 700), (70, 100)])
 @pytest.mark.parametrize("size", [0.0, 1e-38, 1e-20, 1e-3, 30.0])
 def test_queries_of_any_size(hip, rows, offset, size):
