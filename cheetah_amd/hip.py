@@ -394,6 +394,9 @@ class Kv8Cache:
             raise ValueError("rows of kv_heads * head_dim values")
         n = k.size // width
         self._listed(offset // KV8_BLOCK * KV8_BLOCK, offset + n)
+        written = self.table[offset // self.page_size:-(-(offset + n) // self.page_size)]
+        if np.unique(written).size < written.size:
+            raise ValueError("an append that writes a page twice")
         kd, vd = DeviceBuffer.from_array(k), DeviceBuffer.from_array(v)
         check(lib().cheetah_hip_kv8_append(kd.ptr, vd.ptr, int(k.dtype == np.float32), n, width, offset,
                                            _c.byref(self.view)))

@@ -167,7 +167,8 @@ int cheetah_hip_tree_commit(const cheetah_hip_kv_view *views, size_t nviews, uin
  *   scales [pages][kv_heads][page_size / 32] bytes
  * page_size is a multiple of 64, head_dim 64 or 128; codes are 16-byte aligned,
  * the four pools do not overlap. page_table (device int32) maps logical pages;
- * entries of pages that a call neither writes nor reads may hold anything.
+ * entries of pages that a call neither writes nor reads may hold anything. The
+ * pages that one append writes differ.
  * ---------------------------------------------------------------------- */
 #define CHEETAH_HIP_KV8_BLOCK 32
 typedef struct cheetah_hip_kv8_view {
@@ -185,12 +186,11 @@ typedef struct cheetah_hip_kv8_view {
  * (k and v may point into packed projections), row_format 0 = BF16, 1 = f32. A
  * block's scale is the least with |x| <= 448 * 2^e for its rows, codes round to
  * nearest (ties to even). Rows of the block before `offset` (written before, from
- * its first on) keep their values; a
- * scale that later rows raise rounds them again (only values below 2^-13 of the
- * block's largest move, by at most 2^-16 of it), and it does not fall before the
- * block's first position is written again. Rows behind the last new
- * one keep their codes, not their values. An infinity or a NaN is kept as NaN and
- * does not count for the scale; magnitudes past 448 * 2^119 become that. */
+ * its first on) keep their values; a scale that later rows raise rounds them again
+ * (only values below 2^-13 of the block's largest move, by at most 2^-16 of it), and
+ * it does not fall before the block's first position is written again. Rows behind
+ * the last new one keep their codes, not their values. An infinity or a NaN is kept
+ * as NaN and does not count for the scale; magnitudes past 448 * 2^119 become that. */
 int cheetah_hip_kv8_append(const void *k, const void *v, uint32_t row_format, size_t rows, size_t stride, size_t offset,
                            const cheetah_hip_kv8_view *kv);
 /* The cached K and V rows of positions begin .. begin + n - 1 as [n][kv_heads *

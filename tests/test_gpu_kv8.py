@@ -244,6 +244,20 @@ def test_the_wrapper_refuses_positions_that_the_table_does_not_list(hip):
         hip.Kv8Cache(100, 1, 64, table=np.array([2**32, 1]), pages=3)
 
 
+def test_a_page_listed_twice_is_read_twice_and_written_once(hip):
+    rng = np.random.default_rng(3)
+    k, v = ref.some_rows(rng, 128, 1, 64)
+    dev, cpu = hip.Kv8Cache(192, 1, 64, table=np.array([1, 0, 1]), pages=2), ref.Cache(192, 1, 64)
+    dev.append(k, v, 0)
+    cpu.append(k, v, 0)
+    cpu.append(k[:64], v[:64], 128)
+    same(dev, cpu, 0, 192)
+    q = rng.standard_normal((5, 4 * 64)).astype(np.float32)
+    assert rel_err(dev.attention(q, 4, 187), ref.attention64(q, *cpu.values(0, 192), 4, 187)) < TOL
+    with pytest.raises(ValueError, match="a page twice"):
+        dev.append(np.concatenate([k, k])[:192], np.concatenate([v, v])[:192], 0)
+
+
 @pytest.mark.parametrize("order", [[0, 1, 2], [2, 1, 0]])
 def test_calls_of_growing_and_shrinking_size_share_their_scratch(hip, order):
     """Calls with many splits, few and none, back to back on one stream: each is
