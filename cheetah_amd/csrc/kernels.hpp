@@ -281,16 +281,19 @@ struct Kv8Cache {
     Kv8Geom g;
 };
 // Rows of K and V (f32 or BF16, `stride` elements apart, kv_heads * head_dim
-// each) quantised into positions offset .. offset + rows - 1, or from *pos_dev on.
+// each) quantised into positions offset .. offset + rows - 1.
 struct Kv8AppendJob {
     const void *k = nullptr, *v = nullptr;
     bool f32 = true;
     size_t stride = 0, rows = 0, offset = 0;
     size_t head_stride = 0;  // elements between a row's KV heads (0: head_dim)
-    const int32_t *pos_dev = nullptr;
     Kv8Cache kv;
 };
 int launch_kv8_append(const Kv8AppendJob &job, hipStream_t s);
+// Decode: one row [q | k | v] at position *pos_dev, rotated (launch_rope_append's
+// arithmetic) into q and into the cache.
+int launch_kv8_rope_append(const float *qkv, float *q, int q_heads, const Kv8Cache &kv, const float *rope_cos,
+                           const float *rope_sin, int rotary_dim, const int32_t *pos_dev, hipStream_t s);
 // Positions begin .. begin + n - 1 as rows of kv_heads * head_dim f32 or BF16 values.
 int launch_kv8_read(const Kv8Cache &kv, size_t begin, size_t n, bool f32, void *k_out, void *v_out, hipStream_t s);
 // Causal attention of `rows` rows from position `offset` on; window 0: over all

@@ -101,7 +101,6 @@ struct AppendArgs {
     long stride, head_stride;
     uint8_t *codes[2], *scales[2];
     Kv8Geom g;
-    const int32_t *pos_dev;  // the first row's position, where set
     long offset;
     int rows;
 };
@@ -131,7 +130,7 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
     const int tid = threadIdx.x, head = blockIdx.y, which = blockIdx.z;
     const int mine = tid / HD, u = tid % HD;
     const int d = u % (HD / 8) * 8, p = u / (HD / 8) * 4;
-    const long offset = a.pos_dev ? (long)*a.pos_dev : a.offset;
+    const long offset = a.offset;
     const long first = (offset / kBlock + (long)blockIdx.x * kRun<HD> + mine) * kBlock;  // the block's first position
     const int keep = (int)max(offset - first, 0l);                                       // its earlier rows
     const int stop = (int)max(min(offset + a.rows - first, (long)kBlock), 0l);           // new rows end here
@@ -214,6 +213,76 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
         }
         to[j] = w;
     }
+}
+
+// ---------------------------------------------------------------------------
+// A decode step's row: RoPE on its query and key heads, its K and V quantised into
+// the position that the device holds; a thread an element, HD of them a head. The
+// bits of a rotation by launch_rope_append and an append, which took 3.5 us a layer
+// more. Bound by its round trips: position, page, scale.
+// ---------------------------------------------------------------------------
+struct RopeArgs {
+    const float *qkv;  // [q | k | v]
+    float *q;
+    Kv8Cache kv;
+    int q_heads, rotary_dim;
+    const float *cos, *sin;  // [position][rotary_dim / 2]
+    const int32_t *pos_dev;
+};
+
+template <int HD>
+__global__ __launch_bounds__(kThreads) void kv8_rope_append_kernel(RopeArgs a) {
+    __shared__ float s_max[kThreads / 64];
+    const int tid = threadIdx.x, d = tid % HD, kvh = a.kv.g.kv_heads;
+    const int head = (int)blockIdx.x * (kThreads / HD) + tid / HD;  // q, then k, then v heads
+    const bool there = head < a.q_heads + 2 * kvh, v = head >= a.q_heads + kvh;
+    const float *src = a.qkv + (size_t)(there ? head : 0) * HD;
+    const int pos = *a.pos_dev, keep = pos % kBlock, half = a.rotary_dim / 2;
+    const float *cr = a.cos + (size_t)pos * half, *sr = a.sin + (size_t)pos * half;
+    const float x = v ? src[d] : rope_elem(src, d, half, a.rotary_dim, cr, sr);
+    float most = fabsf(x);
+    most = wave_max(most < INFINITY ? most : 0.f);
+    if constexpr (HD > 64) {  // two waves a head
+        if ((tid & 63) == 0) s_max[tid >> 6] = most;
+        __syncthreads();
+        most = fmaxf(s_max[tid / HD * 2], s_max[tid / HD * 2 + 1]);
+    }
+    uint8_t *codes = nullptr, *scale = nullptr;
+    int e_old = kScaleLeast;
+    const bool writes = there && head >= a.q_heads;
+    if (there && !writes) a.q[(size_t)head * HD + d] = x;
+    if (writes) {
+        const int page = a.kv.g.page_table[pos / a.kv.g.page_size];
+        const BlockAt at = block_at(a.kv.g, page, pos % a.kv.g.page_size / kBlock, (head - a.q_heads) % kvh, HD);
+        codes = (v ? a.kv.v : a.kv.k) + at.codes;
+        scale = (v ? a.kv.v_scales : a.kv.k_scales) + at.scale;
+        if (keep) e_old = min(max((int)*scale - 127, kScaleLeast), kScaleMost);
+    }
+    if constexpr (HD > 64) __syncthreads();  // both waves have the scale before one writes it
+    if (!writes) return;
+    const int e = max(exponent_for(most), e_old);
+    const uint32_t code = codes_of(f32x4{x, 0.f, 0.f, 0.f}, two_to(-e)) & 0xFFu;
+    if (d == 0) *scale = (uint8_t)(e + 127);
+    if (e > e_old && keep) {  // earlier rows: 32 bytes a thread, of K a position's, of V a dim's
+        const float grown = two_to(max(e_old - e, -126));
+        u32x4 *to = (u32x4 *)(codes + d * kBlock);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const u32x4 o = to[j];
+            u32x4 w = o;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int n = v ? min(max(keep - (16 * j + 4 * k), 0), 4) : d % kBlock < keep ? 4 : 0;  // bytes of them
+                const uint32_t old = n == 4 ? ~0u : (1u << (8 * n)) - 1;
+                w[k] = (rescaled(o[k], grown) & old) | (o[k] & ~old);
+                if (v && (keep - 16 * j) / 4 == k && keep / 16 == j)
+                    w[k] = (w[k] & ~(0xFFu << (8 * (keep % 4)))) | code << (8 * (keep % 4));
+            }
+            if (v || d % kBlock < keep) to[j] = w;
+        }
+        if (v) return;
+    }
+    codes[v ? d * kBlock + keep : d / 32 * (kBlock * 32) + keep * 32 + d % 32] = (uint8_t)code;
 }
 
 // ---------------------------------------------------------------------------
@@ -454,10 +523,10 @@ __host__ __device__ __forceinline__ Reach reach_of(int pos_lo, int pos_hi, int w
 // copies fill three tiles of LDS, a barrier a tile.
 //
 // Bound: with many rows the matrix cores, at the rate that a large F16 product of
-// the library reaches (512 rows on 4,096, 32 / 8 heads of 128: 74.8 us, of which the
+// the library reaches (512 rows on 4,096, 32 / 8 heads of 128: 73.1 us, of which the
 // loop is 60 at 1.16 PFLOP/s of the two part products; queries in and outputs out
 // take the rest); with one row round trips, then memory (32,767 positions, 28 / 4
-// heads of 128: 13.4 us with the merge, 33 MB in 5.2 of them).
+// heads of 128: 12.9 us with the merge, 33 MB in 5.2 of them).
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -938,7 +1007,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         return S == 1 ? 1.0f / sum : 1.f;
     };
     // A few rows: every thread finds its row's factors, a barrier less (6.6 -> 6.1 us for
-    // one token on 576). Many: a thread a row (1,000 windowed rows 42.7 -> 41.7).
+    // one token on 576). Many: a thread a row (1,000 windowed rows 42.7 -> 41.9).
     if constexpr (WR > 1) {
         const int r = (int)threadIdx.x;
         if (r < held_rows) {
@@ -1089,19 +1158,29 @@ int launch_kv8_append(const Kv8AppendJob &j, hipStream_t s) {
     a.head_stride = (long)(j.head_stride ? j.head_stride : (size_t)j.kv.g.head_dim);
     a.codes[0] = j.kv.k, a.codes[1] = j.kv.v, a.scales[0] = j.kv.k_scales, a.scales[1] = j.kv.v_scales;
     a.g = j.kv.g;
-    a.pos_dev = j.pos_dev;
     a.offset = (long)j.offset;
     a.rows = (int)j.rows;
-    // With the position on the device a chunk may reach one block more.
     const size_t run = kThreads / (size_t)j.kv.g.head_dim;
-    const size_t blocks = ((j.pos_dev ? (j.rows + kBlock - 2) / kBlock + 1
-                                      : (j.offset + j.rows - 1) / kBlock - j.offset / kBlock + 1) + run - 1) / run;
+    const size_t blocks = ((j.offset + j.rows - 1) / kBlock - j.offset / kBlock + 1 + run - 1) / run;
     const size_t unit = j.f32 ? 4 : 2;
     const bool vec = ((uintptr_t)j.k | (uintptr_t)j.v | (j.stride * unit) | (a.head_stride * unit)) % 16 == 0;
     const unsigned n = (unsigned)blocks;
     if (j.kv.g.head_dim == 64)
         return j.f32 ? launch_append<64, float>(j, a, vec, n, s) : launch_append<64, uint16_t>(j, a, vec, n, s);
     return j.f32 ? launch_append<128, float>(j, a, vec, n, s) : launch_append<128, uint16_t>(j, a, vec, n, s);
+}
+
+int launch_kv8_rope_append(const float *qkv, float *q, int q_heads, const Kv8Cache &kv, const float *rope_cos,
+                           const float *rope_sin, int rotary_dim, const int32_t *pos_dev, hipStream_t s) {
+    if (rotary_dim <= 0 || rotary_dim > kv.g.head_dim || rotary_dim % 2)
+        return fail("HIP backend: rotary_dim must be even and at most head_dim.");
+    const RopeArgs a{qkv, q, kv, q_heads, rotary_dim, rope_cos, rope_sin, pos_dev};
+    const int heads = kThreads / kv.g.head_dim;  // a block
+    const dim3 grid((unsigned)((q_heads + 2 * kv.g.kv_heads + heads - 1) / heads));
+    if (kv.g.head_dim == 64) hipLaunchKernelGGL((kv8_rope_append_kernel<64>), grid, dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL((kv8_rope_append_kernel<128>), grid, dim3(kThreads), 0, s, a);
+    CHIP_CHECK(hipGetLastError());
+    return 0;
 }
 
 int launch_kv8_read(const Kv8Cache &kv, size_t begin, size_t n, bool f32, void *k_out, void *v_out, hipStream_t s) {

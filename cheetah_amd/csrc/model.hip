@@ -855,10 +855,9 @@ Kv8AttnJob kv8_job(const cheetah_hip_model *m, const Layer *L, size_t rows, size
 }
 
 // RoPE on a chunk's packed rows, its K and V rows into the 8-bit cache of layer L
-// (launch_rope_append's arguments): rotated into kv_rows, then quantised. One row of
-// a captured step comes with its position on the device.
-int kv8_rope_append(cheetah_hip_model *m, const Layer &L, size_t rows, size_t pos, const int32_t *pos_dev,
-                    const float *ws = nullptr, int nchunks = 0, const float *sc = nullptr, const float *bias = nullptr) {
+// (launch_rope_append's arguments): rotated into kv_rows, then quantised.
+int kv8_append_chunk(cheetah_hip_model *m, const Layer &L, size_t rows, size_t pos, const float *ws, int nchunks,
+                     const float *sc, const float *bias) {
     const Shared &sh = *m->sh;
     const size_t R = sh.max_chunk, hd = C(m).head_dim, kvh = C(m).kv_heads;
     KvLayer to;
@@ -867,8 +866,7 @@ int kv8_rope_append(cheetah_hip_model *m, const Layer &L, size_t rows, size_t po
     // One page of R positions, its table the last word of row_pos.
     const KvGeom g{m->row_pos + sh.kv_capacity, (int)R, (int)kvh, (int)hd, 1};
     CHIP_TRY(launch_rope_append(m->qkv, m->qrot, rows, (int)C(m).q_heads, g, to, sh.rope_cos, sh.rope_sin,
-                                (int)C(m).rotary_dim, 0, nullptr, m->stream, ws, nchunks, sc, bias,
-                                pos_dev ? pos_dev : m->row_pos + pos));
+                                (int)C(m).rotary_dim, 0, nullptr, m->stream, ws, nchunks, sc, bias, m->row_pos + pos));
     Kv8AppendJob a;
     a.k = to.k;
     a.v = to.v;
@@ -876,7 +874,6 @@ int kv8_rope_append(cheetah_hip_model *m, const Layer &L, size_t rows, size_t po
     a.head_stride = R * hd;
     a.rows = rows;
     a.offset = pos;
-    a.pos_dev = pos_dev;
     a.kv = kv8_cache(m, L);
     return launch_kv8_append(a, m->stream);
 }
@@ -985,7 +982,8 @@ int enqueue_decode(cheetah_hip_model *m, int splits, bool sample) {
         qkv.y = m->qkv;
         CHIP_TRY(launch_gemv(qkv, s));
         if (sh.kv8) {
-            CHIP_TRY(kv8_rope_append(m, L, 1, 0, pos));
+            CHIP_TRY(launch_kv8_rope_append(m->qkv, m->qrot, (int)c.q_heads, kv8_cache(m, L), sh.rope_cos, sh.rope_sin,
+                                            (int)c.rotary_dim, pos, s));
             Kv8AttnJob j = kv8_job(m, &L, 1, 0);
             j.pos_dev = pos;
             j.splits = splits;
@@ -1155,7 +1153,7 @@ int enqueue_chunk(cheetah_hip_model *m, const uint32_t *tokens_dev, size_t rows,
         qkv.deferred = &qkv_chunks;
         CHIP_TRY(launch_gemm(qkv, s));
         if (sh.kv8)
-            CHIP_TRY(kv8_rope_append(m, L, rows, pos, nullptr, m->gemm_ws, qkv_chunks, L.qkv.scales(), L.qkv_bias));
+            CHIP_TRY(kv8_append_chunk(m, L, rows, pos, m->gemm_ws, qkv_chunks, L.qkv.scales(), L.qkv_bias));
         else
             CHIP_TRY(launch_rope_append(m->qkv, m->qrot, rows, (int)c.q_heads, geom(m), L.kv, sh.rope_cos, sh.rope_sin,
                                     (int)c.rotary_dim, pos, nullptr, s, m->gemm_ws, qkv_chunks, L.qkv.scales(),

@@ -135,6 +135,46 @@ def test_sliding_window(hip, window):
             hip.HipForward(shape, weights(shape)[0], kv=kv)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_step_that_raises_a_scale(hip, hd):
+    """Decode steps whose K and V outgrow their block: its earlier rows are rounded
+    again (normal codes, from 2^-6 of the new scale on, keep their values; others
+    move by at most half a step, 2^-10), other blocks are as they were."""
+    shape = configs.TINY_QWEN2 if hd == 64 else configs.TINY_LLAMA
+    assert shape.head_dim == hd
+    units = dict(weights(shape)[0])
+    loud = 77
+    x = synth.bf16_to_f32(units["model.embed_tokens.weight"]).reshape(shape.vocab_size, -1)[loud]
+    for name in ("k", "v"):
+        key = f"model.layers.0.self_attn.{name}_proj.weight"
+        w = synth.bf16_to_f32(units[key]).reshape(-1, x.size)
+        w = w + np.where(np.arange(len(w)) % 5 == 0, 4.0, 0.0)[:, None] * (x / np.linalg.norm(x))[None]
+        units[key] = synth.f32_to_bf16(w.astype(np.float32)).reshape(units[key].shape)
+    g = hip.HipForward(shape, units, kv_capacity=1024, max_chunk_rows=64, kv="e4m3")
+    tokens = [t for t in synth.make_tokens(shape.vocab_size, 200) if t != loud][:70]
+    g.forward(tokens, 0)
+    raised = moved = 0
+    for step in range(60):
+        n = 70 + step
+        before = g.kv_rows(0, 0, n)
+        g.forward([loud if step % 13 == 5 else 3 * step + 200], n)
+        for old, new in zip(before, g.kv_rows(0, 0, n + 1)):
+            b = n // 32 * 32
+            np.testing.assert_array_equal(old[:b], new[:b])
+            _, e = np.frexp(np.abs(new[b:]).max((0, 2)) / 448)  # 2^e: at least the block's scale, at most twice
+            unit = 2.0 ** e[None, :, None]
+            move = np.abs(old[b:].astype(np.float64) - new[b:n])
+            assert (move <= unit * 2.0 ** -10).all()
+            assert (move[np.abs(old[b:]) >= unit * 2.0 ** -6] == 0).all()
+            moved += int((move > 0).any())
+            raised += int(n > b and (np.abs(new[n]).max(1) > 2 * np.abs(old[b:]).max((0, 2), initial=0)).any())
+            last = np.abs(new[n]).max(1)
+            assert (last > 0).all() and np.isfinite(new).all()
+    # Two blocks have a first loud row, for K and for V; values far enough below it to
+    # move (2^-13.8) are a hundredth of all.
+    assert raised >= 4 and moved >= 1
+
+
 @pytest.mark.parametrize("window", [2**31 - 1, 2**31, 2**32 - 1])
 def test_a_window_past_every_position_is_none(hip, window):
     shape = configs.TINY_LLAMA
