@@ -175,6 +175,43 @@ def test_a_step_that_raises_a_scale(hip, hd):
     assert raised >= 4 and moved >= 1
 
 
+ODD = configs.TINY_QWEN2.replace(name="tiny-odd", q_heads=5, kv_heads=1, head_dim=128)
+
+
+@pytest.mark.parametrize("graph", ["1", "0"])
+@pytest.mark.parametrize("shape", [configs.TINY_QWEN2, GROUP7, ODD], ids=lambda s: s.name)
+def test_cached_rows_are_the_rotated_ones_quantised(hip, shape, graph, monkeypatch):
+    """With k_proj and v_proj zero a row is the bias, K's rotated: the rows that a
+    model with an f32 cache holds. The 8-bit cache holds exactly these, quantised in
+    the same pieces, through prefill and decode. (The first pair of K, 4 long, turns
+    past 3.5 = 448 * 2^-7 at position 33 and not at 32: the block's scale rises.)"""
+    monkeypatch.setenv("CHEETAH_HIP_GRAPH", graph)
+    units = dict(weights(shape)[0])
+    for layer in range(shape.num_layers):
+        p = f"model.layers.{layer}.self_attn."
+        for name in ("k_proj", "v_proj"):
+            units[p + name + ".weight"] = np.zeros_like(units[p + name + ".weight"])
+        bias = synth.bf16_to_f32(units[p + "k_proj.bias"]).reshape(shape.kv_heads, -1).copy()
+        bias[:, 0], bias[:, shape.head_dim // 2] = 4, 0
+        units[p + "k_proj.bias"] = synth.f32_to_bf16(bias.astype(np.float32)).reshape(units[p + "k_proj.bias"].shape)
+    tokens = synth.make_tokens(shape.vocab_size, 100)
+    models = [hip.HipForward(shape, units, kv_capacity=256, max_chunk_rows=64, kv=kv) for kv in ("f32", "e4m3")]
+    for g in models:
+        g.forward(tokens[:20], 0)
+        for pos in range(20, 100):
+            g.forward(tokens[pos:pos + 1], pos)
+    for layer in range(shape.num_layers):
+        rows = models[0].kv_rows(layer, 0, 100)
+        cpu = ref.Cache(100, shape.kv_heads, shape.head_dim)
+        cpu.append(*(x[:20] for x in rows), 0)
+        for pos in range(20, 100):
+            risen = cpu.exps[0, pos // 32, 0]
+            cpu.append(*(x[pos:pos + 1] for x in rows), pos)
+            assert pos != 33 or cpu.exps[0, 1, 0] == risen + 1
+        for got, want in zip(models[1].kv_rows(layer, 0, 100), cpu.values(0, 100)):
+            np.testing.assert_array_equal(got, want)
+
+
 @pytest.mark.parametrize("window", [2**31 - 1, 2**31, 2**32 - 1])
 def test_a_window_past_every_position_is_none(hip, window):
     shape = configs.TINY_LLAMA
