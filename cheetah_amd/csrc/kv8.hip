@@ -101,8 +101,7 @@ struct AppendArgs {
     long stride, head_stride;
     uint8_t *codes[2], *scales[2];
     Kv8Geom g;
-    long offset;
-    int rows;
+    int offset, rows;  // (positions are below 2^31, block bounds behind the last too)
 };
 
 template <class T, bool VEC>
@@ -130,12 +129,11 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
     const int tid = threadIdx.x, head = blockIdx.y, which = blockIdx.z;
     const int mine = tid / HD, u = tid % HD;
     const int d = u % (HD / 8) * 8, p = u / (HD / 8) * 4;
-    const long offset = a.offset;
-    const long first = (offset / kBlock + (long)blockIdx.x * kRun<HD> + mine) * kBlock;  // the block's first position
-    const int keep = (int)max(offset - first, 0l);                                       // its earlier rows
-    const int stop = (int)max(min(offset + a.rows - first, (long)kBlock), 0l);           // new rows end here
+    const int first = (a.offset / kBlock + (int)blockIdx.x * kRun<HD> + mine) * kBlock;  // the block's first position
+    const int keep = max(a.offset - first, 0);                                           // its earlier rows
+    const int stop = max(min(a.offset + a.rows - first, kBlock), 0);                     // new rows end here
     const bool any = stop > keep;  // (a wave's threads share a block)
-    const T *x = (const T *)(which ? a.x[1] : a.x[0]) + (first - offset) * a.stride + head * a.head_stride;
+    const T *x = (const T *)(which ? a.x[1] : a.x[0]) + (first - a.offset) * a.stride + head * a.head_stride;
     f32x4 v[4][2];
     float most = 0.f;
 #pragma unroll
@@ -146,12 +144,17 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
     uint8_t *codes = nullptr, *scale = nullptr;
     int e_old = kScaleLeast;
     if (any) {
-        const int page = a.g.page_table[first / a.g.page_size];
-        const BlockAt at = block_at(a.g, page, (int)(first % a.g.page_size) / kBlock, head, HD);
+        const uint32_t page = (uint32_t)first / (uint32_t)a.g.page_size;
+        const BlockAt at = block_at(a.g, a.g.page_table[page], (first - (int)page * a.g.page_size) / kBlock, head, HD);
         codes = (which ? a.codes[1] : a.codes[0]) + at.codes;
         scale = (which ? a.scales[1] : a.scales[0]) + at.scale;
         if (keep) e_old = min(max((int)*scale - 127, kScaleLeast), kScaleMost);
     }
+    // V's codes that stay, on their way with the scale.
+    const bool whole = keep == 0 && stop == kBlock;
+    u32x4 *const v_to = (u32x4 *)(codes + u * kBlock);  // dim u's 32 positions
+    u32x4 stay[2] = {};
+    if (which && any && !whole) stay[0] = v_to[0], stay[1] = v_to[1];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -195,13 +198,11 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
     }
     __syncthreads();
     if (!any) return;
-    u32x4 *to = (u32x4 *)(codes + u * kBlock);  // dim u's 32 positions
-    const bool whole = keep == 0 && stop == kBlock;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         u32x4 w = *(const u32x4 *)(s_v[mine] + turn_at(u) + 16 * j);
         if (!whole) {
-            const u32x4 o = to[j];
+            const u32x4 o = stay[j];
             auto below = [](int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1; };  // the first n bytes
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -211,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void kv8_append_kernel(AppendArgs a) {
                 w[k] = (w[k] & fresh) | (kept & old) | (o[k] & ~(fresh | old));
             }
         }
-        to[j] = w;
+        v_to[j] = w;
     }
 }
 
@@ -293,8 +294,7 @@ __global__ __launch_bounds__(kThreads) void kv8_rope_append_kernel(RopeArgs a) {
 struct ReadArgs {
     const uint8_t *codes[2], *scales[2];
     Kv8Geom g;
-    long begin;
-    long n;
+    int begin, n;
     void *out[2];
 };
 
@@ -315,12 +315,11 @@ __global__ __launch_bounds__(kThreads) void kv8_read_kernel(ReadArgs a) {
     constexpr int RB = kRun<HD>;
     __shared__ __attribute__((aligned(16))) uint8_t s_v[RB][HD * kTurnRow];
     const int tid = threadIdx.x, head = blockIdx.y, which = blockIdx.z;
-    const long first = a.begin / kBlock, last = (a.begin + a.n - 1) / kBlock;
+    const int first = a.begin / kBlock, last = (a.begin + a.n - 1) / kBlock;
     const int mine = tid / HD;  // of the run's blocks
-    const long blk = min(first + (long)blockIdx.x * RB + mine, last);
-    const int per = a.g.page_size / kBlock;
-    const int page = a.g.page_table[blk / per];
-    const BlockAt at = block_at(a.g, page, (int)(blk % per), head, HD);
+    const int blk = min(first + (int)blockIdx.x * RB + mine, last);
+    const uint32_t per = (uint32_t)a.g.page_size / kBlock, page = (uint32_t)blk / per;
+    const BlockAt at = block_at(a.g, a.g.page_table[page], blk - (int)(page * per), head, HD);
     const uint8_t *codes = (which ? a.codes[1] : a.codes[0]) + at.codes;
     const float scale = two_to((int)(which ? a.scales[1] : a.scales[0])[at.scale] - 127);
     const int u = tid % HD, d = u % (HD / 8) * 8, p = u / (HD / 8) * 4;
@@ -347,11 +346,11 @@ __global__ __launch_bounds__(kThreads) void kv8_read_kernel(ReadArgs a) {
         turn4(x4, lo);
         turn4(y4, hi);
     }
-    if (first + (long)blockIdx.x * RB + mine > last) return;
+    if (first + (int)blockIdx.x * RB + mine > last) return;
     T *out = (T *)(which ? a.out[1] : a.out[0]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const long row = blk * kBlock + p + i - a.begin;
+        const int row = blk * kBlock + p + i - a.begin;
         if (row < 0 || row >= a.n) continue;
         store8(out + (size_t)row * a.g.kv_heads * HD + (size_t)head * HD + d, code_values(lo[i]) * scale,
                code_values(hi[i]) * scale);
@@ -1158,7 +1157,7 @@ int launch_kv8_append(const Kv8AppendJob &j, hipStream_t s) {
     a.head_stride = (long)(j.head_stride ? j.head_stride : (size_t)j.kv.g.head_dim);
     a.codes[0] = j.kv.k, a.codes[1] = j.kv.v, a.scales[0] = j.kv.k_scales, a.scales[1] = j.kv.v_scales;
     a.g = j.kv.g;
-    a.offset = (long)j.offset;
+    a.offset = (int)j.offset;
     a.rows = (int)j.rows;
     const size_t run = kThreads / (size_t)j.kv.g.head_dim;
     const size_t blocks = ((j.offset + j.rows - 1) / kBlock - j.offset / kBlock + 1 + run - 1) / run;
@@ -1187,8 +1186,8 @@ int launch_kv8_read(const Kv8Cache &kv, size_t begin, size_t n, bool f32, void *
     ReadArgs a;
     a.codes[0] = kv.k, a.codes[1] = kv.v, a.scales[0] = kv.k_scales, a.scales[1] = kv.v_scales;
     a.g = kv.g;
-    a.begin = (long)begin;
-    a.n = (long)n;
+    a.begin = (int)begin;
+    a.n = (int)n;
     a.out[0] = k_out, a.out[1] = v_out;
     const size_t blocks = (begin + n - 1) / kBlock - begin / kBlock + 1, run = kThreads / (size_t)kv.g.head_dim;
     const dim3 grid((unsigned)((blocks + run - 1) / run), kv.g.kv_heads, 2), threads(kThreads);
