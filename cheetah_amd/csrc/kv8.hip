@@ -288,7 +288,7 @@ __global__ __launch_bounds__(kThreads) void kv8_rope_append_kernel(RopeArgs a) {
 
 // ---------------------------------------------------------------------------
 // Read: threads and their values as in the append. 32,768 positions of 4 KV heads
-// of 128 as BF16 (100 MB): 17.3 us, 5.8 TB/s (21.9 with a byte at a time from LDS and
+// of 128 as BF16 (100 MB): 16.3 us, 6.2 TB/s (21.9 with a byte at a time from LDS and
 // stores that pass through the caches).
 // ---------------------------------------------------------------------------
 struct ReadArgs {
