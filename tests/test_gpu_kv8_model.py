@@ -1,5 +1,7 @@
 """A model over an 8-bit K/V cache (kv="e4m3"): prefill, decode, windows,
 snapshots and clones, scoring, host-tier weights; what it refuses."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -281,6 +283,35 @@ def test_host_tier_weights_give_the_same_bits(hip):
     assert g.evict_unit("model.layers.0.self_attn.q_proj.weight")
     np.testing.assert_array_equal(g.forward(tokens, 0), plain.forward(tokens, 0))
     np.testing.assert_array_equal(g.forward([5], 70), plain.forward([5], 70))
+
+
+@pytest.mark.parametrize("window", [0, 60])
+def test_clones_in_threads(hip, window):
+    """Clones share pages (a prefix ends inside a block) and nothing else: each in a
+    thread of its own gives what it gives alone."""
+    shape = configs.TINY_LLAMA.replace(sliding_window=window)
+    base = model(hip, shape, capacity=4096)
+    prefix = synth.make_tokens(shape.vocab_size, 77)
+    base.forward(prefix, 0)
+    snap = base.kv_snapshot()
+    texts = [synth.make_tokens(shape.vocab_size, n, seed=n) for n in (2, 30, 101, 400)]
+
+    def run(text, out):
+        g = base.clone()
+        g.restore_kv_prefix(snap, len(prefix))
+        token = g.forward_greedy(text, len(prefix))
+        out.append(g.decode_greedy(token, len(prefix) + len(text), 50).tolist())
+        out.append([x.tobytes() for layer in range(2) for x in g.kv_rows(layer, 0, g.kv_len())])
+
+    alone, together = [[] for _ in texts], [[] for _ in texts]
+    for args in zip(texts, alone):
+        run(*args)
+    threads = [threading.Thread(target=run, args=args) for args in zip(texts, together)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert together == alone and len({x[0][0] for x in alone}) > 1
 
 
 def test_drafted_tokens_are_refused(hip):
