@@ -439,8 +439,8 @@ __device__ __attribute__((noinline)) void plain_row(Kv8KernArgs args, int row, i
             float dot = 0.f;
 #pragma unroll 1
             for (int c = 0; c < C; ++c) {
-                const u32x4 w = *(const u32x4 *)(a.k + at.codes + c * (kBlock * 32) + n * 32 + 16 * half);
-#pragma unroll
+                const uint32_t *w = (const uint32_t *)(a.k + at.codes + c * (kBlock * 32) + n * 32 + 16 * half);
+#pragma unroll 1
                 for (int i = 0; i < 4; ++i) {
                     const f32x4 k = code_values(w[i]), x = *(const f32x4 *)(q + 32 * c + 4 * i);
 #pragma unroll
@@ -519,13 +519,13 @@ __host__ __device__ __forceinline__ Reach reach_of(int pos_lo, int pos_hi, int w
 // times as many take other blocks of positions (so that a short call fills its CUs
 // without a second launch); two waves a SIMD of 230 to 250 registers. One row wave:
 // K and V go from memory into registers, no wave waits for another. More: direct
-// copies fill three tiles of LDS, a barrier a tile.
+// copies fill three tiles of LDS, a barrier a tile. (At most 8 M rows have a kernel of
+// their own, kv8_few_kernel.)
 //
 // Bound: with many rows the matrix cores, at the rate that a large F16 product of
 // the library reaches (512 rows on 4,096, 32 / 8 heads of 128: 73.1 us, of which the
 // loop is 60 at 1.16 PFLOP/s of the two part products; queries in and outputs out
-// take the rest); with one row round trips, then memory (32,767 positions, 28 / 4
-// heads of 128: 12.9 us with the merge, 33 MB in 5.2 of them).
+// take the rest); with few round trips (13 rows on 1,999: 10.3 us with the merge).
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -563,6 +563,30 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32
 __device__ __forceinline__ uint32_t seen_bits(int base, int last, int first, int sinks) {
     auto below = [](int n) { return 0xFFFFu >> (16 - min(max(n, 0), 16)); };  // the first n
     return below(last - base + 1) & (~below(first - base) | below(sinks - base));
+}
+
+// The factors of a row's waves in the sum of their outputs, from words of each
+// (maximum, weight sum, unit), `stride` apart; returned: what the sum is multiplied
+// with, 1 / (weight sum), or with `ml` (a split's word) 1. A wave that saw nothing
+// counts nothing; a NaN sum shows. (The quotient comes last: with the least unit a
+// factor divided by a large sum would be no normal number.)
+template <int N>
+__device__ __forceinline__ float wave_factors(const f32x4 *words, int stride, float (&f)[N], bool one, float2 *ml) {
+    f32x4 word[N];
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        word[k] = words[k * stride];
+        top = fmaxf(top, word[k][0]);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const float m = word[k][0], w = m == -INFINITY && word[k][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        sum += w != 0.f || word[k][1] != word[k][1] ? w * word[k][1] : 0.f;
+        f[k] = w * word[k][2];
+    }
+    if (ml) *ml = make_float2(top, sum);
+    return one ? 1.0f / sum : 1.f;
 }
 
 constexpr int kWaves = 8;
@@ -984,29 +1008,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         const int row = over_g(m0 + r);
         return (size_t)row * a.q_heads + g * G + (m0 + r - row * G);
     };
-    // The factors of a row's waves, with one split of its weight sum too. (A wave that
-    // saw nothing counts nothing; a NaN sum shows.)
-    // The quotient comes last: with the least unit a factor divided by a large sum would
-    // be no normal number.
     auto factors = [&](int r, float (&f)[WK], bool to_part) {
-        f32x4 word[WK];
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < WK; ++k) {
-            word[k] = words[k * WR * 32 + r];
-            top = fmaxf(top, word[k][0]);
-        }
-#pragma unroll
-        for (int k = 0; k < WK; ++k) {
-            const float m = word[k][0], w = m == -INFINITY && word[k][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top);
-            sum += w != 0.f || word[k][1] != word[k][1] ? w * word[k][1] : 0.f;
-            f[k] = w * word[k][2];
-        }
-        if (to_part) a.ml[item_of(r) * S + split] = make_float2(top, sum);
-        return S == 1 ? 1.0f / sum : 1.f;
+        return wave_factors(words + r, WR * 32, f, S == 1, to_part ? a.ml + item_of(r) * S + split : nullptr);
     };
-    // A few rows: every thread finds its row's factors, a barrier less (6.6 -> 6.1 us for
-    // one token on 576). Many: a thread a row (1,000 windowed rows 42.7 -> 41.9).
+    // A few rows: every thread finds its row's factors, a barrier less (6.3 -> 5.9 us for
+    // 333 rows of 14 / 2 heads of 64 on nothing). Many: a thread a row (1,000 windowed rows 42.7 -> 41.9).
     if constexpr (WR > 1) {
         const int r = (int)threadIdx.x;
         if (r < held_rows) {
@@ -1048,6 +1054,266 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     for (int r = wave; r < held_rows; r += kWaves)
         if (uniform(odd[r / 32]) >> (r % 32) & 1)
             plain_row<HD>(kernel_args(), over_g(m0 + r), g * G + (m0 + r - over_g(m0 + r) * G));
+}
+
+// ---------------------------------------------------------------------------
+// At most 8 M rows (a token's heads of a group): v_mfma_f32_16x16x32_f16, whose 16
+// columns are the rows' high parts and their low parts, so that one product takes
+// both (a quarter of the 32-wide products' time).
+//   S^T = K Q^T     two tiles of 16 positions; A = K: lane (n, q) takes 16 dims
+//                   64 c + 16 q .. of position 8 (n / 4) + 4 t + n % 4 of tile t; the
+//                   columns' sum, n and n + 8, is the score.
+//   O^T += V^T P^T  A = V^T: lane (n, q) takes positions 8 q .. + 7 of dim 16 u + n;
+//                   lane (m, q) holds the probabilities of its row there.
+// Blocks of 8 waves, one a CU, every wave with blocks of positions of its own, K and V
+// from memory into registers. 1 on 576 (14 / 2 heads of 64) 5.7 us (6.3 with 32-wide
+// products), 1 on 32,767 (28 / 4 of 128) 12.2 (12.9), under a window of 4,096 8.5 (9.5);
+// 16 waves 6.4 / 14.2 / 10.9, two blocks a CU 5.7 / 13.2 / 8.5, two blocks of positions
+// in flight 5.8 / 13.5 / 9.2. Bound by round trips (page, K and V, the join) and the
+// merge's launch.
+// ---------------------------------------------------------------------------
+constexpr int kFewWaves = 8, kFewRows = 8;
+template <int HD>
+constexpr size_t kFewQueries = kFewWaves * kFewRows * kRowPad<HD> * 4;  // behind the waves' sums
+template <int HD>
+constexpr int kFewQRow = HD * 2 + 16;  // bytes of a row's part
+template <int HD>
+constexpr size_t kFewWords = kFewQueries<HD> + 2 * kFewRows * kFewQRow<HD>;
+template <int HD>
+constexpr size_t kFewLds = kFewWords<HD> + kFewWaves * kFewRows * 16 + kFewRows * 4 + 16;
+
+// A lane's value and that of the lane 16 away, and of the four rows of 16 lanes.
+template <class F>
+__device__ __forceinline__ float over_quads(float x, F f) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+template <int HD>
+__global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, int S) {
+    constexpr int W = kFewWaves, CC = HD / 64, U = HD / 16, BB = kBlock * HD;
+    extern __shared__ __attribute__((aligned(256))) uint8_t smem[];
+    uint8_t *sq = smem + kFewQueries<HD>;
+    f32x4 *words = (f32x4 *)(smem + kFewWords<HD>);
+    int *sq_exp = (int *)(words + W * kFewRows), *odd = sq_exp + kFewRows;
+    auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+    const int n = lane & 15, quad = lane >> 4, r = n % kFewRows;
+    const int G = a.q_heads / a.g.kv_heads, M = a.rows * G;
+    auto over_g = [&](int x) { return G == 1 ? x : (int)__umulhi((uint32_t)x, a.over_group); };
+    const int total = S * a.g.kv_heads, run = (total + 7) / 8;
+    const int work = (int)blockIdx.x % 8 * run + (int)blockIdx.x / 8;
+    if (work >= total) return;
+    const int g = uniform(work % a.g.kv_heads), split = uniform(work / a.g.kv_heads);
+    const int offset = uniform(first_pos(a)), pos_hi = offset + a.rows - 1;
+    const int pos = r < M ? offset + over_g(r) : offset, lo = window_start(a, pos);
+    const int seen_lo = window_start(a, offset), all_first = window_start(a, pos_hi);
+    const Reach reach = reach_of(offset, pos_hi, a.window, a.sinks);
+    const int each = reach.count / S, extra = reach.count % S;
+    const int begin = uniform(split * each + min(split, extra)), end = uniform(begin + each + (split < extra));
+    const int mine = max(end - begin - wave + W - 1, 0) / W;
+
+    // Where this wave's next 64 blocks lie and their scales, a lane each.
+    int held_at = 0;
+    uint32_t held_k = 0, held_v = 0;
+    auto look_up = [&](int i0) {
+        const int b = reach.block(min(begin + wave + min(i0 + lane, max(mine - 1, 0)) * W, reach.count - 1));
+        const int per = a.g.page_size / kBlock;
+        const int page = a.g.page_table[b / per];
+        held_at = (page * a.g.kv_heads + g) * per + b % per;
+    };
+    auto look_up_scales = [&]() {
+        held_k = a.k_scales[held_at];
+        held_v = a.v_scales[held_at];
+    };
+    auto landed = [&]() { asm volatile("" : "+v"(held_k), "+v"(held_v)); };
+    auto at_of = [&](int i) { return (size_t)(uint32_t)__builtin_amdgcn_readlane(held_at, i & 63); };
+    const int koff = quad / 2 * 1024 + (8 * (n / 4) + n % 4) * 32 + 16 * (quad % 2), voff = n * kBlock + 8 * quad;
+    u32x4 kr[CC][2];
+    uint2 vr[U];
+    auto load_k = [&](size_t at) {
+#pragma unroll
+        for (int c = 0; c < CC; ++c)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) kr[c][t] = *(const u32x4 *)(a.k + at * BB + 2048 * c + 128 * t + koff);
+    };
+    auto load_v = [&](size_t at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) vr[u] = *(const uint2 *)(a.v + at * BB + 16 * kBlock * u + voff);
+    };
+
+    // The start, as kv8_attn_kernel's: a wave loads 256 floats of the queries.
+    look_up(0);
+    constexpr int LPR = HD / 4, RPI = 64 / LPR;  // lanes a row, rows a load
+    const int row = wave * RPI + lane / LPR;
+    const bool queries = wave < kFewRows / RPI;
+    f32x4 raw = {0.f, 0.f, 0.f, 0.f};
+    if (queries) {
+        const int rr = min(row, M - 1);
+        raw = *(const f32x4 *)(a.q + ((size_t)over_g(rr) * a.q_heads + g * G + rr - over_g(rr) * G) * HD + lane % LPR * 4);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    look_up_scales();
+    load_k(at_of(0)), load_v(at_of(0));
+    __builtin_amdgcn_sched_barrier(0);
+    if (queries) {
+        const float sl2 = (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f;
+        f32x4 v = raw * (row < M ? sl2 : 0.f);
+        float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+        for (int d = 1; d < LPR; d <<= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
+        const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -112), 127) - 14;
+        v *= two_to(-e);
+        uint2 hi, lw;
+        split_f16(v[0], v[1], hi.x, lw.x);
+        split_f16(v[2], v[3], hi.y, lw.y);
+        *(uint2 *)(sq + row * kFewQRow<HD> + lane % LPR * 8) = hi;
+        *(uint2 *)(sq + (kFewRows + row) * kFewQRow<HD> + lane % LPR * 8) = lw;
+        if (lane % LPR == 0) sq_exp[row] = e;
+    }
+    if (threadIdx.x == 0) *odd = 0;
+    landed();
+    lds_barrier();
+    f16x8 qo[CC][2];
+    const int q_exp = sq_exp[r];
+#pragma unroll
+    for (int c = 0; c < CC; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) qo[c][i] = *(const f16x8 *)(sq + n * kFewQRow<HD> + 128 * c + 32 * quad + 16 * i);
+
+    f32x4 o[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m2 = -INFINITY, l = 0.f;
+    int v_exp = 0;  // o is in units of 2^v_exp
+    uint32_t now_k = held_k, now_v = held_v;
+    for (int i = 0; i < mine; ++i) {
+        if (i > 0 && (i & 63) == 0) now_k = held_k, now_v = held_v;
+        if (((i + 1) & 63) == 0 && i + 1 < mine) look_up(i + 1), look_up_scales(), landed();
+        const size_t at_next = at_of(i + 1);
+        const int p0 = reach.block(begin + wave + i * W) * kBlock;
+        f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int c = 0; c < CC; ++c)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const u32x4 x = kr[c][t];
+                st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(x[0], x[1], 1.f), qo[c][0], st[t], 0, 0, 0);
+                st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(x[2], x[3], 1.f), qo[c][1], st[t], 0, 0, 0);
+            }
+        if (i + 1 < mine) load_k(at_next);
+        __builtin_amdgcn_sched_barrier(0);
+        constexpr int kOther = 0x128;  // row_ror:8: the column 8 away
+        float s[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] = st[k / 4][k % 4] + dpp_mov<kOther>(st[k / 4][k % 4]);
+        if (p0 + kBlock - 1 > offset || (p0 < all_first && p0 + kBlock > a.sinks)) {
+            const uint32_t bits = seen_bits(p0 + 8 * quad, pos, lo, a.sinks);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s[k] = bits >> k & 1 ? s[k] : -INFINITY;
+        }
+        const float fs = ldexpf(1.f, max(q_exp + (int)__builtin_amdgcn_readlane(now_k, i & 63) - 127, -126));
+        float tmax = s[0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) tmax = fmaxf(tmax, s[k]);
+        tmax = over_quads(tmax, [](float x, float y) { return fmaxf(x, y); }) * fs;
+        if (__any(tmax > m2 + 8.0f)) {  // (as kv8_attn_kernel's: p <= 2^8)
+            const bool raise = tmax > m2 + 8.0f;
+            const float mnew = raise ? tmax : m2, alpha = raise ? __builtin_amdgcn_exp2f(m2 - mnew) : 1.f;
+            l *= alpha;
+#pragma unroll
+            for (int u = 0; u < U; ++u) o[u] *= alpha;
+            m2 = mnew;
+        }
+        const float mref = m2 == -INFINITY ? 0.f : m2;
+        uint32_t p[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * k], fs, -mref)), y = __builtin_amdgcn_exp2f(fmaf(s[2 * k + 1], fs, -mref));
+            l += x;
+            l += y;
+            uint32_t hi, lw;
+            split_f16(x, y, hi, lw);
+            p[k] = n < kFewRows ? hi : lw;
+        }
+        if (p0 + kBlock - 1 > pos_hi || (p0 < seen_lo && p0 + kBlock > a.sinks)) {
+            // Positions that no row sees may hold anything: zeros.
+            const uint32_t bits = seen_bits(p0 + 8 * quad, pos_hi, seen_lo, a.sinks);
+            const uint32_t b0 = ((bits & 15) * 0x204081u & 0x01010101u) * 0xFFu, b1 = ((bits >> 4 & 15) * 0x204081u & 0x01010101u) * 0xFFu;
+#pragma unroll
+            for (int u = 0; u < U; ++u) vr[u].x &= b0, vr[u].y &= b1;
+        }
+        // V under 2^(e_v - v_exp): exact in F16 for differences of -15 .. 7.
+        const int e_v = (int)__builtin_amdgcn_readlane(now_v, i & 63) - 127;
+        if (i == 0) v_exp = e_v;
+        if (e_v - v_exp > 7 || e_v - v_exp < -15) {
+            uint32_t codes = 0, sums = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                codes |= vr[u].x | vr[u].y;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sums |= __float_as_uint(o[u][k]);
+            }
+            // Far steps could lose the sums' values: the rows are computed again; a block
+            // of zeros takes any scale.
+            if (__any(codes & 0x7F7F7F7Fu)) {
+                if (abs(e_v - v_exp) > 100 && __any(sums << 1)) l = NAN;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[u][k] = ldexpf(o[u][k], v_exp - e_v);
+                v_exp = e_v;
+            }
+        }
+        const float vs = two_to(min(max(e_v - v_exp, -126), 127));
+        const f16x8 pp = __builtin_bit_cast(f16x8, u32x4{p[0], p[1], p[2], p[3]});
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            o[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(vr[u].x, vr[u].y, vs), pp, o[u], 0, 0, 0);
+        if (i + 1 < mine) load_v(at_next);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // The waves' parts meet in LDS.
+    l = over_quads(l, [](float x, float y) { return x + y; });
+    float *so = (float *)smem + (size_t)(wave * kFewRows + r) * kRowPad<HD> + 4 * quad;
+#pragma unroll
+    for (int u = 0; u < U; u += 2) {  // (a row's two columns take turns to write)
+        f32x4 v[2];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[0][k] = o[u][k] + dpp_mov<0x128>(o[u][k]);
+            v[1][k] = o[u + 1][k] + dpp_mov<0x128>(o[u + 1][k]);
+        }
+        if (r < M) *(f32x4 *)(so + 16 * (u + n / kFewRows)) = n < kFewRows ? v[0] : v[1];
+    }
+    if (lane < kFewRows) words[wave * kFewRows + r] = f32x4{m2, l, two_to(v_exp), 0.f};
+    __syncthreads();
+    for (int u = (int)threadIdx.x; u < M * (HD / 4); u += 64 * W) {  // 4 dims of a row
+        const int rr = u / (HD / 4), d = u % (HD / 4) * 4, at = over_g(rr);
+        const size_t item = (size_t)at * a.q_heads + g * G + (rr - at * G);
+        float f[W], v[4] = {0.f, 0.f, 0.f, 0.f};
+        const float inv = wave_factors(words + rr, kFewRows, f, S == 1, S > 1 && d == 0 ? a.ml + item * S + split : nullptr);
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const f32x4 x = *(const f32x4 *)((const float *)smem + (size_t)(k * kFewRows + rr) * kRowPad<HD> + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(f[k], x[e], v[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= inv;
+        if (S == 1) {
+            store_out<4>(a, item * HD + d, v);
+            if (!(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY))
+                atomicOr(odd, 1 << rr);
+        } else {
+            *(f32x4 *)(a.part + (item * S + split) * HD + d) = f32x4{v[0], v[1], v[2], v[3]};
+        }
+    }
+    if (S > 1) return;
+    __syncthreads();
+    if (wave < M && (uniform(*odd) >> wave & 1)) plain_row<HD>(kernel_args(), over_g(wave), g * G + (wave - over_g(wave) * G));
 }
 
 // The splits of a row and head, joined by W waves (each takes every W-th); the
@@ -1127,8 +1393,17 @@ int launch_attn_blocks(const Kv8AttnArgs &a, int S, hipStream_t s) {
 }
 
 template <int HD>
+int launch_few(const Kv8AttnArgs &a, int S, hipStream_t s) {
+    const unsigned blocks = (unsigned)((S * a.g.kv_heads + 7) / 8 * 8);
+    hipLaunchKernelGGL((kv8_few_kernel<HD>), dim3(blocks), dim3(64 * kFewWaves), kFewLds<HD>, s, a, S);
+    CHIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+template <int HD>
 int launch_attn(const Kv8AttnArgs &a, int wr, int S, hipStream_t s) {
-    if (wr == 1) CHIP_TRY((launch_attn_blocks<HD, 1>(a, S, s)));
+    if (wr == 0) CHIP_TRY((launch_few<HD>(a, S, s)));
+    else if (wr == 1) CHIP_TRY((launch_attn_blocks<HD, 1>(a, S, s)));
     else if (wr == 2) CHIP_TRY((launch_attn_blocks<HD, 2>(a, S, s)));
     else CHIP_TRY((launch_attn_blocks<HD, 4>(a, S, s)));
     if (S == 1) return 0;
@@ -1208,7 +1483,9 @@ int launch_kv8_read(const Kv8Cache &kv, size_t begin, size_t n, bool f32, void *
 // of positions at two waves a SIMD, 6 for the start and the end of a round of
 // blocks, 4.5 TB/s for a merge's partials and 3 for its launch. Blocks of one row
 // wave read K and V from the caches for every 32 rows, four row waves for 128:
-// ties go to more.
+// ties go to more. At most 8 M rows: kv8_few_kernel (row waves 0), 0.95 (0.7) a step and
+// 2.4 for a merge (one token on 767, 32 / 8 heads of 128, three steps: 7.0 us, with
+// splits 7.6; on 2,047, eight steps: 11.8, with splits 7.8).
 struct Cut {
     int wr, splits;
 };
@@ -1218,6 +1495,17 @@ static Cut cut_of(const Kv8AttnJob &j) {
     const int last = (int)(j.offset + j.rows - 1);
     Cut best{1, 1};
     double least = 0;
+    if (M <= (size_t)kFewRows) {
+        const size_t reach = (size_t)reach_of((int)j.offset, last, (int)j.window, (int)j.sinks).count;
+        const size_t most = std::max<size_t>(1, std::min<size_t>(kMaxSplits, std::min((reach + kFewWaves - 1) / kFewWaves, cus / kvh)));
+        for (size_t S = 1; S <= most; S = S < most && S * 2 > most ? most : S * 2) {
+            const double steps = (double)((reach + S * kFewWaves - 1) / (S * kFewWaves));
+            double us = steps * (hd == 64 ? 0.7 : 0.95);
+            if (S > 1) us += 2.4 + 2.0 * (double)(j.rows * j.q_heads * S * hd * 4) / 4.5e6;
+            if (least == 0 || us < least) least = us, best = Cut{0, (int)S};
+        }
+        return best;
+    }
     for (int wr = 4; wr >= 1; wr /= 2) {
         if (wr > 1 && tiles <= (size_t)wr / 2) continue;  // row waves without rows
         const size_t wk = kWaves / wr, blocks = (tiles + wr - 1) / wr * kvh;
@@ -1246,7 +1534,8 @@ size_t kv8_attention_part_most(int head_dim) { return (size_t)std::max(device_cu
 
 template <int HD>
 static int prepare() {
-    static std::atomic<uint64_t> set[3];
+    static std::atomic<uint64_t> set[4];
+    CHIP_TRY(allow_dynamic_lds((const void *)kv8_few_kernel<HD>, kFewLds<HD>, set[3]));
     CHIP_TRY(allow_dynamic_lds((const void *)kv8_attn_kernel<HD, 1>, kv8_attn_lds_bytes<HD, 1>(), set[0]));
     CHIP_TRY(allow_dynamic_lds((const void *)kv8_attn_kernel<HD, 2>, kv8_attn_lds_bytes<HD, 2>(), set[1]));
     return allow_dynamic_lds((const void *)kv8_attn_kernel<HD, 4>, kv8_attn_lds_bytes<HD, 4>(), set[2]);

@@ -232,6 +232,42 @@ def test_pools_past_four_gigabytes(hip):
         np.testing.assert_array_equal(far.attention(q, 32, n - rows), near.attention(q, 32, n - rows))
 
 
+def test_a_wave_with_more_blocks_than_lanes(hip):
+    """256 KV heads leave each one block of waves, of which one takes more than 64
+    blocks of positions, so page entries and scales are looked up again on the way.
+    Every head has the same rows and queries of its own. (2e-5 has room for 16,600
+    keys: their weights' roundings are 1.7 times those of 6,000.)"""
+    rng, n, kvh, hd = np.random.default_rng(5), 16600, 256, 64
+    k, v = ref.some_rows(rng, n, 1, hd)
+    k, v = (synth.f32_to_bf16(x.reshape(n, hd)) for x in (k, v))
+    dev, cpu = make(hip, rng, n, kvh, hd, 128), ref.Cache(n, 1, hd)
+    for at in range(0, n, 3300):
+        dev.append(np.tile(k[at:at + 3300], kvh), np.tile(v[at:at + 3300], kvh), at)
+        cpu.append(*(synth.bf16_to_f32(x[at:at + 3300]) for x in (k, v)), at)
+    k, v = (x[:, 0] for x in cpu.values(0, n))
+    for rows, window in [(1, 0), (8, 0), (9, 0), (40, 0), (100, 0), (3, 16450)]:
+        q = rng.standard_normal((rows, kvh * hd)).astype(np.float32)
+        got = dev.attention(q, kvh, n - rows, window)
+        for i in {0, rows // 3, rows // 2, rows - 1}:
+            pos = n - rows + i
+            seen = slice(max(pos + 1 - window, 0) if window else 0, pos + 1)
+            s = q[i].astype(np.float64).reshape(kvh, hd) @ k[seen].T / np.sqrt(hd)
+            w = np.exp(s - s.max(1, keepdims=True))
+            want = (w @ v[seen] / w.sum(1, keepdims=True)).reshape(-1)
+            assert rel_err(got[i], want) < TOL, (rows, window, i)
+
+
+@pytest.mark.parametrize("q_heads,kvh,hd", [(4, 4, 64), (8, 4, 128), (12, 4, 64), (16, 2, 128), (4, 1, 64)])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("offset,window,sinks", [(0, 0, 0), (29, 0, 0), (700, 0, 0), (700, 5, 2), (3000, 1000, 40)])
+def test_few_rows(hip, q_heads, kvh, hd, rows, offset, window, sinks):
+    """Up to 8 query rows x heads of a group, and a few more."""
+    rng, dev, cpu = filled(hip, rows + offset, offset + rows, kvh, hd)
+    q = rng.standard_normal((rows, q_heads * hd)).astype(np.float32)
+    want = ref.attention64(q, *cpu.values(0, offset + rows), q_heads, offset, window, sinks)
+    assert rel_err(dev.attention(q, q_heads, offset, window, sinks), want) < TOL
+
+
 def test_the_wrapper_refuses_positions_that_the_table_does_not_list(hip):
     cache = hip.Kv8Cache(200, 1, 64, table=np.array([2, 0, -1, 1], np.int64), pages=3)
     rows = np.zeros((10, 64), np.float32)
