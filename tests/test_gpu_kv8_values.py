@@ -9,8 +9,8 @@ from test_gpu_kv8 import TOL, filled, make, rel_err
 
 pytestmark = pytest.mark.gpu
 
-# One split, several, and many rows (shared tiles).
-SHAPES = [(1, 40), (1, 700), (1, 5000), (9, 300), (70, 1500), (300, 200)]
+# One split, several, two rows (8 with their heads), and many rows (shared tiles).
+SHAPES = [(1, 40), (1, 700), (1, 5000), (2, 45), (2, 600), (9, 300), (70, 1500), (300, 200)]
 
 
 @pytest.fixture(scope="module")
