@@ -133,6 +133,7 @@ struct Shared {
     WMat head;
     uint16_t *final_norm = nullptr;
     float *rope_cos = nullptr, *rope_sin = nullptr;
+    int32_t *row_pos = nullptr;  // 8-bit cache: 0, 1, .. kv_capacity - 1, 0
     int num_pages = 0;
     size_t page_elems = 0;  // elements of one page of one layer (K or V)
     size_t page_bytes() const { return page_elems * (kv8 ? 1 : kv_f32 ? 4 : 2); }
@@ -209,10 +210,8 @@ struct cheetah_hip_model {
     float *hidden = nullptr, *normed = nullptr, *qkv = nullptr, *qrot = nullptr, *attn = nullptr, *act = nullptr;
     float *logits = nullptr, *part = nullptr;
     // 8-bit cache: a chunk's rotated K and V rows on their way to it, laid out as an
-    // f32 cache of one page ([kv_head][max_chunk][head_dim] each), and device words
-    // 0, 1, .. kv_capacity - 1, 0.
+    // f32 cache of one page ([kv_head][max_chunk][head_dim] each).
     float *kv_rows = nullptr;
-    int32_t *row_pos = nullptr;
     size_t part_floats = 0;
     float *gemm_ws = nullptr;  // split-K chunk sums of the prefill GEMMs
     size_t gemm_ws_floats = 0;
@@ -454,6 +453,15 @@ int finalize(cheetah_hip_model *m) {
     CHIP_TRY(sh.mem.alloc(&sh.rope_sin, sn.size()));
     CHIP_CHECK(hipMemcpy(sh.rope_cos, cs.data(), cs.size() * 4, hipMemcpyHostToDevice));
     CHIP_CHECK(hipMemcpy(sh.rope_sin, sn.data(), sn.size() * 4, hipMemcpyHostToDevice));
+
+    // (Here, not with an instance's buffers: a copy on the legacy stream would end the
+    // capture of a clone's decode step in another thread.)
+    if (sh.kv8) {
+        std::vector<int32_t> at(sh.kv_capacity + 1, 0);
+        for (size_t i = 0; i < sh.kv_capacity; ++i) at[i] = (int32_t)i;
+        CHIP_TRY(sh.mem.alloc(&sh.row_pos, at.size()));
+        CHIP_CHECK(hipMemcpy(sh.row_pos, at.data(), at.size() * sizeof(int32_t), hipMemcpyHostToDevice));
+    }
 
     // KV pool.
     sh.num_pages = (int)((sh.kv_capacity + kPageSize - 1) / kPageSize);
@@ -718,10 +726,6 @@ int init_instance(cheetah_hip_model *m) {
         m->part_floats = kv8_attention_part_most((int)c.head_dim);
         CHIP_TRY(kv8_attention_prepare((int)c.head_dim));
         CHIP_TRY(m->mem.alloc(&m->kv_rows, 2 * R * kvd));
-        CHIP_TRY(m->mem.alloc(&m->row_pos, sh.kv_capacity + 1));
-        std::vector<int32_t> at(sh.kv_capacity + 1, 0);  // positions in order, then a 0
-        for (size_t i = 0; i < sh.kv_capacity; ++i) at[i] = (int32_t)i;
-        CHIP_CHECK(hipMemcpy(m->row_pos, at.data(), at.size() * sizeof(int32_t), hipMemcpyHostToDevice));
     }
     CHIP_TRY(m->mem.alloc(&m->part, m->part_floats));
     {
@@ -864,9 +868,9 @@ int kv8_append_chunk(cheetah_hip_model *m, const Layer &L, size_t rows, size_t p
     to.k = m->kv_rows;
     to.v = m->kv_rows + R * kvh * hd;
     // One page of R positions, its table the last word of row_pos.
-    const KvGeom g{m->row_pos + sh.kv_capacity, (int)R, (int)kvh, (int)hd, 1};
+    const KvGeom g{sh.row_pos + sh.kv_capacity, (int)R, (int)kvh, (int)hd, 1};
     CHIP_TRY(launch_rope_append(m->qkv, m->qrot, rows, (int)C(m).q_heads, g, to, sh.rope_cos, sh.rope_sin,
-                                (int)C(m).rotary_dim, 0, nullptr, m->stream, ws, nchunks, sc, bias, m->row_pos + pos));
+                                (int)C(m).rotary_dim, 0, nullptr, m->stream, ws, nchunks, sc, bias, sh.row_pos + pos));
     Kv8AppendJob a;
     a.k = to.k;
     a.v = to.v;
