@@ -519,13 +519,13 @@ __host__ __device__ __forceinline__ Reach reach_of(int pos_lo, int pos_hi, int w
 // times as many take other blocks of positions (so that a short call fills its CUs
 // without a second launch); two waves a SIMD of 230 to 250 registers. One row wave:
 // K and V go from memory into registers, no wave waits for another. More: direct
-// copies fill three tiles of LDS, a barrier a tile. (At most 8 M rows have a kernel of
-// their own, kv8_few_kernel.)
+// copies fill three tiles of LDS, a barrier a tile. (Few rows have a kernel of their
+// own, kv8_few_kernel.)
 //
 // Bound: with many rows the matrix cores, at the rate that a large F16 product of
 // the library reaches (512 rows on 4,096, 32 / 8 heads of 128: 73.1 us, of which the
 // loop is 60 at 1.16 PFLOP/s of the two part products; queries in and outputs out
-// take the rest); with few round trips (13 rows on 1,999: 10.3 us with the merge).
+// take the rest); with few round trips.
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -1057,30 +1057,32 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
 }
 
 // ---------------------------------------------------------------------------
-// At most 8 M rows (a token's heads of a group): v_mfma_f32_16x16x32_f16, whose 16
-// columns are the rows' high parts and their low parts, so that one product takes
-// both (a quarter of the 32-wide products' time).
+// Few M rows: v_mfma_f32_16x16x32_f16 over blocks of R = 8 or 16 of them. The 16
+// columns of 8 rows (a token's heads of a group) are their high parts and their low
+// parts, so that one product takes both, a quarter of the 32-wide products' time; 16
+// rows take two products.
 //   S^T = K Q^T     two tiles of 16 positions; A = K: lane (n, q) takes 16 dims
-//                   64 c + 16 q .. of position 8 (n / 4) + 4 t + n % 4 of tile t; the
-//                   columns' sum, n and n + 8, is the score.
+//                   64 c + 16 q .. of position 8 (n / 4) + 4 t + n % 4 of tile t; of 8
+//                   rows the columns' sum, n and n + 8, is the score.
 //   O^T += V^T P^T  A = V^T: lane (n, q) takes positions 8 q .. + 7 of dim 16 u + n;
 //                   lane (m, q) holds the probabilities of its row there.
-// Blocks of 8 waves, one a CU, every wave with blocks of positions of its own, K and V
-// from memory into registers. 1 on 576 (14 / 2 heads of 64) 5.7 us (6.3 with 32-wide
-// products), 1 on 32,767 (28 / 4 of 128) 12.2 (12.9), under a window of 4,096 8.5 (9.5);
-// 16 waves 6.4 / 14.2 / 10.9, two blocks a CU 5.7 / 13.2 / 8.5, two blocks of positions
-// in flight 5.8 / 13.5 / 9.2. Bound by round trips (page, K and V, the join) and the
-// merge's launch.
+// Blocks of 8 waves, every one with blocks of positions of its own, K and V from
+// memory into registers. 1 on 576 (14 / 2 heads of 64) 5.6 us (6.3 with 32-wide
+// products), 1 on 32,767 (28 / 4 of 128) 12.2 (12.9), under a window of 4,096 8.5 (9.5),
+// 13 on 1,999 (32 / 8 of 128) 9.9 (11.0). Of 8 rows 16 waves 6.4 / 14.2 / 10.9, two
+// blocks a CU 5.7 / 13.2 / 8.5, two blocks of positions in flight 5.8 / 13.5 / 9.2.
+// Bound by round trips (page, K and V, the join) and the merge's launch.
 // ---------------------------------------------------------------------------
-constexpr int kFewWaves = 8, kFewRows = 8;
-template <int HD>
-constexpr size_t kFewQueries = kFewWaves * kFewRows * kRowPad<HD> * 4;  // behind the waves' sums
+constexpr int kFewWaves = 8;
+constexpr int kFew8 = -8, kFew16 = -16;  // a cut's rows in place of row waves
+template <int HD, int R>
+constexpr size_t kFewQueries = kFewWaves * R * kRowPad<HD> * 4;  // behind the waves' sums
 template <int HD>
 constexpr int kFewQRow = HD * 2 + 16;  // bytes of a row's part
-template <int HD>
-constexpr size_t kFewWords = kFewQueries<HD> + 2 * kFewRows * kFewQRow<HD>;
-template <int HD>
-constexpr size_t kFewLds = kFewWords<HD> + kFewWaves * kFewRows * 16 + kFewRows * 4 + 16;
+template <int HD, int R>
+constexpr size_t kFewWords = kFewQueries<HD, R> + 2 * R * kFewQRow<HD>;
+template <int HD, int R>
+constexpr size_t kFewLds = kFewWords<HD, R> + kFewWaves * R * 16 + R * 4 + 16;
 
 // A lane's value and that of the lane 16 away, and of the four rows of 16 lanes.
 template <class F>
@@ -1091,26 +1093,29 @@ __device__ __forceinline__ float over_quads(float x, F f) {
     return f(__uint_as_float(t[0]), __uint_as_float(t[1]));
 }
 
-template <int HD>
+template <int HD, int R>
 __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, int S) {
     constexpr int W = kFewWaves, CC = HD / 64, U = HD / 16, BB = kBlock * HD;
+    constexpr int P = R / 8;  // products for the two parts
     extern __shared__ __attribute__((aligned(256))) uint8_t smem[];
-    uint8_t *sq = smem + kFewQueries<HD>;
-    f32x4 *words = (f32x4 *)(smem + kFewWords<HD>);
-    int *sq_exp = (int *)(words + W * kFewRows), *odd = sq_exp + kFewRows;
+    uint8_t *sq = smem + kFewQueries<HD, R>;
+    f32x4 *words = (f32x4 *)(smem + kFewWords<HD, R>);
+    int *sq_exp = (int *)(words + W * R), *odd = sq_exp + R;
     auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
-    const int n = lane & 15, quad = lane >> 4, r = n % kFewRows;
-    const int G = a.q_heads / a.g.kv_heads, M = a.rows * G;
+    const int n = lane & 15, quad = lane >> 4, r = n % R;
+    const int G = a.q_heads / a.g.kv_heads, M = a.rows * G, RB = (M + R - 1) / R;
     auto over_g = [&](int x) { return G == 1 ? x : (int)__umulhi((uint32_t)x, a.over_group); };
-    const int total = S * a.g.kv_heads, run = (total + 7) / 8;
+    const int total = RB * S * a.g.kv_heads, run = (total + 7) / 8;
     const int work = (int)blockIdx.x % 8 * run + (int)blockIdx.x / 8;
     if (work >= total) return;
-    const int g = uniform(work % a.g.kv_heads), split = uniform(work / a.g.kv_heads);
-    const int offset = uniform(first_pos(a)), pos_hi = offset + a.rows - 1;
-    const int pos = r < M ? offset + over_g(r) : offset, lo = window_start(a, pos);
-    const int seen_lo = window_start(a, offset), all_first = window_start(a, pos_hi);
-    const Reach reach = reach_of(offset, pos_hi, a.window, a.sinks);
+    const int pair = work / RB, m0 = uniform(work % RB * R), rows = min(R, M - m0);  // of the block
+    const int g = uniform(pair % a.g.kv_heads), split = uniform(pair / a.g.kv_heads);
+    const int offset = uniform(first_pos(a));
+    const int pos_lo = uniform(offset + over_g(m0)), pos_hi = uniform(offset + over_g(m0 + rows - 1));
+    const int pos = r < rows ? offset + over_g(m0 + r) : pos_lo, lo = window_start(a, pos);
+    const int seen_lo = window_start(a, pos_lo), all_first = window_start(a, pos_hi);
+    const Reach reach = reach_of(pos_lo, pos_hi, a.window, a.sinks);
     const int each = reach.count / S, extra = reach.count % S;
     const int begin = uniform(split * each + min(split, extra)), end = uniform(begin + each + (split < extra));
     const int mine = max(end - begin - wave + W - 1, 0) / W;
@@ -1148,10 +1153,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
     look_up(0);
     constexpr int LPR = HD / 4, RPI = 64 / LPR;  // lanes a row, rows a load
     const int row = wave * RPI + lane / LPR;
-    const bool queries = wave < kFewRows / RPI;
+    const bool queries = wave < R / RPI;
     f32x4 raw = {0.f, 0.f, 0.f, 0.f};
     if (queries) {
-        const int rr = min(row, M - 1);
+        const int rr = m0 + min(row, rows - 1);
         raw = *(const f32x4 *)(a.q + ((size_t)over_g(rr) * a.q_heads + g * G + rr - over_g(rr) * G) * HD + lane % LPR * 4);
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -1160,7 +1165,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
     __builtin_amdgcn_sched_barrier(0);
     if (queries) {
         const float sl2 = (1.0f / sqrtf((float)HD)) * 1.44269504088896340736f;
-        f32x4 v = raw * (row < M ? sl2 : 0.f);
+        f32x4 v = raw * (row < rows ? sl2 : 0.f);
         float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
         for (int d = 1; d < LPR; d <<= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
@@ -1170,19 +1175,27 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
         split_f16(v[0], v[1], hi.x, lw.x);
         split_f16(v[2], v[3], hi.y, lw.y);
         *(uint2 *)(sq + row * kFewQRow<HD> + lane % LPR * 8) = hi;
-        *(uint2 *)(sq + (kFewRows + row) * kFewQRow<HD> + lane % LPR * 8) = lw;
+        *(uint2 *)(sq + (R + row) * kFewQRow<HD> + lane % LPR * 8) = lw;
         if (lane % LPR == 0) sq_exp[row] = e;
     }
     if (threadIdx.x == 0) *odd = 0;
     landed();
     lds_barrier();
-    f16x8 qo[CC][2];
+    f16x8 qo[P][CC][2];
     const int q_exp = sq_exp[r];
 #pragma unroll
-    for (int c = 0; c < CC; ++c)
+    for (int j = 0; j < P; ++j)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) qo[c][i] = *(const f16x8 *)(sq + n * kFewQRow<HD> + 128 * c + 32 * quad + 16 * i);
+        for (int c = 0; c < CC; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                qo[j][c][i] = *(const f16x8 *)(sq + (j * R + n) * kFewQRow<HD> + 128 * c + 32 * quad + 16 * i);
 
+    // A row's value from its columns: the high and the low part's, 8 away (row_ror:8).
+    auto whole_row = [](float x) {
+        if constexpr (P == 1) return x + dpp_mov<0x128>(x);
+        else return x;
+    };
     f32x4 o[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1200,16 +1213,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const u32x4 x = kr[c][t];
-                st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(x[0], x[1], 1.f), qo[c][0], st[t], 0, 0, 0);
-                st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(x[2], x[3], 1.f), qo[c][1], st[t], 0, 0, 0);
+                const f16x8 x0 = codes_f16(x[0], x[1], 1.f), x1 = codes_f16(x[2], x[3], 1.f);
+#pragma unroll
+                for (int j = 0; j < P; ++j) {
+                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, qo[j][c][0], st[t], 0, 0, 0);
+                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, qo[j][c][1], st[t], 0, 0, 0);
+                }
             }
         if (i + 1 < mine) load_k(at_next);
         __builtin_amdgcn_sched_barrier(0);
-        constexpr int kOther = 0x128;  // row_ror:8: the column 8 away
         float s[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s[k] = st[k / 4][k % 4] + dpp_mov<kOther>(st[k / 4][k % 4]);
-        if (p0 + kBlock - 1 > offset || (p0 < all_first && p0 + kBlock > a.sinks)) {
+        for (int k = 0; k < 8; ++k) s[k] = whole_row(st[k / 4][k % 4]);
+        if (p0 + kBlock - 1 > pos_lo || (p0 < all_first && p0 + kBlock > a.sinks)) {
             const uint32_t bits = seen_bits(p0 + 8 * quad, pos, lo, a.sinks);
 #pragma unroll
             for (int k = 0; k < 8; ++k) s[k] = bits >> k & 1 ? s[k] : -INFINITY;
@@ -1228,7 +1244,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
             m2 = mnew;
         }
         const float mref = m2 == -INFINITY ? 0.f : m2;
-        uint32_t p[4];
+        uint32_t p[P][4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * k], fs, -mref)), y = __builtin_amdgcn_exp2f(fmaf(s[2 * k + 1], fs, -mref));
@@ -1236,7 +1252,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
             l += y;
             uint32_t hi, lw;
             split_f16(x, y, hi, lw);
-            p[k] = n < kFewRows ? hi : lw;
+            p[0][k] = n < R ? hi : lw;
+            if constexpr (P == 2) p[1][k] = lw;
         }
         if (p0 + kBlock - 1 > pos_hi || (p0 < seen_lo && p0 + kBlock > a.sinks)) {
             // Positions that no row sees may hold anything: zeros.
@@ -1268,36 +1285,39 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
             }
         }
         const float vs = two_to(min(max(e_v - v_exp, -126), 127));
-        const f16x8 pp = __builtin_bit_cast(f16x8, u32x4{p[0], p[1], p[2], p[3]});
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            o[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(vr[u].x, vr[u].y, vs), pp, o[u], 0, 0, 0);
+        for (int u = 0; u < U; ++u) {
+            const f16x8 x = codes_f16(vr[u].x, vr[u].y, vs);
+#pragma unroll
+            for (int j = 0; j < P; ++j)
+                o[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(f16x8, u32x4{p[j][0], p[j][1], p[j][2], p[j][3]}),
+                                                              o[u], 0, 0, 0);
+        }
         if (i + 1 < mine) load_v(at_next);
         __builtin_amdgcn_sched_barrier(0);
     }
     // The waves' parts meet in LDS.
     l = over_quads(l, [](float x, float y) { return x + y; });
-    float *so = (float *)smem + (size_t)(wave * kFewRows + r) * kRowPad<HD> + 4 * quad;
+    float *so = (float *)smem + (size_t)(wave * R + r) * kRowPad<HD> + 4 * quad;
 #pragma unroll
-    for (int u = 0; u < U; u += 2) {  // (a row's two columns take turns to write)
-        f32x4 v[2];
+    for (int u = 0; u < U; u += 3 - P) {  // (a row's two columns take turns to write)
+        f32x4 v[3 - P];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            v[0][k] = o[u][k] + dpp_mov<0x128>(o[u][k]);
-            v[1][k] = o[u + 1][k] + dpp_mov<0x128>(o[u + 1][k]);
-        }
-        if (r < M) *(f32x4 *)(so + 16 * (u + n / kFewRows)) = n < kFewRows ? v[0] : v[1];
+        for (int i = 0; i < 3 - P; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i][k] = whole_row(o[u + i][k]);
+        if (r < rows) *(f32x4 *)(so + 16 * (u + n / R)) = n < R ? v[0] : v[2 - P];
     }
-    if (lane < kFewRows) words[wave * kFewRows + r] = f32x4{m2, l, two_to(v_exp), 0.f};
+    if (lane < R) words[wave * R + r] = f32x4{m2, l, two_to(v_exp), 0.f};
     __syncthreads();
-    for (int u = (int)threadIdx.x; u < M * (HD / 4); u += 64 * W) {  // 4 dims of a row
-        const int rr = u / (HD / 4), d = u % (HD / 4) * 4, at = over_g(rr);
-        const size_t item = (size_t)at * a.q_heads + g * G + (rr - at * G);
+    for (int u = (int)threadIdx.x; u < rows * (HD / 4); u += 64 * W) {  // 4 dims of a row
+        const int rr = u / (HD / 4), d = u % (HD / 4) * 4, at = over_g(m0 + rr);
+        const size_t item = (size_t)at * a.q_heads + g * G + (m0 + rr - at * G);
         float f[W], v[4] = {0.f, 0.f, 0.f, 0.f};
-        const float inv = wave_factors(words + rr, kFewRows, f, S == 1, S > 1 && d == 0 ? a.ml + item * S + split : nullptr);
+        const float inv = wave_factors(words + rr, R, f, S == 1, S > 1 && d == 0 ? a.ml + item * S + split : nullptr);
 #pragma unroll
         for (int k = 0; k < W; ++k) {
-            const f32x4 x = *(const f32x4 *)((const float *)smem + (size_t)(k * kFewRows + rr) * kRowPad<HD> + d);
+            const f32x4 x = *(const f32x4 *)((const float *)smem + (size_t)(k * R + rr) * kRowPad<HD> + d);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = fmaf(f[k], x[e], v[e]);
         }
@@ -1313,7 +1333,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
     }
     if (S > 1) return;
     __syncthreads();
-    if (wave < M && (uniform(*odd) >> wave & 1)) plain_row<HD>(kernel_args(), over_g(wave), g * G + (wave - over_g(wave) * G));
+    for (int rr = wave; rr < rows; rr += W)
+        if (uniform(*odd) >> rr & 1)
+            plain_row<HD>(kernel_args(), over_g(m0 + rr), g * G + (m0 + rr - over_g(m0 + rr) * G));
 }
 
 // The splits of a row and head, joined by W waves (each takes every W-th); the
@@ -1392,17 +1414,19 @@ int launch_attn_blocks(const Kv8AttnArgs &a, int S, hipStream_t s) {
     return 0;
 }
 
-template <int HD>
+template <int HD, int R>
 int launch_few(const Kv8AttnArgs &a, int S, hipStream_t s) {
-    const unsigned blocks = (unsigned)((S * a.g.kv_heads + 7) / 8 * 8);
-    hipLaunchKernelGGL((kv8_few_kernel<HD>), dim3(blocks), dim3(64 * kFewWaves), kFewLds<HD>, s, a, S);
+    const long M = (long)a.rows * (a.q_heads / a.g.kv_heads);
+    const long blocks = ((M + R - 1) / R * S * a.g.kv_heads + 7) / 8 * 8;
+    hipLaunchKernelGGL((kv8_few_kernel<HD, R>), dim3((unsigned)blocks), dim3(64 * kFewWaves), (kFewLds<HD, R>), s, a, S);
     CHIP_CHECK(hipGetLastError());
     return 0;
 }
 
 template <int HD>
 int launch_attn(const Kv8AttnArgs &a, int wr, int S, hipStream_t s) {
-    if (wr == 0) CHIP_TRY((launch_few<HD>(a, S, s)));
+    if (wr == kFew8) CHIP_TRY((launch_few<HD, 8>(a, S, s)));
+    else if (wr == kFew16) CHIP_TRY((launch_few<HD, 16>(a, S, s)));
     else if (wr == 1) CHIP_TRY((launch_attn_blocks<HD, 1>(a, S, s)));
     else if (wr == 2) CHIP_TRY((launch_attn_blocks<HD, 2>(a, S, s)));
     else CHIP_TRY((launch_attn_blocks<HD, 4>(a, S, s)));
@@ -1477,15 +1501,15 @@ int launch_kv8_read(const Kv8Cache &kv, size_t begin, size_t n, bool f32, void *
     return 0;
 }
 
-// How a call is cut: row waves of a block (the other waves of eight split its keys
-// in LDS) and splits of the keys (a block each, joined by a merge kernel). The
-// cheapest by an estimate, in us: 1.85 (half that at head_dim 64) for a wave's block
-// of positions at two waves a SIMD, 6 for the start and the end of a round of
-// blocks, 4.5 TB/s for a merge's partials and 3 for its launch. Blocks of one row
-// wave read K and V from the caches for every 32 rows, four row waves for 128:
-// ties go to more. At most 8 M rows: kv8_few_kernel (row waves 0), 0.95 (0.7) a step and
-// 2.4 for a merge (one token on 767, 32 / 8 heads of 128, three steps: 7.0 us, with
-// splits 7.6; on 2,047, eight steps: 11.8, with splits 7.8).
+// How a call is cut: rows a block (its waves split its keys in LDS) and splits of the
+// keys (a block each, joined by a merge kernel). The cheapest by an estimate, in us:
+// for a round of blocks, one a CU, its start and end and a step a block of positions
+// of a wave; for splits a merge's launch and 4.5 TB/s for its partials. kv8_attn_kernel
+// with one row wave reads K and V from the caches for every 32 rows, with four for
+// 128: ties go to more. Rows of 32 / 8 heads of 128, 16-row blocks against its own:
+// 64 on nothing 6.0 us, 12.2; 13 on 1,023 9.6, 10.6; 20 on 4,095 11.7, 15.4; 64 on
+// 16,383 45.4, 42.5; 180 on 1,023 18.8, 14.4. 8-row blocks with and without splits: 1 on
+// 767 7.6, 7.0; 1 on 2,047 7.8, 11.8.
 struct Cut {
     int wr, splits;
 };
@@ -1495,30 +1519,26 @@ static Cut cut_of(const Kv8AttnJob &j) {
     const int last = (int)(j.offset + j.rows - 1);
     Cut best{1, 1};
     double least = 0;
-    if (M <= (size_t)kFewRows) {
-        const size_t reach = (size_t)reach_of((int)j.offset, last, (int)j.window, (int)j.sinks).count;
-        const size_t most = std::max<size_t>(1, std::min<size_t>(kMaxSplits, std::min((reach + kFewWaves - 1) / kFewWaves, cus / kvh)));
-        for (size_t S = 1; S <= most; S = S < most && S * 2 > most ? most : S * 2) {
-            const double steps = (double)((reach + S * kFewWaves - 1) / (S * kFewWaves));
-            double us = steps * (hd == 64 ? 0.7 : 0.95);
-            if (S > 1) us += 2.4 + 2.0 * (double)(j.rows * j.q_heads * S * hd * 4) / 4.5e6;
-            if (least == 0 || us < least) least = us, best = Cut{0, (int)S};
-        }
-        return best;
-    }
-    for (int wr = 4; wr >= 1; wr /= 2) {
-        if (wr > 1 && tiles <= (size_t)wr / 2) continue;  // row waves without rows
-        const size_t wk = kWaves / wr, blocks = (tiles + wr - 1) / wr * kvh;
-        const int first = std::max(last + 1 - (int)std::min<size_t>(j.rows, (32 * wr + G - 1) / G + 1), 0);
+    auto consider = [&](int kind, size_t rows, size_t wk, double base, double step, double merge) {
+        const size_t blocks = (M + rows - 1) / rows * kvh;
+        const int first = std::max(last + 1 - (int)std::min<size_t>(j.rows, (rows + G - 1) / G + 1), 0);
         const size_t reach = (size_t)reach_of(first, last, (int)j.window, (int)j.sinks).count;
         const size_t most = std::max<size_t>(1, std::min<size_t>(kMaxSplits, std::min((reach + wk - 1) / wk, cus / blocks)));
         for (size_t S = 1; S <= most; S = S < most && S * 2 > most ? most : S * 2) {
             const double rounds = (double)((blocks * S + cus - 1) / cus), steps = (double)((reach + S * wk - 1) / (S * wk));
-            double us = rounds * (6 + steps * (hd == 64 ? 0.95 : 1.85));
-            if (S > 1) us += 3 + 2.0 * (double)(j.rows * j.q_heads * S * hd * 4) / 4.5e6;
-            if (least == 0 || us < least) least = us, best = Cut{wr, (int)S};
+            double us = rounds * (base + steps * step);
+            if (S > 1) us += merge + 2.0 * (double)(j.rows * j.q_heads * S * hd * 4) / 4.5e6;
+            if (least == 0 || us < least) least = us, best = Cut{kind, (int)S};
         }
+    };
+    if (M <= 8) {
+        consider(kFew8, 8, kFewWaves, 4.2, hd == 64 ? 0.7 : 0.95, 2.4);
+        return best;
     }
+    for (int wr = 4; wr >= 1; wr /= 2)
+        if (wr == 1 || tiles > (size_t)wr / 2)  // (else row waves without rows)
+            consider(wr, 32 * wr, kWaves / wr, 5.5, hd == 64 ? 0.9 : 1.7, 3);
+    consider(kFew16, 16, kFewWaves, hd == 64 ? 3.8 : 4.7, hd == 64 ? 0.72 : 1, 3.1);
     return best;
 }
 
@@ -1534,8 +1554,9 @@ size_t kv8_attention_part_most(int head_dim) { return (size_t)std::max(device_cu
 
 template <int HD>
 static int prepare() {
-    static std::atomic<uint64_t> set[4];
-    CHIP_TRY(allow_dynamic_lds((const void *)kv8_few_kernel<HD>, kFewLds<HD>, set[3]));
+    static std::atomic<uint64_t> set[5];
+    CHIP_TRY(allow_dynamic_lds((const void *)kv8_few_kernel<HD, 8>, kFewLds<HD, 8>, set[3]));
+    CHIP_TRY(allow_dynamic_lds((const void *)kv8_few_kernel<HD, 16>, kFewLds<HD, 16>, set[4]));
     CHIP_TRY(allow_dynamic_lds((const void *)kv8_attn_kernel<HD, 1>, kv8_attn_lds_bytes<HD, 1>(), set[0]));
     CHIP_TRY(allow_dynamic_lds((const void *)kv8_attn_kernel<HD, 2>, kv8_attn_lds_bytes<HD, 2>(), set[1]));
     return allow_dynamic_lds((const void *)kv8_attn_kernel<HD, 4>, kv8_attn_lds_bytes<HD, 4>(), set[2]);
