@@ -245,7 +245,7 @@ def test_a_wave_with_more_blocks_than_lanes(hip):
         dev.append(np.tile(k[at:at + 3300], kvh), np.tile(v[at:at + 3300], kvh), at)
         cpu.append(*(synth.bf16_to_f32(x[at:at + 3300]) for x in (k, v)), at)
     k, v = (x[:, 0] for x in cpu.values(0, n))
-    for rows, window in [(1, 0), (8, 0), (9, 0), (40, 0), (100, 0), (3, 16450)]:
+    for rows, window in [(1, 0), (8, 0), (9, 0), (30, 0), (40, 0), (100, 0), (3, 16450)]:
         q = rng.standard_normal((rows, kvh * hd)).astype(np.float32)
         got = dev.attention(q, kvh, n - rows, window)
         for i in {0, rows // 3, rows // 2, rows - 1}:
