@@ -369,7 +369,7 @@ struct Kv8AttnArgs {
     uint32_t over_group;  // ceil(2^32 / G) for G > 1 query heads per KV head
     float *out;
     float *part;  // [row][head][split][HD]: weighted sums
-    float2 *ml;   // [row][head][split]: maximum (log2 units), weight sum
+    float2 *ml;   // [row][head][split]: reference (log2 units), weight sum
     const int32_t *pos_dev;     // offset's word on the device (null: offset)
     uint16_t *out_hi, *out_lo;  // BF16 halves of out (null: not written); out may then be null
 };
@@ -510,22 +510,26 @@ __host__ __device__ __forceinline__ Reach reach_of(int pos_lo, int pos_hi, int w
 //                   32 u + n; B = the probabilities: with that kpos lane (m, h)
 //                   holds those of its row at positions 16 h .. + 15, where the
 //                   first product leaves them.
-// Codes are exact F16 numbers. Queries (by a power of two of their own a row, so
-// that they fill F16's range) and probabilities are two F16 parts, 22 bits. A
-// K scale multiplies the scores, a V scale comes with the conversion, relative
+// Codes are exact F16 numbers. Queries are two F16 parts, 22 bits of a row's largest
+// (a power of two of each row's own fills F16's range). Probabilities are two parts as
+// well; a long tail behind one large weight (a sink, whose value may be 0) is made of
+// weights far below F16's normal numbers, so the low part carries 2^11 and meets V times
+// 2^-11: 22 bits for a weight of 2^-21 of the largest that a wave has seen and more, for
+// smaller ones 2^-44 of it. (Low parts without a factor lose weights below 2^-25: 3 % of
+// the time of 512 rows on 4,096, 73.5 against 75.9 us, for outputs 1e-4 off.) A K scale
+// multiplies the scores, a V scale comes with the conversion, relative
 // to one that the running sums carry (a power of two, changed without rounding).
 //
 // Blocks of 8 waves, one a CU: WR of them hold 32 M rows each, the other 8 / WR - 1
 // times as many take other blocks of positions (so that a short call fills its CUs
-// without a second launch); two waves a SIMD of 230 to 250 registers. One row wave:
+// without a second launch); two waves a SIMD of 220 to 256 registers. One row wave:
 // K and V go from memory into registers, no wave waits for another. More: direct
 // copies fill three tiles of LDS, a barrier a tile. (Few rows have a kernel of their
 // own, kv8_few_kernel.)
 //
 // Bound: with many rows the matrix cores, at the rate that a large F16 product of
-// the library reaches (512 rows on 4,096, 32 / 8 heads of 128: 73.1 us, of which the
-// loop is 60 at 1.16 PFLOP/s of the two part products; queries in and outputs out
-// take the rest); with few round trips.
+// the library reaches (512 rows on 4,096, 32 / 8 heads of 128: 75.9 us, of which
+// queries in and outputs out take 12); with few round trips.
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -558,6 +562,36 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32
     lo = __builtin_bit_cast(uint32_t, f16x2{(_Float16)(a - ha), (_Float16)(b - hb)});
 }
 
+// Two weights' F16 parts: the first 11 bits of each, and the rest times 2^11, which
+// meets V times 2^-11 (kLow): a weight below F16's normal numbers keeps its bits
+// down to 2^-35. Rounded once, by at most 2^-36 or 2^-23 of it.
+constexpr float kLowUp = 0x1p11f;
+constexpr _Float16 kLow = (_Float16)0x1p-11f;
+__device__ __forceinline__ void split_weights(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, f16x2{(_Float16)fmaf((float)h[0], -kLowUp, a * kLowUp),
+                                            (_Float16)fmaf((float)h[1], -kLowUp, b * kLowUp)});
+}
+// Weights are taken against a reference kLift powers of two below the largest score,
+// raised when a score passes it by more than kLift + kRaise: 2^14 at most (F16 ends
+// at 2^16), 2^8 at least for the largest key of a wave. (Of a key 2^-25 of it 2^-17 is
+// left, 18 bits.) The factor is in weights and sums alike and drops out in the quotient.
+constexpr float kLift = 8.0f, kRaise = 6.0f;
+
+// A block's weights, added up, onto the sum of all: compensated, so that a long tail
+// behind one large weight is not lost to it (N weights of 2^-26 of it are N 2^-26 of
+// the sum, each below its last bit). Four instructions a block.
+struct WeightSum {
+    float sum = 0.f, over = 0.f;  // the true sum is sum - over
+    __device__ __forceinline__ void add(float x) {
+        const float y = x - over, t = sum + y;
+        over = (t - sum) - y;
+        sum = t;
+    }
+    __device__ __forceinline__ void scale(float f) { sum *= f, over *= f; }
+};
+
 // Which of the positions base .. base + 15 lie at or below `last` and at or above
 // `first` or below `sinks`, a bit each.
 __device__ __forceinline__ uint32_t seen_bits(int base, int last, int first, int sinks) {
@@ -566,7 +600,7 @@ __device__ __forceinline__ uint32_t seen_bits(int base, int last, int first, int
 }
 
 // The factors of a row's waves in the sum of their outputs, from words of each
-// (maximum, weight sum, unit), `stride` apart; returned: what the sum is multiplied
+// (reference, weight sum, unit), `stride` apart; returned: what the sum is multiplied
 // with, 1 / (weight sum), or with `ml` (a split's word) 1. A wave that saw nothing
 // counts nothing; a NaN sum shows. (The quotient comes last: with the least unit a
 // factor divided by a large sum would be no normal number.)
@@ -597,7 +631,7 @@ template <int HD>
 constexpr int kQRow = HD * 4 + 16;     // bytes of a query row's parts in LDS: high, low, padding
 // A block's LDS: tiles, then the waves' sums in their place; query rows on their way
 // to the operands (of one row wave behind the sums, else in the third tile's place
-// and behind it); a word of each wave and row (maximum, weight sum, the sums' unit);
+// and behind it); a word of each wave and row (reference, weight sum, the sums' unit);
 // the query rows' exponents; rows to compute again.
 template <int HD, int WR>
 constexpr size_t kQueriesAt = WR == 1 ? kWaves * 32 * kRowPad<HD> * 4 : kStage / 3 * 2;
@@ -754,7 +788,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     f32x16 o[C];
 #pragma unroll
     for (int u = 0; u < C; ++u) o[u] = f32x16{};
-    float m2 = -INFINITY, l = 0.f;
+    float m2 = -INFINITY;
+    WeightSum l;
     int v_exp = 0;  // o is in units of 2^v_exp
     uint32_t now_k = held_k, now_v = held_v, next_k = 0, next_v = 0;  // (the next ones are looked up a tile ahead)
     auto lds_at = [&](int i) { return smem + (i % (3 * NB) * WK + wk) * 2 * BB + 16 * lane; };
@@ -799,14 +834,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     auto scale_of = [&](int i) {  // of block i's scores
         return ldexpf(1.f, max(q_exp + (int)__builtin_amdgcn_readlane(now_k, i & 63) - 127, -126));
     };
-    // Exponentials against a maximum that is raised when a score exceeds it by more
-    // than 8 (so p <= 2^8); the running sums are rescaled only then.
+    // The running sums are rescaled only where the reference is raised.
     auto raise_to = [&](float tmax) {
-        const bool raise = tmax > m2 + 8.0f;
+        const bool raise = tmax > m2 + (kLift + kRaise);
         if (__any(raise)) {
-            const float mnew = raise ? tmax : m2;
+            const float mnew = raise ? tmax - kLift : m2;
             const float alpha = raise ? __builtin_amdgcn_exp2f(m2 - mnew) : 1.f;
-            l *= alpha;
+            l.scale(alpha);
 #pragma unroll
             for (int u = 0; u < C; ++u)
 #pragma unroll
@@ -817,12 +851,12 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     f32x16 s;
     float fs = 0.f;
     auto reference = [&]() { return m2 == -INFINITY ? 0.f : m2; };
-    // V under 2^(e_v - v_exp): exact in F16 for differences of -15 .. 7. The factor of
-    // block i's codes.
+    // V under 2^(e_v - v_exp): exact in F16, times 2^-11 too, for differences of -4 .. 7.
+    // The factor of block i's codes.
     auto value_scale = [&](int i) {
         const int e_v = (int)__builtin_amdgcn_readlane(now_v, i & 63) - 127;
         if (i == 0) v_exp = e_v;
-        if (e_v - v_exp > 7 || e_v - v_exp < -15) {
+        if (e_v - v_exp > 7 || e_v - v_exp < -4) {
             // Steps that could lose the sums' values: the rows are computed again. (A block
             // of zeros, whose scale is the least, and sums that are 0 lose nothing.)
             if (abs(e_v - v_exp) > 100) {
@@ -835,7 +869,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                     for (int r = 0; r < 16; ++r) sums |= __float_as_uint(o[u][r]);
                 }
                 if (!__any(codes & 0x7F7F7F7Fu)) return 1.f;
-                if (__any(sums << 1)) l = NAN;
+                if (__any(sums << 1)) l.sum = NAN;
             }
 #pragma unroll
             for (int u = 0; u < C; ++u)
@@ -861,11 +895,13 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     // Probability r - 1 of a block from its score's exponential, in two F16 parts (a
     // pair at a time), and the exponential of score r, so that none is waited for.
     uint32_t ph[8], pl[8];
-    auto exponential = [&](int r, float mref) {
+    float block_sum = 0.f;
+    auto exponential = [&](int r, float mref, f32x16 &s) {
         if (r < 16) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], fs, -mref));
-        if (r > 0) l += s[r - 1];
+        if (r > 0) block_sum = r == 1 ? s[0] : block_sum + s[r - 1];
+        if (r == 16) l.add(block_sum);
         if (r > 0 && r % 2 == 0) {
-            split_f16(s[r - 2], s[r - 1], ph[r / 2 - 1], pl[r / 2 - 1]);
+            split_weights(s[r - 2], s[r - 1], ph[r / 2 - 1], pl[r / 2 - 1]);
         }
     };
     auto part = [&](const uint32_t (&p)[8], int k) {
@@ -886,16 +922,16 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             raise_to(largest(s) * fs);
             const float mref = reference();
 #pragma unroll
-            for (int r = 0; r <= 16; ++r) exponential(r, mref);
+            for (int r = 0; r <= 16; ++r) exponential(r, mref, s);
             clear_v(i);
             const float vs = value_scale(i);
 #pragma unroll
             for (int u = 0; u < C; ++u) {
                 const f16x8 v0 = codes_f16(vr[u][0], vr[u][1], vs), v1 = codes_f16(vr[u][2], vr[u][3], vs);
                 o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, part(ph, 0), o[u], 0, 0, 0);
-                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, part(pl, 0), o[u], 0, 0, 0);
                 o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, part(ph, 1), o[u], 0, 0, 0);
-                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, part(pl, 1), o[u], 0, 0, 0);
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0 * kLow, part(pl, 0), o[u], 0, 0, 0);
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1 * kLow, part(pl, 1), o[u], 0, 0, 0);
             }
             if (i + 1 < mine) load_v(at_next);
             __builtin_amdgcn_sched_barrier(0);
@@ -905,7 +941,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
         // scores, and the next maxima between its own V products: a wave's vector
         // instructions run while its matrix instructions do, and two waves of a SIMD that
         // do the same thing at the same time do not overlap. K and V are read from LDS
-        // one phase before their use.
+        // one phase before their use. Two steps a turn, so that scores change places
+        // without moves (512 rows on 4,096 77.1 -> 75.9 us).
         // The first tile has landed (copies end in order; one block a tile: the second too).
         constexpr int LATER = NB == 1 ? 0 : NB * PIECES;
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(LATER) : "memory");
@@ -919,8 +956,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             if (mine > 1) read_k(1);
         }
         constexpr int E = 4 / C;  // exponentials for a product
-        for (int i = 0; i < steps; ++i) {
-            f32x16 t = f32x16{};
+        auto step = [&](int i, f32x16 &s, f32x16 &t) {
+            t = f32x16{};
             float vs = 0.f;
             if (i < mine) {
                 read_v(i);
@@ -939,11 +976,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                         __builtin_amdgcn_sched_barrier(0);
                         if (c + 1 < C) k4[q] = codes_f16x4(kr[c + 1][q], 1.f);
 #pragma unroll
-                        for (int x = 0; x < E; ++x) exponential((4 * c + q) * E + x, mref);
+                        for (int x = 0; x < E; ++x) exponential((4 * c + q) * E + x, mref, s);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-                exponential(16, mref);
+                exponential(16, mref, s);
             }
             // The tile of block i + 2: it has landed, and V of block i and all before is read
             // by all; the tile after it takes the place of the one before the last.
@@ -953,7 +990,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 for (int j = ahead; j < min(ahead + NB, mine); ++j) copy(at_of(j), j);
             }
-            if (i >= mine) continue;
+            if (i >= mine) return;
             if (i + 2 < mine) read_k(i + 2);
             clear_v(i);
             vs = value_scale(i);
@@ -964,12 +1001,12 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             for (int q = 0; q < 4; ++q) v4[q] = codes_f16x4(vr[0][q], vs);
 #pragma unroll
             for (int u = 0; u < C; ++u) {
-                const f16x8 v0 = operand(v4[0], v4[1]), v1 = operand(v4[2], v4[3]);
+                f16x8 v[2] = {operand(v4[0], v4[1]), operand(v4[2], v4[3])};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q < 2 ? v0 : v1, q & 1 ? part(pl, q / 2) : part(ph, q / 2), o[u], 0, 0,
-                                                                  0);
+                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[q & 1], q < 2 ? part(ph, q) : part(pl, q - 2), o[u], 0, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
+                    if (q < 2) v[q] *= kLow;
                     if (u + 1 < C) v4[q] = codes_f16x4(vr[u + 1][q], vs);
 #pragma unroll
                     for (int x = 0; x < E; ++x) tmax = fmaxf(tmax, t[(4 * u + q) * E + x]);
@@ -981,12 +1018,16 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
                 fs = scale_of(i + 1);
                 raise_to(max_halves(tmax) * fs);
             }
-            s = t;
+        };
+        f32x16 t;
+        for (int i = 0; i < steps; i += 2) {
+            step(i, s, t);
+            if (i + 1 < steps) step(i + 1, t, s);
         }
     }
     // The key waves' parts meet in LDS. (In the tiles' place: their last reads are
     // done, and copies that nothing reads.)
-    l += __shfl_xor(l, 32, 64);
+    l.sum += __shfl_xor(l.sum, 32, 64);
     if constexpr (!DIRECT) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -1000,7 +1041,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             for (int q = 0; q < 4; ++q)
                 *(f32x4 *)(so + 32 * u + 8 * q + 4 * half) =
                     f32x4{o[u][4 * q], o[u][4 * q + 1], o[u][4 * q + 2], o[u][4 * q + 3]};
-        if (half == 0) words[wave * 32 + n] = f32x4{m2, l, two_to(v_exp), 0.f};
+        if (half == 0) words[wave * 32 + n] = f32x4{m2, l.sum, two_to(v_exp), 0.f};
     }
     if (threadIdx.x < WR) odd[threadIdx.x] = 0;
     __syncthreads();
@@ -1199,7 +1240,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
     f32x4 o[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m2 = -INFINITY, l = 0.f;
+    float m2 = -INFINITY;
+    WeightSum l;
     int v_exp = 0;  // o is in units of 2^v_exp
     uint32_t now_k = held_k, now_v = held_v;
     for (int i = 0; i < mine; ++i) {
@@ -1235,26 +1277,28 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
 #pragma unroll
         for (int k = 1; k < 8; ++k) tmax = fmaxf(tmax, s[k]);
         tmax = over_quads(tmax, [](float x, float y) { return fmaxf(x, y); }) * fs;
-        if (__any(tmax > m2 + 8.0f)) {  // (as kv8_attn_kernel's: p <= 2^8)
-            const bool raise = tmax > m2 + 8.0f;
-            const float mnew = raise ? tmax : m2, alpha = raise ? __builtin_amdgcn_exp2f(m2 - mnew) : 1.f;
-            l *= alpha;
+        if (__any(tmax > m2 + (kLift + kRaise))) {
+            const bool raise = tmax > m2 + (kLift + kRaise);
+            const float mnew = raise ? tmax - kLift : m2, alpha = raise ? __builtin_amdgcn_exp2f(m2 - mnew) : 1.f;
+            l.scale(alpha);
 #pragma unroll
             for (int u = 0; u < U; ++u) o[u] *= alpha;
             m2 = mnew;
         }
         const float mref = m2 == -INFINITY ? 0.f : m2;
         uint32_t p[P][4];
+        float block_sum = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float x = __builtin_amdgcn_exp2f(fmaf(s[2 * k], fs, -mref)), y = __builtin_amdgcn_exp2f(fmaf(s[2 * k + 1], fs, -mref));
-            l += x;
-            l += y;
+            block_sum += x;
+            block_sum += y;
             uint32_t hi, lw;
-            split_f16(x, y, hi, lw);
+            split_weights(x, y, hi, lw);
             p[0][k] = n < R ? hi : lw;
             if constexpr (P == 2) p[1][k] = lw;
         }
+        l.add(block_sum);
         if (p0 + kBlock - 1 > pos_hi || (p0 < seen_lo && p0 + kBlock > a.sinks)) {
             // Positions that no row sees may hold anything: zeros.
             const uint32_t bits = seen_bits(p0 + 8 * quad, pos_hi, seen_lo, a.sinks);
@@ -1262,10 +1306,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
 #pragma unroll
             for (int u = 0; u < U; ++u) vr[u].x &= b0, vr[u].y &= b1;
         }
-        // V under 2^(e_v - v_exp): exact in F16 for differences of -15 .. 7.
+        // V under 2^(e_v - v_exp): exact in F16 for differences of -15 .. 7, of -4 .. 7
+        // where the low parts meet it times 2^-11 (of 8 rows their columns carry that).
         const int e_v = (int)__builtin_amdgcn_readlane(now_v, i & 63) - 127;
         if (i == 0) v_exp = e_v;
-        if (e_v - v_exp > 7 || e_v - v_exp < -15) {
+        if (e_v - v_exp > 7 || e_v - v_exp < (P == 1 ? -15 : -4)) {
             uint32_t codes = 0, sums = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -1276,7 +1321,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
             // Far steps could lose the sums' values: the rows are computed again; a block
             // of zeros takes any scale.
             if (__any(codes & 0x7F7F7F7Fu)) {
-                if (abs(e_v - v_exp) > 100 && __any(sums << 1)) l = NAN;
+                if (abs(e_v - v_exp) > 100 && __any(sums << 1)) l.sum = NAN;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -1290,25 +1335,26 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
             const f16x8 x = codes_f16(vr[u].x, vr[u].y, vs);
 #pragma unroll
             for (int j = 0; j < P; ++j)
-                o[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(f16x8, u32x4{p[j][0], p[j][1], p[j][2], p[j][3]}),
-                                                              o[u], 0, 0, 0);
+                o[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    j == 0 ? x : x * kLow, __builtin_bit_cast(f16x8, u32x4{p[j][0], p[j][1], p[j][2], p[j][3]}), o[u], 0, 0, 0);
         }
         if (i + 1 < mine) load_v(at_next);
         __builtin_amdgcn_sched_barrier(0);
     }
     // The waves' parts meet in LDS.
-    l = over_quads(l, [](float x, float y) { return x + y; });
+    l.sum = over_quads(l.sum, [](float x, float y) { return x + y; });
     float *so = (float *)smem + (size_t)(wave * R + r) * kRowPad<HD> + 4 * quad;
+    const float column = n < R ? 1.f : 1.f / kLowUp;  // a low part's
 #pragma unroll
     for (int u = 0; u < U; u += 3 - P) {  // (a row's two columns take turns to write)
         f32x4 v[3 - P];
 #pragma unroll
         for (int i = 0; i < 3 - P; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[i][k] = whole_row(o[u + i][k]);
+            for (int k = 0; k < 4; ++k) v[i][k] = whole_row(o[u + i][k] * column);
         if (r < rows) *(f32x4 *)(so + 16 * (u + n / R)) = n < R ? v[0] : v[2 - P];
     }
-    if (lane < R) words[wave * R + r] = f32x4{m2, l, two_to(v_exp), 0.f};
+    if (lane < R) words[wave * R + r] = f32x4{m2, l.sum, two_to(v_exp), 0.f};
     __syncthreads();
     for (int u = (int)threadIdx.x; u < rows * (HD / 4); u += 64 * W) {  // 4 dims of a row
         const int rr = u / (HD / 4), d = u % (HD / 4) * 4, at = over_g(m0 + rr);

@@ -1,0 +1,85 @@
+"""Attention over an 8-bit cache where weights differ by many powers of two: one key
+far above a long tail (an attention sink), large values behind small weights. Each
+row and head is measured by its own largest output."""
+import numpy as np
+import pytest
+
+import kv8_reference as ref
+from test_gpu_kv8 import TOL, make
+
+pytestmark = pytest.mark.gpu
+
+# (q heads, KV heads, head dim, rows, offset, window, sinks): a token over short and
+# long contexts and a window, blocks of 16 rows, chunks whose keys are split and not.
+CALLS = [(4, 1, 128, 1, 3000, 0, 0), (14, 2, 64, 1, 575, 0, 0), (28, 4, 128, 1, 31999, 0, 0),
+         (32, 8, 128, 1, 5999, 2048, 4), (32, 8, 128, 13, 1999, 0, 0), (5, 1, 64, 3, 1200, 0, 0),
+         (14, 2, 64, 333, 0, 0, 0), (32, 8, 128, 512, 4096, 0, 0), (28, 4, 128, 1000, 1088, 1024, 16),
+         (28, 4, 128, 300, 16000, 0, 0), (8, 8, 64, 700, 3000, 0, 0)]
+
+
+@pytest.fixture(scope="module")
+def hip():
+    from cheetah_amd import hip as h
+    h.init(0)
+    return h
+
+
+def filled(hip, rng, call, k, v):
+    _, kvh, hd, rows, offset, *_ = call
+    n = offset + rows
+    dev, cpu = make(hip, rng, n, kvh, hd), ref.Cache(n, kvh, hd)
+    dev.append(k.reshape(n, -1), v.reshape(n, -1), 0)
+    cpu.append(k, v, 0)
+    return dev, cpu.values(0, n)
+
+
+def check(call, dev, held, q, what=""):
+    """Some rows of the call against 64 bits over what the cache holds."""
+    q_heads, _, hd, rows, offset, window, sinks = call
+    got = dev.attention(q.reshape(rows, -1), q_heads, offset, window, sinks).reshape(rows, q_heads, hd)
+    for i in sorted({0, rows // 7, rows // 2, 2 * rows // 3, rows - 2, rows - 1} & set(range(rows))):
+        want = ref.attention64(q[i].reshape(1, -1), *held, q_heads, offset + i, window, sinks).reshape(q_heads, hd)
+        off, most = np.abs(got[i] - want).max(1), np.abs(want).max(1)
+        assert (off <= TOL * most).all(), (what, i, off, most)
+
+
+@pytest.mark.parametrize("value", [0.0, 0.02])
+@pytest.mark.parametrize("call", CALLS)
+def test_one_key_far_above_a_long_tail(hip, call, value):
+    """The first position scores `gap` powers of two above the others, whose scores
+    are equal or nearly so, and its value is small or zero: the output is the tail's.
+    TOL holds: 22 bits of the query put up to 26 * 2^-22 = 6.2e-6 between the key and
+    the tail, exponents of up to 26 in f32 2^-20 = 1e-6, a tail's weight of at least
+    2^-18 in the wave of the key rounds by 2^-36, 4e-6 of it: 1.2e-5."""
+    q_heads, kvh, hd, rows, offset, *_ = call
+    rng = np.random.default_rng(rows + hd)
+    n = offset + rows
+    k, v = (rng.standard_normal((n, kvh, hd)).astype(np.float32) for _ in "kv")
+    k[..., 0] = 0
+    k[0] = 0
+    k[0, :, 0] = 16
+    v[0] *= np.float32(value)
+    dev, held = filled(hip, rng, call, k, v)
+    for gap in (8, 13, 18, 26):
+        for spread in (0, 0.3):
+            q = (spread * rng.standard_normal((rows, q_heads, hd))).astype(np.float32)
+            q[..., 0] = gap * np.log(2) * np.sqrt(hd) / 16
+            check(call, dev, held, q, (gap, spread))
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_large_values_behind_small_weights(hip, call):
+    """Every fourth block scores 25 powers of two below the others and holds values
+    2^18 times theirs: some 2^-8 of the outputs is theirs (weights of 2^-17 that round
+    by 2^-36: 2^-19 of that)."""
+    q_heads, kvh, hd, rows, offset, *_ = call
+    rng = np.random.default_rng(rows + hd)
+    n = offset + rows
+    k, v = (rng.standard_normal((n, kvh, hd)).astype(np.float32) for _ in "kv")
+    far = np.arange(n) // 32 % 4 == 1
+    k[..., 0] = 0
+    k[far, :, 0] = -16
+    v[far] *= 2.0 ** 18
+    q = (0.3 * rng.standard_normal((rows, q_heads, hd))).astype(np.float32)
+    q[..., 0] = 25 * np.log(2) * np.sqrt(hd) / 16
+    check(call, *filled(hip, rng, call, k, v), q)
