@@ -592,6 +592,33 @@ struct WeightSum {
     __device__ __forceinline__ void scale(float f) { sum *= f, over *= f; }
 };
 
+// A wave's output sums are in units of 2^e; V's codes meet them under 2^(e_v - e), which
+// is exact in F16 for differences of -down .. 7. Past these the sums move to the block's
+// unit, a power of two away, without rounding. Where units have come to lie more than
+// 2^kFar apart, the rows are computed again (a NaN weight sum): weights are right to
+// 2^-44 of the largest alone, which is not enough for a value 2^44 times as large, and
+// sums could end behind the type's range, in one step or in several. A block of zeros
+// takes any unit, and sums that are 0 have none.
+constexpr int kFar = 20;
+struct ValueUnit {
+    int e = 0, least = 0, most = 0;
+    // The factor of a block's codes; `codes` and `sums` return the bits of all that a lane
+    // holds of either, `move` multiplies the sums by 2^n.
+    template <class Codes, class Sums, class Move>
+    __device__ __forceinline__ float factor(int e_v, bool first, int down, WeightSum &l, Codes codes, Sums sums, Move move) {
+        if (first) e = least = most = e_v;
+        if (e_v - e > 7 || e_v - e < -down) {
+            if (!__any(codes() & 0x7F7F7F7Fu)) return 1.f;
+            if (!__any(sums() << 1)) least = most = e_v;
+            least = min(least, e_v), most = max(most, e_v);
+            if (most - least > kFar) l.sum = NAN;
+            move(e - e_v);
+            e = e_v;
+        }
+        return two_to(e_v - e);
+    }
+};
+
 // Which of the positions base .. base + 15 lie at or below `last` and at or above
 // `first` or below `sinks`, a bit each.
 __device__ __forceinline__ uint32_t seen_bits(int base, int last, int first, int sinks) {
@@ -790,7 +817,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     for (int u = 0; u < C; ++u) o[u] = f32x16{};
     float m2 = -INFINITY;
     WeightSum l;
-    int v_exp = 0;  // o is in units of 2^v_exp
+    ValueUnit unit;  // of o
     uint32_t now_k = held_k, now_v = held_v, next_k = 0, next_v = 0;  // (the next ones are looked up a tile ahead)
     auto lds_at = [&](int i) { return smem + (i % (3 * NB) * WK + wk) * 2 * BB + 16 * lane; };
     auto read_k = [&](int i) {
@@ -851,33 +878,32 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
     f32x16 s;
     float fs = 0.f;
     auto reference = [&]() { return m2 == -INFINITY ? 0.f : m2; };
-    // V under 2^(e_v - v_exp): exact in F16, times 2^-11 too, for differences of -4 .. 7.
-    // The factor of block i's codes.
+    // The factor of block i's codes, exact in F16 times 2^-11 too.
     auto value_scale = [&](int i) {
-        const int e_v = (int)__builtin_amdgcn_readlane(now_v, i & 63) - 127;
-        if (i == 0) v_exp = e_v;
-        if (e_v - v_exp > 7 || e_v - v_exp < -4) {
-            // Steps that could lose the sums' values: the rows are computed again. (A block
-            // of zeros, whose scale is the least, and sums that are 0 lose nothing.)
-            if (abs(e_v - v_exp) > 100) {
-                uint32_t codes = 0, sums = 0;
+        return unit.factor(
+            (int)__builtin_amdgcn_readlane(now_v, i & 63) - 127, i == 0, 4, l,
+            [&]() {
+                uint32_t codes = 0;
 #pragma unroll
-                for (int u = 0; u < C; ++u) {
+                for (int u = 0; u < C; ++u)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) codes |= vr[u][j];
+                return codes;
+            },
+            [&]() {
+                uint32_t sums = 0;
+#pragma unroll
+                for (int u = 0; u < C; ++u)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) sums |= __float_as_uint(o[u][r]);
-                }
-                if (!__any(codes & 0x7F7F7F7Fu)) return 1.f;
-                if (__any(sums << 1)) l.sum = NAN;
-            }
+                return sums;
+            },
+            [&](int n) {
 #pragma unroll
-            for (int u = 0; u < C; ++u)
+                for (int u = 0; u < C; ++u)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[u][r] = ldexpf(o[u][r], v_exp - e_v);
-            v_exp = e_v;
-        }
-        return two_to(e_v - v_exp);
+                    for (int r = 0; r < 16; ++r) o[u][r] = ldexpf(o[u][r], n);
+            });
     };
     // Positions that no row of the block sees may hold anything: zeros.
     auto clear_v = [&](int i) {
@@ -1041,7 +1067,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
             for (int q = 0; q < 4; ++q)
                 *(f32x4 *)(so + 32 * u + 8 * q + 4 * half) =
                     f32x4{o[u][4 * q], o[u][4 * q + 1], o[u][4 * q + 2], o[u][4 * q + 3]};
-        if (half == 0) words[wave * 32 + n] = f32x4{m2, l.sum, two_to(v_exp), 0.f};
+        if (half == 0) words[wave * 32 + n] = f32x4{m2, l.sum, two_to(unit.e), 0.f};
     }
     if (threadIdx.x < WR) odd[threadIdx.x] = 0;
     __syncthreads();
@@ -1242,7 +1268,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
     for (int u = 0; u < U; ++u) o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m2 = -INFINITY;
     WeightSum l;
-    int v_exp = 0;  // o is in units of 2^v_exp
+    ValueUnit unit;  // of o
     uint32_t now_k = held_k, now_v = held_v;
     for (int i = 0; i < mine; ++i) {
         if (i > 0 && (i & 63) == 0) now_k = held_k, now_v = held_v;
@@ -1306,30 +1332,29 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
 #pragma unroll
             for (int u = 0; u < U; ++u) vr[u].x &= b0, vr[u].y &= b1;
         }
-        // V under 2^(e_v - v_exp): exact in F16 for differences of -15 .. 7, of -4 .. 7
-        // where the low parts meet it times 2^-11 (of 8 rows their columns carry that).
-        const int e_v = (int)__builtin_amdgcn_readlane(now_v, i & 63) - 127;
-        if (i == 0) v_exp = e_v;
-        if (e_v - v_exp > 7 || e_v - v_exp < (P == 1 ? -15 : -4)) {
-            uint32_t codes = 0, sums = 0;
+        // (Of 8 rows the low parts' columns carry the 2^-11, not V.)
+        const float vs = unit.factor(
+            (int)__builtin_amdgcn_readlane(now_v, i & 63) - 127, i == 0, P == 1 ? 15 : 4, l,
+            [&]() {
+                uint32_t codes = 0;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                codes |= vr[u].x | vr[u].y;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) sums |= __float_as_uint(o[u][k]);
-            }
-            // Far steps could lose the sums' values: the rows are computed again; a block
-            // of zeros takes any scale.
-            if (__any(codes & 0x7F7F7F7Fu)) {
-                if (abs(e_v - v_exp) > 100 && __any(sums << 1)) l.sum = NAN;
+                for (int u = 0; u < U; ++u) codes |= vr[u].x | vr[u].y;
+                return codes;
+            },
+            [&]() {
+                uint32_t sums = 0;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) o[u][k] = ldexpf(o[u][k], v_exp - e_v);
-                v_exp = e_v;
-            }
-        }
-        const float vs = two_to(min(max(e_v - v_exp, -126), 127));
+                    for (int k = 0; k < 4; ++k) sums |= __float_as_uint(o[u][k]);
+                return sums;
+            },
+            [&](int by) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[u][k] = ldexpf(o[u][k], by);
+            });
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const f16x8 x = codes_f16(vr[u].x, vr[u].y, vs);
@@ -1354,7 +1379,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void kv8_few_kernel(Kv8AttnArgs a, 
             for (int k = 0; k < 4; ++k) v[i][k] = whole_row(o[u + i][k] * column);
         if (r < rows) *(f32x4 *)(so + 16 * (u + n / R)) = n < R ? v[0] : v[2 - P];
     }
-    if (lane < R) words[wave * R + r] = f32x4{m2, l.sum, two_to(v_exp), 0.f};
+    if (lane < R) words[wave * R + r] = f32x4{m2, l.sum, two_to(unit.e), 0.f};
     __syncthreads();
     for (int u = (int)threadIdx.x; u < rows * (HD / 4); u += 64 * W) {  // 4 dims of a row
         const int rr = u / (HD / 4), d = u % (HD / 4) * 4, at = over_g(m0 + rr);

@@ -83,3 +83,51 @@ def test_large_values_behind_small_weights(hip, call):
     q = (0.3 * rng.standard_normal((rows, q_heads, hd))).astype(np.float32)
     q[..., 0] = 25 * np.log(2) * np.sqrt(hd) / 16
     check(call, *filled(hip, rng, call, k, v), q)
+
+
+# 256 KV heads of the same rows: a few rows are a block a CU, whose waves see every 8th,
+# 4th, 2nd or each block of positions. Blocks of 8 rows, of 16, of one, two and four
+# waves of 32.
+HEADS = 256
+
+
+def alike(hip, rng, k, v, rows, hd, far):
+    """Attention of the last `rows` of the positions, rows of queries whose channel 0
+    puts `far` powers of two between k's of 16 and -16, and its 64 bits."""
+    n = len(k)
+    dev, cpu = make(hip, rng, n, HEADS, hd), ref.Cache(n, 1, hd)
+    dev.append(np.tile(k, HEADS), np.tile(v, HEADS), 0)
+    cpu.append(k, v, 0)
+    q = (0.3 * rng.standard_normal((rows, HEADS, hd))).astype(np.float32)
+    q[..., 0] = far * np.log(2) * np.sqrt(hd) / 32
+    got = dev.attention(q.reshape(rows, -1), HEADS, n - rows).reshape(q.shape)
+    ck, cv = (x[:, 0] for x in cpu.values(0, n))
+    want = np.empty(q.shape)
+    for i, x in enumerate(q.astype(np.float64)):
+        s = x @ ck[:n - rows + i + 1].T / np.sqrt(hd)
+        w = np.exp(s - s.max(1, keepdims=True))
+        want[i] = w @ cv[:n - rows + i + 1] / w.sum(1, keepdims=True)
+    return got, want
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [1, 16, 32, 64, 128])
+@pytest.mark.parametrize("sizes", [(-90, 0, 90), (-60, -20, 60), (-9, 0, 9), (90, 0, -90), (0, -200, 0), (-200, 0, 0)])
+def test_values_that_grow_and_shrink_in_steps(hip, rows, hd, sizes):
+    """The first eight blocks hold values of one size and all of the weight, the next
+    eight and the rest others (2^-200: zeros), whose weights are 2^-300: none of it shows,
+    in whatever steps a wave's sums change their unit. Scores are +-150 powers of two, so
+    each of the hd sums that make one rounds by up to 2^-17 (half of the last bit of 128 to
+    256), 2^-17 sqrt(hd / 3) at random, times ln 2 in the weight: 2.0e-5 (hd 64) and 3.4e-5
+    of a weight, as much of an output, at most three deviations of it 1e-4 = 5 TOL."""
+    rng = np.random.default_rng(rows + hd)
+    n = 1120 + rows
+    k, v = (rng.standard_normal((n, hd)).astype(np.float32) for _ in "kv")
+    block = np.arange(n) // 32
+    k[:, 0] = np.where(block < 8, 16, -16)
+    v = (v.astype(np.float64) * 2.0 ** np.array(sizes)[np.minimum(block // 8, 2)][:, None]).astype(np.float32)
+    got, want = alike(hip, rng, k, v, rows, hd, 300)
+    if sizes[0] == -200:  # the weight is all on values of 0
+        assert (got == 0).all()
+        return
+    assert (np.abs(got - want).max(2) <= 5 * TOL * np.abs(want).max(2)).all()
