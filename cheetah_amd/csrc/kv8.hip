@@ -436,13 +436,15 @@ __device__ __attribute__((noinline)) void plain_row(Kv8KernArgs args, int row, i
             if (b * kBlock >= sinks && (b + 1) * kBlock <= lo) b = lo / kBlock;
             const int page = a.g.page_table[(size_t)b * kBlock / a.g.page_size];
             const BlockAt at = block_at(a.g, page, b % (a.g.page_size / kBlock), g, HD);
+            // (Scaled values, not codes: those over large queries could pass the range.)
+            const float k_scale = two_to((int)a.k_scales[at.scale] - 127);
             float dot = 0.f;
 #pragma unroll 1
             for (int c = 0; c < C; ++c) {
                 const uint32_t *w = (const uint32_t *)(a.k + at.codes + c * (kBlock * 32) + n * 32 + 16 * half);
 #pragma unroll 1
                 for (int i = 0; i < 4; ++i) {
-                    const f32x4 k = code_values(w[i]), x = *(const f32x4 *)(q + 32 * c + 4 * i);
+                    const f32x4 k = code_values(w[i]) * k_scale, x = *(const f32x4 *)(q + 32 * c + 4 * i);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) dot = fmaf(k[e], x[e], dot);
                 }
@@ -450,7 +452,7 @@ __device__ __attribute__((noinline)) void plain_row(Kv8KernArgs args, int row, i
             dot += __shfl_xor(dot, 32, 64);
             const int p = b * kBlock + n;
             const bool seen = p <= pos && (p >= lo || p < sinks);
-            const float s = seen ? dot * two_to((int)a.k_scales[at.scale] - 127) * sl2 : -INFINITY;
+            const float s = seen ? dot * sl2 : -INFINITY;
             if (pass == 0) {
                 const float mn = fmaxf(m, wave_max(s));
                 const float w = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - mn);

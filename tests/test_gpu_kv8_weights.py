@@ -131,3 +131,28 @@ def test_values_that_grow_and_shrink_in_steps(hip, rows, hd, sizes):
         assert (got == 0).all()
         return
     assert (np.abs(got - want).max(2) <= 5 * TOL * np.abs(want).max(2)).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [1, 16, 32, 64, 128])
+def test_large_queries_over_tiny_keys_computed_again(hip, rows, hd):
+    """Values near the largest, so that every row is computed again (their sums pass the
+    type's range), and queries of 2^122 over keys near the least: products of codes and
+    queries pass it too, those of values do not. Channels 0 and 1 cancel exactly."""
+    rng = np.random.default_rng(rows + hd)
+    n = 300 + rows
+    k = (rng.standard_normal((n, hd)) * 2.0 ** -117).astype(np.float32)
+    k[:, :2] = 64 * 2.0 ** -117
+    v = (3e38 * rng.uniform(0.5, 1.0, (n, hd))).astype(np.float32)
+    dev, cpu = make(hip, rng, n, HEADS, hd), ref.Cache(n, 1, hd)
+    dev.append(np.tile(k, HEADS), np.tile(v, HEADS), 0)
+    cpu.append(k, v, 0)
+    q = (2.0 ** 117 * rng.standard_normal((rows, HEADS, hd))).astype(np.float32)
+    q[..., 0], q[..., 1] = 2.0 ** 122, -2.0 ** 122
+    got = dev.attention(q.reshape(rows, -1), HEADS, n - rows).reshape(q.shape)
+    ck, cv = (x[:, 0] for x in cpu.values(0, n))
+    for i, x in enumerate(q.astype(np.float64)):
+        s = x @ ck[:n - rows + i + 1].T / np.sqrt(hd)
+        w = np.exp(s - s.max(1, keepdims=True))
+        want = w @ cv[:n - rows + i + 1] / w.sum(1, keepdims=True)
+        assert (np.abs(got[i] - want).max(1) <= TOL * np.abs(want).max(1)).all()
