@@ -414,6 +414,8 @@ class Kv8Cache:
         """cheetah_hip_kv8_attention: q f32 [rows, q_heads * head_dim]."""
         q = np.ascontiguousarray(q, np.float32).reshape(-1, q_heads * self.head_dim)
         rows = q.shape[0]
+        if window < 0 or sinks < 0:
+            raise ValueError("a window and sinks count positions: not below 0")
         first = max(offset + 1 - window, 0) if window else 0
         self._listed(0, min(sinks, first))
         self._listed(first, offset + rows)

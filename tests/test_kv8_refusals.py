@@ -128,3 +128,20 @@ def test_the_reference_grows_a_scale_without_moving_normal_codes():
     a, b = whole.values(0, 20)[0], pieces.values(0, 20)[0]
     most = np.abs(a).max()
     assert (np.abs(a - b)[np.abs(a) >= most * 2.0 ** -13] == 0).all() and np.abs(a - b).max() <= most * 2.0 ** -16.8
+
+
+def wrapper(hip, table):
+    """A cache's Python side alone, over a table."""
+    cache = hip.Kv8Cache.__new__(hip.Kv8Cache)
+    cache.table, cache.page_size, cache.kv_heads, cache.head_dim = np.asarray(table, np.int32), 64, 1, 64
+    cache.view = view(hip, kvh=1)
+    return cache
+
+
+@pytest.mark.parametrize("kw", [dict(window=-1), dict(window=64, sinks=-1), dict(window=-64, sinks=3)])
+def test_the_wrapper_refuses_negative_windows_and_sinks(hip, kw):
+    """Taken as whole numbers without a sign they would reach every page, those that the
+    table does not list among them."""
+    cache = wrapper(hip, [-1, -1, 0, 1])
+    with pytest.raises(ValueError, match="window"):
+        cache.attention(np.zeros((1, 64), np.float32), 1, 200, **kw)
