@@ -529,9 +529,10 @@ __host__ __device__ __forceinline__ Reach reach_of(int pos_lo, int pos_hi, int w
 // copies fill three tiles of LDS, a barrier a tile. (Few rows have a kernel of their
 // own, kv8_few_kernel.)
 //
-// Bound: with many rows the matrix cores, at the rate that a large F16 product of
-// the library reaches (512 rows on 4,096, 32 / 8 heads of 128: 75.9 us, of which
-// queries in and outputs out take 12); with few round trips.
+// Bound: with many rows vector and matrix instructions, which hardly overlap (512 rows
+// on 4,096, 32 / 8 heads of 128: 76.9 us, vector instructions in 55 % of the SIMDs'
+// cycles, matrix ones in 46 %; queries in and outputs out take 12); with few round
+// trips.
 // ---------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -1136,9 +1137,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))
 //   O^T += V^T P^T  A = V^T: lane (n, q) takes positions 8 q .. + 7 of dim 16 u + n;
 //                   lane (m, q) holds the probabilities of its row there.
 // Blocks of 8 waves, every one with blocks of positions of its own, K and V from
-// memory into registers. 1 on 576 (14 / 2 heads of 64) 5.6 us (6.3 with 32-wide
-// products), 1 on 32,767 (28 / 4 of 128) 12.2 (12.9), under a window of 4,096 8.5 (9.5),
-// 13 on 1,999 (32 / 8 of 128) 9.9 (11.0). Of 8 rows 16 waves 6.4 / 14.2 / 10.9, two
+// memory into registers. 1 on 576 (14 / 2 heads of 64) 5.5 us (6.3 with 32-wide
+// products), 1 on 32,767 (28 / 4 of 128) 12.2 (12.9), under a window of 4,096 8.9 (9.5),
+// 13 on 1,999 (32 / 8 of 128) 9.0 (11.0). Of 8 rows 16 waves 6.4 / 14.2 / 10.9, two
 // blocks a CU 5.7 / 13.2 / 8.5, two blocks of positions in flight 5.8 / 13.5 / 9.2.
 // Bound by round trips (page, K and V, the join) and the merge's launch.
 // ---------------------------------------------------------------------------

@@ -257,9 +257,12 @@ typedef struct cheetah_hip_snapshot cheetah_hip_snapshot;
  * ops.rs:1533-1537). kv_format: element type of the paged KV cache, 0 = BF16
  * (half the KV bytes), 1 = f32 (the reference's own cache precision,
  * ops.rs:995-999), 2 = 8 bits (a quarter; cheetah_hip_kv8_append's codes and
- * scales: K and V are rounded, by up to 2^-4 of a value). Over an 8-bit cache a
- * position's results depend, in their last bits, on how the text was cut into
- * chunks, and drafted tokens are refused. kv_capacity: positions the KV pool holds across this
+ * scales: K and V are rounded, by up to 2^-4 of a value; values below 2^-13.8 of
+ * the largest of their block, by up to 2^-17.8 of that, so that small ones can
+ * vanish). Over an 8-bit cache a position's results depend, in their last bits, on
+ * how the text was cut into chunks and, behind a prefix restored up to a position
+ * inside a block, on the rows cut off (the block's scale stays theirs), and drafted
+ * tokens are refused. kv_capacity: positions the KV pool holds across this
  * model, its clones and its snapshots (0 = 65536). max_chunk_rows: largest
  * prefill chunk (0 = 1024). */
 cheetah_hip_model *cheetah_hip_model_create(const cheetah_hip_config *cfg, uint32_t quant_format,
