@@ -67,6 +67,28 @@ def test_one_key_far_above_a_long_tail(hip, call, value):
             check(call, dev, held, q, (gap, spread))
 
 
+@pytest.mark.parametrize("call", [c for c in CALLS if not c[5] and c[4]])
+def test_keys_that_dominate_some_heads_in_mid_context(hip, call):
+    """Keys of one value each at two thirds and at nine tenths of the context, far above
+    the rest for some rows and heads of a tile and far below it for others: sums move to
+    the later maxima and the tails on either side keep their weights (as above)."""
+    q_heads, kvh, hd, rows, offset, *_ = call
+    rng = np.random.default_rng(rows + hd)
+    n = offset + rows
+    k, v = (rng.standard_normal((n, kvh, hd)).astype(np.float32) for _ in "kv")
+    k[..., :2] = 0
+    for c, at in enumerate((offset * 2 // 3, offset * 9 // 10)):
+        k[at] = 0
+        k[at, :, c] = 16
+        v[at] = 0
+    dev, held = filled(hip, rng, call, k, v)
+    q = (0.3 * rng.standard_normal((rows, q_heads, hd))).astype(np.float32)
+    gap = rng.integers(-26, 25, (rows, q_heads))
+    q[..., 0] = gap * np.log(2) * np.sqrt(hd) / 16
+    q[..., 1] = (gap + 2) * np.log(2) * np.sqrt(hd) / 16
+    check(call, dev, held, q)
+
+
 @pytest.mark.parametrize("call", CALLS)
 def test_large_values_behind_small_weights(hip, call):
     """Every fourth block scores 25 powers of two below the others and holds values
